@@ -13,6 +13,10 @@ import torch  # noqa: F401  (must be imported before the HIP library is loaded)
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libco_alibi.so")
 
+# Most new tokens per sequence of co_alibi_decode_tree, and most logits per row of co_alibi_sample.
+MAX_TREE_TOKENS = 64
+MAX_VOCAB = 1 << 20
+
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 SUPPORTED_HEAD_DIMS = (16, 32, 64, 128, 256)
 
@@ -41,6 +45,10 @@ EXPORTS = (
     "co_alibi_decode_splits",
     "co_alibi_decode",
     "co_alibi_decode_noalloc",
+    "co_alibi_decode_tree_workspace_bytes",
+    "co_alibi_decode_tree",
+    "co_alibi_cache_append",
+    "co_alibi_sample",
     "co_alibi_probe_mfma",
     "co_alibi_last_error",
     "co_alibi_abi_version",
@@ -51,6 +59,8 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 _Z = ctypes.c_size_t
 _L = ctypes.POINTER(ctypes.c_longlong)
+_LL = ctypes.c_longlong
+_D = ctypes.c_double
 
 _SIGNATURES = {
     "co_alibi_stats_numel": (_Z, [_I, _I, _I, _I]),
@@ -86,6 +96,16 @@ _SIGNATURES = {
     "co_alibi_decode_splits": (_I, [_I, _I, _I, _I, _I, _I]),
     "co_alibi_decode": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _P, _Z, _I, _I, _I, _I, _I, _I, _F, _P]),
     "co_alibi_decode_noalloc": (_I, [_I, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _P]),
+    "co_alibi_decode_tree_workspace_bytes": (_Z, [_I] * 7),
+    "co_alibi_decode_tree": (
+        _I,
+        [_I, _P, _P, _P, _P, _P, _L, _P, _P, _P, _I, _P, _I, _I, _I, _P, _P, _P, _Z, _I, _I, _I, _I, _I, _I, _F, _P],
+    ),
+    "co_alibi_cache_append": (
+        _I,
+        [_I, _P, _P, _P, _P, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
+    ),
+    "co_alibi_sample": (_I, [_I, _P, _LL, _P, _I, _P, _P, _P, _P, _D, _I, _D, _D, _P, _I, _I, _P]),
     "co_alibi_probe_mfma": (_I, [_P, _P, _I, _I, _P]),
     "co_alibi_last_error": (ctypes.c_char_p, []),
     "co_alibi_abi_version": (_I, []),

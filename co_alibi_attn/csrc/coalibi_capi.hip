@@ -735,6 +735,208 @@ int co_alibi_decode_noalloc(int dtype, const void* q, const void* k_cache, const
                      heads_q, heads_kv, seq_kv, kv_capacity, head_dim, sm_scale, stream);
 }
 
+}  // extern "C"
+
+// ------------------------------------------------------------------------- serving step
+
+namespace {
+
+// A cache's place arguments: without a block table page_size is a sequence's capacity.
+int check_place(const char* fn, const int* block_table, int blocks_per_seq, int num_pages, int page_size, int batch,
+                coalibi::CachePlace* out, long long* capacity) {
+  if (page_size < 1) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": page_size must be >= 1");
+  if (block_table == nullptr) {
+    *out = {nullptr, 0, batch, 31};
+    *capacity = page_size;
+    return CO_ALIBI_OK;
+  }
+  if (!aligned(block_table, 4)) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": block_table is not 4-byte aligned");
+  if (page_size < 16 || (page_size & (page_size - 1)) != 0)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": page_size must be a power of two >= 16, got " +
+                                     std::to_string(page_size));
+  if (blocks_per_seq < 1 || num_pages < 1)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": blocks_per_seq and num_pages must be >= 1");
+  int shift = 4;
+  while ((1 << shift) < page_size) ++shift;
+  *out = {block_table, blocks_per_seq, num_pages, shift};
+  *capacity = static_cast<long long>(blocks_per_seq) * page_size;
+  return CO_ALIBI_OK;
+}
+
+// Layout i of a call's strides (three values each), or the contiguous one.
+int layout_at(const char* fn, const char* name, const long long* strides, int i, int dtype, int H, int S, int D,
+              coalibi::Layout* out) {
+  return read_layout(fn, name, strides == nullptr ? nullptr : strides + 3 * i, dtype, H, S, D, out);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t co_alibi_decode_tree_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,
+                                            int head_dim) {
+  return 0;
+}
+
+int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v, const void* k_cache,
+                         const void* v_cache, const long long* strides, const float* slopes, const int* seq_lens,
+                         const int* parents, int parents_per_seq, const int* block_table, int blocks_per_seq,
+                         int num_pages, int page_size, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                         int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim, float sm_scale,
+                         void* stream) {
+  const char* fn = "co_alibi_decode_tree";
+  const Shape s{batch, heads_q, heads_kv, tokens, seq_kv > 0 ? seq_kv : 1, head_dim};
+  int rc;
+  if ((rc = check_shape(fn, dtype, s))) return rc;
+  if (head_dim == 256 && dtype == CO_ALIBI_F32)
+    return fail(CO_ALIBI_EUNSUPPORTED, std::string(fn) + ": head_dim 256 needs fp16 or bf16");
+  if (tokens > coalibi::kMaxTreeTokens)
+    return fail(CO_ALIBI_EUNSUPPORTED, std::string(fn) + ": at most " + std::to_string(coalibi::kMaxTreeTokens) +
+                                           " new tokens per sequence, got " + std::to_string(tokens));
+  coalibi::TreeArgs a{};
+  long long capacity = 0;
+  if ((rc = check_place(fn, block_table, blocks_per_seq, num_pages, page_size, batch, &a.place, &capacity))) return rc;
+  if (seq_kv < 0 || seq_kv > capacity)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": seq_kv must be in [0, " + std::to_string(capacity) + "]");
+  if ((rc = check_ptr(fn, "q", q, 16)) || (rc = check_ptr(fn, "k", k, 16)) || (rc = check_ptr(fn, "v", v, 16)) ||
+      (rc = check_ptr(fn, "k_cache", k_cache, 16)) || (rc = check_ptr(fn, "v_cache", v_cache, 16)) ||
+      (rc = check_ptr(fn, "o", o, 16)) || (rc = check_ptr(fn, "slopes", slopes, 4)) ||
+      (rc = check_opt_ptr(fn, "seq_lens", seq_lens, 4)) || (rc = check_opt_ptr(fn, "parents", parents, 4)) ||
+      (rc = check_opt_ptr(fn, "lse", lse, 4)))
+    return rc;
+  if (!std::isfinite(sm_scale)) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": sm_scale must be finite");
+  if ((rc = layout_at(fn, "q", strides, 0, dtype, heads_q, tokens, head_dim, &a.ql)) ||
+      (rc = layout_at(fn, "k", strides, 1, dtype, heads_kv, tokens, head_dim, &a.kl)) ||
+      (rc = layout_at(fn, "v", strides, 2, dtype, heads_kv, tokens, head_dim, &a.vl)) ||
+      (rc = layout_at(fn, "k_cache", strides, 3, dtype, heads_kv, page_size, head_dim, &a.kcl)) ||
+      (rc = layout_at(fn, "v_cache", strides, 4, dtype, heads_kv, page_size, head_dim, &a.vcl)))
+    return rc;
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.kc = k_cache;
+  a.vc = v_cache;
+  a.slopes = slopes;
+  a.o = o;
+  a.lse = lse;
+  a.seq_lens = seq_lens;
+  a.parents = parents;
+  a.parents_stride = parents_per_seq != 0 ? tokens : 0;
+  a.B = batch;
+  a.Hq = heads_q;
+  a.Hkv = heads_kv;
+  a.G = heads_q / heads_kv;
+  a.T = tokens;
+  a.L = seq_kv;
+  a.D = head_dim;
+  a.sc2 = sm_scale * coalibi::kLog2eHost;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e;
+  switch (dtype) {
+    case CO_ALIBI_F16: e = coalibi::launch_tree<_Float16>(a, st); break;
+    case CO_ALIBI_BF16: e = coalibi::launch_tree<__bf16>(a, st); break;
+    default: e = coalibi::launch_tree<float>(a, st); break;
+  }
+  if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+  return CO_ALIBI_OK;
+}
+
+int co_alibi_cache_append(int dtype, const void* k, const void* v, void* k_cache, void* v_cache,
+                          const long long* strides, const int* seq_lens, const int* counts, const int* rows,
+                          int new_rows, const int* block_table, int blocks_per_seq, int num_pages, int page_size,
+                          int batch, int heads_kv, int tokens, int head_dim, void* stream) {
+  const char* fn = "co_alibi_cache_append";
+  const Shape s{batch, heads_kv, heads_kv, tokens, 1, head_dim};
+  int rc;
+  if ((rc = check_shape(fn, dtype, s))) return rc;
+  if (new_rows < 1) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": new_rows must be >= 1");
+  if (rows == nullptr && new_rows > tokens)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": new_rows is above tokens and there is no rows array");
+  coalibi::AppendArgs a{};
+  long long capacity = 0;
+  if ((rc = check_place(fn, block_table, blocks_per_seq, num_pages, page_size, batch, &a.place, &capacity))) return rc;
+  const int elem = dtype == CO_ALIBI_F32 ? 4 : 2;
+  if (static_cast<double>(new_rows) * heads_kv * head_dim * elem / 16 > 1e9 || capacity > (1ll << 30))
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
+  if ((rc = check_ptr(fn, "k", k, 16)) || (rc = check_ptr(fn, "v", v, 16)) ||
+      (rc = check_ptr(fn, "k_cache", k_cache, 16)) || (rc = check_ptr(fn, "v_cache", v_cache, 16)) ||
+      (rc = check_ptr(fn, "seq_lens", seq_lens, 4)) || (rc = check_opt_ptr(fn, "counts", counts, 4)) ||
+      (rc = check_opt_ptr(fn, "rows", rows, 4)))
+    return rc;
+  const int units = block_table != nullptr ? num_pages : batch;
+  if ((rc = layout_at(fn, "k", strides, 0, dtype, heads_kv, tokens, head_dim, &a.kl)) ||
+      (rc = layout_at(fn, "v", strides, 1, dtype, heads_kv, tokens, head_dim, &a.vl)) ||
+      (rc = layout_at(fn, "k_cache", strides, 2, dtype, heads_kv, page_size, head_dim, &a.kcl)) ||
+      (rc = layout_at(fn, "v_cache", strides, 3, dtype, heads_kv, page_size, head_dim, &a.vcl)) ||
+      (rc = check_output(fn, "k_cache", a.kcl, units, heads_kv, page_size, head_dim)) ||
+      (rc = check_output(fn, "v_cache", a.vcl, units, heads_kv, page_size, head_dim)))
+    return rc;
+  a.k = k;
+  a.v = v;
+  a.kc = k_cache;
+  a.vc = v_cache;
+  a.seq_lens = seq_lens;
+  a.counts = counts;
+  a.rows = rows;
+  a.B = batch;
+  a.Hkv = heads_kv;
+  a.T = tokens;
+  a.N = new_rows;
+  a.capacity = static_cast<int>(capacity);
+  a.row_chunks = head_dim * elem / 16;
+  a.elem = elem;
+  const hipError_t e = coalibi::launch_append(a, static_cast<hipStream_t>(stream));
+  if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+  return CO_ALIBI_OK;
+}
+
+int co_alibi_sample(int dtype, const void* logits, long long row_stride, const void* uniforms, int uniforms_f64,
+                    const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                    double temperature_all, int top_k_all, double top_p_all, double min_p_all, long long* tokens,
+                    int batch, int vocab, void* stream) {
+  const char* fn = "co_alibi_sample";
+  if (dtype != CO_ALIBI_F32 && dtype != CO_ALIBI_F16 && dtype != CO_ALIBI_BF16)
+    return fail(CO_ALIBI_EUNSUPPORTED, std::string(fn) + ": dtype must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+  if (batch < 1) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": batch must be >= 1");
+  if (vocab < 1 || vocab > coalibi::kMaxVocab)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": vocab must be in [1, " + std::to_string(coalibi::kMaxVocab) + "]");
+  if (row_stride < 0) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": row_stride must be >= 0");
+  int rc;
+  if ((rc = check_ptr(fn, "logits", logits, dtype == CO_ALIBI_F32 ? 4 : 2)) ||
+      (rc = check_ptr(fn, "uniforms", uniforms, uniforms_f64 != 0 ? 8 : 4)) ||
+      (rc = check_ptr(fn, "tokens", tokens, 8)) || (rc = check_opt_ptr(fn, "temperature", temperature, 4)) ||
+      (rc = check_opt_ptr(fn, "top_k", top_k, 4)) || (rc = check_opt_ptr(fn, "top_p", top_p, 4)) ||
+      (rc = check_opt_ptr(fn, "min_p", min_p, 4)))
+    return rc;
+  coalibi::SampleArgs a{};
+  a.logits = logits;
+  a.row_stride = row_stride;
+  a.uniforms = uniforms;
+  a.uniforms_f64 = uniforms_f64 != 0;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.temperature_all = temperature_all;
+  a.top_k_all = top_k_all;
+  a.top_p_all = top_p_all;
+  a.min_p_all = min_p_all;
+  a.tokens = tokens;
+  a.B = batch;
+  a.V = vocab;
+  a.mass_bits = 62;
+  while ((1ll << (62 - a.mass_bits)) < vocab) --a.mass_bits;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e;
+  switch (dtype) {
+    case CO_ALIBI_F16: e = coalibi::launch_sample<_Float16>(a, st); break;
+    case CO_ALIBI_BF16: e = coalibi::launch_sample<__bf16>(a, st); break;
+    default: e = coalibi::launch_sample<float>(a, st); break;
+  }
+  if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+  return CO_ALIBI_OK;
+}
+
 const char* co_alibi_last_error(void) { return g_last_error.c_str(); }
 
 int co_alibi_abi_version(void) { return 6; }

@@ -359,9 +359,85 @@ hipError_t launch_fwd(const FwdArgs& a, hipStream_t stream);
 template <typename T, int D>
 hipError_t launch_decode(const DecodeArgs& a, hipStream_t stream);
 
+// Where the rows of a key / value cache lie: row r of kv head h of sequence b is row r % 2^page_shift of
+// head h of unit table[b][r / 2^page_shift]; without a table the unit is b, one per sequence.
+struct CachePlace {
+  const int* table;  // (B, table_stride), or NULL
+  int table_stride;
+  int units;       // pages of the pool, or sequences: a table entry outside [0, units) is none
+  int page_shift;  // without a table 31: every row lies in page 0
+};
+
+// Tree decode: q/o (B, Hq, T, D), k/v (B, Hkv, T, D) the step's own tokens; kc/vc the caches (their
+// layouts' b is the stride from unit to unit).  Row g * T + t of a kv head is query head hkv * G + g of
+// node t.
+constexpr int kMaxTreeTokens = 64;  // a node's ancestors are the bits of one 64-bit mask
+struct TreeArgs {
+  Layout ql, kl, vl, kcl, vcl;
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* kc;
+  const void* vc;
+  CachePlace place;
+  const float* slopes;  // (Hq,)
+  void* o;
+  float* lse;            // (B, Hq, T) or NULL
+  const int* seq_lens;   // (B,) filled rows, clamped to [0, L], or NULL (all L)
+  const int* parents;    // (B, T) or (T,), or NULL: a chain
+  int parents_stride;    // T, or 0: one tree for every sequence
+  int B, Hq, Hkv, G, T, L, D;
+  float sc2;
+};
+
+// Cache append: row i of sequence b, new row rows[b][i] (or i) of k / v, goes to cache row lens[b] + i, for
+// i < counts[b] (or N).
+struct AppendArgs {
+  Layout kl, vl, kcl, vcl;
+  const void* k;
+  const void* v;
+  void* kc;
+  void* vc;
+  CachePlace place;
+  const int* seq_lens;  // (B,)
+  const int* counts;    // (B,) or NULL
+  const int* rows;      // (B, N) or NULL
+  int B, Hkv, T, N;
+  int capacity;    // cache rows a sequence has room for
+  int row_chunks;  // 16-byte chunks per row
+  int elem;        // bytes per element
+};
+
+// Sampling: one token per row of logits (B, V), rows row_stride elements apart.  A setting's array holds
+// one value per row; without it the value beside it is every row's.
+constexpr int kMaxVocab = 1 << 20;
+struct SampleArgs {
+  const void* logits;
+  long long row_stride;
+  const void* uniforms;  // (B,) fp32, or fp64 with uniforms_f64
+  bool uniforms_f64;
+  const float* temperature;
+  const int* top_k;
+  const float* top_p;
+  const float* min_p;
+  double temperature_all, top_p_all, min_p_all;
+  int top_k_all;
+  long long* tokens;  // (B,)
+  int B, V;
+  int mass_bits;  // a weight of 1 in units of mass: 2^mass_bits, and V * 2^mass_bits <= 2^62
+};
+
 // stages: bit 0 = pass 1 (dq, dsum, and zb / cb or the score store), bit 1 = pass 2 (dk, dv; needs pass
 // 1's output).
 template <typename T, int D, bool CAUSAL>
 hipError_t launch_bwd(const BwdArgs& a, int stages, hipStream_t stream);
+
+template <typename T>
+hipError_t launch_tree(const TreeArgs& a, hipStream_t stream);
+
+hipError_t launch_append(const AppendArgs& a, hipStream_t stream);
+
+template <typename T>
+hipError_t launch_sample(const SampleArgs& a, hipStream_t stream);
 
 }  // namespace coalibi

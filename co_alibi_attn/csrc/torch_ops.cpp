@@ -6,9 +6,13 @@
 //   co_alibi::fwd_qkv(qkv, slopes, causal, sm_scale, with_stats) -> (o, lse, stats)
 //   co_alibi::bwd_qkv(do, qkv, o, lse, stats, slopes, causal, sm_scale) -> dqkv
 //   co_alibi::decode(q, k_cache, v_cache, slopes, seq_lens, max_seq_len, sm_scale, with_lse) -> (o, lse)
+//   co_alibi::decode_tree(q, k, v, k_cache, v_cache, slopes, seq_lens, parents, block_table, max_seq_len, sm_scale,
+//                         with_lse) -> (o, lse)
+//   co_alibi::cache_append(k, v, k_cache!, v_cache!, seq_lens, counts, rows, block_table) -> ()
+//   co_alibi::sample(logits, uniforms, temperature, top_k, top_p, min_p, their four values for every row) -> tokens
 //
 // They replace the reference's two Triton launches with their buffer set-up
-// (co_alibi_attn/co_alibi_attn.py:35-57 and :83-133); decode has no counterpart there.  Each
+// (co_alibi_attn/co_alibi_attn.py:35-57 and :83-133); decode and the operators after it have no counterpart there.  Each
 // kernel runs on the caller's current HIP stream under a device guard of the inputs' device and
 // allocates only through torch's caching allocator, so the operators can be captured in a HIP
 // graph.  co_alibi::fwd carries its backward as a C++ autograd kernel: dQ alone runs backward
@@ -336,6 +340,208 @@ std::tuple<Tensor, Tensor> decode_hip(const Tensor& q_in, const Tensor& k_in, co
   return {o, lse};
 }
 
+// ----------------------------------------------------------------------- serving step
+
+// An index array as the kernels read it (int32, dense, on `like`'s device); 64-bit values that do not fit are
+// clamped, not wrapped into the valid range.
+Tensor index_i32(const Tensor& t, const Tensor& like) {
+  TORCH_CHECK_TYPE(t.scalar_type() == at::kInt || t.scalar_type() == at::kLong,
+                   "co_alibi: lengths, tables and indices must be int32 or int64, got ", t.scalar_type());
+  const Tensor d = t.to(like.device());
+  if (d.scalar_type() == at::kInt) return d.contiguous();
+  return d.clamp(std::numeric_limits<int>::min(), std::numeric_limits<int>::max()).to(at::kInt).contiguous();
+}
+const int* data_or_null(const Tensor& t) { return t.defined() ? t.data_ptr<int>() : nullptr; }
+bool given(const c10::optional<Tensor>& t) { return t.has_value() && t->defined(); }
+
+// The caches of a call over `batch` sequences: pools of pages with a table, else one cache per sequence.  They
+// are read and written in place, never copied, so a layout the kernels cannot address is refused.
+struct Caches {
+  Tensor table;  // int32 (batch, blocks), or undefined
+  int64_t blocks = 0, units = 0, page = 0, capacity = 0;
+};
+Caches check_caches(const char* fn, const Tensor& like, int64_t batch, const Tensor& k_cache, const Tensor& v_cache,
+                    const c10::optional<Tensor>& block_table) {
+  TORCH_CHECK_VALUE(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes(), fn,
+                    ": k_cache and v_cache must be 4-dimensional and of one shape, got ", k_cache.sizes(), " and ",
+                    v_cache.sizes());
+  TORCH_CHECK_TYPE(k_cache.scalar_type() == like.scalar_type() && v_cache.scalar_type() == like.scalar_type(), fn,
+                   ": the caches' dtype must be the new tokens', ", like.scalar_type(), ", got ", k_cache.scalar_type(),
+                   " and ", v_cache.scalar_type());
+  TORCH_CHECK_VALUE(k_cache.device() == like.device() && v_cache.device() == like.device(), fn,
+                    ": the caches must be on the new tokens' device");
+  Caches c;
+  c.units = k_cache.size(0);
+  c.page = k_cache.size(2);
+  if (given(block_table)) {
+    TORCH_CHECK_VALUE(block_table->dim() == 2 && block_table->size(0) == batch, fn, ": block_table must be (", batch,
+                      ", blocks), got ", block_table->sizes());
+    c.table = index_i32(*block_table, like);
+    c.blocks = c.table.size(1);
+    TORCH_CHECK_VALUE(c.page >= 16 && (c.page & (c.page - 1)) == 0, fn, ": a page must hold a power of two >= 16 rows, got ",
+                      c.page);
+    c.capacity = c.blocks * c.page;
+  } else {
+    TORCH_CHECK_VALUE(c.units == batch, fn, ": without a block_table the caches hold one entry per sequence, got ", c.units,
+                      " for ", batch);
+    c.capacity = c.page;
+  }
+  TORCH_CHECK_VALUE(c.capacity <= 1 << 30, fn, ": a sequence's cache holds at most 2^30 rows");
+  if (k_cache.numel() != 0)
+    TORCH_CHECK_VALUE(readable(k_cache) && readable(v_cache), fn,
+                      ": a cache's rows must be dense, 16-byte aligned and at most 2^20 elements apart");
+  return c;
+}
+int as_int(const char* fn, const char* name, int64_t x) {
+  TORCH_CHECK_VALUE(x >= 0 && x <= std::numeric_limits<int>::max(), fn, ": ", name, " out of range: ", x);
+  return static_cast<int>(x);
+}
+
+std::tuple<Tensor, Tensor> decode_tree_hip(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
+                                           const Tensor& k_cache, const Tensor& v_cache, const Tensor& slopes,
+                                           const c10::optional<Tensor>& seq_lens, const c10::optional<Tensor>& parents,
+                                           const c10::optional<Tensor>& block_table, int64_t max_seq_len, double sm_scale,
+                                           bool with_lse) {
+  const char* fn = "co_alibi::decode_tree";
+  TORCH_CHECK_VALUE(q_in.dim() == 4 && k_in.dim() == 4 && v_in.sizes() == k_in.sizes(), fn,
+                    ": q must be (B, Hq, T, D) and k, v (B, Hkv, T, D), got ", q_in.sizes(), ", ", k_in.sizes(), " and ",
+                    v_in.sizes());
+  const int64_t batch = q_in.size(0), heads_q = q_in.size(1), tokens = q_in.size(2), head_dim = q_in.size(3);
+  const int64_t heads_kv = k_in.size(1);
+  TORCH_CHECK_VALUE(k_in.size(0) == batch && k_in.size(2) == tokens && k_in.size(3) == head_dim, fn,
+                    ": k and v must hold q's batch, tokens and head dim, got ", k_in.sizes(), " for ", q_in.sizes());
+  TORCH_CHECK_TYPE(k_in.scalar_type() == q_in.scalar_type() && v_in.scalar_type() == q_in.scalar_type(), fn,
+                   ": q, k and v must share one dtype");
+  TORCH_CHECK_VALUE(k_in.device() == q_in.device() && v_in.device() == q_in.device(), fn,
+                    ": q, k and v must be on one device");
+  const int code = dtype_code(q_in.scalar_type());
+  c10::hip::HIPGuard guard(q_in.device().index());
+  const Caches c = check_caches(fn, q_in, batch, k_cache, v_cache, block_table);
+  TORCH_CHECK_VALUE(k_cache.size(1) == heads_kv && k_cache.size(3) == head_dim, fn,
+                    ": the caches must have k's heads and head dim, got ", k_cache.sizes(), " for ", k_in.sizes());
+  TORCH_CHECK_VALUE(slopes.dim() == 1 && slopes.size(0) == heads_q, fn, ": slopes must be (", heads_q, ",), got ", slopes.sizes());
+  TORCH_CHECK_VALUE(max_seq_len >= 0 && max_seq_len <= c.capacity, fn, ": max_seq_len must be in [0, ", c.capacity, "], got ",
+                    max_seq_len);
+  Tensor lens, par;
+  if (given(seq_lens)) {
+    TORCH_CHECK_VALUE(seq_lens->dim() == 1 && seq_lens->size(0) == batch, fn, ": seq_lens must be (", batch, ",), got ",
+                      seq_lens->sizes());
+    lens = index_i32(*seq_lens, q_in);
+  }
+  if (given(parents)) {
+    const bool one = parents->dim() == 1 && parents->size(0) == tokens;
+    TORCH_CHECK_VALUE(one || (parents->dim() == 2 && parents->size(0) == batch && parents->size(1) == tokens), fn,
+                      ": parents must be (", tokens, ",) or (", batch, ", ", tokens, "), got ", parents->sizes());
+    par = index_i32(*parents, q_in);
+  }
+  const auto f32 = q_in.options().dtype(at::kFloat);
+  Tensor o = at::empty(q_in.sizes(), q_in.options());
+  Tensor lse = with_lse ? at::empty({batch, heads_q, tokens}, f32) : empty_stats(q_in);
+  if (q_in.numel() == 0) return {o, lse};
+  const Tensor q = in_place(q_in), k = in_place(k_in), v = in_place(v_in);
+  // A pool without rows is never read; the launch wants an address all the same.
+  const Tensor kc = k_cache.numel() != 0 ? k_cache : k, vc = v_cache.numel() != 0 ? v_cache : v;
+  TORCH_CHECK_VALUE(k_cache.numel() != 0 || max_seq_len == 0, fn, ": the caches hold no rows");
+  const Tensor sl = slopes_f32(slopes, q);
+  const size_t ws_bytes = co_alibi_decode_tree_workspace_bytes(code, as_int(fn, "batch", batch), as_int(fn, "heads", heads_q),
+                                                               as_int(fn, "heads", heads_kv), as_int(fn, "tokens", tokens),
+                                                               as_int(fn, "max_seq_len", max_seq_len),
+                                                               as_int(fn, "head_dim", head_dim));
+  Tensor ws;
+  if (ws_bytes != 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+  const auto strides = all_strides<5>({q, k, v, kc, vc});
+  const bool none = k_cache.numel() == 0;
+  check(co_alibi_decode_tree(code, q.data_ptr(), k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), strides.data(),
+                             sl.data_ptr<float>(), data_or_null(lens), data_or_null(par),
+                             par.defined() && par.dim() == 2 ? 1 : 0, none ? nullptr : data_or_null(c.table),
+                             as_int(fn, "blocks", c.blocks), as_int(fn, "pages", c.units),
+                             none ? 1 : as_int(fn, "page", c.page), o.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr,
+                             ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, batch, heads_q, heads_kv, tokens, max_seq_len,
+                             head_dim, static_cast<float>(sm_scale), current_stream(q)));
+  return {o, lse};
+}
+
+void cache_append_hip(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache, const Tensor& v_cache,
+                      const Tensor& seq_lens, const c10::optional<Tensor>& counts, const c10::optional<Tensor>& rows,
+                      const c10::optional<Tensor>& block_table) {
+  const char* fn = "co_alibi::cache_append";
+  TORCH_CHECK_VALUE(k_in.dim() == 4 && v_in.sizes() == k_in.sizes(), fn, ": k and v must be (B, Hkv, T, D), got ",
+                    k_in.sizes(), " and ", v_in.sizes());
+  TORCH_CHECK_TYPE(v_in.scalar_type() == k_in.scalar_type(), fn, ": k and v must share one dtype");
+  TORCH_CHECK_VALUE(v_in.device() == k_in.device(), fn, ": k and v must be on one device");
+  const int64_t batch = k_in.size(0), heads_kv = k_in.size(1), tokens = k_in.size(2), head_dim = k_in.size(3);
+  const int code = dtype_code(k_in.scalar_type());
+  c10::hip::HIPGuard guard(k_in.device().index());
+  const Caches c = check_caches(fn, k_in, batch, k_cache, v_cache, block_table);
+  TORCH_CHECK_VALUE(k_cache.size(1) == heads_kv && k_cache.size(3) == head_dim, fn,
+                    ": the caches must have k's heads and head dim, got ", k_cache.sizes(), " for ", k_in.sizes());
+  TORCH_CHECK_VALUE(seq_lens.dim() == 1 && seq_lens.size(0) == batch, fn, ": seq_lens must be (", batch, ",), got ",
+                    seq_lens.sizes());
+  const Tensor lens = index_i32(seq_lens, k_in);
+  Tensor cnt, idx;
+  if (given(counts)) {
+    TORCH_CHECK_VALUE(counts->dim() == 1 && counts->size(0) == batch, fn, ": counts must be (", batch, ",), got ",
+                      counts->sizes());
+    cnt = index_i32(*counts, k_in);
+  }
+  int64_t new_rows = tokens;
+  if (given(rows)) {
+    TORCH_CHECK_VALUE(rows->dim() == 2 && rows->size(0) == batch, fn, ": rows must be (", batch, ", n), got ", rows->sizes());
+    idx = index_i32(*rows, k_in);
+    new_rows = idx.size(1);
+  }
+  if (k_in.numel() == 0 || new_rows == 0 || k_cache.numel() == 0) return;
+  const Tensor k = in_place(k_in), v = in_place(v_in);
+  const auto strides = all_strides<4>({k, v, k_cache, v_cache});
+  check(co_alibi_cache_append(code, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides.data(),
+                              lens.data_ptr<int>(), data_or_null(cnt), data_or_null(idx), as_int(fn, "rows", new_rows),
+                              data_or_null(c.table), as_int(fn, "blocks", c.blocks), as_int(fn, "pages", c.units),
+                              as_int(fn, "page", c.page), as_int(fn, "batch", batch), as_int(fn, "heads", heads_kv),
+                              as_int(fn, "tokens", tokens), as_int(fn, "head_dim", head_dim), current_stream(k)));
+  for (const Tensor* t : {&k_cache, &v_cache})  // autograd's record of a write in place
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+// A setting with one value per row, as the kernel reads it.
+template <typename V>
+const V* setting(const char* fn, const char* name, const c10::optional<Tensor>& t, const Tensor& logits, at::ScalarType type,
+                 Tensor& keep) {
+  if (!given(t)) return nullptr;
+  TORCH_CHECK_VALUE(t->dim() == 1 && t->size(0) == logits.size(0), fn, ": ", name, " must be one value or (", logits.size(0),
+                    ",), got ", t->sizes());
+  keep = type == at::kInt ? index_i32(*t, logits) : t->to(logits.device(), type).contiguous();
+  return keep.data_ptr<V>();
+}
+
+Tensor sample_hip(const Tensor& logits_in, const Tensor& uniforms, const c10::optional<Tensor>& temperature,
+                  const c10::optional<Tensor>& top_k, const c10::optional<Tensor>& top_p, const c10::optional<Tensor>& min_p,
+                  double temperature_all, int64_t top_k_all, double top_p_all, double min_p_all) {
+  const char* fn = "co_alibi::sample";
+  TORCH_CHECK_VALUE(logits_in.dim() == 2, fn, ": logits must be (B, V), got ", logits_in.sizes());
+  const int64_t batch = logits_in.size(0), vocab = logits_in.size(1);
+  const int code = dtype_code(logits_in.scalar_type());
+  TORCH_CHECK_VALUE(uniforms.dim() == 1 && uniforms.size(0) == batch, fn, ": uniforms must be (", batch, ",), got ",
+                    uniforms.sizes());
+  TORCH_CHECK_TYPE(uniforms.scalar_type() == at::kFloat || uniforms.scalar_type() == at::kDouble, fn,
+                   ": uniforms must be float32 or float64, got ", uniforms.scalar_type());
+  c10::hip::HIPGuard guard(logits_in.device().index());
+  Tensor tokens = at::empty({batch}, logits_in.options().dtype(at::kLong));
+  if (batch == 0) return tokens;
+  const Tensor logits = logits_in.stride(1) == 1 || vocab == 1 ? logits_in : logits_in.contiguous();
+  const Tensor uni = uniforms.to(logits.device()).contiguous();
+  Tensor keep[4];
+  const float* t = setting<float>(fn, "temperature", temperature, logits, at::kFloat, keep[0]);
+  const int* k = setting<int>(fn, "top_k", top_k, logits, at::kInt, keep[1]);
+  const float* p = setting<float>(fn, "top_p", top_p, logits, at::kFloat, keep[2]);
+  const float* m = setting<float>(fn, "min_p", min_p, logits, at::kFloat, keep[3]);
+  check(co_alibi_sample(code, logits.data_ptr(), batch == 1 ? vocab : logits.stride(0), uni.data_ptr(),
+                        uni.scalar_type() == at::kDouble ? 1 : 0, t, k, p, m, temperature_all,
+                        static_cast<int>(std::min<int64_t>(std::max<int64_t>(top_k_all, 0), vocab)), top_p_all, min_p_all,
+                        reinterpret_cast<long long*>(tokens.data_ptr<int64_t>()), as_int(fn, "batch", batch),
+                        as_int(fn, "vocab", vocab), current_stream(logits)));
+  return tokens;
+}
+
 // --------------------------------------------------------------------------- autograd
 
 // The operators called below autograd (the forward kernel) and from the backward.
@@ -463,6 +669,12 @@ TORCH_LIBRARY(co_alibi, m) {
         "float sm_scale) -> Tensor");
   m.def("decode(Tensor q, Tensor k_cache, Tensor v_cache, Tensor slopes, Tensor? seq_lens, SymInt max_seq_len, "
         "float sm_scale, bool with_lse) -> (Tensor, Tensor)");
+  m.def("decode_tree(Tensor q, Tensor k, Tensor v, Tensor k_cache, Tensor v_cache, Tensor slopes, Tensor? seq_lens, "
+        "Tensor? parents, Tensor? block_table, SymInt max_seq_len, float sm_scale, bool with_lse) -> (Tensor, Tensor)");
+  m.def("cache_append(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor seq_lens, Tensor? counts, "
+        "Tensor? rows, Tensor? block_table) -> ()");
+  m.def("sample(Tensor logits, Tensor uniforms, Tensor? temperature, Tensor? top_k, Tensor? top_p, Tensor? min_p, "
+        "float temperature_all, SymInt top_k_all, float top_p_all, float min_p_all) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(co_alibi, CUDA, m) {
@@ -472,6 +684,9 @@ TORCH_LIBRARY_IMPL(co_alibi, CUDA, m) {
   m.impl("fwd_qkv", &fwd_qkv_hip);
   m.impl("bwd_qkv", &bwd_qkv_hip);
   m.impl("decode", &decode_hip);
+  m.impl("decode_tree", &decode_tree_hip);
+  m.impl("cache_append", &cache_append_hip);
+  m.impl("sample", &sample_hip);
 }
 
 TORCH_LIBRARY_IMPL(co_alibi, Autograd, m) {

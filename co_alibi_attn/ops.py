@@ -1,5 +1,6 @@
 """PyTorch operators over the native library: ``co_alibi::fwd``, ``co_alibi::bwd``, ``co_alibi::bwd_dq``,
-``co_alibi::fwd_qkv``, ``co_alibi::bwd_qkv``, ``co_alibi::decode``.
+``co_alibi::fwd_qkv``, ``co_alibi::bwd_qkv``, ``co_alibi::decode``, ``co_alibi::decode_tree``,
+``co_alibi::cache_append``, ``co_alibi::sample``.
 
 The operators are defined in C++ (``csrc/torch_ops.cpp``, built into
 ``_lib/libco_alibi_torch.so`` and loaded here): each one is one C-ABI launch
@@ -16,7 +17,8 @@ They replace the reference's two Triton launches with their buffer set-up:
 ``_co_alibi_fwd_kernel[grid](...)`` with the O / LSE / RowSigTotal allocations
 (co_alibi_attn/co_alibi_attn.py:35-57) and ``_co_alibi_bwd_kernel[grid](...)`` with its
 dK / dV partial buffers and their reduction (:83-133).  ``co_alibi::decode`` has no
-counterpart in the reference (its forward with Sq = 1 over a cache).
+counterpart in the reference (its forward with Sq = 1 over a cache), nor have the three after it.
+``co_alibi::cache_append`` writes its two cache operands in place.
 
 Operands are (B, H, S, D) tensors as in include/co_alibi.h.  The forward, and the backward on
 its score-store path, read them in place in any layout whose rows are consecutive and 16-byte
@@ -32,7 +34,8 @@ from torch import Tensor
 
 from . import _native
 
-__all__ = ["fwd", "bwd", "bwd_dq", "fwd_qkv", "bwd_qkv", "backward_for", "decode", "stats_numel", "TORCH_LIB_PATH"]
+__all__ = ["fwd", "bwd", "bwd_dq", "fwd_qkv", "bwd_qkv", "backward_for", "decode", "decode_tree",
+           "cache_append", "sample", "stats_numel", "TORCH_LIB_PATH"]
 
 TORCH_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libco_alibi_torch.so")
 
@@ -74,8 +77,11 @@ if _MISSING is None:
     fwd_qkv = torch.ops.co_alibi.fwd_qkv
     bwd_qkv = torch.ops.co_alibi.bwd_qkv
     decode = torch.ops.co_alibi.decode
+    decode_tree = torch.ops.co_alibi.decode_tree
+    cache_append = torch.ops.co_alibi.cache_append
+    sample = torch.ops.co_alibi.sample
 else:
-    fwd = bwd = bwd_dq = fwd_qkv = bwd_qkv = decode = _unavailable
+    fwd = bwd = bwd_dq = fwd_qkv = bwd_qkv = decode = decode_tree = cache_append = sample = _unavailable
 
 
 def stats_numel(batch: int, heads_q: int, seq_q: int, seq_kv: int) -> int:
@@ -157,6 +163,21 @@ def _register_fakes() -> None:
         o = torch.empty_like(q, memory_format=torch.contiguous_format)
         lse = q.new_empty((batch, heads_q, 1), dtype=torch.float32) if with_lse else _empty_stats(q)
         return o, lse
+
+    @torch.library.register_fake("co_alibi::decode_tree")
+    def _decode_tree_fake(q, k, v, k_cache, v_cache, slopes, seq_lens, parents, block_table, max_seq_len, sm_scale, with_lse):
+        """o (B, Hq, T, D) in q.dtype and, with with_lse, the natural-log LSE (B, Hq, T) in fp32."""
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
+        return o, q.new_empty(q.shape[:3], dtype=torch.float32) if with_lse else _empty_stats(q)
+
+    @torch.library.register_fake("co_alibi::cache_append")
+    def _cache_append_fake(k, v, k_cache, v_cache, seq_lens, counts, rows, block_table):
+        """Nothing: k_cache and v_cache are written in place."""
+
+    @torch.library.register_fake("co_alibi::sample")
+    def _sample_fake(logits, uniforms, temperature, top_k, top_p, min_p, temperature_all, top_k_all, top_p_all, min_p_all):
+        """One int64 token per row of logits."""
+        return logits.new_empty(logits.shape[:1], dtype=torch.int64)
 
 
 if _MISSING is None:

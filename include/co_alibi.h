@@ -11,8 +11,11 @@
  *                 in co_alibi_attn/co_alibi_attn.py:101-123 together with the
  *                 dK/dV partial buffers and their reduction (:83-99, :132-133).
  *
- * and a decode step the reference does not have, co_alibi_decode: its forward
- * with Sq = 1 over a key / value cache, as one split-K pass over the cache.
+ * a decode step the reference does not have, co_alibi_decode: its forward
+ * with Sq = 1 over a key / value cache, as one split-K pass over the cache;
+ * and the rest of a serving step around it, without counterparts there either:
+ * co_alibi_decode_tree (several new tokens, paged caches), co_alibi_cache_append
+ * and co_alibi_sample.
  *
  * Tensor layout (except the _strided calls): contiguous row-major, q / o / dout / dq are (B, Hq, Sq, D),
  * k / v / dk / dv are (B, Hkv, Skv, D); query head h attends key/value head
@@ -212,6 +215,64 @@ int co_alibi_decode_noalloc(int dtype, const void* q, const void* k_cache, const
                             const float* slopes, const int* seq_lens, void* o, float* lse, int batch,
                             int heads_q, int heads_kv, int seq_kv, int kv_capacity, int head_dim,
                             float sm_scale, void* stream);
+
+/* The calls below take key / value caches as pages or as one contiguous cache per sequence.  With a
+ * block_table (batch x blocks_per_seq int32 on the device) the caches are pools of num_pages pages (page,
+ * heads_kv, page_size, head_dim), page_size a power of two >= 16, and cache row r of sequence b is row
+ * r % page_size of page block_table[b][r / page_size].  Without one (NULL) they are (batch, heads_kv,
+ * page_size, head_dim), page_size being the capacity, and blocks_per_seq and num_pages are not read.  Strides
+ * follow co_alibi_fwd_strided's rules (k and v may differ), from page to page in place of the batch stride;
+ * NULL: everything is contiguous. */
+
+/* Tree decode: the attention of `tokens` new tokens per sequence (1 to 64) over a cache and each other.
+ * q and o are (B, Hq, tokens, D), o contiguous; k and v (B, Hkv, tokens, D) are the new tokens' own keys and
+ * values, which the cache does not hold yet.  Token t sees the sequence's filled rows and, after them, its
+ * chain of parents up to itself: parents (int32 on the device; tokens values for every sequence, or with
+ * parents_per_seq != 0 batch x tokens) holds in [-1, t) the token that t comes after, -1 for the cache's last
+ * row.  NULL is a chain: t after t - 1.  Any other value makes the token absent, and every token whose
+ * chain meets it: o = 0 and lse = -inf there.  The result for token t is co_alibi_decode's for its query with
+ * the chain's keys and values appended to the cache.  Filled rows: seq_lens (B int32 on the device) clamped to
+ * [0, seq_kv], or NULL for seq_kv (>= 0).  A sequence whose filled rows lie on a page outside the pool gets
+ * NaN.  Rows past the filled ones, pages that hold none, and keys and values of tokens outside a token's chain
+ * do not reach its result whatever they hold.  Head dims 16 to 256 (256 in fp16 / bf16 only).  strides: those
+ * of q, k, v, k_cache and v_cache (15 values) or NULL.  workspace holds
+ * co_alibi_decode_tree_workspace_bytes(...) bytes (256-byte aligned; may be NULL when that is 0). */
+size_t co_alibi_decode_tree_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,
+                                            int head_dim);
+int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v, const void* k_cache,
+                         const void* v_cache, const long long* strides, const float* slopes, const int* seq_lens,
+                         const int* parents, int parents_per_seq, const int* block_table, int blocks_per_seq,
+                         int num_pages, int page_size, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                         int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim, float sm_scale,
+                         void* stream);
+
+/* Cache append: writes new keys and values (k, v: (B, Hkv, tokens, D)) into the caches behind each sequence's
+ * filled rows.  Row i of sequence b, for i < counts[b] (B int32, or NULL: new_rows), is new row rows[b][i]
+ * (batch x new_rows int32, or NULL: row i) and goes to cache row seq_lens[b] + i.  seq_lens itself is the
+ * caller's to advance.  Counts are clamped to [0, new_rows]; a source row outside [0, tokens), a cache row
+ * outside the capacity and a page outside the pool write nothing.  Every other byte of the caches keeps its
+ * value.  The caches must not overlap k and v, and no two sequences may write one page's same row.
+ * strides: those of k, v, k_cache and v_cache (12 values) or NULL. */
+int co_alibi_cache_append(int dtype, const void* k, const void* v, void* k_cache, void* v_cache,
+                          const long long* strides, const int* seq_lens, const int* counts, const int* rows,
+                          int new_rows, const int* block_table, int blocks_per_seq, int num_pages, int page_size,
+                          int batch, int heads_kv, int tokens, int head_dim, void* stream);
+
+/* Sampling: one token per row of logits (batch rows of vocab elements, row_stride elements apart; element
+ * aligned; vocab at most 2^20).  With a row's tokens in order (logit descending, then index ascending) and
+ * weights exp((logit - max) / temperature): top_k keeps the first top_k (<= 0: all); top_p of those the ones
+ * before which less than top_p times the top_k's total weight lies (>= 1: all); min_p of those the ones of
+ * weight >= min_p (<= 0: all).  The first token is always kept.  The result is the first token in that order
+ * whose inclusive weight sum exceeds uniform times the kept sum (uniforms: batch fp32, or fp64 with
+ * uniforms_f64 != 0, in [0, 1); values outside are taken as 0 or as the last kept token).  temperature <= 0
+ * takes the first token.  A row with a NaN, or with no logit above -inf, gives -1.  Of several +inf logits all have
+ * weight 1 and the others 0.  temperature, top_k, top_p and min_p are arrays of one value per row on the
+ * device, or NULL: then the _all value is every row's.  Weights are summed exactly in integers, so a call's
+ * result does not depend on the order of its sums. */
+int co_alibi_sample(int dtype, const void* logits, long long row_stride, const void* uniforms, int uniforms_f64,
+                    const float* temperature, const int* top_k, const float* top_p, const float* min_p,
+                    double temperature_all, int top_k_all, double top_p_all, double min_p_all, long long* tokens,
+                    int batch, int vocab, void* stream);
 
 /* Measurement helper with no counterpart in the reference: `blocks` work-groups of 256
  * threads each issue `iters` rounds of four independent fp16 32x32x16 MFMAs per
