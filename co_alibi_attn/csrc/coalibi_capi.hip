@@ -769,13 +769,44 @@ int layout_at(const char* fn, const char* name, const long long* strides, int i,
   return read_layout(fn, name, strides == nullptr ? nullptr : strides + 3 * i, dtype, H, S, D, out);
 }
 
+template <typename T>
+hipError_t tree_dispatch_d(const coalibi::TreeArgs& a, int D, hipStream_t st) {
+  switch (D) {
+    case 16: return coalibi::launch_tree<T, 16>(a, st);
+    case 32: return coalibi::launch_tree<T, 32>(a, st);
+    case 64: return coalibi::launch_tree<T, 64>(a, st);
+    case 256:
+      if constexpr (sizeof(T) == 2) return coalibi::launch_tree<T, 256>(a, st);
+      return hipErrorInvalidValue;
+    default: return coalibi::launch_tree<T, 128>(a, st);
+  }
+}
+
+// How a tree decode is split: `splits` runs of `cps` chunks per sequence.
+struct TreePlan {
+  int row_blocks, splits, cps;
+  size_t parts;  // partials: (query row, split) pairs
+};
+TreePlan tree_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim) {
+  const int rows = heads_q / heads_kv * tokens, block = coalibi::tree_block_rows(rows);
+  const int row_blocks = (rows + block - 1) / block;
+  const int chunks = std::max((seq_kv + coalibi::kTreeChunkKeys - 1) / coalibi::kTreeChunkKeys, 1);
+  const int per_cu = head_dim * (dtype == CO_ALIBI_F32 ? 4 : 2) <= 256 ? 2 : 1;
+  const long long units = static_cast<long long>(batch) * heads_kv * row_blocks;
+  const long long want = std::max<long long>(per_cu * device_cus() / units, 1);
+  const int most = static_cast<int>(std::min<long long>({want, chunks, coalibi::kMaxTreeSplits}));
+  const int cps = (chunks + most - 1) / most, splits = (chunks + cps - 1) / cps;
+  return {row_blocks, splits, cps, splits == 1 ? 0 : static_cast<size_t>(batch) * heads_q * tokens * splits};
+}
+
 }  // namespace
 
 extern "C" {
 
 size_t co_alibi_decode_tree_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,
                                             int head_dim) {
-  return 0;
+  if (batch < 1 || heads_kv < 1 || heads_q < heads_kv || tokens < 1 || seq_kv < 0 || head_dim < 1) return 0;
+  return decode_partials_bytes(tree_plan(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim).parts, head_dim);
 }
 
 int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v, const void* k_cache,
@@ -805,6 +836,15 @@ int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v,
       (rc = check_opt_ptr(fn, "lse", lse, 4)))
     return rc;
   if (!std::isfinite(sm_scale)) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": sm_scale must be finite");
+  const TreePlan plan = tree_plan(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim);
+  if (static_cast<double>(batch) * heads_kv * plan.row_blocks * plan.splits > 2.1e9 ||
+      static_cast<double>(batch) * heads_q * tokens > 2.1e9)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
+  const size_t need = decode_partials_bytes(plan.parts, head_dim);
+  if (workspace_bytes < need)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": workspace of " + std::to_string(workspace_bytes) +
+                                     " bytes, need " + std::to_string(need));
+  if (need != 0 && (rc = check_ptr(fn, "workspace", workspace, 256))) return rc;
   if ((rc = layout_at(fn, "q", strides, 0, dtype, heads_q, tokens, head_dim, &a.ql)) ||
       (rc = layout_at(fn, "k", strides, 1, dtype, heads_kv, tokens, head_dim, &a.kl)) ||
       (rc = layout_at(fn, "v", strides, 2, dtype, heads_kv, tokens, head_dim, &a.vl)) ||
@@ -828,14 +868,24 @@ int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v,
   a.G = heads_q / heads_kv;
   a.T = tokens;
   a.L = seq_kv;
-  a.D = head_dim;
+  a.row_blocks = plan.row_blocks;
+  a.nSplits = plan.splits;
+  a.cps = plan.cps;
+  const size_t stat_bytes = round_up(plan.parts * sizeof(float), 256);
+  char* ws = static_cast<char*>(workspace);
+  if (need != 0) {
+    a.pmax = reinterpret_cast<float*>(ws);
+    a.psum = reinterpret_cast<float*>(ws + stat_bytes);
+    a.psig = reinterpret_cast<float*>(ws + 2 * stat_bytes);
+    a.pout = reinterpret_cast<float*>(ws + 3 * stat_bytes);
+  }
   a.sc2 = sm_scale * coalibi::kLog2eHost;
   hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e;
   switch (dtype) {
-    case CO_ALIBI_F16: e = coalibi::launch_tree<_Float16>(a, st); break;
-    case CO_ALIBI_BF16: e = coalibi::launch_tree<__bf16>(a, st); break;
-    default: e = coalibi::launch_tree<float>(a, st); break;
+    case CO_ALIBI_F16: e = tree_dispatch_d<_Float16>(a, head_dim, st); break;
+    case CO_ALIBI_BF16: e = tree_dispatch_d<__bf16>(a, head_dim, st); break;
+    default: e = tree_dispatch_d<float>(a, head_dim, st); break;
   }
   if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
   return CO_ALIBI_OK;

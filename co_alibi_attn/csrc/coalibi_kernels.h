@@ -371,7 +371,14 @@ struct CachePlace {
 // Tree decode: q/o (B, Hq, T, D), k/v (B, Hkv, T, D) the step's own tokens; kc/vc the caches (their
 // layouts' b is the stride from unit to unit).  Row g * T + t of a kv head is query head hkv * G + g of
 // node t.
+// Split s of a sequence covers chunks [s*cps, (s+1)*cps) of kTreeChunkKeys cache rows, its last split also the new
+// tokens.  Partials per (row (b*Hkv + hkv)*G*T + g*T + t, split): pmax / psum / psig (rows, nSplits) and pout (rows,
+// nSplits, D), fp32; unused with one split.
 constexpr int kMaxTreeTokens = 64;  // a node's ancestors are the bits of one 64-bit mask
+constexpr int kTreeChunkKeys = 128;
+constexpr int kMaxTreeSplits = 512;  // merge weights in LDS
+// Query rows (of the G*T of a kv head) per work-group: one, two or four 32-row tiles.
+constexpr int tree_block_rows(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
 struct TreeArgs {
   Layout ql, kl, vl, kcl, vcl;
   const void* q;
@@ -386,7 +393,13 @@ struct TreeArgs {
   const int* seq_lens;   // (B,) filled rows, clamped to [0, L], or NULL (all L)
   const int* parents;    // (B, T) or (T,), or NULL: a chain
   int parents_stride;    // T, or 0: one tree for every sequence
-  int B, Hq, Hkv, G, T, L, D;
+  float* pmax;
+  float* psum;
+  float* psig;
+  float* pout;
+  int B, Hq, Hkv, G, T, L;
+  int row_blocks;  // work-groups per (split, batch, kv head)
+  int nSplits, cps;
   float sc2;
 };
 
@@ -432,7 +445,7 @@ struct SampleArgs {
 template <typename T, int D, bool CAUSAL>
 hipError_t launch_bwd(const BwdArgs& a, int stages, hipStream_t stream);
 
-template <typename T>
+template <typename T, int D>
 hipError_t launch_tree(const TreeArgs& a, hipStream_t stream);
 
 hipError_t launch_append(const AppendArgs& a, hipStream_t stream);

@@ -7,6 +7,21 @@
 //   t_j = sm_scale*log2(e) * q.k_j,   sigma_j = sigmoid(t_j / log2(e)),
 //   z_j = sum_{k >= j} sigma_k,       a_j = t_j - slope*log2(e) * z_j,
 //   O   = sum_j 2^(a_j - m) v_j / sum_j 2^(a_j - m),   LSE = (m + log2 l) * ln 2.
+//
+// The R = G*T query rows of a kv head (row g*T + t) read the same keys, so a work-group takes up to 128 of them
+// over a run of 128-key chunks (a split), from its newest chunk to its oldest; the sequence's newest split
+// starts with the new keys as a chunk of their own, masked by the ancestor bits.  Splits know only their own
+// keys' z; the merge shifts each one's maximum by the sigma of the splits after it (as the decode's does).
+// The four wavefronts of a work-group are laid out by R: WR of them over 32-row tiles and 4 / WR over the
+// chunk's keys, so that small R still has four wavefronts of key tiles and large R reads each tile once for 128 rows.
+//   S^T = K Q^T and O^T += V^T P^T on MFMA, keys on the accumulator rows of S^T (in the kRowOfReg order: a lane holds 16
+// consecutive keys of one query row, so the suffix sums are register-local) and query rows on the
+// columns of both, so every per-row factor is a lane's own.  K and V come in by buffer-to-LDS DMA, one chunk ahead,
+// each tile's next chunk as soon as the tile has been read.  LDS rows are not padded: the 16-byte pieces of a
+// row are stored in an order XORed with its index (the DMA lanes fetch them so), which keeps the
+// operand reads off each other's banks and every DMA lane busy.
+#include <type_traits>
+
 #include "coalibi_common.h"
 #include "coalibi_kernels.h"
 
@@ -14,133 +29,669 @@ namespace coalibi {
 
 namespace {
 
-constexpr int kTreeThreads = 256;
+constexpr int kTreeWaves = 4;
+constexpr int kTreeThreads = 64 * kTreeWaves;
+static_assert(kTreeWaves * kWaveKeys == kTreeChunkKeys, "every wavefront brings in 32 keys of a chunk");
+// O is rescaled when a row's maximum grows by more than 2^8, as in the forward: P stays at most 256.
+constexpr float kTreeRescale = 8.0f;
+
+// A partial's sum in the newest split where the row's node is absent.
+constexpr float kAbsent = -1.0f;
 
 __device__ __forceinline__ int filled_rows(const TreeArgs& a, int b) {
   return a.seq_lens == nullptr ? a.L : min(max(a.seq_lens[b], 0), a.L);
 }
 
-// The new keys node t sees (bit j: key j), or 0 for an absent node: one whose chain of parents leaves
-// [-1, own index).
-__device__ __forceinline__ unsigned long long ancestors(const TreeArgs& a, int b, int t) {
-  if (a.parents == nullptr) return t == 63 ? ~0ull : (2ull << t) - 1;
-  const int* par = a.parents + (size_t)b * a.parents_stride;
-  unsigned long long m = 0;
-  while (t >= 0) {
-    m |= 1ull << t;
-    const int p = par[t];
-    if (p < -1 || p >= t) return 0;
-    t = p;
-  }
-  return m;
+// The sequence's splits that hold keys (the newest one also the new tokens): at least one.
+__device__ __forceinline__ int used_splits(const TreeArgs& a, int L) {
+  const int chunks = (L + kTreeChunkKeys - 1) / kTreeChunkKeys;
+  return max((chunks + a.cps - 1) / a.cps, 1);
 }
 
-template <typename F>
-__device__ __forceinline__ float block_reduce(float x, float* red, const F& f) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int off = 32; off > 0; off >>= 1) x = f(x, __shfl_xor(x, off, 64));
-  if (lane == 0) red[wave] = x;
-  __syncthreads();
-  x = red[0];
-  for (int w = 1; w < kTreeThreads / 64; ++w) x = f(x, red[w]);
-  __syncthreads();
-  return x;
-}
-
-// One work-group per (batch, query head, node), its keys 256 at a time from the newest on.
-template <typename T>
-__global__ __launch_bounds__(kTreeThreads) void coalibi_tree_kernel(TreeArgs a) {
-  __shared__ float sq[256], sp[kTreeThreads], red[kTreeThreads / 64];
-  __shared__ const T* srow[kTreeThreads];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int id = blockIdx.x, t = id % a.T, h = id / a.T % a.Hq, b = id / a.T / a.Hq, hkv = h / a.G;
-  const float lam2 = a.slopes[h] * kLog2e;
-  const int L = filled_rows(a, b);
-  const unsigned long long sees = ancestors(a, b, t);
-  T* const orow = static_cast<T*>(a.o) + (size_t)id * a.D;
-  if (sees == 0) {
-    for (int d = tid; d < a.D; d += kTreeThreads) orow[d] = T(0);
-    if (tid == 0 && a.lse != nullptr) a.lse[id] = kNegInf;
-    return;
-  }
-  const T* const q = head_at(static_cast<const T*>(a.q), a.ql, b, h) + (size_t)t * a.ql.r;
-  if (tid < a.D) sq[tid] = static_cast<float>(q[tid]);
-  __syncthreads();
-  const T* const knew = head_at(static_cast<const T*>(a.k), a.kl, b, hkv);
-  const T* const vnew = head_at(static_cast<const T*>(a.v), a.vl, b, hkv);
-  float m = kNegInf, l = 0.f, carry = 0.f, acc = 0.f;
-  bool lost = false;  // a visible row lies on no page of the pool
-  // Step -1: the new tokens; then the cache's rows from its end on.
-  for (int k0 = -1; k0 == -1 || k0 * kTreeThreads < L; ++k0) {
-    const int j = k0 < 0 ? tid : L - 1 - k0 * kTreeThreads - (kTreeThreads - 1 - tid);
-    const bool ok = k0 < 0 ? tid < a.T && (sees >> tid & 1) : j >= 0;
-    float s = kNegInf, sig = 0.f;
-    const T* vrow = nullptr;
-    if (ok) {
-      const T* krow;
-      if (k0 < 0) {
-        krow = knew + (size_t)j * a.kl.r;
-        vrow = vnew + (size_t)j * a.vl.r;
-      } else {
-        int unit = b, r = j;
-        if (a.place.table != nullptr) {
-          unit = a.place.table[(size_t)b * a.place.table_stride + (j >> a.place.page_shift)];
-          r = j & ((1 << a.place.page_shift) - 1);
-          if (unit < 0 || unit >= a.place.units) lost = true, unit = 0;
-        }
-        krow = head_at(static_cast<const T*>(a.kc), a.kcl, unit, hkv) + (size_t)r * a.kcl.r;
-        vrow = head_at(static_cast<const T*>(a.vc), a.vcl, unit, hkv) + (size_t)r * a.vcl.r;
-      }
-      s = 0.f;
-      for (int d = 0; d < a.D; ++d) s += sq[d] * static_cast<float>(krow[d]);
-      s *= a.sc2;
-      sig = sigmoid_log2(s);
+// Lane t: the new keys that node t sees (bit j: key j), or 0 for an absent node -- one whose chain of parents
+// leaves [-1, own index).  Six steps of doubling: after step i a lane has gathered 2^i ancestors.
+__device__ __forceinline__ unsigned long long ancestors(const TreeArgs& a, int b, int lane) {
+  if (a.parents == nullptr) return lane == 63 ? ~0ull : (2ull << lane) - 1;
+  const int p = lane < a.T ? a.parents[(size_t)b * a.parents_stride + lane] : -1;
+  const bool valid = p >= -1 && p < lane;
+  unsigned lo = lane < 32 ? 1u << lane : 0u, hi = lane < 32 ? 0u : 1u << (lane - 32);
+  int bad = valid ? 0 : 1, up = valid ? p : -1;
+#pragma unroll
+  for (int i = 0; i < 6; ++i) {
+    const int from = max(up, 0);
+    const unsigned olo = __shfl(lo, from, 64), ohi = __shfl(hi, from, 64);
+    const int obad = __shfl(bad, from, 64), oup = __shfl(up, from, 64);
+    if (up >= 0) {
+      lo |= olo;
+      hi |= ohi;
+      bad |= obad;
+      up = oup;
     }
-    srow[tid] = vrow;
-    float suf = sig;  // suffix sum over the block
+  }
+  return bad ? 0ull : (unsigned long long)hi << 32 | lo;
+}
+
+template <typename T, int D>
+struct TreeCfg {
+  static constexpr int E = sizeof(T);
+  static constexpr int ROWB = D * E;       // bytes per key in LDS
+  static constexpr int CPR = ROWB / 16;    // 16-byte pieces of them
+  static constexpr int KS = D / 16;        // k16 steps over the head dim
+  static constexpr int DT = D < 32 ? 1 : D / 32;  // 32-row tiles of O^T
+  static constexpr int HALF_INSTR = 16 * ROWB >= 1024 ? 16 * ROWB / 1024 : 1;  // DMA instructions per 16 keys
+  static constexpr int TILE_INSTR = 2 * HALF_INSTR;
+  static constexpr int TILES = 2 * kTreeChunkKeys * ROWB;  // bytes of the K and the V chunk
+  // At the end the wavefronts' O rows (fp32, rows 16 bytes apart from a power of two) alias the chunks.
+  static constexpr int LDO = D + 4;
+  static constexpr int O_BYTES = kTreeWaves * 32 * LDO * 4;
+  static constexpr int LDS_BYTES = TILES > O_BYTES ? TILES : O_BYTES;
+  static constexpr int WGS_PER_CU = LDS_BYTES <= 76 * 1024 ? 2 : 1;
+};
+
+// The XOR of a key's piece order, by the key's index in its 32-key tile.  K: a read pass is 16 bytes of 16
+// consecutive A-operand rows R (key kRowOfReg(R)).  V: a transpose read's pass is 64 bytes of 4 consecutive
+// keys; fp32 reads 128 bytes of keys k and k + 16.  A pass covers the 64 banks (256 bytes) once.
+template <int CPR>
+__device__ __forceinline__ constexpr int swizzle_k(int R) {
+  return CPR >= 16 ? R & 15 : CPR == 8 ? (R >> 1) & 7 : CPR == 4 ? (R >> 2) & 3 : (R >> 3) & 1;
+}
+template <int CPR, int E>
+__device__ __forceinline__ constexpr int swizzle_v(int key) {
+  if (E == 4) return CPR >= 16 ? ((key >> 4) & 1) << 3 : 0;
+  return CPR >= 16 ? (key & 3) << 2 : CPR == 8 ? ((key >> 1) & 1) << 2 : 0;
+}
+
+// dma16_to_lds_untracked with the non-temporal policy.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void dma16_to_lds_untracked_nt(__amdgpu_buffer_rsrc_t rsrc, unsigned lds_byte, int voffset) {
+  asm volatile(
+      "s_nop 4\n\t"
+      "s_mov_b32 m0, %0\n\t"
+      "s_nop 0\n\t"
+      "buffer_load_dwordx4 %1, %2, 0 offen nt lds"
+      :
+      : "s"(lds_byte), "v"(voffset), "s"(rsrc)
+      : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// DMA of 16 keys (half `half` of a tile) whose rows start at `base`, `rows` of them valid (the others land as
+// zeros), to LDS byte address lds.  Ordered by the caller's waits (dma16_to_lds_untracked's rules).
+template <typename T, int D, bool V, bool NT>
+__device__ __forceinline__ void dma_half(const T* base, int rows, int ld, unsigned lds, int half, int lane) {
+  using C = TreeCfg<T, D>;
+  const __amdgpu_buffer_rsrc_t r = tile_rsrc(base, row_span(rows, ld, D));
+  // Recomputed at every issue from an opaque copy of the lane index, as in dma_wave_rows.
+  int ln;
+  asm volatile("v_mov_b32 %0, %1" : "=v"(ln) : "v"(lane));
+#pragma unroll
+  for (int m = 0; m < C::HALF_INSTR; ++m) {
+    const int at = m * 64 + ln, key = at / C::CPR, piece = at % C::CPR;
+    const int in_tile = 16 * half + key;
+    const int x = V ? swizzle_v<C::CPR, C::E>(in_tile) : swizzle_k<C::CPR>(kRegOfRow(in_tile & 31));
+    const int off = key * ld * C::E + ((piece ^ x) << 4);
+    if (16 * C::ROWB >= 1024 || ln < 16 * C::ROWB / 16) {
+      if constexpr (NT)
+        dma16_to_lds_untracked_nt(r, lds + m * 1024, off);
+      else
+        dma16_to_lds_untracked(r, lds + m * 1024, off);
+    }
+  }
+}
+
+// A wave-uniform int from the constant address space: a scalar load, whatever the memory clobbers around it.
+__device__ __forceinline__ int scalar_load(const int* p) {
+  return *(const __attribute__((address_space(4))) int*)(size_t)p;
+}
+
+template <typename T>
+__device__ __forceinline__ bool not_finite(T x) {
+  if constexpr (sizeof(T) == 4) return (__builtin_bit_cast(unsigned, x) & 0x7f800000u) == 0x7f800000u;
+  constexpr unsigned exp_bits = __is_same(T, __bf16) ? 0x7f80u : 0x7c00u;
+  if constexpr (sizeof(T) == 2) return (__builtin_bit_cast(unsigned short, x) & exp_bits) == exp_bits;
+}
+
+// WR: wavefronts over the query rows.  NT: the cache is read once (one row block), so its DMA does not keep it in L2.
+template <typename T, int D, int WR, bool NT>
+__global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coalibi_tree_split_kernel(TreeArgs a) {
+  using C = TreeCfg<T, D>;
+  using M = Mfma<T>;
+  using V8 = typename M::vec8;
+  constexpr int WK = kTreeWaves / WR;            // wavefronts over the chunk's keys
+  constexpr int NTILE = WR == 1 ? 1 : 2;         // 32-key tiles a wavefront handles at once
+  constexpr int STEPS = 4 / (WK * NTILE);        // times per chunk
+  __shared__ __align__(1024) char smem[C::LDS_BYTES];
+  __shared__ float sSig[2][WK][WR * 32];
+  __shared__ float sMax[WK][WR * 32], sSum[WK][WR * 32], sScale[WK][WR * 32];
+  __shared__ unsigned long long sBad;  // new keys whose values hold an infinity or a NaN
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hl = lane & 31, hh = lane >> 5;
+  const int wr = wave % WR, wk = wave / WR;
+  // Ids: the row blocks of an item (split, sequence, kv head) 8 apart, so that they share an XCD and its L2.
+  const int RB = a.row_blocks, id = blockIdx.x;
+  const int rb = (id >> 3) % RB, item = (id / (8 * RB)) * 8 + (id & 7);
+  const int nS = a.nSplits;
+  if (item >= nS * a.B * a.Hkv) return;
+  const int bhk = item / nS, split = item - bhk * nS;
+  const int b = bhk / a.Hkv, hkv = bhk - b * a.Hkv;
+  const int L = __builtin_amdgcn_readfirstlane(filled_rows(a, b));
+  const int used = used_splits(a, L);
+  if (split >= used) return;  // past this sequence's keys: the merge reads no such partial
+  const bool newest = split == used - 1;
+  const int c_first = split * a.cps;
+  const int c_cache = min(c_first + a.cps, (L + kTreeChunkKeys - 1) / kTreeChunkKeys) - 1;  // newest cache chunk
+  const int c_top = newest ? c_cache + 1 : c_cache;  // chunk c_cache + 1: the new keys
+
+  const int R = a.G * a.T, row = rb * (WR * 32) + wr * 32 + hl;
+  const bool row_ok = row < R;
+  const int rsafe = row_ok ? row : 0;
+  const int g = rsafe / a.T, t = rsafe - g * a.T, h = hkv * a.G + g;
+  const float lam2 = a.slopes[h] * kLog2e;
+
+  unsigned long long sees = 0;
+  if (newest) {
+    const unsigned long long all = ancestors(a, b, lane);
+    sees = (unsigned long long)__shfl((unsigned)(all >> 32), t, 64) << 32 | __shfl((unsigned)all, t, 64);
+    if (tid == 0) sBad = 0;
+  }
+
+  const T* const kn = head_at(static_cast<const T*>(a.k), a.kl, b, hkv);
+  const T* const vn = head_at(static_cast<const T*>(a.v), a.vl, b, hkv);
+  const T* const kc = static_cast<const T*>(a.kc) + (size_t)hkv * a.kcl.h;
+  const T* const vc = static_cast<const T*>(a.vc) + (size_t)hkv * a.vcl.h;
+  const unsigned ldsK = lds_address(smem), ldsV = ldsK + kTreeChunkKeys * C::ROWB;
+
+  // This wavefront's 32 keys of chunk c: the unit and the row in it of each 16-key half.  `lost`: a filled row lies
+  // on no page of the pool (the pages are then read from unit 0 and the results made NaN at the end).
+  bool lost = false;
+  struct Halves {
+    int unit[2], row[2];
+  };
+  auto find = [&](int c) {
+    Halves f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = c * kTreeChunkKeys + wave * kWaveKeys + 16 * i;
+      f.unit[i] = b;
+      f.row[i] = r;
+      if (a.place.table != nullptr) {
+        f.unit[i] = 0;
+        f.row[i] = r & ((1 << a.place.page_shift) - 1);
+        if (r < L) {
+          const int u = scalar_load(a.place.table + (size_t)b * a.place.table_stride + (r >> a.place.page_shift));
+          const bool in = u >= 0 && u < a.place.units;
+          lost |= !in;
+          f.unit[i] = in ? u : 0;
+        }
+      }
+    }
+    return f;
+  };
+  // A chunk's K or V tile of this wavefront (NT: the cache's rows; the new tokens' are read by every row block).
+  auto issue = [&](auto is_v, int c, const Halves& f) {
+    constexpr bool V = decltype(is_v)::value;
+    const unsigned lds = (V ? ldsV : ldsK) + wave * kWaveKeys * C::ROWB;
+    if (c > c_cache) {
+      const T* const n = V ? vn : kn;
+      const int ld = V ? a.vl.r : a.kl.r;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = wave * kWaveKeys + 16 * i;
+        dma_half<T, D, V, false>(n + (size_t)r * ld, min(max(a.T - r, 0), 16), ld, lds + 16 * i * C::ROWB, i, lane);
+      }
+    } else {
+      const T* const base = V ? vc : kc;
+      const Layout& l = V ? a.vcl : a.kcl;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = c * kTreeChunkKeys + wave * kWaveKeys + 16 * i;
+        dma_half<T, D, V, NT>(base + (size_t)f.unit[i] * l.b + (size_t)f.row[i] * l.r, min(max(L - r, 0), 16), l.r,
+                              lds + 16 * i * C::ROWB, i, lane);
+      }
+    }
+  };
+  using K_t = std::false_type;
+  using V_t = std::true_type;
+
+  // Q^T fragments: lane l holds query row l%32 of its tile (zero past R).
+  V8 qf[C::KS];
+  {
+    const T* const q = head_at(static_cast<const T*>(a.q), a.ql, b, h) + (size_t)t * a.ql.r + hh * 8;
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks) qf[ks] = row_ok ? ld_vec8(q + ks * 16) : zero_vec8<T>();
+  }
+  Halves cur = c_top > c_cache ? Halves{} : find(c_top);
+  issue(K_t{}, c_top, cur);
+  issue(V_t{}, c_top, cur);
+  // Wait here for Q: the compiler would place this wait inside the loop, as a vmcnt(0) of every chunk.
+  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+
+  // State of the lane's row: scale (maximum, lazily followed), this half's share of the sum, O^T, and the sigma of
+  // the keys after the current ones.
+  float m2 = kNegInf, lsum = 0.f, carry = 0.f;
+  f32x16 acc[C::DT];
+#pragma unroll
+  for (int j = 0; j < C::DT; ++j) acc[j] = f32x16{};
+
+  // Lane constants of the operand reads.
+  const int kx = swizzle_k<C::CPR>(hl);
+  const char* const kread = smem + kRowOfReg(hl) * C::ROWB;
+  const char* const vtile = smem + kTreeChunkKeys * C::ROWB;
+  const int vi = lane & 15, vg = lane >> 4;
+  int par = 0;
+
+  for (int c = c_top; c >= c_first; --c) {
+    const bool more = c > c_first, fresh = c > c_cache;
+    Halves next{};
+    if (more) next = find(c - 1);
+    // This chunk's K has landed once at most its V (issued after it) is outstanding.
+    wait_vm<C::TILE_INSTR>();
+    if constexpr (WR > 1) lds_barrier();
+    const int key0 = c * kTreeChunkKeys;
+#pragma unroll
+    for (int step = 0; step < STEPS; ++step) {
+      const int tile0 = WR == 4 ? 2 - 2 * step : wk * NTILE;  // first 32-key tile of this step
+      f32x16 sacc[NTILE];
+#pragma unroll
+      for (int st = 0; st < NTILE; ++st) {
+        sacc[st] = f32x16{};
+        const char* const kt = kread + (tile0 + st) * kWaveKeys * C::ROWB;
+#pragma unroll
+        for (int ks = 0; ks < C::KS; ++ks) {
+          V8 kf;
+          if constexpr (C::E == 2) {
+            kf = *reinterpret_cast<const V8*>(kt + (((2 * ks + hh) ^ kx) << 4));
+          } else {
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(kt + (((4 * ks + 2 * hh) ^ kx) << 4));
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(kt + (((4 * ks + 2 * hh + 1) ^ kx) << 4));
+            kf = V8{lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+          }
+          sacc[st] = M::k16(kf, qf[ks], sacc[st]);
+        }
+      }
+      if (step == STEPS - 1 && more) {  // the K tiles have been read: the next chunk's come in
+        wait_lds();
+        if constexpr (WR > 1) lds_barrier();
+        issue(K_t{}, c - 1, next);
+      }
+
+      // Scores in log2 units; -inf for keys the row does not see: sigma 0, weight 0.  loc: the suffix sums of sigma
+      // inside each lane's 16 keys.
+      float loc[NTILE][16], tot[NTILE];
+      const bool masked = fresh || key0 + (tile0 + NTILE) * kWaveKeys > L;
+#pragma unroll
+      for (int st = 0; st < NTILE; ++st) {
+        const int kt = (tile0 + st) * kWaveKeys + 16 * hh;  // the lane's first key in the chunk
+        if (masked) {
+          const int left = L - key0 - kt;
+          const unsigned ok = fresh ? (kt < 64 ? (unsigned)(sees >> (kt & 63)) : 0u)
+                                    : left >= 16 ? 0xffffu : (1u << max(left, 0)) - 1u;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sacc[st][r] = ok >> r & 1 ? sacc[st][r] * a.sc2 : kNegInf;
+        } else {
+#pragma unroll
+          for (int r = 0; r < 16; ++r) sacc[st][r] *= a.sc2;
+        }
+        float run = 0.f;
+#pragma unroll
+        for (int r = 15; r >= 0; --r) {
+          run += sigmoid_log2(sacc[st][r]);
+          loc[st][r] = run;
+        }
+        tot[st] = run;
+      }
+      // off: the sigma after each lane's run.  Runs right to left: (tile 1, half 1), (1, 0), (0, 1), (0, 0).
+      float off[NTILE], sum = 0.f;
+#pragma unroll
+      for (int st = NTILE - 1; st >= 0; --st) {
+        const float oth = other_half(tot[st]);
+        off[st] = sum + (hh ? 0.f : oth);
+        sum += hh ? tot[st] + oth : oth + tot[st];
+      }
+      float after = carry;
+      if constexpr (WK > 1) {
+        if (hh == 0) sSig[par][wk][wr * 32 + hl] = sum;
+        lds_barrier();  // the DMA in flight goes on
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const float sw = sSig[par][w][wr * 32 + hl];
+          after += w > wk ? sw : 0.f;
+          carry += sw;
+        }
+        par ^= 1;
+      } else {
+        carry += sum;
+      }
+
+      // a relative to the row's scale, and the scale's update.
+      const float mb = m2 == kNegInf ? 0.f : m2;
+      float mt = kNegInf;
+#pragma unroll
+      for (int st = 0; st < NTILE; ++st) {
+        const float cst = mb + lam2 * (after + off[st]);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          sacc[st][r] = fmaf(-lam2, loc[st][r], sacc[st][r] - cst);
+          mt = fmaxf(mt, sacc[st][r]);
+        }
+      }
+      mt = fmaxf(mt, other_half(mt));
+      const bool need = m2 == kNegInf ? mt > kNegInf : mt > kTreeRescale;
+      if (__any(need)) {
+        const float delta = need ? mt : 0.f;
+        const float alpha = need ? (m2 == kNegInf ? 0.f : fast_exp2(-delta)) : 1.f;
+        m2 = need ? mb + delta : m2;
+        lsum *= alpha;
+#pragma unroll
+        for (int j = 0; j < C::DT; ++j) acc[j] *= alpha;
+#pragma unroll
+        for (int st = 0; st < NTILE; ++st) sacc[st] -= delta;
+      }
+      V8 pb[NTILE][2];
+#pragma unroll
+      for (int st = 0; st < NTILE; ++st)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          f32x8 p;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            p[e] = fast_exp2(sacc[st][8 * s + e]);
+            lsum += p[e];  // before the rounding for the product: the LSE is fp32's
+          }
+          pb[st][s] = M::pack(p);
+        }
+
+      if (step == 0) {
+        // This chunk's V has landed once at most the next chunk's K is outstanding (issued by now with one step).
+        if (STEPS == 1 && more)
+          wait_vm<C::TILE_INSTR>();
+        else
+          wait_vm<0>();
+        if constexpr (WR > 1) lds_barrier();
+        if (fresh) {
+          // A product with a weight of 0 would carry an infinity or a NaN of a value to rows that do not see it: such
+          // values become 0 here and are added to the rows that do below.
+          char* const tile = smem + kTreeChunkKeys * C::ROWB + wave * kWaveKeys * C::ROWB;
+          for (int i = lane; i < kWaveKeys * C::CPR; i += 64) {
+            typedef T pieces __attribute__((ext_vector_type(16 / C::E)));
+            pieces x = *reinterpret_cast<pieces*>(tile + i * 16);
+            bool any = false;
+#pragma unroll
+            for (int e = 0; e < 16 / C::E; ++e)
+              if (not_finite(static_cast<T>(x[e]))) {
+                any = true;
+                x[e] = T(0);
+              }
+            if (any) {
+              *reinterpret_cast<pieces*>(tile + i * 16) = x;
+              atomicOr(&sBad, 1ull << ((wave * kWaveKeys + i / C::CPR) & 63));
+            }
+          }
+          lds_barrier();
+        }
+      }
+      // O^T[d][row] += V^T[d][key] P^T[key][row]; keys 8*s + 16*(l/32) + e of each tile, as in pb.
+#pragma unroll
+      for (int j = 0; j < C::DT; ++j)
+#pragma unroll
+        for (int st = 0; st < NTILE; ++st) {
+          const char* const vt = vtile + (tile0 + st) * kWaveKeys * C::ROWB;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            V8 va;
+            if constexpr (C::E == 2) {
+              const int r0 = 8 * s + (vg >> 1) * 16 + (vi >> 2), col = (32 * j + 16 * (vg & 1) + 4 * (vi & 3)) & (D - 1);
+              const char* const at = vt + r0 * C::ROWB + (((col >> 3) ^ swizzle_v<C::CPR, 2>(vi >> 2)) << 4) + (col & 7) * 2;
+              const u32x2 lo = lds_tr4(reinterpret_cast<const T*>(at));
+              const u32x2 hi = lds_tr4(reinterpret_cast<const T*>(at + 4 * C::ROWB));
+              va = __builtin_bit_cast(V8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+            } else {
+              const int d = (32 * j + hl) & (D - 1);
+              const char* const at = vt + (8 * s + 16 * hh) * C::ROWB + (((d >> 2) ^ swizzle_v<C::CPR, 4>(16 * hh)) << 4) + (d & 3) * 4;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) va[e] = *reinterpret_cast<const float*>(at + e * C::ROWB);
+            }
+            acc[j] = M::k16(va, pb[st][s], acc[j]);
+          }
+        }
+    }
+    if (fresh) {
+      unsigned long long bad = sBad;
+      if (bad != 0) {
+        for (int key = 0; key < a.T; ++key) {
+          // The wavefront whose keys they are adds them (one of the WK), to rows that see the key.
+          if (!(bad >> key & 1) || (WK > 1 && key / (kWaveKeys * NTILE) != wk) || !(sees >> key & 1)) continue;
+#pragma unroll
+          for (int j = 0; j < C::DT; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int d = 32 * j + (r >> 2) * 8 + hh * 4 + (r & 3);
+              if (d >= D) continue;
+              const T x = vn[(size_t)key * a.vl.r + d];
+              if (not_finite(x)) acc[j][r] += static_cast<float>(x);
+            }
+        }
+      }
+      __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+    }
+    if (more) {
+      wait_lds();  // the V tiles have been read
+      if constexpr (WR > 1) lds_barrier();
+      issue(V_t{}, c - 1, next);
+    }
+  }
+
+  // The row's sum over both halves, then over the wavefronts of its keys (in one z frame: the split's own keys).
+  float l = lsum + other_half(lsum);
+  if (lost) l = __builtin_nanf("");
+  const int rl = wr * 32 + hl;
+  if (hh == 0) {
+    sMax[wk][rl] = m2;
+    sSum[wk][rl] = l;
+  }
+  __syncthreads();  // and every wavefront is done with the tiles (no DMA in flight)
+  if (tid < WR * 32) {
+    float m = kNegInf;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) m = fmaxf(m, sMax[w][tid]);
+    float ls = 0.f;
+#pragma unroll
+    for (int w = 0; w < WK; ++w) {
+      const float f = sMax[w][tid] == kNegInf ? 0.f : fast_exp2(sMax[w][tid] - m);
+      sScale[w][tid] = f;
+      ls += sMax[w][tid] == kNegInf && sSum[w][tid] == 0.f ? 0.f : f * sSum[w][tid];
+    }
+    // tid == wr * 32 + hl of wavefront wr only for the lanes that hold that row: `carry` comes from there below.
+    sMax[0][tid] = m;
+    sSum[0][tid] = ls;
+  }
+  __syncthreads();
+  float* const so = reinterpret_cast<float*>(smem) + (size_t)(wk * WR + wr) * 32 * C::LDO;
+  const float f = sScale[wk][rl];
+#pragma unroll
+  for (int j = 0; j < C::DT; ++j)
+#pragma unroll
+    for (int q4 = 0; q4 < 4; ++q4) {
+      const int d = 32 * j + q4 * 8 + hh * 4;
+      if (d < D)
+        *reinterpret_cast<f32x4*>(so + hl * C::LDO + d) =
+            f32x4{acc[j][4 * q4] * f, acc[j][4 * q4 + 1] * f, acc[j][4 * q4 + 2] * f, acc[j][4 * q4 + 3] * f};
+    }
+  const size_t row0 = (size_t)bhk * R + rb * (WR * 32);  // the block's first row in o, lse and the partials
+  const int rows = min(R - rb * (WR * 32), WR * 32);
+  const bool direct = nS == 1;
+  if (wk == 0 && hh == 0 && row_ok) {
+    const bool absent = newest && sees == 0;
+    if (direct) {
+      const float ls = sSum[0][rl];
+      if (a.lse != nullptr) a.lse[row0 + rl] = absent ? kNegInf : (sMax[0][rl] + log2f(ls)) * kLn2;
+      sScale[0][rl] = absent ? 0.f : 1.f / ls;
+      sMax[0][rl] = absent ? 0.f : 1.f;
+    } else {
+      const size_t pi = (row0 + rl) * nS + split;
+      a.pmax[pi] = sMax[0][rl];
+      a.psum[pi] = absent ? kAbsent : sSum[0][rl];
+      a.psig[pi] = carry;
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * (D / 4); i += kTreeThreads) {
+    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+    f32x4 s = f32x4{};
+#pragma unroll
+    for (int w = 0; w < WK; ++w)
+      s += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(smem) + ((size_t)w * WR * 32 + r) * C::LDO + d);
+    if (direct) {
+      typedef T out4 __attribute__((ext_vector_type(4)));
+      const bool there = sMax[0][r] != 0.f;
+      const float inv = sScale[0][r];
+      out4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(there ? s[e] * inv : 0.f);
+      *reinterpret_cast<out4*>(static_cast<T*>(a.o) + (row0 + r) * D + d) = v;
+    } else {
+      *reinterpret_cast<f32x4*>(a.pout + ((row0 + r) * nS + split) * D + d) = s;
+    }
+  }
+}
+
+constexpr int kTreeMergeThreads = 256;
+
+// O and LSE of a query row from its split partials: WPR wavefronts per row (one where rows are many, four where
+// few rows have many splits each).
+template <typename T, int D, int WPR>
+__global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(TreeArgs a) {
+  constexpr int ROWS = kTreeMergeThreads / 64 / WPR;  // rows per work-group
+  constexpr int LPS = D / 4;                          // lanes per split's O
+  constexpr int PER = 64 / LPS;                       // splits per wavefront and load
+  __shared__ float sW[kTreeMergeThreads / 64][kMaxTreeSplits];
+  __shared__ __align__(16) float sO[kTreeMergeThreads / 64][D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, part = wave % WPR;
+  const long long total = (long long)a.B * a.Hq * a.T;
+  const long long mine = (long long)blockIdx.x * ROWS + wave / WPR;
+  const long long row = mine < total ? mine : total - 1;  // every wavefront meets the barrier
+  const int bh = (int)(row / a.T), b = bh / a.Hq;
+  const float lam2 = a.slopes[bh - b * a.Hq] * kLog2e;
+  const int n = used_splits(a, filled_rows(a, b));
+  const float* const pmax = a.pmax + row * a.nSplits;
+  const float* const psum = a.psum + row * a.nSplits;
+  const float* const psig = a.psig + row * a.nSplits;
+  float* const w = sW[wave];
+  const bool absent = psum[n - 1] == kAbsent;
+
+  // Split maxima shifted by the sigma of the splits after them; each wavefront computes all of them.
+  float carry = 0.f, mx = kNegInf;
+  for (int base = (n - 1) / 64 * 64; base >= 0; base -= 64) {
+    const int s = base + lane;
+    const bool ok = s < n;
+    const float x = ok ? psig[s] : 0.f, pm = ok ? pmax[s] : kNegInf;
+    float suf = x;
+#pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
       const float y = __shfl_down(suf, off, 64);
       if (lane + off < 64) suf += y;
     }
-    if (lane == 0) red[wave] = suf;
-    __syncthreads();
-    float after = carry, all = 0.f;
-    for (int w = 0; w < kTreeThreads / 64; ++w) {
-      if (w > wave) after += red[w];
-      all += red[w];
-    }
-    __syncthreads();
-    const float av = ok ? s - lam2 * (after + suf) : kNegInf;
-    carry += all;
-    const float mt = block_reduce(av, red, [](float x, float y) { return fmaxf(x, y); });
-    const float mn = fmaxf(m, mt), mref = mn == kNegInf ? 0.f : mn;
-    const float p = fast_exp2(av - mref), fold = fast_exp2(m - mref);
-    m = mn;
-    l = l * fold + block_reduce(p, red, [](float x, float y) { return x + y; });
-    sp[tid] = p;
-    __syncthreads();
-    acc *= fold;
-    if (tid < a.D)
-      for (int e = 0; e < kTreeThreads; ++e)
-        if (srow[e] != nullptr) acc += sp[e] * static_cast<float>(srow[e][tid]);
-    __syncthreads();
+    const float m = pm - lam2 * (carry + (suf - x));
+    if (ok) w[s] = m;
+    mx = fmaxf(mx, m);
+    carry += __shfl(suf, 0, 64);
   }
-  if (__syncthreads_or(lost)) l = __builtin_nanf("");
-  if (tid < a.D) orow[tid] = static_cast<T>(acc / l);
-  if (tid == 0 && a.lse != nullptr) a.lse[id] = (m + log2f(l)) * kLn2;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
+  const float mref = mx == kNegInf ? 0.f : mx;
+  float l = 0.f;
+  for (int s = lane; s < n; s += 64) {  // a lane reads back what it wrote itself
+    const float f = fast_exp2(w[s] - mref);
+    w[s] = f;
+    l = fmaf(f, psum[s], l);
+  }
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
+  wait_lds();  // the weights are read across lanes below (LDS operations of a wavefront complete in order)
+
+  const int sub = lane / LPS, d = (lane % LPS) * 4;
+  const float* const po = a.pout + row * a.nSplits * D + d;
+  f32x4 acc[4] = {};
+  constexpr int STRIDE = PER * WPR;
+  int s = part * PER + sub;
+  for (; s + 3 * STRIDE < n; s += 4 * STRIDE)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) acc[u] += w[s + u * STRIDE] * *reinterpret_cast<const f32x4*>(po + (size_t)(s + u * STRIDE) * D);
+  for (; s < n; s += STRIDE) acc[0] += w[s] * *reinterpret_cast<const f32x4*>(po + (size_t)s * D);
+  f32x4 o = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+#pragma unroll
+  for (int off = LPS; off < 64; off <<= 1)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], off, 64);
+  if constexpr (WPR > 1) {
+    if (sub == 0) *reinterpret_cast<f32x4*>(&sO[wave][d]) = o;
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int p = 1; p < WPR; ++p) o += *reinterpret_cast<const f32x4*>(&sO[wave + p][d]);
+  }
+  if (mine >= total) return;
+  if (sub == 0) {
+    typedef T out4 __attribute__((ext_vector_type(4)));
+    const float inv = 1.f / l;
+    out4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(absent ? 0.f : o[e] * inv);
+    *reinterpret_cast<out4*>(static_cast<T*>(a.o) + row * D + d) = v;
+  }
+  if (part == 0 && lane == 0 && a.lse != nullptr) a.lse[row] = absent ? kNegInf : (mx + log2f(l)) * kLn2;
+}
+
+template <typename T, int D, int WR>
+hipError_t launch_split(const TreeArgs& a, hipStream_t stream) {
+  const long long items = (long long)a.nSplits * a.B * a.Hkv;
+  const dim3 grid(static_cast<unsigned>((items + 7) / 8 * 8 * a.row_blocks));
+  if (a.row_blocks == 1)
+    hipLaunchKernelGGL((coalibi_tree_split_kernel<T, D, WR, true>), grid, dim3(kTreeThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((coalibi_tree_split_kernel<T, D, WR, false>), grid, dim3(kTreeThreads), 0, stream, a);
+  return hipGetLastError();
 }
 
 }  // namespace
 
-template <typename T>
+template <typename T, int D>
 hipError_t launch_tree(const TreeArgs& a, hipStream_t stream) {
-  const dim3 grid(static_cast<unsigned>(a.B) * a.Hq * a.T);
-  hipLaunchKernelGGL((coalibi_tree_kernel<T>), grid, dim3(kTreeThreads), 0, stream, a);
+  const int R = a.G * a.T;
+  hipError_t e;
+  if (R <= 32)
+    e = launch_split<T, D, 1>(a, stream);
+  else if (R <= 64)
+    e = launch_split<T, D, 2>(a, stream);
+  else
+    e = launch_split<T, D, 4>(a, stream);
+  if (e != hipSuccess || a.nSplits == 1) return e;
+  const long long rows = (long long)a.B * a.Hq * a.T;
+  if (rows <= 2048)
+    hipLaunchKernelGGL((coalibi_tree_merge_kernel<T, D, 4>), dim3(static_cast<unsigned>(rows)), dim3(kTreeMergeThreads), 0,
+                       stream, a);
+  else
+    hipLaunchKernelGGL((coalibi_tree_merge_kernel<T, D, 1>), dim3(static_cast<unsigned>((rows + 3) / 4)),
+                       dim3(kTreeMergeThreads), 0, stream, a);
   return hipGetLastError();
 }
 
-template hipError_t launch_tree<_Float16>(const TreeArgs&, hipStream_t);
-template hipError_t launch_tree<__bf16>(const TreeArgs&, hipStream_t);
-template hipError_t launch_tree<float>(const TreeArgs&, hipStream_t);
+#define COALIBI_INST_TREE(T, D) template hipError_t launch_tree<T, D>(const TreeArgs&, hipStream_t);
+COALIBI_INST_TREE(_Float16, 16)
+COALIBI_INST_TREE(_Float16, 32)
+COALIBI_INST_TREE(_Float16, 64)
+COALIBI_INST_TREE(_Float16, 128)
+COALIBI_INST_TREE(_Float16, 256)
+COALIBI_INST_TREE(__bf16, 16)
+COALIBI_INST_TREE(__bf16, 32)
+COALIBI_INST_TREE(__bf16, 64)
+COALIBI_INST_TREE(__bf16, 128)
+COALIBI_INST_TREE(__bf16, 256)
+COALIBI_INST_TREE(float, 16)
+COALIBI_INST_TREE(float, 32)
+COALIBI_INST_TREE(float, 64)
+COALIBI_INST_TREE(float, 128)
 
 }  // namespace coalibi
