@@ -976,6 +976,7 @@ int co_alibi_sample(int dtype, const void* logits, long long row_stride, const v
   a.V = vocab;
   a.mass_bits = 62;
   while ((1ll << (62 - a.mass_bits)) < vocab) --a.mass_bits;
+  a.mass_bits = std::min(a.mass_bits, 50);
   hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e;
   switch (dtype) {

@@ -437,7 +437,7 @@ struct SampleArgs {
   int top_k_all;
   long long* tokens;  // (B,)
   int B, V;
-  int mass_bits;  // a weight of 1 in units of mass: 2^mass_bits, and V * 2^mass_bits <= 2^62
+  int mass_bits;  // a weight of 1 in units of mass: 2^mass_bits, at most 2^50, and V * 2^mass_bits <= 2^62
 };
 
 // stages: bit 0 = pass 1 (dq, dsum, and zb / cb or the score store), bit 1 = pass 2 (dk, dv; needs pass

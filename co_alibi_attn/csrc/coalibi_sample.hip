@@ -5,16 +5,23 @@
 //   top-k keeps the first k;  top-p of those the ones whose weights before them sum to less than p times
 //   the sum of the top-k's;  min-p of those the ones with w_i >= min_p (max w is 1).  What is kept is a prefix
 //   and never empty.  The token is the first whose inclusive sum of weights exceeds u times the kept sum.
+// So every step asks for a position along that order, by count or by weight, and nothing needs the whole order.
 //
-// Nothing is sorted.  Every step is a search for a position along that order, by count or by weight, and a
-// position is found digit by digit of the logit's order-preserving integer key (radix select): a histogram
-// of one digit, a scan from its largest value, and the next digit within the bin that holds the
-// position.  Tokens of one key have one weight, so the position among them is a division.
-//   Weights are integers, 2^mass_bits * w rounded (mass_bits = 62 - ceil(log2 V), 46 for 50304 tokens): integer
-// sums do not depend on the order in which atomics add, and the same call gives the same token.  The rounding
-// moves a border by less than V * 2^-63 of the largest weight.  They are computed in fp64: with fp32
-// exponentials (2^-22) a border between 50304 tokens would move past the uniform number in one draw of about a
+// Weights are integers, 2^mass_bits * w rounded (mass_bits = min(50, 62 - ceil(log2 V)), 46 for 50304 tokens):
+// integer sums do not depend on the order in which atomics add, and the same call gives the same token.  The
+// rounding moves a border by less than V * 2^-(mass_bits + 1) of the largest weight.  They are computed in fp64: with
+// fp32 exponentials a border between 50304 tokens would move past the uniform number in one draw of about a
 // thousand.
+//
+// One work-group per row, passes over it from L2 after the first:
+//   1. the largest logit;
+//   2. short lists: where top-k (or min-p) leaves few tokens, those above a bound are gathered in LDS -- for top-k the
+//      k-th largest of the threads' own maxima, below which no token of the first k lies -- and all positions are
+//      found among them;
+//   3. otherwise a histogram of the weights over 2048 bins of the logits' distance from the largest.  Its sums bound every
+//      position to a bin or two; the tokens of those bins are gathered and the positions found among them;
+//   4. where a list does not fit (many equal logits), radix select: positions are found digit by digit of the logit's
+//      order-preserving integer key, with a histogram per digit, and among equal tokens by division.
 #include <cmath>
 
 #include "coalibi_common.h"
@@ -30,6 +37,12 @@ constexpr int kSampleThreads = 1024;
 constexpr int kSampleWaves = kSampleThreads / 64;
 constexpr int kDigitBits = 11;
 constexpr int kBins = 1 << kDigitBits;
+static_assert(kBins == 2 * kSampleThreads, "a thread scans two bins");
+constexpr int kMaxList = 1024;
+// Largest top-k that is tried as a list.  Among 1024 threads' maxima the bound for k leaves about k + k^2 / 2048 tokens.
+constexpr int kMaxListK = 512;
+constexpr int kIndexBits = 20;
+static_assert(kMaxVocab <= 1 << kIndexBits, "an index fits an entry");
 
 // A logit's key: unsigned integers in the logits' order, with -0 taken for +0.
 template <typename T>
@@ -53,82 +66,186 @@ struct Key {
       return static_cast<float>(__builtin_bit_cast(T, static_cast<unsigned short>(u)));
   }
 };
+__device__ __forceinline__ unsigned key32(float x) { return Key<float>::of(x); }
+
+// A listed token: its bin (larger logits first), key and index, complemented so that the order of the tokens is the
+// descending order of the words, and its weight.
+struct Entry {
+  u64 word;
+  u64 mass;  // set by weigh_list
+};
+__device__ __forceinline__ u64 entry_word(int bin, float x, int i) {
+  return (u64)(0xfffu - bin) << 52 | (u64)key32(x) << kIndexBits | ((1u << kIndexBits) - 1 - i);
+}
+__device__ __forceinline__ float entry_logit(u64 word) { return Key<float>::value((unsigned)(word >> kIndexBits)); }
+__device__ __forceinline__ int entry_index(u64 word) { return (1 << kIndexBits) - 1 - (int)(word & ((1u << kIndexBits) - 1)); }
+
+// What a thread knows of its entry in the list: what lies before it in the row, by count and by mass.
+struct Listed {
+  u64 before_cnt, before_mass, mass;
+  int token;
+  bool mine;
+};
 
 struct SampleLds {
+  u64 mass[kBins];  // a histogram's bins; then what lies before each
   unsigned cnt[kBins];
-  u64 mass[kBins];
+  Entry list[kMaxList];
+  double exp2_table[32];
+  u64 wmass[kSampleWaves], wmass2[kSampleWaves];
   unsigned wcnt[kSampleWaves];
-  u64 wmass[kSampleWaves];
+  unsigned char flag[kBins];
   int bin;
   u64 before_cnt, before_mass;
-  u64 sum;
-  unsigned key;
-  int flag, token;
+  int listed, token, found;
+  Listed at;
 };
 
-// The weights of one row.
+// The weights of one row: 2^y with y = (x - max) * log2(e) / T.
 struct Weights {
-  double top, temp, one;
-  __device__ __forceinline__ double w(float x) const {
-    const double d = static_cast<double>(x) - top;
-    return x == static_cast<float>(top) ? 1.0 : d == -__builtin_inf() ? 0.0 : exp(d / temp);
+  float top;
+  double top64, c, one;  // c = log2(e) / T, one = 2^mass_bits
+  float reach;           // logits further than this below the largest have weight 0
+  const double* table;   // 2^(i/32)
+
+  // 2^mass_bits * w, before its rounding to an integer: y = i/32 + r with |r| <= 1/64, 2^r by its series up to r^5 (the next
+  // term is below 2^-48).
+  __device__ __forceinline__ double scaled(float x) const {
+    if (x == top) return one;
+    const float d = top - x;
+    if (!(d <= reach)) return 0.0;  // also -inf, and anything below a +inf
+    const double y = (static_cast<double>(x) - top64) * c;
+    const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer, in the low bits
+    const double t = fma(y, 32.0, magic);
+    const int i = static_cast<int>(static_cast<unsigned>(__builtin_bit_cast(u64, t)));
+    const double r = fma(t - magic, -0.03125, y) * 0.69314718055994530942;
+    double p = fma(r, 1.0 / 120, 1.0 / 24);
+    p = fma(p, r, 1.0 / 6);
+    p = fma(p, r, 0.5);
+    p = fma(p, r, 1.0);
+    p = fma(p, r, 1.0);
+    return ldexp(p * table[i & 31] * one, i >> 5);
   }
-  __device__ __forceinline__ u64 mass(double w) const { return static_cast<u64>(w * one + 0.5); }
+  static __device__ __forceinline__ u64 mass(double scaled) {
+    return __builtin_bit_cast(u64, scaled + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52: scaled <= 2^50
+  }
+  __device__ __forceinline__ u64 operator()(float x) const { return mass(scaled(x)); }
 };
+
+// f(x, index) over the row, each thread its own tokens, 16 bytes a load whatever the row's alignment and U loads in
+// flight (few copies of a long f); the last V % VEC tokens one by one.
+template <int U, typename T, typename F>
+__device__ __forceinline__ void for_row(const T* row, int V, const F& f) {
+  constexpr int VEC = 16 / (int)sizeof(T);
+  typedef T vec __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
+  const int n = V / VEC;
+  const vec* const v = reinterpret_cast<const vec*>(row);
+  for (int j = threadIdx.x; j < n; j += U * kSampleThreads) {
+    vec x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = v[min(j + u * kSampleThreads, n - 1)];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u == 0 || j + u * kSampleThreads < n)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) f(static_cast<T>(x[u][e]), (j + u * kSampleThreads) * VEC + e);
+  }
+  const int i = n * VEC + threadIdx.x;
+  if (i < V) f(row[i], i);
+}
+
+__device__ __forceinline__ u64 block_sum(u64 x, SampleLds& s) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
+  if (lane == 0) s.wmass[wave] = x;
+  __syncthreads();
+  x = 0;
+#pragma unroll
+  for (int w = 0; w < kSampleWaves; ++w) x += s.wmass[w];
+  __syncthreads();
+  return x;
+}
+
+// ------------------------------------------------------------------ positions in a list
+
+// Each of the n entries learns from all others what lies before it in its bin (s.mass / s.cnt: what lies before the
+// bin; `flat`: one bin, nothing before it).  `share` threads, a power of two within a wavefront, split an
+// entry's walk over the list, and the first of them has it.
+__device__ __forceinline__ Listed place_listed(SampleLds& s, int n, bool flat) {
+  int share = 64;
+  while (share * n > kSampleThreads) share >>= 1;
+  const int i = threadIdx.x / share, part = threadIdx.x - i * share;
+  Listed r{0, 0, 0, 0, false};
+  if (i < n) {
+    const Entry e = s.list[i];
+    u64 mass = 0;
+    unsigned cnt = 0;
+    for (int j = part; j < n; j += share) {
+      const Entry o = s.list[j];
+      if (o.word > e.word && (o.word ^ e.word) >> 52 == 0) {
+        mass += o.mass;
+        ++cnt;
+      }
+    }
+    for (int off = 1; off < share; off <<= 1) {
+      mass += __shfl_xor(mass, off, 64);
+      cnt += __shfl_xor(cnt, off, 64);
+    }
+    const int bin = 0xfff - (int)(e.word >> 52);
+    r = {(flat ? 0 : s.cnt[bin]) + (u64)cnt, (flat ? 0 : s.mass[bin]) + mass, e.mass, entry_index(e.word), part == 0};
+  }
+  return r;
+}
+
+// The listed token at position `pos` (by count, or by mass), into s.at; false: not in the list.
+__device__ __forceinline__ bool find_listed(SampleLds& s, const Listed& l, u64 pos, bool by_mass) {
+  if (threadIdx.x == 0) s.found = 0;
+  __syncthreads();
+  const u64 before = by_mass ? l.before_mass : l.before_cnt, own = by_mass ? l.mass : 1;
+  if (l.mine && pos >= before && pos - before < own) {
+    s.at = l;
+    s.found = 1;
+  }
+  __syncthreads();
+  const bool found = s.found != 0;
+  __syncthreads();  // before another call clears it
+  return found;
+}
+
+// ------------------------------------------------------------------ radix select
 
 // The histogram of the digit at bits [shift, shift + kDigitBits) of the keys, over the tokens whose key bits
-// from `top` on are `prefix`'s; ends with a barrier.  Returns this thread's part of the mass of the tokens
-// with w >= min_p.
+// from `top` on are `prefix`'s; ends with a barrier.
 template <typename T>
-__device__ u64 histogram(SampleLds& s, const T* row, int V, unsigned prefix, int top, int shift, const Weights& ws,
-                         double min_p) {
+__device__ __forceinline__ void digit_histogram(SampleLds& s, const T* row, int V, unsigned prefix, int top, int shift, const Weights& ws) {
   const int tid = threadIdx.x;
   for (int i = tid; i < kBins; i += kSampleThreads) s.cnt[i] = 0, s.mass[i] = 0;
   __syncthreads();
-  u64 heavy = 0;
-  for (int i = tid; i < V; i += kSampleThreads) {
-    const T x = row[i];
+  for_row<1>(row, V, [&](T x, int) {
     const unsigned k = Key<T>::of(x);
-    if (top < Key<T>::kBits && (k ^ prefix) >> top != 0) continue;
-    const double w = ws.w(static_cast<float>(x));
-    const u64 m = ws.mass(w);
+    if (top < Key<T>::kBits && (k ^ prefix) >> top != 0) return;
+    const u64 m = ws(static_cast<float>(x));
     const int bin = k >> shift & (kBins - 1);
     atomicAdd(&s.cnt[bin], 1u);
     if (m != 0) atomicAdd(&s.mass[bin], m);
-    if (w >= min_p) heavy += m;
-  }
+  });
   __syncthreads();
-  return heavy;
 }
 
-// The bin that holds position `pos` (counted by tokens, or by mass with by_mass) among the histogram's bins
-// from the largest down, and what lies before it, into s.bin / s.before_*: each thread scans two bins.
-__device__ void find_bin(SampleLds& s, u64 pos, bool by_mass) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int b0 = kBins - 1 - 2 * tid, b1 = b0 - 1;
-  const u64 c0 = s.cnt[b0], c1 = s.cnt[b1], m0 = s.mass[b0], m1 = s.mass[b1];
-  u64 c = c0 + c1, m = m0 + m1;
+// Inclusive sums over the bins up to this thread's second one, bins first, first + step, ... in this order.
+__device__ __forceinline__ void scan_bins(SampleLds& s, int b0, int b1, u64& cnt, u64& mass) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  cnt = (u64)s.cnt[b0] + s.cnt[b1];
+  mass = s.mass[b0] + s.mass[b1];
+#pragma unroll
   for (int off = 1; off < 64; off <<= 1) {
-    const u64 oc = __shfl_up(c, off, 64), om = __shfl_up(m, off, 64);
-    if (lane >= off) c += oc, m += om;
+    const u64 oc = __shfl_up(cnt, off, 64), om = __shfl_up(mass, off, 64);
+    if (lane >= off) cnt += oc, mass += om;
   }
-  if (lane == 63) s.wcnt[wave] = (unsigned)c, s.wmass[wave] = m;
+  if (lane == 63) s.wcnt[wave] = (unsigned)cnt, s.wmass[wave] = mass;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) c += s.wcnt[w], m += s.wmass[w];
-  // [before, before + own) of each of the two bins.
-  u64 cb = c - c0 - c1, mb = m - m0 - m1;
-  for (int e = 0; e < 2; ++e) {
-    const u64 oc = e == 0 ? c0 : c1, om = e == 0 ? m0 : m1;
-    const u64 before = by_mass ? mb : cb, own = by_mass ? om : oc;
-    if (pos >= before && pos - before < own) {
-      s.bin = e == 0 ? b0 : b1;
-      s.before_cnt = cb;
-      s.before_mass = mb;
-    }
-    cb += oc;
-    mb += om;
-  }
-  __syncthreads();
+  for (int w = 0; w < wave; ++w) cnt += s.wcnt[w], mass += s.wmass[w];
 }
 
 struct Place {
@@ -136,16 +253,27 @@ struct Place {
   u64 before_cnt, before_mass;  // of the tokens with larger keys
 };
 
+// The key at position `pos`.
 template <typename T>
-__device__ Place locate(SampleLds& s, const T* row, int V, u64 pos, bool by_mass, const Weights& ws) {
+__device__ __forceinline__ Place locate(SampleLds& s, const T* row, int V, u64 pos, bool by_mass, const Weights& ws) {
   Place p{0, 0, 0};
+  const int b0 = kBins - 1 - 2 * threadIdx.x, b1 = b0 - 1;
+#pragma unroll 1
   for (int top = Key<T>::kBits; top > 0; top -= kDigitBits) {
     const int shift = max(top - kDigitBits, 0);
     // The last digit reaches above `top` where the key's bits are no multiple of a digit's; the tokens agree there.
-    histogram(s, row, V, p.key, top, shift, ws, 0.0);
-    find_bin(s, pos, by_mass);
-    const unsigned digit = s.bin;
-    p.key = (p.key & ~((unsigned)(kBins - 1) << shift)) | digit << shift;
+    digit_histogram(s, row, V, p.key, top, shift, ws);
+    u64 c, m;
+    scan_bins(s, b0, b1, c, m);
+    for (int e = 1; e >= 0; --e) {
+      const int bin = e == 0 ? b0 : b1;
+      c -= s.cnt[bin];
+      m -= s.mass[bin];
+      const u64 before = by_mass ? m : c, own = by_mass ? s.mass[bin] : s.cnt[bin];
+      if (pos >= before && pos - before < own) s.bin = bin, s.before_cnt = c, s.before_mass = m;
+    }
+    __syncthreads();
+    p.key = (p.key & ~((unsigned)(kBins - 1) << shift)) | (unsigned)s.bin << shift;
     p.before_cnt += s.before_cnt;
     p.before_mass += s.before_mass;
     pos -= by_mass ? s.before_mass : s.before_cnt;
@@ -154,24 +282,14 @@ __device__ Place locate(SampleLds& s, const T* row, int V, u64 pos, bool by_mass
   return p;
 }
 
-__device__ u64 block_sum(u64 x, SampleLds& s) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-  if (lane == 0) s.wmass[wave] = x;
-  __syncthreads();
-  x = 0;
-  for (int w = 0; w < kSampleWaves; ++w) x += s.wmass[w];
-  __syncthreads();
-  return x;
-}
-
 // The index of the token of key `key` that `nth` others of that key precede.
 template <typename T>
-__device__ int nth_token(SampleLds& s, const T* row, int V, unsigned key, u64 nth) {
+__device__ __forceinline__ int nth_token(SampleLds& s, const T* row, int V, unsigned key, u64 nth) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int per = (V + kSampleThreads - 1) / kSampleThreads * 64, lo = min(wave * per, V), hi = min(lo + per, V);
   unsigned n = 0;
   for (int i = lo + lane; i < hi; i += 64) n += Key<T>::of(row[i]) == key;
+#pragma unroll
   for (int off = 32; off > 0; off >>= 1) n += __shfl_xor(n, off, 64);
   if (lane == 0) s.wcnt[wave] = n;
   __syncthreads();
@@ -190,10 +308,48 @@ __device__ int nth_token(SampleLds& s, const T* row, int V, unsigned key, u64 nt
   return s.token;
 }
 
+// ------------------------------------------------------------------ the cuts
+
+// The last position by mass that top-p keeps of a top-k of mass `kept`: tokens are kept while the mass before them is
+// below p * kept.
+__device__ __forceinline__ u64 top_p_position(double p, u64 kept) {
+  return static_cast<u64>(fmax(ceil(p * static_cast<double>(kept)), 1.0)) - 1;
+}
+// The position the uniform number draws of a kept mass.
+__device__ __forceinline__ u64 draw_position(double uni, u64 kept) {
+  const double at = uni > 0.0 ? uni * static_cast<double>(kept) : 0.0;
+  return at < static_cast<double>(kept) ? min(static_cast<u64>(at), kept - 1) : kept - 1;
+}
+
+// A bound that at least k (1 to 1024) of the threads' values reach: the k-th largest of them, its key cut to 16 bits.
+// Two bits a round, from the top.
+__device__ __forceinline__ float kth_of_threads(SampleLds& s, float mine, int k) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const unsigned key = key32(mine);
+  unsigned bound = 0;
+#pragma unroll
+  for (int bit = 30; bit >= 16; bit -= 2) {
+    // How many reach bound + 1, + 2 and + 3 units of these bits, 16 bits each.
+    u64 c = 0;
+#pragma unroll
+    for (unsigned d = 1; d < 4; ++d) c |= (u64)__popcll(__ballot(key >= (bound | d << bit))) << (16 * (d - 1));
+    u64* const w = bit & 2 ? s.wmass : s.wmass2;  // a buffer per parity: one barrier a round
+    if (lane == 0) w[wave] = c;
+    __syncthreads();
+    u64 n = 0;
+#pragma unroll
+    for (int i = 0; i < kSampleWaves; ++i) n += w[i];
+    const unsigned kk = k, n1 = n & 0xffff, n2 = n >> 16 & 0xffff, n3 = n >> 32;
+    bound |= (n3 >= kk ? 3u : n2 >= kk ? 2u : n1 >= kk ? 1u : 0u) << bit;
+  }
+  __syncthreads();
+  return bound <= key32(kNegInf) ? kNegInf : Key<float>::value(bound);
+}
+
 template <typename T>
 __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleArgs a) {
   __shared__ SampleLds s;
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x, V = a.V;
   const T* const row = static_cast<const T*>(a.logits) + b * a.row_stride;
   const double temp = a.temperature != nullptr ? static_cast<double>(a.temperature[b]) : a.temperature_all;
   const int top_k = a.top_k != nullptr ? a.top_k[b] : a.top_k_all;
@@ -201,56 +357,211 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
   const double min_p = a.min_p != nullptr ? static_cast<double>(a.min_p[b]) : a.min_p_all;
   const double uni = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[b]
                                     : static_cast<double>(static_cast<const float*>(a.uniforms)[b]);
-  // The largest key, and whether a logit is NaN.
-  unsigned kmax = 0;
-  bool nan = false;
-  for (int i = tid; i < a.V; i += kSampleThreads) {
-    const T x = row[i];
-    nan |= static_cast<float>(x) != static_cast<float>(x);
-    kmax = max(kmax, Key<T>::of(x));
-  }
-  for (int off = 32; off > 0; off >>= 1) kmax = max(kmax, (unsigned)__shfl_xor((int)kmax, off, 64));
-  if (lane == 0) s.wcnt[wave] = kmax;
-  nan = __syncthreads_or(nan);
-  for (int w = 0; w < kSampleWaves; ++w) kmax = max(kmax, s.wcnt[w]);
-  const float top = Key<T>::value(kmax);
+  if (tid < 32) s.exp2_table[tid] = exp2(tid / 32.0);
+  if (tid == 0) s.listed = 0;
+
+  // 1. The largest logit, and whether one is NaN (magnitude bits above the infinities').
+  float mine = kNegInf;
+  unsigned magnitude = 0;
+  for_row<4>(row, V, [&](T x, int) {
+    const float f = static_cast<float>(x);
+    mine = fmaxf(mine, f);
+    magnitude = max(magnitude, __builtin_bit_cast(unsigned, f) & 0x7fffffffu);
+  });
+  float top = mine;
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if (lane == 0) s.wcnt[wave] = __builtin_bit_cast(unsigned, top);
+  const bool nan = __syncthreads_or(magnitude > 0x7f800000u);
+#pragma unroll
+  for (int w = 0; w < kSampleWaves; ++w) top = fmaxf(top, __builtin_bit_cast(float, s.wcnt[w]));
   __syncthreads();
   if (nan || top == kNegInf) {
     if (tid == 0) a.tokens[b] = -1;
     return;
   }
-  unsigned key = kmax;
+  unsigned key = Key<T>::of(static_cast<T>(top));
   u64 nth = 0;
-  if (temp > 0.0) {  // else (0, negative, NaN): the first of the largest logits
-    const Weights ws{static_cast<double>(top), temp, static_cast<double>(1ull << a.mass_bits)};
-    const u64 heavy = block_sum(histogram(s, row, a.V, 0u, Key<T>::kBits, Key<T>::kBits - kDigitBits, ws, min_p), s);
-    u64 all = 0;
-    for (int i = tid; i < kBins; i += kSampleThreads) all += s.mass[i];
-    all = block_sum(all, s);
-    u64 kept = all;
-    if (top_k > 0 && top_k < a.V) {
-      const Place p = locate(s, row, a.V, top_k - 1, false, ws);
-      kept = p.before_mass + (top_k - p.before_cnt) * ws.mass(ws.w(Key<T>::value(p.key)));
-    }
-    u64 cut = kept;
-    if (top_p < 1.0) {
-      // Tokens are kept while the mass before them is below the bound: up to the one at its last unit.
-      const double bound = fmax(ceil(top_p * static_cast<double>(kept)), 1.0);
-      const u64 pos = static_cast<u64>(bound) - 1;
-      if (pos < all) {
-        const Place p = locate(s, row, a.V, pos, true, ws);
-        const u64 w = ws.mass(ws.w(Key<T>::value(p.key)));
-        cut = min(cut, p.before_mass + ((pos - p.before_mass) / w + 1) * w);
+  if (temp > 0.0) {  // else (0, negative or NaN) the first of the largest logits
+    Weights ws;
+    ws.top = top;
+    ws.top64 = static_cast<double>(top);
+    ws.c = 1.4426950408889634074 / temp;
+    ws.one = static_cast<double>(1ull << a.mass_bits);
+    ws.reach = static_cast<float>(fmin((a.mass_bits + 2) / ws.c, 3.4028234e38));
+    ws.table = s.exp2_table;
+    const bool cut_k = top_k > 0 && top_k < V, cut_p = top_p < 1.0, cut_m = min_p > 0.0;
+    const double min_scaled = min_p * ws.one;
+    const u64 one = static_cast<u64>(1) << a.mass_bits;  // the first token's weight
+
+    auto list = [&](int bin, float x, int i) {
+      const int at = atomicAdd(&s.listed, 1);
+      if (at < kMaxList) s.list[at].word = entry_word(bin, x, i);
+    };
+    // Sets the list's weights; returns this thread's entry's.
+    auto weigh_list = [&](int n) {
+      const double w = tid < n ? ws.scaled(entry_logit(s.list[tid].word)) : 0.0;
+      if (tid < n) s.list[tid].mass = Weights::mass(w);
+      return w;
+    };
+
+    // 2. A short list: the first k and what ties with their bound, or (without top-k) the tokens near or above min-p's
+    // bound; top-p then also needs the sum of all weights.
+    if ((cut_k && top_k <= kMaxListK) || (!cut_k && cut_m)) {
+      float bound;
+      if (cut_k) {
+        bound = kth_of_threads(s, mine, top_k);
+      } else {
+        const double below = fmax(-log2(min_p), 0.0) / ws.c;
+        bound = top - static_cast<float>(below * 1.00001);
+        bound -= 1e-6f * (fabsf(top) + fabsf(bound));  // the weights decide at the border, not this rounding
+        if (top == __builtin_inff()) bound = top;
+      }
+      for_row<4>(row, V, [&](T x, int i) {
+        if (static_cast<float>(x) >= bound) list(0, static_cast<float>(x), i);
+      });
+      __syncthreads();
+      const int n = s.listed;
+      if (n <= kMaxList) {
+        u64 all = 0;
+        if (!cut_k && cut_p) {
+          for_row<1>(row, V, [&](T x, int) { all += ws(static_cast<float>(x)); });
+          all = block_sum(all, s);
+        }
+        const double w = weigh_list(n);
+        const u64 sum = block_sum(Weights::mass(w), s);
+        const Listed l = place_listed(s, n, true);
+        u64 kept = sum;
+        if (cut_k && n > top_k) {
+          find_listed(s, l, top_k - 1, false);
+          kept = s.at.before_mass + s.at.mass;
+        }
+        u64 cut = kept;
+        // Past the list's end (only without top-k) min-p is the closer cut.
+        if (cut_p && find_listed(s, l, top_p_position(top_p, cut_k ? kept : all), true))
+          cut = min(cut, s.at.before_mass + s.at.mass);
+        if (cut_m) cut = min(cut, max(block_sum(w >= min_scaled ? Weights::mass(w) : 0, s), one));
+        find_listed(s, l, draw_position(uni, cut), true);
+        if (tid == 0) a.tokens[b] = s.at.token;
+        return;
       }
     }
-    if (min_p > 0.0) cut = min(cut, max(heavy, ws.mass(1.0)));
-    const double at = uni > 0.0 ? uni * static_cast<double>(cut) : 0.0;
-    const u64 pos = at < static_cast<double>(cut) ? min(static_cast<u64>(at), cut - 1) : cut - 1;
-    const Place p = locate(s, row, a.V, pos, true, ws);
-    key = p.key;
-    nth = (pos - p.before_mass) / ws.mass(ws.w(Key<T>::value(key)));
+
+    // 3. Weights by distance from the largest logit, in bins of reach / kBins (the last also holds what has no weight).
+    const float per_bin = kBins / ws.reach;
+    auto bin_of = [&](float x) {
+      const float d = x == top ? 0.f : (top - x) * per_bin;
+      return d < kBins - 1 ? static_cast<int>(d) : kBins - 1;
+    };
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kSampleThreads) s.cnt[i] = 0, s.mass[i] = 0;
+    if (tid == 0) s.listed = 0;
+    __syncthreads();
+    u64 heavy = 0;
+    for_row<1>(row, V, [&](T x, int) {
+      const float f = static_cast<float>(x);
+      const double w = ws.scaled(f);
+      const u64 m = Weights::mass(w);
+      const int bin = bin_of(f);
+      if (cut_k) atomicAdd(&s.cnt[bin], 1u);
+      if (m != 0) atomicAdd(&s.mass[bin], m);
+      if (w >= min_scaled) heavy += m;
+    });
+    __syncthreads();
+    if (cut_m) heavy = max(block_sum(heavy, s), one);
+    const int b0 = 2 * tid, b1 = b0 + 1;
+    const u64 m0 = s.mass[b0], m1 = s.mass[b1];
+    const unsigned c0 = s.cnt[b0], c1 = s.cnt[b1];
+    u64 c_in, m_in;
+    scan_bins(s, b0, b1, c_in, m_in);
+    // What lies before this thread's bins takes their place.
+    const u64 cb1 = c_in - c1, cb0 = cb1 - c0, mb1 = m_in - m1, mb0 = mb1 - m0;
+    __syncthreads();
+    s.mass[b0] = mb0;
+    s.mass[b1] = mb1;
+    s.cnt[b0] = (unsigned)cb0;
+    s.cnt[b1] = (unsigned)cb1;
+    if (tid == kSampleThreads - 1) s.before_mass = m_in;
+    __syncthreads();
+    const u64 all = s.before_mass;
+    __syncthreads();
+    bool f0 = false, f1 = false;
+    // Flags the bins that hold positions lo .. hi by mass (or a position by count); `from` and `to`: the masses before the
+    // first such bin and up to the end of the last.
+    auto flag = [&](bool by_mass, u64 lo, u64 hi, u64& from, u64& to) {
+      const u64 B0 = by_mass ? mb0 : cb0, B1 = by_mass ? mb1 : cb1, E0 = B0 + (by_mass ? m0 : c0), E1 = B1 + (by_mass ? m1 : c1);
+      f0 |= B0 <= hi && lo < E0;
+      f1 |= B1 <= hi && lo < E1;
+      if (B0 <= lo && lo < E0) s.before_mass = mb0;
+      if (B1 <= lo && lo < E1) s.before_mass = mb1;
+      if (B0 <= hi && hi < E0) s.before_cnt = mb0 + m0;
+      if (B1 <= hi && hi < E1) s.before_cnt = mb1 + m1;
+      __syncthreads();
+      from = s.before_mass;
+      to = s.before_cnt;
+      __syncthreads();
+    };
+    u64 lo = all, hi = all;  // the kept mass lies in [lo, hi]
+    if (cut_k) flag(false, top_k - 1, top_k - 1, lo, hi);
+    if (cut_p) {
+      u64 p_lo, p_hi;
+      flag(true, top_p_position(top_p, lo), top_p_position(top_p, hi), p_lo, p_hi);
+      lo = min(lo, p_lo);
+      hi = min(hi, p_hi);
+    }
+    if (cut_m) lo = min(lo, heavy), hi = min(hi, heavy);
+    lo = max(lo, one);
+    hi = max(hi, lo);
+    u64 from, to;
+    flag(true, draw_position(uni, lo), draw_position(uni, hi), from, to);
+    s.flag[b0] = f0;
+    s.flag[b1] = f1;
+    __syncthreads();
+    for_row<4>(row, V, [&](T x, int i) {
+      const float f = static_cast<float>(x);
+      const int bin = bin_of(f);
+      if (s.flag[bin]) list(bin, f, i);
+    });
+    __syncthreads();
+    const int n = s.listed;
+    if (n <= kMaxList) {
+      weigh_list(n);
+      __syncthreads();
+      const Listed l = place_listed(s, n, false);
+      u64 cut = all;
+      if (cut_k) {
+        find_listed(s, l, top_k - 1, false);
+        cut = s.at.before_mass + s.at.mass;
+      }
+      if (cut_p) {
+        find_listed(s, l, top_p_position(top_p, cut), true);
+        cut = min(cut, s.at.before_mass + s.at.mass);
+      }
+      if (cut_m) cut = min(cut, heavy);
+      find_listed(s, l, draw_position(uni, cut), true);
+      if (tid == 0) a.tokens[b] = s.at.token;
+      return;
+    }
+
+    // 4. Radix select: the end of the top-k, the end of the top-p, the draw.
+    u64 cut = all;
+#pragma unroll 1
+    for (int step = 0; step < 3; ++step) {
+      if (step == 2 && cut_m) cut = min(cut, heavy);
+      if ((step == 0 && !cut_k) || (step == 1 && !cut_p)) continue;
+      const u64 pos = step == 0 ? top_k - 1 : step == 1 ? top_p_position(top_p, cut) : draw_position(uni, cut);
+      const Place p = locate(s, row, V, pos, step > 0, ws);
+      const u64 w = ws(Key<T>::value(p.key));
+      const u64 at = step == 0 ? pos - p.before_cnt : (pos - p.before_mass) / w;  // among the tokens of this key
+      if (step < 2) {
+        cut = min(cut, p.before_mass + (at + 1) * w);
+      } else {
+        key = p.key;
+        nth = at;
+      }
+    }
   }
-  const int token = nth_token(s, row, a.V, key, nth);
+  const int token = nth_token(s, row, V, key, nth);
   if (tid == 0) a.tokens[b] = token;
 }
 

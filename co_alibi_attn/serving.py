@@ -26,11 +26,18 @@ __all__ = ["co_alibi_decode_tree", "co_alibi_cache_append", "co_alibi_sample"]
 
 
 def _check_new(names: str, *tensors: torch.Tensor) -> None:
-    if not all(t.is_cuda for t in tensors):
-        raise AssertionError("Inputs must be CUDA tensors")
-    if len({t.dtype for t in tensors}) != 1 or tensors[0].dtype not in _native.DTYPE_CODES:
-        raise TypeError(f"{names} must share one dtype of float32/float16/bfloat16, got "
-                        + ", ".join(str(t.dtype) for t in tensors))
+    dtype = tensors[0].dtype
+    for t in tensors:
+        if not t.is_cuda:
+            raise AssertionError("Inputs must be CUDA tensors")
+        if t.dtype != dtype or dtype not in _native.DTYPE_CODES:
+            raise TypeError(f"{names} must share one dtype of float32/float16/bfloat16, got "
+                            + ", ".join(str(x.dtype) for x in tensors))
+
+
+def _detached(t: torch.Tensor) -> torch.Tensor:
+    """t without its gradient record (t itself where there is none: detaching costs the host a microsecond)."""
+    return t.detach() if t.requires_grad else t
 
 
 def _capacity(k_cache: torch.Tensor, block_table: torch.Tensor | None) -> int:
@@ -92,8 +99,8 @@ def co_alibi_decode_tree(q, k, v, k_cache, v_cache, seq_len=None, parents=None, 
     if sm_scale is None:
         sm_scale = 1.0 / (head_dim ** 0.5)
     slopes = _device_slopes(num_heads, bias_max, q.dtype, q.device)
-    o, lse = ops.decode_tree(q.detach(), k.detach(), v.detach(), k_cache.detach(), v_cache.detach(), slopes, lens, parents,
-                             block_table, bound, float(sm_scale), bool(return_lse))
+    o, lse = ops.decode_tree(_detached(q), _detached(k), _detached(v), _detached(k_cache), _detached(v_cache), slopes, lens,
+                             parents, block_table, bound, float(sm_scale), bool(return_lse))
     return (o, lse) if return_lse else o
 
 
@@ -116,7 +123,7 @@ def co_alibi_cache_append(k, v, k_cache, v_cache, seq_lens, block_table=None, ro
     _check_table(block_table, k.shape[0])
     if k_cache.requires_grad or v_cache.requires_grad:
         raise ValueError("the caches are written in place and cannot require gradients")
-    ops.cache_append(k.detach(), v.detach(), k_cache, v_cache, seq_lens, counts, rows, block_table)
+    ops.cache_append(_detached(k), _detached(v), k_cache, v_cache, seq_lens, counts, rows, block_table)
 
 
 def _setting(name, x, low, high):
@@ -159,5 +166,5 @@ def co_alibi_sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p
     k, k_all = _setting("top_k", top_k, 0, math.inf)
     p, p_all = _setting("top_p", top_p, 0.0, 1.0)
     m, m_all = _setting("min_p", min_p, 0.0, 1.0)
-    return ops.sample(logits.detach(), uniforms.detach(), t, k, p, m, float(t_all), int(min(k_all, _native.MAX_VOCAB)),
+    return ops.sample(_detached(logits), _detached(uniforms), t, k, p, m, float(t_all), int(min(k_all, _native.MAX_VOCAB)),
                       float(p_all), float(m_all))
