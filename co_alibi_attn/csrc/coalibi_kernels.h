@@ -371,14 +371,16 @@ struct CachePlace {
 // Tree decode: q/o (B, Hq, T, D), k/v (B, Hkv, T, D) the step's own tokens; kc/vc the caches (their
 // layouts' b is the stride from unit to unit).  Row g * T + t of a kv head is query head hkv * G + g of
 // node t.
-// Split s of a sequence covers chunks [s*cps, (s+1)*cps) of kTreeChunkKeys cache rows, its last split also the new
-// tokens.  Partials per (row (b*Hkv + hkv)*G*T + g*T + t, split): pmax / psum / psig (rows, nSplits) and pout (rows,
+// A sequence's chunks are runs of `chunk` cache rows, then one of the new tokens; split s of it covers chunks [s*cps,
+// (s+1)*cps).  Partials per (row (b*Hkv + hkv)*G*T + g*T + t, split): pmax / psum / psig (rows, nSplits) and pout (rows,
 // nSplits, D), fp32; unused with one split.
-constexpr int kMaxTreeTokens = 64;  // a node's ancestors are the bits of one 64-bit mask
-constexpr int kTreeChunkKeys = 128;
+constexpr int kMaxTreeTokens = 64;   // a node's ancestors are the bits of one 64-bit mask
 constexpr int kMaxTreeSplits = 512;  // merge weights in LDS
 // Query rows (of the G*T of a kv head) per work-group: one, two or four 32-row tiles.
 constexpr int tree_block_rows(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
+// Keys held in LDS, and keys per chunk: one buffer of 128, or two of 64 where four wavefronts share every tile.
+constexpr int kTreeLdsKeys = 128;
+constexpr int tree_chunk_keys(int block_rows) { return block_rows == 128 ? 64 : 128; }
 struct TreeArgs {
   Layout ql, kl, vl, kcl, vcl;
   const void* q;
@@ -398,8 +400,13 @@ struct TreeArgs {
   float* psig;
   float* pout;
   int B, Hq, Hkv, G, T, L;
+  int chunk;       // tree_chunk_keys of the launch
   int row_blocks;  // work-groups per (split, batch, kv head)
-  int nSplits, cps;
+  int nSplits;     // most splits of any sequence: the partials' stride
+  int cps;         // chunks per split (with a plan the kernels share the chunks out)
+  int slots;       // resident work-groups the splits are sized for
+  int slack;       // the plan's (decode_cps)
+  bool plan;       // splits sized by the lengths in seq_lens
   float sc2;
 };
 

@@ -101,30 +101,31 @@ struct SampleLds {
   Listed at;
 };
 
-// The weights of one row: 2^y with y = (x - max) * log2(e) / T.
+// The weights of one row: 2^(y / 32) with y = (x - max) * 32 log2(e) / T.
 struct Weights {
-  float top;
-  double top64, c, one;  // c = log2(e) / T, one = 2^mass_bits
-  float reach;           // logits further than this below the largest have weight 0
-  const double* table;   // 2^(i/32)
+  float top, reach;  // the largest logit; logits further than `reach` below it have weight 0
+  double top64, c;   // c = 32 log2(e) / T
+  double one;        // 2^mass_bits
+  const double* table;  // 2^mass_bits * 2^(i / 32)
 
-  // 2^mass_bits * w, before its rounding to an integer: y = i/32 + r with |r| <= 1/64, 2^r by its series up to r^5 (the next
-  // term is below 2^-48).
+  // 2^mass_bits * w, before its rounding to an integer: y = i + r with an integer i and |r| <= 1/2, 2^(r/32) by its
+  // series up to r^5 (the next term is below 2^-48 of it).
   __device__ __forceinline__ double scaled(float x) const {
-    if (x == top) return one;
-    const float d = top - x;
-    if (!(d <= reach)) return 0.0;  // also -inf, and anything below a +inf
-    const double y = (static_cast<double>(x) - top64) * c;
+    const double d = static_cast<double>(x) - top64;
     const double magic = 6755399441055744.0;  // 1.5 * 2^52: adding it rounds to an integer, in the low bits
-    const double t = fma(y, 32.0, magic);
+    const double t = fma(d, c, magic);
     const int i = static_cast<int>(static_cast<unsigned>(__builtin_bit_cast(u64, t)));
-    const double r = fma(t - magic, -0.03125, y) * 0.69314718055994530942;
-    double p = fma(r, 1.0 / 120, 1.0 / 24);
-    p = fma(p, r, 1.0 / 6);
-    p = fma(p, r, 0.5);
+    const double r = fma(d, c, magic - t);
+    constexpr double k = 0.69314718055994530942 / 32;
+    double p = fma(r, k * k * k * k * k / 120, k * k * k * k / 24);
+    p = fma(p, r, k * k * k / 6);
+    p = fma(p, r, k * k / 2);
+    p = fma(p, r, k);
     p = fma(p, r, 1.0);
-    p = fma(p, r, 1.0);
-    return ldexp(p * table[i & 31] * one, i >> 5);
+    // The table's entry times 2^(i >> 5), through its exponent: the result is normal where it is used.
+    const u64 e = __builtin_bit_cast(u64, table[i & 31]) + ((u64)(unsigned)((i >> 5) << 20) << 32);
+    const double w = p * __builtin_bit_cast(double, e);
+    return x == top ? one : top - x <= reach ? w : 0.0;  // 0 also for -inf, and for what is below a +inf
   }
   static __device__ __forceinline__ u64 mass(double scaled) {
     return __builtin_bit_cast(u64, scaled + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52: scaled <= 2^50
@@ -357,13 +358,13 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
   const double min_p = a.min_p != nullptr ? static_cast<double>(a.min_p[b]) : a.min_p_all;
   const double uni = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[b]
                                     : static_cast<double>(static_cast<const float*>(a.uniforms)[b]);
-  if (tid < 32) s.exp2_table[tid] = exp2(tid / 32.0);
+  if (tid < 32) s.exp2_table[tid] = ldexp(exp2(tid / 32.0), a.mass_bits);
   if (tid == 0) s.listed = 0;
 
   // 1. The largest logit, and whether one is NaN (magnitude bits above the infinities').
   float mine = kNegInf;
   unsigned magnitude = 0;
-  for_row<4>(row, V, [&](T x, int) {
+  for_row<8>(row, V, [&](T x, int) {
     const float f = static_cast<float>(x);
     mine = fmaxf(mine, f);
     magnitude = max(magnitude, __builtin_bit_cast(unsigned, f) & 0x7fffffffu);
@@ -386,9 +387,9 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
     Weights ws;
     ws.top = top;
     ws.top64 = static_cast<double>(top);
-    ws.c = 1.4426950408889634074 / temp;
+    ws.c = 32.0 * 1.4426950408889634074 / temp;
     ws.one = static_cast<double>(1ull << a.mass_bits);
-    ws.reach = static_cast<float>(fmin((a.mass_bits + 2) / ws.c, 3.4028234e38));
+    ws.reach = static_cast<float>(fmin((a.mass_bits + 2) * 32.0 / ws.c, 3.4028234e38));
     ws.table = s.exp2_table;
     const bool cut_k = top_k > 0 && top_k < V, cut_p = top_p < 1.0, cut_m = min_p > 0.0;
     const double min_scaled = min_p * ws.one;
@@ -412,22 +413,26 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
       if (cut_k) {
         bound = kth_of_threads(s, mine, top_k);
       } else {
-        const double below = fmax(-log2(min_p), 0.0) / ws.c;
+        const double below = fmax(-log2(min_p), 0.0) * 32.0 / ws.c;
         bound = top - static_cast<float>(below * 1.00001);
         bound -= 1e-6f * (fabsf(top) + fabsf(bound));  // the weights decide at the border, not this rounding
         if (top == __builtin_inff()) bound = top;
       }
-      for_row<4>(row, V, [&](T x, int i) {
-        if (static_cast<float>(x) >= bound) list(0, static_cast<float>(x), i);
-      });
+      u64 all = 0;
+      if (!cut_k && cut_p) {
+        for_row<2>(row, V, [&](T x, int i) {
+          all += ws(static_cast<float>(x));
+          if (static_cast<float>(x) >= bound) list(0, static_cast<float>(x), i);
+        });
+        all = block_sum(all, s);
+      } else {
+        for_row<8>(row, V, [&](T x, int i) {
+          if (static_cast<float>(x) >= bound) list(0, static_cast<float>(x), i);
+        });
+      }
       __syncthreads();
       const int n = s.listed;
       if (n <= kMaxList) {
-        u64 all = 0;
-        if (!cut_k && cut_p) {
-          for_row<1>(row, V, [&](T x, int) { all += ws(static_cast<float>(x)); });
-          all = block_sum(all, s);
-        }
         const double w = weigh_list(n);
         const u64 sum = block_sum(Weights::mass(w), s);
         const Listed l = place_listed(s, n, true);
@@ -458,7 +463,7 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
     if (tid == 0) s.listed = 0;
     __syncthreads();
     u64 heavy = 0;
-    for_row<1>(row, V, [&](T x, int) {
+    for_row<2>(row, V, [&](T x, int) {
       const float f = static_cast<float>(x);
       const double w = ws.scaled(f);
       const u64 m = Weights::mass(w);

@@ -9,17 +9,19 @@
 //   O   = sum_j 2^(a_j - m) v_j / sum_j 2^(a_j - m),   LSE = (m + log2 l) * ln 2.
 //
 // The R = G*T query rows of a kv head (row g*T + t) read the same keys, so a work-group takes up to 128 of them
-// over a run of 128-key chunks (a split), from its newest chunk to its oldest; the sequence's newest split
-// starts with the new keys as a chunk of their own, masked by the ancestor bits.  Splits know only their own
-// keys' z; the merge shifts each one's maximum by the sigma of the splits after it (as the decode's does).
+// over a run of key chunks (a split), from its newest chunk to its oldest; the sequence's newest chunk is
+// the new keys, masked by the ancestor bits.  Splits know only their own keys' z; the merge shifts each
+// one's maximum by the sigma of the splits after it (as the decode's does).
 // The four wavefronts of a work-group are laid out by R: WR of them over 32-row tiles and 4 / WR over the
 // chunk's keys, so that small R still has four wavefronts of key tiles and large R reads each tile once for 128 rows.
 //   S^T = K Q^T and O^T += V^T P^T on MFMA, keys on the accumulator rows of S^T (in the kRowOfReg order: a lane holds 16
 // consecutive keys of one query row, so the suffix sums are register-local) and query rows on the
-// columns of both, so every per-row factor is a lane's own.  K and V come in by buffer-to-LDS DMA, one chunk ahead,
-// each tile's next chunk as soon as the tile has been read.  LDS rows are not padded: the 16-byte pieces of a
-// row are stored in an order XORed with its index (the DMA lanes fetch them so), which keeps the
-// operand reads off each other's banks and every DMA lane busy.
+// columns of both, so every per-row factor is a lane's own.  K and V come in by buffer-to-LDS DMA, one chunk ahead.
+// Where wavefronts share the tiles of all keys (WR 4) there are two buffers of 64 keys and one barrier per chunk; else
+// one buffer of 128 keys, each tile's next chunk issued as soon as the tile has been read.  LDS rows are not
+// padded: the 16-byte pieces of a row are stored in an order XORed with its index (the DMA lanes fetch them so), which
+// keeps the operand reads off each other's banks and every DMA lane busy.
+#include <algorithm>
 #include <type_traits>
 
 #include "coalibi_common.h"
@@ -31,21 +33,82 @@ namespace {
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = 64 * kTreeWaves;
-static_assert(kTreeWaves * kWaveKeys == kTreeChunkKeys, "every wavefront brings in 32 keys of a chunk");
 // O is rescaled when a row's maximum grows by more than 2^8, as in the forward: P stays at most 256.
 constexpr float kTreeRescale = 8.0f;
 
 // A partial's sum in the newest split where the row's node is absent.
 constexpr float kAbsent = -1.0f;
 
+template <typename V, typename F>
+__device__ __forceinline__ V wave_all(V x, const F& f) {
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) x = f(x, __shfl_xor(x, off, 64));
+  return x;
+}
+
 __device__ __forceinline__ int filled_rows(const TreeArgs& a, int b) {
   return a.seq_lens == nullptr ? a.L : min(max(a.seq_lens[b], 0), a.L);
 }
+// A sequence's chunks: of its filled rows, and the new keys' (the last).
+__device__ __forceinline__ int chunks_of(const TreeArgs& a, int len) { return (len + a.chunk - 1) / a.chunk + 1; }
 
-// The sequence's splits that hold keys (the newest one also the new tokens): at least one.
-__device__ __forceinline__ int used_splits(const TreeArgs& a, int L) {
-  const int chunks = (L + kTreeChunkKeys - 1) / kTreeChunkKeys;
-  return max((chunks + a.cps - 1) / a.cps, 1);
+// Chunks per split of a launch with a plan (every wavefront computes the same): the splits share out the batch's real
+// chunks over one round of work-groups, as the decode's plan does.
+__device__ __forceinline__ int plan_cps(const TreeArgs& a, int lane) {
+  int total = 0, longest = 0;
+  for (int b = lane; b < a.B; b += 64) {
+    const int n = chunks_of(a, filled_rows(a, b));
+    total += n;
+    longest = max(longest, n);
+  }
+  total = wave_all(total, [](int x, int y) { return x + y; });
+  longest = wave_all(longest, [](int x, int y) { return max(x, y); });
+  const long long heads = (long long)a.Hkv * a.row_blocks;
+  return decode_cps(total * heads, longest, a.slots, a.nSplits, a.slack, longest, [&](int c) {
+    int n = 0;
+    for (int b = lane; b < a.B; b += 64) n += (chunks_of(a, filled_rows(a, b)) + c - 1) / c;
+    return wave_all(n, [](int x, int y) { return x + y; }) * heads;
+  });
+}
+
+// A sequence's splits: `used` of them, of cps chunks each (the last may be shorter).
+struct TreeSplits {
+  int cps, used;
+};
+__device__ __forceinline__ TreeSplits splits_of(const TreeArgs& a, int cps, int chunks) {
+  if (a.plan) {  // as many as the plan's cps make, then of equal length
+    const int n = (chunks + cps - 1) / cps;
+    cps = (chunks + n - 1) / n;
+  }
+  return {cps, (chunks + cps - 1) / cps};
+}
+
+// The (sequence and kv head, split) of item `id` under a plan: items run over the sequences' own splits, split
+// fastest; ids past the last one have none (bhk < 0).
+struct TreeItem {
+  int bhk, split;
+};
+__device__ __forceinline__ TreeItem plan_item(const TreeArgs& a, int cps, int id, int lane) {
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int b = b0 + lane;
+    const int n = b < a.B ? splits_of(a, cps, chunks_of(a, filled_rows(a, b))).used : 0;
+    int incl = n * a.Hkv;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int o = __shfl_up(incl, off, 64);
+      if (lane >= off) incl += o;
+    }
+    const unsigned long long in = __ballot(id < before + incl);
+    if (in != 0) {
+      const int l = __ffsll(in) - 1;
+      const int splits = __shfl(n, l, 64), at = id - before - (__shfl(incl, l, 64) - splits * a.Hkv);
+      const int hkv = at / splits;
+      return {__builtin_amdgcn_readfirstlane((b0 + l) * a.Hkv + hkv), __builtin_amdgcn_readfirstlane(at - hkv * splits)};
+    }
+    before += __shfl(incl, 63, 64);
+  }
+  return {-1, 0};
 }
 
 // Lane t: the new keys that node t sees (bit j: key j), or 0 for an absent node -- one whose chain of parents
@@ -79,8 +142,7 @@ struct TreeCfg {
   static constexpr int KS = D / 16;        // k16 steps over the head dim
   static constexpr int DT = D < 32 ? 1 : D / 32;  // 32-row tiles of O^T
   static constexpr int HALF_INSTR = 16 * ROWB >= 1024 ? 16 * ROWB / 1024 : 1;  // DMA instructions per 16 keys
-  static constexpr int TILE_INSTR = 2 * HALF_INSTR;
-  static constexpr int TILES = 2 * kTreeChunkKeys * ROWB;  // bytes of the K and the V chunk
+  static constexpr int TILES = 2 * kTreeLdsKeys * ROWB;  // bytes of the K and V buffers
   // At the end the wavefronts' O rows (fp32, rows 16 bytes apart from a power of two) alias the chunks.
   static constexpr int LDO = D + 4;
   static constexpr int O_BYTES = kTreeWaves * 32 * LDO * 4;
@@ -101,42 +163,66 @@ __device__ __forceinline__ constexpr int swizzle_v(int key) {
   return CPR >= 16 ? (key & 3) << 2 : CPR == 8 ? ((key >> 1) & 1) << 2 : 0;
 }
 
-// dma16_to_lds_untracked with the non-temporal policy.
+// N buffer-to-LDS DMA instructions at LDS byte address lds, lds + 1024, ..., ordered by the caller's waits
+// (dma16_to_lds_untracked's rules); one run, so that only the first waits out the writes of its scalar operands.
+// Every m0 comes from the scalar address: added to itself, m0 lost its upper bits for LDS addresses past 64 KB.
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
-__device__ __forceinline__ void dma16_to_lds_untracked_nt(__amdgpu_buffer_rsrc_t rsrc, unsigned lds_byte, int voffset) {
-  asm volatile(
-      "s_nop 4\n\t"
-      "s_mov_b32 m0, %0\n\t"
-      "s_nop 0\n\t"
-      "buffer_load_dwordx4 %1, %2, 0 offen nt lds"
-      :
-      : "s"(lds_byte), "v"(voffset), "s"(rsrc)
-      : "memory", "m0");
+#define COALIBI_DMA_FIRST(V, NT) "s_nop 4\n\ts_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 " V ", %1, 0 offen" NT " lds"
+#define COALIBI_DMA_NEXT(V, AT, NT) "\n\ts_add_u32 m0, %0, " AT "\n\ts_nop 0\n\tbuffer_load_dwordx4 " V ", %1, 0 offen" NT " lds"
+#define COALIBI_DMA1(NT) COALIBI_DMA_FIRST("%2", NT)
+#define COALIBI_DMA2(NT) COALIBI_DMA1(NT) COALIBI_DMA_NEXT("%3", "0x400", NT)
+#define COALIBI_DMA4(NT) COALIBI_DMA2(NT) COALIBI_DMA_NEXT("%4", "0x800", NT) COALIBI_DMA_NEXT("%5", "0xc00", NT)
+template <int N, bool NT>
+__device__ __forceinline__ void dma_run(__amdgpu_buffer_rsrc_t r, unsigned lds, const int* v) {
+  if constexpr (N == 1 && NT) {
+    asm volatile(COALIBI_DMA1(" nt")::"s"(lds), "s"(r), "v"(v[0]) : "memory", "m0");
+  } else if constexpr (N == 1) {
+    asm volatile(COALIBI_DMA1("")::"s"(lds), "s"(r), "v"(v[0]) : "memory", "m0");
+  } else if constexpr (N == 2 && NT) {
+    asm volatile(COALIBI_DMA2(" nt")::"s"(lds), "s"(r), "v"(v[0]), "v"(v[1]) : "memory", "m0", "scc");
+  } else if constexpr (N == 2) {
+    asm volatile(COALIBI_DMA2("")::"s"(lds), "s"(r), "v"(v[0]), "v"(v[1]) : "memory", "m0", "scc");
+  } else if constexpr (N == 4 && NT) {
+    asm volatile(COALIBI_DMA4(" nt")::"s"(lds), "s"(r), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]) : "memory", "m0", "scc");
+  } else if constexpr (N == 4) {
+    asm volatile(COALIBI_DMA4("")::"s"(lds), "s"(r), "v"(v[0]), "v"(v[1]), "v"(v[2]), "v"(v[3]) : "memory", "m0", "scc");
+  } else {
+    dma_run<N / 2, NT>(r, lds, v);
+    dma_run<N / 2, NT>(r, lds + N / 2 * 1024, v + N / 2);
+  }
 }
+#undef COALIBI_DMA1
+#undef COALIBI_DMA2
+#undef COALIBI_DMA4
+#undef COALIBI_DMA_FIRST
+#undef COALIBI_DMA_NEXT
 #pragma clang diagnostic pop
 
-// DMA of 16 keys (half `half` of a tile) whose rows start at `base`, `rows` of them valid (the others land as
-// zeros), to LDS byte address lds.  Ordered by the caller's waits (dma16_to_lds_untracked's rules).
-template <typename T, int D, bool V, bool NT>
-__device__ __forceinline__ void dma_half(const T* base, int rows, int ld, unsigned lds, int half, int lane) {
+// DMA of HALVES runs of 16 keys of a tile, the first of them half `half0` of its 32 keys, to LDS byte address lds.  Run
+// i's rows start at base[i], rows[i] of them valid (the others land as zeros).
+//   Lane ln of instruction m brings in piece ln % CPR of key m * KPI + ln / CPR.  The XOR patterns are linear in the key's
+// bits, so their part that depends on m and on the half is a constant on top of the lane's own.
+template <typename T, int D, bool V, bool NT, int HALVES>
+__device__ __forceinline__ void dma_halves(const T* const (&base)[HALVES], const int (&rows)[HALVES], int ld, unsigned lds,
+                                           int half0, int lane) {
   using C = TreeCfg<T, D>;
-  const __amdgpu_buffer_rsrc_t r = tile_rsrc(base, row_span(rows, ld, D));
+  constexpr int KPI = C::CPR >= 64 ? 1 : 64 / C::CPR;  // keys per instruction
+  auto pattern = [](int key) { return V ? swizzle_v<C::CPR, C::E>(key) : swizzle_k<C::CPR>(kRegOfRow(key)); };
   // Recomputed at every issue from an opaque copy of the lane index, as in dma_wave_rows.
   int ln;
   asm volatile("v_mov_b32 %0, %1" : "=v"(ln) : "v"(lane));
+  const int key = ln / C::CPR & 15, piece = ln % C::CPR;
+  const int row = key * (ld * C::E), own = (piece ^ pattern(key)) << 4, step = KPI * ld * C::E;
 #pragma unroll
-  for (int m = 0; m < C::HALF_INSTR; ++m) {
-    const int at = m * 64 + ln, key = at / C::CPR, piece = at % C::CPR;
-    const int in_tile = 16 * half + key;
-    const int x = V ? swizzle_v<C::CPR, C::E>(in_tile) : swizzle_k<C::CPR>(kRegOfRow(in_tile & 31));
-    const int off = key * ld * C::E + ((piece ^ x) << 4);
-    if (16 * C::ROWB >= 1024 || ln < 16 * C::ROWB / 16) {
-      if constexpr (NT)
-        dma16_to_lds_untracked_nt(r, lds + m * 1024, off);
-      else
-        dma16_to_lds_untracked(r, lds + m * 1024, off);
-    }
+  for (int i = 0; i < HALVES; ++i) {
+    const __amdgpu_buffer_rsrc_t r = tile_rsrc(base[i], row_span(rows[i], ld, D));
+    // One half at a time: which one is a wave-uniform value there.
+    const int hx = (HALVES == 2 ? i : half0) * (pattern(16) << 4);
+    int off[C::HALF_INSTR];
+#pragma unroll
+    for (int m = 0; m < C::HALF_INSTR; ++m) off[m] = row + m * step + (own ^ (pattern(m * KPI) << 4) ^ hx);
+    if (16 * C::ROWB >= 1024 || ln < C::ROWB) dma_run<C::HALF_INSTR, NT>(r, lds + 16 * i * C::ROWB, off);
   }
 }
 
@@ -158,9 +244,13 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
   using C = TreeCfg<T, D>;
   using M = Mfma<T>;
   using V8 = typename M::vec8;
-  constexpr int WK = kTreeWaves / WR;            // wavefronts over the chunk's keys
-  constexpr int NTILE = WR == 1 ? 1 : 2;         // 32-key tiles a wavefront handles at once
-  constexpr int STEPS = 4 / (WK * NTILE);        // times per chunk
+  constexpr int WK = kTreeWaves / WR;             // wavefronts over the chunk's keys
+  constexpr int NTILE = WR == 1 ? 1 : 2;          // 32-key tiles of a wavefront
+  constexpr int CHUNK = tree_chunk_keys(32 * WR);  // keys
+  constexpr int NBUF = kTreeLdsKeys / CHUNK;      // LDS buffers
+  static_assert(CHUNK == WK * NTILE * kWaveKeys, "the wavefronts share out a chunk");
+  constexpr int HALVES = CHUNK / kTreeWaves / 16;  // runs of 16 keys a wavefront brings in
+  constexpr int INSTR = HALVES * C::HALF_INSTR;   // DMA instructions of its K (or V) of a chunk
   __shared__ __align__(1024) char smem[C::LDS_BYTES];
   __shared__ float sSig[2][WK][WR * 32];
   __shared__ float sMax[WK][WR * 32], sSum[WK][WR * 32], sScale[WK][WR * 32];
@@ -173,16 +263,26 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
   const int RB = a.row_blocks, id = blockIdx.x;
   const int rb = (id >> 3) % RB, item = (id / (8 * RB)) * 8 + (id & 7);
   const int nS = a.nSplits;
-  if (item >= nS * a.B * a.Hkv) return;
-  const int bhk = item / nS, split = item - bhk * nS;
-  const int b = bhk / a.Hkv, hkv = bhk - b * a.Hkv;
+  int cps = a.cps;
+  TreeItem it{item / nS, item % nS};
+  if (a.plan) {
+    cps = plan_cps(a, lane);
+    it = plan_item(a, cps, item, lane);
+    if (it.bhk < 0) return;
+  } else if (it.bhk >= a.B * a.Hkv) {
+    return;
+  }
+  // Wave-uniform, which the divisions behind them hide from the compiler.
+  const int bhk = __builtin_amdgcn_readfirstlane(it.bhk), split = __builtin_amdgcn_readfirstlane(it.split);
+  const int b = __builtin_amdgcn_readfirstlane(bhk / a.Hkv), hkv = bhk - b * a.Hkv;
   const int L = __builtin_amdgcn_readfirstlane(filled_rows(a, b));
-  const int used = used_splits(a, L);
-  if (split >= used) return;  // past this sequence's keys: the merge reads no such partial
-  const bool newest = split == used - 1;
-  const int c_first = split * a.cps;
-  const int c_cache = min(c_first + a.cps, (L + kTreeChunkKeys - 1) / kTreeChunkKeys) - 1;  // newest cache chunk
-  const int c_top = newest ? c_cache + 1 : c_cache;  // chunk c_cache + 1: the new keys
+  const int chunks = __builtin_amdgcn_readfirstlane(chunks_of(a, L));
+  TreeSplits sp = splits_of(a, cps, chunks);
+  sp = {__builtin_amdgcn_readfirstlane(sp.cps), __builtin_amdgcn_readfirstlane(sp.used)};
+  if (split >= sp.used) return;  // past this sequence's keys: the merge reads no such partial
+  const bool newest = split == sp.used - 1;
+  const int c_first = split * sp.cps, c_top = min(c_first + sp.cps, chunks) - 1;
+  const int c_cache = chunks - 2;  // the newest chunk of filled rows; the one after it is the new keys
 
   const int R = a.G * a.T, row = rb * (WR * 32) + wr * 32 + hl;
   const bool row_ok = row < R;
@@ -201,19 +301,20 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
   const T* const vn = head_at(static_cast<const T*>(a.v), a.vl, b, hkv);
   const T* const kc = static_cast<const T*>(a.kc) + (size_t)hkv * a.kcl.h;
   const T* const vc = static_cast<const T*>(a.vc) + (size_t)hkv * a.vcl.h;
-  const unsigned ldsK = lds_address(smem), ldsV = ldsK + kTreeChunkKeys * C::ROWB;
+  const unsigned ldsK = lds_address(smem), ldsV = ldsK + kTreeLdsKeys * C::ROWB;
 
-  // This wavefront's 32 keys of chunk c: the unit and the row in it of each 16-key half.  `lost`: a filled row lies
+  // This wavefront's keys of chunk c: the unit and the row in it of each run of 16.  `lost`: a filled row lies
   // on no page of the pool (the pages are then read from unit 0 and the results made NaN at the end).
   bool lost = false;
   struct Halves {
-    int unit[2], row[2];
+    int unit[HALVES], row[HALVES];
   };
+  const int my_key = wave * (16 * HALVES);
   auto find = [&](int c) {
     Halves f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int r = c * kTreeChunkKeys + wave * kWaveKeys + 16 * i;
+    for (int i = 0; i < HALVES; ++i) {
+      const int r = c * CHUNK + my_key + 16 * i;
       f.unit[i] = b;
       f.row[i] = r;
       if (a.place.table != nullptr) {
@@ -229,27 +330,31 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
     }
     return f;
   };
-  // A chunk's K or V tile of this wavefront (NT: the cache's rows; the new tokens' are read by every row block).
-  auto issue = [&](auto is_v, int c, const Halves& f) {
+  // This wavefront's part of chunk c's K or V into buffer `buf` (NT: the cache's rows; the new tokens' are read by every
+  // row block).
+  auto issue = [&](auto is_v, int c, const Halves& f, int buf) {
     constexpr bool V = decltype(is_v)::value;
-    const unsigned lds = (V ? ldsV : ldsK) + wave * kWaveKeys * C::ROWB;
+    const unsigned lds = (V ? ldsV : ldsK) + (buf * CHUNK + my_key) * C::ROWB;
+    const T* base[HALVES];
+    int rows[HALVES];
+    const int half0 = HALVES == 2 ? 0 : wave & 1;
     if (c > c_cache) {
-      const T* const n = V ? vn : kn;
       const int ld = V ? a.vl.r : a.kl.r;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = wave * kWaveKeys + 16 * i;
-        dma_half<T, D, V, false>(n + (size_t)r * ld, min(max(a.T - r, 0), 16), ld, lds + 16 * i * C::ROWB, i, lane);
+      for (int i = 0; i < HALVES; ++i) {
+        const int r = my_key + 16 * i;
+        base[i] = (V ? vn : kn) + (size_t)r * ld;
+        rows[i] = min(max(a.T - r, 0), 16);
       }
+      dma_halves<T, D, V, false, HALVES>(base, rows, ld, lds, half0, lane);
     } else {
-      const T* const base = V ? vc : kc;
       const Layout& l = V ? a.vcl : a.kcl;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = c * kTreeChunkKeys + wave * kWaveKeys + 16 * i;
-        dma_half<T, D, V, NT>(base + (size_t)f.unit[i] * l.b + (size_t)f.row[i] * l.r, min(max(L - r, 0), 16), l.r,
-                              lds + 16 * i * C::ROWB, i, lane);
+      for (int i = 0; i < HALVES; ++i) {
+        base[i] = (V ? vc : kc) + (size_t)f.unit[i] * l.b + (size_t)f.row[i] * l.r;
+        rows[i] = min(max(L - (c * CHUNK + my_key + 16 * i), 0), 16);
       }
+      dma_halves<T, D, V, NT, HALVES>(base, rows, l.r, lds, half0, lane);
     }
   };
   using K_t = std::false_type;
@@ -263,8 +368,8 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
     for (int ks = 0; ks < C::KS; ++ks) qf[ks] = row_ok ? ld_vec8(q + ks * 16) : zero_vec8<T>();
   }
   Halves cur = c_top > c_cache ? Halves{} : find(c_top);
-  issue(K_t{}, c_top, cur);
-  issue(V_t{}, c_top, cur);
+  issue(K_t{}, c_top, cur, 0);
+  issue(V_t{}, c_top, cur, 0);
   // Wait here for Q: the compiler would place this wait inside the loop, as a vmcnt(0) of every chunk.
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
 
@@ -278,26 +383,34 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
   // Lane constants of the operand reads.
   const int kx = swizzle_k<C::CPR>(hl);
   const char* const kread = smem + kRowOfReg(hl) * C::ROWB;
-  const char* const vtile = smem + kTreeChunkKeys * C::ROWB;
+  const char* const vtile = smem + kTreeLdsKeys * C::ROWB;
   const int vi = lane & 15, vg = lane >> 4;
-  int par = 0;
+  const int tile0 = wk * NTILE;  // this wavefront's first 32-key tile of a chunk
+  int par = 0, buf = 0;
 
   for (int c = c_top; c >= c_first; --c) {
     const bool more = c > c_first, fresh = c > c_cache;
     Halves next{};
     if (more) next = find(c - 1);
-    // This chunk's K has landed once at most its V (issued after it) is outstanding.
-    wait_vm<C::TILE_INSTR>();
-    if constexpr (WR > 1) lds_barrier();
-    const int key0 = c * kTreeChunkKeys;
-#pragma unroll
-    for (int step = 0; step < STEPS; ++step) {
-      const int tile0 = WR == 4 ? 2 - 2 * step : wk * NTILE;  // first 32-key tile of this step
+    if constexpr (NBUF == 2) {
+      // This chunk has landed, and every wavefront has read the one before it, whose buffer the next one takes.
+      wait_vm<0>();
+      lds_barrier();
+      if (more) {
+        issue(K_t{}, c - 1, next, buf ^ 1);
+        issue(V_t{}, c - 1, next, buf ^ 1);
+      }
+    } else {
+      wait_vm<INSTR>();  // this chunk's K has landed once at most its V (issued after it) is outstanding
+      if constexpr (WR > 1) lds_barrier();
+    }
+    const int key0 = c * CHUNK;
+    {
       f32x16 sacc[NTILE];
 #pragma unroll
       for (int st = 0; st < NTILE; ++st) {
         sacc[st] = f32x16{};
-        const char* const kt = kread + (tile0 + st) * kWaveKeys * C::ROWB;
+        const char* const kt = kread + (buf * CHUNK + (tile0 + st) * kWaveKeys) * C::ROWB;
 #pragma unroll
         for (int ks = 0; ks < C::KS; ++ks) {
           V8 kf;
@@ -311,10 +424,10 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
           sacc[st] = M::k16(kf, qf[ks], sacc[st]);
         }
       }
-      if (step == STEPS - 1 && more) {  // the K tiles have been read: the next chunk's come in
+      if (NBUF == 1 && more) {  // the K tiles have been read: the next chunk's come in
         wait_lds();
         if constexpr (WR > 1) lds_barrier();
-        issue(K_t{}, c - 1, next);
+        issue(K_t{}, c - 1, next, 0);
       }
 
       // Scores in log2 units; -inf for keys the row does not see: sigma 0, weight 0.  loc: the suffix sums of sigma
@@ -403,18 +516,20 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
           pb[st][s] = M::pack(p);
         }
 
-      if (step == 0) {
-        // This chunk's V has landed once at most the next chunk's K is outstanding (issued by now with one step).
-        if (STEPS == 1 && more)
-          wait_vm<C::TILE_INSTR>();
-        else
-          wait_vm<0>();
-        if constexpr (WR > 1) lds_barrier();
+      {
+        if constexpr (NBUF == 1) {
+          // This chunk's V has landed once at most the next chunk's K (issued by now) is outstanding.
+          if (more)
+            wait_vm<INSTR>();
+          else
+            wait_vm<0>();
+          if constexpr (WR > 1) lds_barrier();
+        }
         if (fresh) {
           // A product with a weight of 0 would carry an infinity or a NaN of a value to rows that do not see it: such
           // values become 0 here and are added to the rows that do below.
-          char* const tile = smem + kTreeChunkKeys * C::ROWB + wave * kWaveKeys * C::ROWB;
-          for (int i = lane; i < kWaveKeys * C::CPR; i += 64) {
+          char* const tile = smem + (kTreeLdsKeys + buf * CHUNK + my_key) * C::ROWB;
+          for (int i = lane; i < 16 * HALVES * C::CPR; i += 64) {
             typedef T pieces __attribute__((ext_vector_type(16 / C::E)));
             pieces x = *reinterpret_cast<pieces*>(tile + i * 16);
             bool any = false;
@@ -426,7 +541,7 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
               }
             if (any) {
               *reinterpret_cast<pieces*>(tile + i * 16) = x;
-              atomicOr(&sBad, 1ull << ((wave * kWaveKeys + i / C::CPR) & 63));
+              atomicOr(&sBad, 1ull << ((my_key + i / C::CPR) & 63));
             }
           }
           lds_barrier();
@@ -437,7 +552,7 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
       for (int j = 0; j < C::DT; ++j)
 #pragma unroll
         for (int st = 0; st < NTILE; ++st) {
-          const char* const vt = vtile + (tile0 + st) * kWaveKeys * C::ROWB;
+          const char* const vt = vtile + (buf * CHUNK + (tile0 + st) * kWaveKeys) * C::ROWB;
 #pragma unroll
           for (int s = 0; s < 2; ++s) {
             V8 va;
@@ -476,11 +591,12 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
       }
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     }
-    if (more) {
+    if (NBUF == 1 && more) {
       wait_lds();  // the V tiles have been read
       if constexpr (WR > 1) lds_barrier();
-      issue(V_t{}, c - 1, next);
+      issue(V_t{}, c - 1, next, 0);
     }
+    if constexpr (NBUF == 2) buf ^= 1;
   }
 
   // The row's sum over both halves, then over the wavefronts of its keys (in one z frame: the split's own keys).
@@ -503,7 +619,6 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
       sScale[w][tid] = f;
       ls += sMax[w][tid] == kNegInf && sSum[w][tid] == 0.f ? 0.f : f * sSum[w][tid];
     }
-    // tid == wr * 32 + hl of wavefront wr only for the lanes that hold that row: `carry` comes from there below.
     sMax[0][tid] = m;
     sSum[0][tid] = ls;
   }
@@ -574,7 +689,8 @@ __global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(T
   const long long row = mine < total ? mine : total - 1;  // every wavefront meets the barrier
   const int bh = (int)(row / a.T), b = bh / a.Hq;
   const float lam2 = a.slopes[bh - b * a.Hq] * kLog2e;
-  const int n = used_splits(a, filled_rows(a, b));
+  // The splits that wrote a partial.
+  const int n = splits_of(a, a.plan ? plan_cps(a, lane) : a.cps, chunks_of(a, filled_rows(a, b))).used;
   const float* const pmax = a.pmax + row * a.nSplits;
   const float* const psum = a.psum + row * a.nSplits;
   const float* const psig = a.psig + row * a.nSplits;
@@ -646,7 +762,9 @@ __global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(T
 
 template <typename T, int D, int WR>
 hipError_t launch_split(const TreeArgs& a, hipStream_t stream) {
-  const long long items = (long long)a.nSplits * a.B * a.Hkv;
+  // Under a plan at most one round of work-groups and a rounded-up split per sequence and kv head.
+  const long long heads = (long long)a.B * a.Hkv, even = heads * a.nSplits;
+  const long long items = a.plan ? std::min<long long>(even, a.slots / a.row_blocks + 1 + heads) : even;
   const dim3 grid(static_cast<unsigned>((items + 7) / 8 * 8 * a.row_blocks));
   if (a.row_blocks == 1)
     hipLaunchKernelGGL((coalibi_tree_split_kernel<T, D, WR, true>), grid, dim3(kTreeThreads), 0, stream, a);
