@@ -787,12 +787,8 @@ hipError_t tree_dispatch_d(const coalibi::TreeArgs& a, int D, hipStream_t st) {
 constexpr int kTreePlanWalk = 4;      // chunks per split from which the plan pays
 constexpr int kTreeRaggedSplits = 4;  // times as many splits as by the bound that a longer sequence may get
 struct TreePlan {
-  int chunk, row_blocks, slots, cps, splits, planned;
+  int chunk, row_blocks, cps, splits, planned, share;
   bool plans;
-  size_t parts(long long rows, bool ragged) const {
-    const int n = ragged && plans ? planned : splits;
-    return n == 1 ? 0 : static_cast<size_t>(rows) * n;
-  }
 };
 TreePlan tree_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim) {
   const int rows = heads_q / heads_kv * tokens, block = coalibi::tree_block_rows(rows);
@@ -800,18 +796,24 @@ TreePlan tree_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, 
   p.chunk = coalibi::tree_chunk_keys(block);
   p.row_blocks = (rows + block - 1) / block;
   const int chunks = static_cast<int>((seq_kv + static_cast<long long>(p.chunk) - 1) / p.chunk) + 1;
-  const int per_cu = head_dim * (dtype == CO_ALIBI_F32 ? 4 : 2) <= 256 ? 2 : 1;
-  p.slots = per_cu * device_cus();
+  const int per_cu = head_dim * (dtype == CO_ALIBI_F32 ? 4 : 2) <= 256 ? 2 : 1, slots = per_cu * device_cus();
   const long long heads = static_cast<long long>(heads_kv) * p.row_blocks, units = batch * heads;
-  const int most = static_cast<int>(std::min<long long>({std::max<long long>(p.slots / units, 1), chunks, coalibi::kMaxTreeSplits}));
+  const int most = static_cast<int>(std::min<long long>({std::max<long long>(slots / units, 1), chunks, coalibi::kMaxTreeSplits}));
   p.cps = (chunks + most - 1) / most;
   p.splits = (chunks + p.cps - 1) / p.cps;
-  // One sequence cannot get more than all slots.
-  p.planned = static_cast<int>(std::min<long long>({p.splits * static_cast<long long>(kTreeRaggedSplits), chunks,
-                                                    p.slots / heads + 1, coalibi::kMaxTreeSplits}));
+  p.share = static_cast<int>(std::max<long long>(slots / heads, 1));
+  p.planned = static_cast<int>(std::min<long long>({p.splits * static_cast<long long>(kTreeRaggedSplits), chunks, p.share,
+                                                    coalibi::kMaxTreeSplits}));
   p.planned = std::max(p.planned, p.splits);
   p.plans = p.splits > 1 && p.cps >= kTreePlanWalk;
   return p;
+}
+// Bytes of a launch's workspace: the splits used per sequence and kv head, then the partials.  0 with one split.
+size_t tree_workspace(const TreePlan& p, bool ragged, int batch, int heads_q, int heads_kv, int tokens, int head_dim) {
+  const int splits = ragged && p.plans ? p.planned : p.splits;
+  if (splits == 1) return 0;
+  return round_up(static_cast<size_t>(batch) * heads_kv * sizeof(int), 256) +
+         decode_partials_bytes(static_cast<size_t>(batch) * heads_q * tokens * splits, head_dim);
 }
 
 }  // namespace
@@ -822,7 +824,7 @@ size_t co_alibi_decode_tree_workspace_bytes(int dtype, int batch, int heads_q, i
                                             int head_dim) {
   if (batch < 1 || heads_kv < 1 || heads_q < heads_kv || tokens < 1 || seq_kv < 0 || head_dim < 1) return 0;
   const TreePlan plan = tree_plan(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim);
-  return decode_partials_bytes(plan.parts(static_cast<long long>(batch) * heads_q * tokens, true), head_dim);
+  return tree_workspace(plan, true, batch, heads_q, heads_kv, tokens, head_dim);
 }
 
 int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v, const void* k_cache,
@@ -853,11 +855,10 @@ int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v,
     return rc;
   if (!std::isfinite(sm_scale)) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": sm_scale must be finite");
   const TreePlan plan = tree_plan(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim);
-  if (static_cast<double>(batch) * heads_kv * plan.row_blocks * plan.planned > 2.1e9 ||
+  if (static_cast<double>(batch) * heads_kv * plan.row_blocks * (plan.planned + 8.0) > 2.1e9 ||
       static_cast<double>(batch) * heads_q * tokens > 2.1e9)
     return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
-  const size_t parts = plan.parts(static_cast<long long>(batch) * heads_q * tokens, seq_lens != nullptr);
-  const size_t need = decode_partials_bytes(parts, head_dim);
+  const size_t need = tree_workspace(plan, seq_lens != nullptr, batch, heads_q, heads_kv, tokens, head_dim);
   if (workspace_bytes < need)
     return fail(CO_ALIBI_EINVAL, std::string(fn) + ": workspace of " + std::to_string(workspace_bytes) +
                                      " bytes, need " + std::to_string(need));
@@ -890,11 +891,13 @@ int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v,
   a.plan = seq_lens != nullptr && plan.plans;
   a.nSplits = a.plan ? plan.planned : plan.splits;
   a.cps = plan.cps;
-  a.slots = plan.slots;
-  a.slack = 6;
-  const size_t stat_bytes = round_up(parts * sizeof(float), 256);
-  char* ws = static_cast<char*>(workspace);
+  a.share = plan.share;
   if (need != 0) {
+    const size_t parts = static_cast<size_t>(batch) * heads_q * tokens * a.nSplits;
+    const size_t stat_bytes = round_up(parts * sizeof(float), 256);
+    char* ws = static_cast<char*>(workspace);
+    a.used = reinterpret_cast<int*>(ws);
+    ws += round_up(static_cast<size_t>(batch) * heads_kv * sizeof(int), 256);
     a.pmax = reinterpret_cast<float*>(ws);
     a.psum = reinterpret_cast<float*>(ws + stat_bytes);
     a.psig = reinterpret_cast<float*>(ws + 2 * stat_bytes);

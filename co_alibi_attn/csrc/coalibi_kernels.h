@@ -372,7 +372,7 @@ struct CachePlace {
 // layouts' b is the stride from unit to unit).  Row g * T + t of a kv head is query head hkv * G + g of
 // node t.
 // A sequence's chunks are runs of `chunk` cache rows, then one of the new tokens; split s of it covers chunks [s*cps,
-// (s+1)*cps).  Partials per (row (b*Hkv + hkv)*G*T + g*T + t, split): pmax / psum / psig (rows, nSplits) and pout (rows,
+// (s+1)*cps).  Workspace: the splits used, and partials per (row (b*Hkv + hkv)*G*T + g*T + t, split): pmax / psum / psig (rows, nSplits) and pout (rows,
 // nSplits, D), fp32; unused with one split.
 constexpr int kMaxTreeTokens = 64;   // a node's ancestors are the bits of one 64-bit mask
 constexpr int kMaxTreeSplits = 512;  // merge weights in LDS
@@ -399,13 +399,13 @@ struct TreeArgs {
   float* psum;
   float* psig;
   float* pout;
+  int* used;  // (B*Hkv) the splits of each sequence's heads that wrote partials
   int B, Hq, Hkv, G, T, L;
   int chunk;       // tree_chunk_keys of the launch
   int row_blocks;  // work-groups per (split, batch, kv head)
   int nSplits;     // most splits of any sequence: the partials' stride
   int cps;         // chunks per split (with a plan the kernels share the chunks out)
-  int slots;       // resident work-groups the splits are sized for
-  int slack;       // the plan's (decode_cps)
+  int share;       // the plan's splits of all sequences together, per kv head and row block
   bool plan;       // splits sized by the lengths in seq_lens
   float sc2;
 };

@@ -39,12 +39,20 @@ constexpr float kTreeRescale = 8.0f;
 // A partial's sum in the newest split where the row's node is absent.
 constexpr float kAbsent = -1.0f;
 
-template <typename V, typename F>
-__device__ __forceinline__ V wave_all(V x, const F& f) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) x = f(x, __shfl_xor(x, off, 64));
-  return x;
+// Inclusive sum over the lanes up to each one, by DPP moves (shuffles take an LDS round trip a step).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_add(int x) {
+  return x + __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false);
 }
+__device__ __forceinline__ int wave_prefix(int x) {
+  x = dpp_add<0x111, 0xf>(x);  // row_shr 1, 2, 4 and 8 within 16 lanes
+  x = dpp_add<0x112, 0xf>(x);
+  x = dpp_add<0x114, 0xf>(x);
+  x = dpp_add<0x118, 0xf>(x);
+  x = dpp_add<0x142, 0xa>(x);  // the 16 lanes before
+  return dpp_add<0x143, 0xc>(x);  // the 32 lanes before
+}
+__device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_prefix(x), 63); }
 
 __device__ __forceinline__ int filled_rows(const TreeArgs& a, int b) {
   return a.seq_lens == nullptr ? a.L : min(max(a.seq_lens[b], 0), a.L);
@@ -53,22 +61,27 @@ __device__ __forceinline__ int filled_rows(const TreeArgs& a, int b) {
 __device__ __forceinline__ int chunks_of(const TreeArgs& a, int len) { return (len + a.chunk - 1) / a.chunk + 1; }
 
 // Chunks per split of a launch with a plan (every wavefront computes the same): the splits share out the batch's real
-// chunks over one round of work-groups, as the decode's plan does.
+// chunks over one round of work-groups, a.share splits for all sequences of a kv head and row block together.  An equal
+// share of the chunks each, or up to 3/8 more and one where the rounded-up splits then fit the round.
 __device__ __forceinline__ int plan_cps(const TreeArgs& a, int lane) {
   int total = 0, longest = 0;
-  for (int b = lane; b < a.B; b += 64) {
-    const int n = chunks_of(a, filled_rows(a, b));
-    total += n;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int n = b0 + lane < a.B ? chunks_of(a, filled_rows(a, b0 + lane)) : 0;
+    total += wave_total(n);
     longest = max(longest, n);
   }
-  total = wave_all(total, [](int x, int y) { return x + y; });
-  longest = wave_all(longest, [](int x, int y) { return max(x, y); });
-  const long long heads = (long long)a.Hkv * a.row_blocks;
-  return decode_cps(total * heads, longest, a.slots, a.nSplits, a.slack, longest, [&](int c) {
-    int n = 0;
-    for (int b = lane; b < a.B; b += 64) n += (chunks_of(a, filled_rows(a, b)) + c - 1) / c;
-    return wave_all(n, [](int x, int y) { return x + y; }) * heads;
-  });
+  const int c0 = max((total + a.share - 1) / a.share, 1);
+  for (int c = c0; c <= c0 + 1 + c0 * 3 / 8; c += 1 + c / 16) {
+    if (!__any(longest > c * a.nSplits)) {
+      int splits = 0;
+      for (int b0 = 0; b0 < a.B; b0 += 64)
+        splits += wave_total(b0 + lane < a.B ? (chunks_of(a, filled_rows(a, b0 + lane)) + c - 1) / c : 0);
+      if (splits <= a.share) return c;
+    }
+  }
+  int fit = c0;  // no more than nSplits of any sequence
+  while (__any(longest > fit * a.nSplits)) ++fit;
+  return fit;
 }
 
 // A sequence's splits: `used` of them, of cps chunks each (the last may be shorter).
@@ -93,12 +106,7 @@ __device__ __forceinline__ TreeItem plan_item(const TreeArgs& a, int cps, int id
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int b = b0 + lane;
     const int n = b < a.B ? splits_of(a, cps, chunks_of(a, filled_rows(a, b))).used : 0;
-    int incl = n * a.Hkv;
-#pragma unroll
-    for (int off = 1; off < 64; off <<= 1) {
-      const int o = __shfl_up(incl, off, 64);
-      if (lane >= off) incl += o;
-    }
+    const int incl = wave_prefix(n * a.Hkv);
     const unsigned long long in = __ballot(id < before + incl);
     if (in != 0) {
       const int l = __ffsll(in) - 1;
@@ -106,7 +114,7 @@ __device__ __forceinline__ TreeItem plan_item(const TreeArgs& a, int cps, int id
       const int hkv = at / splits;
       return {__builtin_amdgcn_readfirstlane((b0 + l) * a.Hkv + hkv), __builtin_amdgcn_readfirstlane(at - hkv * splits)};
     }
-    before += __shfl(incl, 63, 64);
+    before += __builtin_amdgcn_readlane(incl, 63);
   }
   return {-1, 0};
 }
@@ -292,6 +300,7 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
 
   unsigned long long sees = 0;
   if (newest) {
+    if (tid == 0 && nS > 1) a.used[bhk] = sp.used;  // every row block writes the same
     const unsigned long long all = ancestors(a, b, lane);
     sees = (unsigned long long)__shfl((unsigned)(all >> 32), t, 64) << 32 | __shfl((unsigned)all, t, 64);
     if (tid == 0) sBad = 0;
@@ -408,11 +417,12 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
     {
       f32x16 sacc[NTILE];
 #pragma unroll
-      for (int st = 0; st < NTILE; ++st) {
-        sacc[st] = f32x16{};
-        const char* const kt = kread + (buf * CHUNK + (tile0 + st) * kWaveKeys) * C::ROWB;
+      for (int st = 0; st < NTILE; ++st) sacc[st] = f32x16{};
 #pragma unroll
-        for (int ks = 0; ks < C::KS; ++ks) {
+      for (int ks = 0; ks < C::KS; ++ks)
+#pragma unroll
+        for (int st = 0; st < NTILE; ++st) {
+          const char* const kt = kread + (buf * CHUNK + (tile0 + st) * kWaveKeys) * C::ROWB;
           V8 kf;
           if constexpr (C::E == 2) {
             kf = *reinterpret_cast<const V8*>(kt + (((2 * ks + hh) ^ kx) << 4));
@@ -423,7 +433,6 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
           }
           sacc[st] = M::k16(kf, qf[ks], sacc[st]);
         }
-      }
       if (NBUF == 1 && more) {  // the K tiles have been read: the next chunk's come in
         wait_lds();
         if constexpr (WR > 1) lds_barrier();
@@ -549,12 +558,12 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
       }
       // O^T[d][row] += V^T[d][key] P^T[key][row]; keys 8*s + 16*(l/32) + e of each tile, as in pb.
 #pragma unroll
-      for (int j = 0; j < C::DT; ++j)
+      for (int st = 0; st < NTILE; ++st)
 #pragma unroll
-        for (int st = 0; st < NTILE; ++st) {
+        for (int s = 0; s < 2; ++s) {
           const char* const vt = vtile + (buf * CHUNK + (tile0 + st) * kWaveKeys) * C::ROWB;
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
+          for (int j = 0; j < C::DT; ++j) {
             V8 va;
             if constexpr (C::E == 2) {
               const int r0 = 8 * s + (vg >> 1) * 16 + (vi >> 2), col = (32 * j + 16 * (vg & 1) + 4 * (vi & 3)) & (D - 1);
@@ -689,8 +698,7 @@ __global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(T
   const long long row = mine < total ? mine : total - 1;  // every wavefront meets the barrier
   const int bh = (int)(row / a.T), b = bh / a.Hq;
   const float lam2 = a.slopes[bh - b * a.Hq] * kLog2e;
-  // The splits that wrote a partial.
-  const int n = splits_of(a, a.plan ? plan_cps(a, lane) : a.cps, chunks_of(a, filled_rows(a, b))).used;
+  const int n = a.used[bh / a.G];  // the splits that wrote a partial
   const float* const pmax = a.pmax + row * a.nSplits;
   const float* const psum = a.psum + row * a.nSplits;
   const float* const psig = a.psig + row * a.nSplits;
@@ -764,7 +772,7 @@ template <typename T, int D, int WR>
 hipError_t launch_split(const TreeArgs& a, hipStream_t stream) {
   // Under a plan at most one round of work-groups and a rounded-up split per sequence and kv head.
   const long long heads = (long long)a.B * a.Hkv, even = heads * a.nSplits;
-  const long long items = a.plan ? std::min<long long>(even, a.slots / a.row_blocks + 1 + heads) : even;
+  const long long items = a.plan ? std::min<long long>(even, ((long long)a.share + a.B) * a.Hkv) : even;
   const dim3 grid(static_cast<unsigned>((items + 7) / 8 * 8 * a.row_blocks));
   if (a.row_blocks == 1)
     hipLaunchKernelGGL((coalibi_tree_split_kernel<T, D, WR, true>), grid, dim3(kTreeThreads), 0, stream, a);
