@@ -207,32 +207,39 @@ __device__ __forceinline__ void dma_run(__amdgpu_buffer_rsrc_t r, unsigned lds, 
 #undef COALIBI_DMA_NEXT
 #pragma clang diagnostic pop
 
-// DMA of HALVES runs of 16 keys of a tile, the first of them half `half0` of its 32 keys, to LDS byte address lds.  Run
-// i's rows start at base[i], rows[i] of them valid (the others land as zeros).
+// The source offsets of a wavefront's DMA of HALVES runs of 16 keys, the first of them half `half0` of its 32-key tile.
 //   Lane ln of instruction m brings in piece ln % CPR of key m * KPI + ln / CPR.  The XOR patterns are linear in the key's
 // bits, so their part that depends on m and on the half is a constant on top of the lane's own.
-template <typename T, int D, bool V, bool NT, int HALVES>
-__device__ __forceinline__ void dma_halves(const T* const (&base)[HALVES], const int (&rows)[HALVES], int ld, unsigned lds,
-                                           int half0, int lane) {
+template <typename T, int D, bool V, int HALVES>
+struct DmaOffsets {
   using C = TreeCfg<T, D>;
-  constexpr int KPI = C::CPR >= 64 ? 1 : 64 / C::CPR;  // keys per instruction
-  auto pattern = [](int key) { return V ? swizzle_v<C::CPR, C::E>(key) : swizzle_k<C::CPR>(kRegOfRow(key)); };
-  // Recomputed at every issue from an opaque copy of the lane index, as in dma_wave_rows.
-  int ln;
-  asm volatile("v_mov_b32 %0, %1" : "=v"(ln) : "v"(lane));
-  const int key = ln / C::CPR & 15, piece = ln % C::CPR;
-  const int row = key * (ld * C::E), own = (piece ^ pattern(key)) << 4, step = KPI * ld * C::E;
-#pragma unroll
-  for (int i = 0; i < HALVES; ++i) {
-    const __amdgpu_buffer_rsrc_t r = tile_rsrc(base[i], row_span(rows[i], ld, D));
-    // One half at a time: which one is a wave-uniform value there.
-    const int hx = (HALVES == 2 ? i : half0) * (pattern(16) << 4);
-    int off[C::HALF_INSTR];
-#pragma unroll
-    for (int m = 0; m < C::HALF_INSTR; ++m) off[m] = row + m * step + (own ^ (pattern(m * KPI) << 4) ^ hx);
-    if (16 * C::ROWB >= 1024 || ln < C::ROWB) dma_run<C::HALF_INSTR, NT>(r, lds + 16 * i * C::ROWB, off);
+  int off[HALVES][C::HALF_INSTR];
+
+  static constexpr __device__ __forceinline__ int pattern(int key) {
+    return V ? swizzle_v<C::CPR, C::E>(key) : swizzle_k<C::CPR>(kRegOfRow(key));
   }
-}
+  __device__ __forceinline__ void init(int ld, int half0, int lane) {
+    constexpr int KPI = 64 / C::CPR;  // keys per instruction
+    const int key = lane / C::CPR & 15, piece = lane % C::CPR;
+    const int row = key * (ld * C::E), own = (piece ^ pattern(key)) << 4, step = KPI * ld * C::E;
+#pragma unroll
+    for (int i = 0; i < HALVES; ++i) {
+      const int hx = (HALVES == 2 ? i : half0) * (pattern(16) << 4);
+#pragma unroll
+      for (int m = 0; m < C::HALF_INSTR; ++m) off[i][m] = row + m * step + (own ^ (pattern(m * KPI) << 4) ^ hx);
+    }
+  }
+  // To LDS byte address lds.  Run i's rows start at base[i], rows[i] of them valid (the others land as zeros).
+  template <bool NT>
+  __device__ __forceinline__ void issue(const T* const (&base)[HALVES], const int (&rows)[HALVES], int ld, unsigned lds,
+                                        int lane) const {
+#pragma unroll
+    for (int i = 0; i < HALVES; ++i) {
+      const __amdgpu_buffer_rsrc_t r = tile_rsrc(base[i], row_span(rows[i], ld, D));
+      if (16 * C::ROWB >= 1024 || lane < C::ROWB) dma_run<C::HALF_INSTR, NT>(r, lds + 16 * i * C::ROWB, off[i]);
+    }
+  }
+};
 
 // A wave-uniform int from the constant address space: a scalar load, whatever the memory clobbers around it.
 __device__ __forceinline__ int scalar_load(const int* p) {
@@ -340,13 +347,17 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
     return f;
   };
   // This wavefront's part of chunk c's K or V into buffer `buf` (NT: the cache's rows; the new tokens' are read by every
-  // row block).
+  // row block).  The cache's source offsets are the same for every chunk.
+  const int half0 = HALVES == 2 ? 0 : wave & 1;
+  DmaOffsets<T, D, false, HALVES> k_off;
+  DmaOffsets<T, D, true, HALVES> v_off;
+  k_off.init(a.kcl.r, half0, lane);
+  v_off.init(a.vcl.r, half0, lane);
   auto issue = [&](auto is_v, int c, const Halves& f, int buf) {
     constexpr bool V = decltype(is_v)::value;
     const unsigned lds = (V ? ldsV : ldsK) + (buf * CHUNK + my_key) * C::ROWB;
     const T* base[HALVES];
     int rows[HALVES];
-    const int half0 = HALVES == 2 ? 0 : wave & 1;
     if (c > c_cache) {
       const int ld = V ? a.vl.r : a.kl.r;
 #pragma unroll
@@ -355,7 +366,9 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
         base[i] = (V ? vn : kn) + (size_t)r * ld;
         rows[i] = min(max(a.T - r, 0), 16);
       }
-      dma_halves<T, D, V, false, HALVES>(base, rows, ld, lds, half0, lane);
+      DmaOffsets<T, D, V, HALVES> off;
+      off.init(ld, half0, lane);
+      off.template issue<false>(base, rows, ld, lds, lane);
     } else {
       const Layout& l = V ? a.vcl : a.kcl;
 #pragma unroll
@@ -363,7 +376,10 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
         base[i] = (V ? vc : kc) + (size_t)f.unit[i] * l.b + (size_t)f.row[i] * l.r;
         rows[i] = min(max(L - (c * CHUNK + my_key + 16 * i), 0), 16);
       }
-      dma_halves<T, D, V, NT, HALVES>(base, rows, l.r, lds, half0, lane);
+      if constexpr (V)
+        v_off.template issue<NT>(base, rows, l.r, lds, lane);
+      else
+        k_off.template issue<NT>(base, rows, l.r, lds, lane);
     }
   };
   using K_t = std::false_type;
@@ -396,7 +412,6 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
   const int vi = lane & 15, vg = lane >> 4;
   const int tile0 = wk * NTILE;  // this wavefront's first 32-key tile of a chunk
   int par = 0, buf = 0;
-
   for (int c = c_top; c >= c_first; --c) {
     const bool more = c > c_first, fresh = c > c_cache;
     Halves next{};
@@ -698,19 +713,22 @@ __global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(T
   const long long row = mine < total ? mine : total - 1;  // every wavefront meets the barrier
   const int bh = (int)(row / a.T), b = bh / a.Hq;
   const float lam2 = a.slopes[bh - b * a.Hq] * kLog2e;
-  const int n = a.used[bh / a.G];  // the splits that wrote a partial
   const float* const pmax = a.pmax + row * a.nSplits;
   const float* const psum = a.psum + row * a.nSplits;
   const float* const psig = a.psig + row * a.nSplits;
   float* const w = sW[wave];
-  const bool absent = psum[n - 1] == kAbsent;
+  // The usual split counts' statistics, read along with the count itself.
+  const bool pre = lane < a.nSplits;
+  const float sig0 = pre ? psig[lane] : 0.f, max0 = pre ? pmax[lane] : 0.f, sum0 = pre ? psum[lane] : 0.f;
+  const int n = a.used[bh / a.G];  // the splits that wrote a partial
+  const bool absent = n <= 64 ? __shfl(sum0, n - 1, 64) == kAbsent : psum[n - 1] == kAbsent;
 
   // Split maxima shifted by the sigma of the splits after them; each wavefront computes all of them.
   float carry = 0.f, mx = kNegInf;
   for (int base = (n - 1) / 64 * 64; base >= 0; base -= 64) {
     const int s = base + lane;
     const bool ok = s < n;
-    const float x = ok ? psig[s] : 0.f, pm = ok ? pmax[s] : kNegInf;
+    const float x = !ok ? 0.f : base == 0 ? sig0 : psig[s], pm = !ok ? kNegInf : base == 0 ? max0 : pmax[s];
     float suf = x;
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -729,21 +747,29 @@ __global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(T
   for (int s = lane; s < n; s += 64) {  // a lane reads back what it wrote itself
     const float f = fast_exp2(w[s] - mref);
     w[s] = f;
-    l = fmaf(f, psum[s], l);
+    l = fmaf(f, s == lane ? sum0 : psum[s], l);
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
   wait_lds();  // the weights are read across lanes below (LDS operations of a wavefront complete in order)
 
+  // A split of weight below 2^-64 is not read: on a steep head all but the newest ones.  (The fp32 tail skip's bound.)
   const int sub = lane / LPS, d = (lane % LPS) * 4;
   const float* const po = a.pout + row * a.nSplits * D + d;
   f32x4 acc[4] = {};
   constexpr int STRIDE = PER * WPR;
-  int s = part * PER + sub;
-  for (; s + 3 * STRIDE < n; s += 4 * STRIDE)
+  for (int s = n - 1 - (part * PER + sub); s >= 0; s -= 4 * STRIDE) {
+    f32x4 x[4];
+    float f[4];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) acc[u] += w[s + u * STRIDE] * *reinterpret_cast<const f32x4*>(po + (size_t)(s + u * STRIDE) * D);
-  for (; s < n; s += STRIDE) acc[0] += w[s] * *reinterpret_cast<const f32x4*>(po + (size_t)s * D);
+    for (int u = 0; u < 4; ++u) {
+      const int at = s - u * STRIDE;
+      f[u] = at >= 0 ? w[at] : 0.f;
+      x[u] = f[u] >= 0x1p-64f || f[u] != f[u] ? *reinterpret_cast<const f32x4*>(po + (size_t)at * D) : f32x4{};
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) acc[u] += f[u] * x[u];
+  }
   f32x4 o = (acc[0] + acc[1]) + (acc[2] + acc[3]);
 #pragma unroll
   for (int off = LPS; off < 64; off <<= 1)
