@@ -33,8 +33,9 @@ namespace {
 
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = 64 * kTreeWaves;
-// O is rescaled when a row's maximum grows by more than 2^8, as in the forward: P stays at most 256.
-constexpr float kTreeRescale = 8.0f;
+// O is rescaled when the weights of a lane's keys of a chunk sum to more than this at the running scale: a weight stays
+// far below fp16's 65504.
+constexpr float kTreeRescale = 4096.0f;
 
 // A partial's sum in the newest split where the row's node is absent.
 constexpr float kAbsent = -1.0f;
@@ -502,21 +503,42 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
         carry += sum;
       }
 
-      // a relative to the row's scale, and the scale's update.
+      // a relative to the row's scale, and its weights.
       const float mb = m2 == kNegInf ? 0.f : m2;
-      float mt = kNegInf;
 #pragma unroll
       for (int st = 0; st < NTILE; ++st) {
         const float cst = mb + lam2 * (after + off[st]);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          sacc[st][r] = fmaf(-lam2, loc[st][r], sacc[st][r] - cst);
-          mt = fmaxf(mt, sacc[st][r]);
-        }
+        for (int r = 0; r < 16; ++r) sacc[st][r] = fmaf(-lam2, loc[st][r], sacc[st][r] - cst);
       }
-      mt = fmaxf(mt, other_half(mt));
-      const bool need = m2 == kNegInf ? mt > kNegInf : mt > kTreeRescale;
-      if (__any(need)) {
+      V8 pb[NTILE][2];
+      auto weights = [&] {
+        float sum_p = 0.f;
+#pragma unroll
+        for (int st = 0; st < NTILE; ++st)
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            f32x8 p;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              p[e] = fast_exp2(sacc[st][8 * s + e]);
+              sum_p += p[e];  // before the rounding for the product: the LSE is fp32's
+            }
+            pb[st][s] = M::pack(p);
+          }
+        return sum_p;
+      };
+      float sum_p = weights();
+      // The scale follows the maximum where the weights' sum says that it has risen far (or has none yet): no maximum is
+      // taken otherwise.
+      if (__any(m2 == kNegInf || sum_p > kTreeRescale)) {
+        float mt = kNegInf;
+#pragma unroll
+        for (int st = 0; st < NTILE; ++st)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sacc[st][r]);
+        mt = fmaxf(mt, other_half(mt));
+        const bool need = mt > (m2 == kNegInf ? kNegInf : 0.f);
         const float delta = need ? mt : 0.f;
         const float alpha = need ? (m2 == kNegInf ? 0.f : fast_exp2(-delta)) : 1.f;
         m2 = need ? mb + delta : m2;
@@ -525,20 +547,9 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
         for (int j = 0; j < C::DT; ++j) acc[j] *= alpha;
 #pragma unroll
         for (int st = 0; st < NTILE; ++st) sacc[st] -= delta;
+        sum_p = weights();
       }
-      V8 pb[NTILE][2];
-#pragma unroll
-      for (int st = 0; st < NTILE; ++st)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          f32x8 p;
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            p[e] = fast_exp2(sacc[st][8 * s + e]);
-            lsum += p[e];  // before the rounding for the product: the LSE is fp32's
-          }
-          pb[st][s] = M::pack(p);
-        }
+      lsum += sum_p;
 
       {
         if constexpr (NBUF == 1) {
