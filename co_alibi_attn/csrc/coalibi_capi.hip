@@ -796,16 +796,21 @@ TreePlan tree_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, 
   p.chunk = coalibi::tree_chunk_keys(block);
   p.row_blocks = (rows + block - 1) / block;
   const int chunks = static_cast<int>((seq_kv + static_cast<long long>(p.chunk) - 1) / p.chunk) + 1;
-  const int per_cu = head_dim * (dtype == CO_ALIBI_F32 ? 4 : 2) <= 256 ? 2 : 1, slots = per_cu * device_cus();
+  const int row_bytes = head_dim * (dtype == CO_ALIBI_F32 ? 4 : 2), cus = device_cus();
+  const int slots = (row_bytes <= 128 ? 3 : row_bytes <= 256 ? 2 : 1) * cus;
+  const int few = block <= 64 && row_bytes > 128 ? cus : slots;
   const long long heads = static_cast<long long>(heads_kv) * p.row_blocks, units = batch * heads;
-  const int most = static_cast<int>(std::min<long long>({std::max<long long>(slots / units, 1), chunks, coalibi::kMaxTreeSplits}));
-  p.cps = (chunks + most - 1) / most;
+  auto walk = [&](long long n) {  // chunks per split of n splits
+    const int most = static_cast<int>(std::min<long long>({std::max(n, 1ll), chunks, coalibi::kMaxTreeSplits}));
+    return (chunks + most - 1) / most;
+  };
+  p.cps = walk(few / units);
   p.splits = (chunks + p.cps - 1) / p.cps;
   p.share = static_cast<int>(std::max<long long>(slots / heads, 1));
   p.planned = static_cast<int>(std::min<long long>({p.splits * static_cast<long long>(kTreeRaggedSplits), chunks, p.share,
                                                     coalibi::kMaxTreeSplits}));
-  p.planned = std::max(p.planned, p.splits);
-  p.plans = p.splits > 1 && p.cps >= kTreePlanWalk;
+  p.planned = std::max({p.planned, p.splits, 2});
+  p.plans = slots / units > 1 && walk(slots / units) >= kTreePlanWalk;
   return p;
 }
 // Bytes of a launch's workspace: the splits used per sequence and kv head, then the partials.  0 with one split.

@@ -372,8 +372,8 @@ struct CachePlace {
 // layouts' b is the stride from unit to unit).  Row g * T + t of a kv head is query head hkv * G + g of
 // node t.
 // A sequence's chunks are runs of `chunk` cache rows, then one of the new tokens; split s of it covers chunks [s*cps,
-// (s+1)*cps).  Workspace: the splits used, and partials per (row (b*Hkv + hkv)*G*T + g*T + t, split): pmax / psum / psig (rows, nSplits) and pout (rows,
-// nSplits, D), fp32; unused with one split.
+// (s+1)*cps).  Workspace: the splits used, and partials per (row (b*Hkv + hkv)*G*T + g*T + t, split): pmax / psum / psig
+// (rows, nSplits) and pout (rows, nSplits, D), fp32; a sequence with one split has none.
 constexpr int kMaxTreeTokens = 64;   // a node's ancestors are the bits of one 64-bit mask
 constexpr int kMaxTreeSplits = 512;  // merge weights in LDS
 // Query rows (of the G*T of a kv head) per work-group: one, two or four 32-row tiles.

@@ -53,6 +53,15 @@ __device__ __forceinline__ int wave_prefix(int x) {
   x = dpp_add<0x142, 0xa>(x);  // the 16 lanes before
   return dpp_add<0x143, 0xc>(x);  // the 32 lanes before
 }
+// The largest of the lanes' values (>= 0), in the same steps.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_max(int x) {
+  return max(x, __builtin_amdgcn_update_dpp(0, x, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ int wave_largest(int x) {
+  x = dpp_max<0x118, 0xf>(dpp_max<0x114, 0xf>(dpp_max<0x112, 0xf>(dpp_max<0x111, 0xf>(x))));
+  return __builtin_amdgcn_readlane(dpp_max<0x143, 0xc>(dpp_max<0x142, 0xa>(x)), 63);
+}
 __device__ __forceinline__ int wave_total(int x) { return __builtin_amdgcn_readlane(wave_prefix(x), 63); }
 
 __device__ __forceinline__ int filled_rows(const TreeArgs& a, int b) {
@@ -61,31 +70,32 @@ __device__ __forceinline__ int filled_rows(const TreeArgs& a, int b) {
 // A sequence's chunks: of its filled rows, and the new keys' (the last).
 __device__ __forceinline__ int chunks_of(const TreeArgs& a, int len) { return (len + a.chunk - 1) / a.chunk + 1; }
 
+// The sequences' splits together, of cps chunks each.
+__device__ __forceinline__ int total_splits(const TreeArgs& a, int cps, int lane) {
+  int n = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64)
+    n += wave_total(b0 + lane < a.B ? (chunks_of(a, filled_rows(a, b0 + lane)) + cps - 1) / cps : 0);
+  return n;
+}
+
 // Chunks per split of a launch with a plan (every wavefront computes the same): the splits share out the batch's real
-// chunks over one round of work-groups, a.share splits for all sequences of a kv head and row block together.  An equal
-// share of the chunks each, or up to 3/8 more and one where the rounded-up splits then fit the round.
+// chunks over one round of `share` work-groups per kv head and row block.  An equal share of the chunks each, or up
+// to 3/8 more and one where the rounded-up splits then fit the round.
 __device__ __forceinline__ int plan_cps(const TreeArgs& a, int lane) {
   int total = 0, longest = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
     const int n = b0 + lane < a.B ? chunks_of(a, filled_rows(a, b0 + lane)) : 0;
     total += wave_total(n);
-    longest = max(longest, n);
+    longest = max(longest, wave_largest(n));
   }
-  const int c0 = max((total + a.share - 1) / a.share, 1);
-  for (int c = c0; c <= c0 + 1 + c0 * 3 / 8; c += 1 + c / 16) {
-    if (!__any(longest > c * a.nSplits)) {
-      int splits = 0;
-      for (int b0 = 0; b0 < a.B; b0 += 64)
-        splits += wave_total(b0 + lane < a.B ? (chunks_of(a, filled_rows(a, b0 + lane)) + c - 1) / c : 0);
-      if (splits <= a.share) return c;
-    }
-  }
-  int fit = c0;  // no more than nSplits of any sequence
-  while (__any(longest > fit * a.nSplits)) ++fit;
-  return fit;
+  // No more than nSplits of any sequence.
+  const int c0 = max((total + a.share - 1) / a.share, (longest + a.nSplits - 1) / a.nSplits);
+  for (int c = c0; c <= c0 + 1 + c0 * 3 / 8; c += 1 + c / 16)
+    if (total_splits(a, c, lane) <= a.share) return c;
+  return c0;
 }
 
-// A sequence's splits: `used` of them, of cps chunks each (the last may be shorter).
+// A sequence's splits: `used` of them, of cps chunks each (the last may have fewer).
 struct TreeSplits {
   int cps, used;
 };
@@ -671,7 +681,7 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
     }
   const size_t row0 = (size_t)bhk * R + rb * (WR * 32);  // the block's first row in o, lse and the partials
   const int rows = min(R - rb * (WR * 32), WR * 32);
-  const bool direct = nS == 1;
+  const bool direct = sp.used == 1;  // the whole sequence: no partials, and the merge leaves its rows alone
   if (wk == 0 && hh == 0 && row_ok) {
     const bool absent = newest && sees == 0;
     if (direct) {
@@ -732,6 +742,7 @@ __global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(T
   const bool pre = lane < a.nSplits;
   const float sig0 = pre ? psig[lane] : 0.f, max0 = pre ? pmax[lane] : 0.f, sum0 = pre ? psum[lane] : 0.f;
   const int n = a.used[bh / a.G];  // the splits that wrote a partial
+  if (WPR > 1 && n == 1) return;   // its only split wrote o (one row per work-group: nobody is left at a barrier)
   const bool absent = n <= 64 ? __shfl(sum0, n - 1, 64) == kAbsent : psum[n - 1] == kAbsent;
 
   // Split maxima shifted by the sigma of the splits after them; each wavefront computes all of them.
@@ -793,7 +804,7 @@ __global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(T
 #pragma unroll
     for (int p = 1; p < WPR; ++p) o += *reinterpret_cast<const f32x4*>(&sO[wave + p][d]);
   }
-  if (mine >= total) return;
+  if (mine >= total || n == 1) return;
   if (sub == 0) {
     typedef T out4 __attribute__((ext_vector_type(4)));
     const float inv = 1.f / l;
@@ -807,8 +818,8 @@ __global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(T
 
 template <typename T, int D, int WR>
 hipError_t launch_split(const TreeArgs& a, hipStream_t stream) {
-  // Under a plan at most one round of work-groups and a rounded-up split per sequence and kv head.
-  const long long heads = (long long)a.B * a.Hkv, even = heads * a.nSplits;
+  // Under a plan at most one round of work-groups and a rounded-up split per sequence.
+  const long long even = (long long)a.B * a.Hkv * a.nSplits;
   const long long items = a.plan ? std::min<long long>(even, ((long long)a.share + a.B) * a.Hkv) : even;
   const dim3 grid(static_cast<unsigned>((items + 7) / 8 * 8 * a.row_blocks));
   if (a.row_blocks == 1)
