@@ -133,14 +133,14 @@ struct Weights {
   __device__ __forceinline__ u64 operator()(float x) const { return mass(scaled(x)); }
 };
 
-// f(x, index) over the row, each thread its own tokens, 16 bytes a load whatever the row's alignment and U loads in
-// flight (few copies of a long f); the last V % VEC tokens one by one.
+// f(x, index) over the row, each thread its own tokens, U loads of 16 bytes in flight (few copies of a long f).  The
+// tokens before the row's first 16-byte boundary and after its last go one by one.
 template <int U, typename T, typename F>
 __device__ __forceinline__ void for_row(const T* row, int V, const F& f) {
   constexpr int VEC = 16 / (int)sizeof(T);
-  typedef T vec __attribute__((ext_vector_type(VEC), aligned(sizeof(T))));
-  const int n = V / VEC;
-  const vec* const v = reinterpret_cast<const vec*>(row);
+  typedef T vec __attribute__((ext_vector_type(VEC)));
+  const int head = min((int)(-reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T), V), n = (V - head) / VEC;
+  const vec* const v = reinterpret_cast<const vec*>(row + head);
   for (int j = threadIdx.x; j < n; j += U * kSampleThreads) {
     vec x[U];
 #pragma unroll
@@ -149,9 +149,9 @@ __device__ __forceinline__ void for_row(const T* row, int V, const F& f) {
     for (int u = 0; u < U; ++u)
       if (u == 0 || j + u * kSampleThreads < n)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) f(static_cast<T>(x[u][e]), (j + u * kSampleThreads) * VEC + e);
+        for (int e = 0; e < VEC; ++e) f(static_cast<T>(x[u][e]), head + (j + u * kSampleThreads) * VEC + e);
   }
-  const int i = n * VEC + threadIdx.x;
+  const int t = threadIdx.x, i = t < head ? t : n * VEC + t;
   if (i < V) f(row[i], i);
 }
 
@@ -420,7 +420,7 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
       }
       u64 all = 0;
       if (!cut_k && cut_p) {
-        for_row<2>(row, V, [&](T x, int i) {
+        for_row<4>(row, V, [&](T x, int i) {
           all += ws(static_cast<float>(x));
           if (static_cast<float>(x) >= bound) list(0, static_cast<float>(x), i);
         });
@@ -463,7 +463,7 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
     if (tid == 0) s.listed = 0;
     __syncthreads();
     u64 heavy = 0;
-    for_row<2>(row, V, [&](T x, int) {
+    for_row<4>(row, V, [&](T x, int) {
       const float f = static_cast<float>(x);
       const double w = ws.scaled(f);
       const u64 m = Weights::mass(w);
