@@ -38,9 +38,11 @@ constexpr int kSampleWaves = kSampleThreads / 64;
 constexpr int kDigitBits = 11;
 constexpr int kBins = 1 << kDigitBits;
 static_assert(kBins == 2 * kSampleThreads, "a thread scans two bins");
-constexpr int kMaxList = 1024;
-// Largest top-k that is tried as a list.  Among 1024 threads' maxima the bound for k leaves about k + k^2 / 2048 tokens.
-constexpr int kMaxListK = 512;
+constexpr int kMaxList = 2048;
+constexpr int kPerThread = kMaxList / kSampleThreads;  // listed tokens
+// Largest top-k that is tried as a list.  Among 1024 threads' maxima the bound for k leaves about -1024 ln(1 - k / 1024)
+// tokens in random order: 1.2 k at 350, 1.6 k at 700.
+constexpr int kMaxListK = 800;
 constexpr int kIndexBits = 20;
 static_assert(kMaxVocab <= 1 << kIndexBits, "an index fits an entry");
 
@@ -72,7 +74,7 @@ __device__ __forceinline__ unsigned key32(float x) { return Key<float>::of(x); }
 // descending order of the words, and its weight.
 struct Entry {
   u64 word;
-  u64 mass;  // set by weigh_list
+  u64 mass;
 };
 __device__ __forceinline__ u64 entry_word(int bin, float x, int i) {
   return (u64)(0xfffu - bin) << 52 | (u64)key32(x) << kIndexBits | ((1u << kIndexBits) - 1 - i);
@@ -80,23 +82,29 @@ __device__ __forceinline__ u64 entry_word(int bin, float x, int i) {
 __device__ __forceinline__ float entry_logit(u64 word) { return Key<float>::value((unsigned)(word >> kIndexBits)); }
 __device__ __forceinline__ int entry_index(u64 word) { return (1 << kIndexBits) - 1 - (int)(word & ((1u << kIndexBits) - 1)); }
 
-// What a thread knows of its entry in the list: what lies before it in the row, by count and by mass.
+// An entry's place: what lies before it in the row, by count and by mass.
 struct Listed {
   u64 before_cnt, before_mass, mass;
-  int token;
-  bool mine;
+  int token;  // -1: no entry
 };
+
+constexpr int kRounds = 8;  // of kth_of_threads
+constexpr int kSums = 3;    // block_sum calls on one way through the kernel
 
 struct SampleLds {
   u64 mass[kBins];  // a histogram's bins; then what lies before each
   unsigned cnt[kBins];
-  Entry list[kMaxList];
+  unsigned cursor[kBins];
+  u64 list[kMaxList];       // the words of the listed tokens, as found
+  Entry grouped[kMaxList];  // by bin
+  u64 prefix[kMaxList];     // the masses before each grouped entry
   double exp2_table[32];
-  u64 wmass[kSampleWaves], wmass2[kSampleWaves];
+  u64 wmass[kSampleWaves];
   unsigned wcnt[kSampleWaves];
+  u64 round[kRounds], sum[kSums];  // zero at the start
   unsigned char flag[kBins];
   int bin;
-  u64 before_cnt, before_mass;
+  u64 before_cnt, before_mass, list_mass;
   int listed, token, found;
   Listed at;
 };
@@ -155,58 +163,110 @@ __device__ __forceinline__ void for_row(const T* row, int V, const F& f) {
   if (i < V) f(row[i], i);
 }
 
-__device__ __forceinline__ u64 block_sum(u64 x, SampleLds& s) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// The sum over the work-group, each call with a slot of its own (integers: any order gives the same).
+__device__ __forceinline__ u64 block_sum(u64 x, SampleLds& s, int slot) {
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) x += __shfl_xor(x, off, 64);
-  if (lane == 0) s.wmass[wave] = x;
+  if ((threadIdx.x & 63) == 0) atomicAdd(&s.sum[slot], x);
   __syncthreads();
-  x = 0;
-#pragma unroll
-  for (int w = 0; w < kSampleWaves; ++w) x += s.wmass[w];
-  __syncthreads();
-  return x;
+  return s.sum[slot];
 }
 
 // ------------------------------------------------------------------ positions in a list
 
-// Each of the n entries learns from all others what lies before it in its bin (s.mass / s.cnt: what lies before the
-// bin; `flat`: one bin, nothing before it).  `share` threads, a power of two within a wavefront, split an
-// entry's walk over the list, and the first of them has it.
-__device__ __forceinline__ Listed place_listed(SampleLds& s, int n, bool flat) {
-  int share = 64;
-  while (share * n > kSampleThreads) share >>= 1;
-  const int i = threadIdx.x / share, part = threadIdx.x - i * share;
-  Listed r{0, 0, 0, 0, false};
-  if (i < n) {
-    const Entry e = s.list[i];
-    u64 mass = 0;
-    unsigned cnt = 0;
-    for (int j = part; j < n; j += share) {
-      const Entry o = s.list[j];
-      if (o.word > e.word && (o.word ^ e.word) >> 52 == 0) {
-        mass += o.mass;
-        ++cnt;
-      }
-    }
-    for (int off = 1; off < share; off <<= 1) {
-      mass += __shfl_xor(mass, off, 64);
-      cnt += __shfl_xor(cnt, off, 64);
-    }
-    const int bin = 0xfff - (int)(e.word >> 52);
-    r = {(flat ? 0 : s.cnt[bin]) + (u64)cnt, (flat ? 0 : s.mass[bin]) + mass, e.mass, entry_index(e.word), part == 0};
+// Each of the n entries of s.list learns what lies before it: the entries are grouped by bin, and within their bin compared
+// with one another.  Before a bin lies what s.mass / s.cnt say, or with `whole` (the list is all that counts) what the list
+// holds before it.  Thread t has the entries t, t + kSampleThreads, ... in `out`, and their weights' sum in s.list_mass.
+__device__ __forceinline__ void place_listed(SampleLds& s, int n, bool whole, const Weights& ws, Listed (&out)[kPerThread]) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  auto bin_of = [](u64 word) { return 0xfff - (int)(word >> 52); };
+  s.cursor[2 * tid] = s.cursor[2 * tid + 1] = 0;
+  __syncthreads();
+  for (int i = tid; i < n; i += kSampleThreads) atomicAdd(&s.cursor[bin_of(s.list[i])], 1u);
+  __syncthreads();
+  const unsigned n0 = s.cursor[2 * tid], n1 = s.cursor[2 * tid + 1];
+  unsigned c = n0 + n1;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const unsigned o = __shfl_up(c, off, 64);
+    if (lane >= off) c += o;
   }
-  return r;
+  if (lane == 63) s.wcnt[wave] = c;
+  __syncthreads();
+  unsigned w = lane < wave ? s.wcnt[lane & (kSampleWaves - 1)] : 0;
+#pragma unroll
+  for (int off = kSampleWaves / 2; off > 0; off >>= 1) w += __shfl_xor(w, off, kSampleWaves);
+  c += __shfl(w, 0, 64) - n0 - n1;  // entries of the bins before this thread's
+  s.cursor[2 * tid] = c;
+  s.cursor[2 * tid + 1] = c + n0;
+  __syncthreads();
+  for (int i = tid; i < n; i += kSampleThreads) {
+    const u64 word = s.list[i];
+    // A bin's cursor ends at the next bin's start.
+    s.grouped[atomicAdd(&s.cursor[bin_of(word)], 1u)] = {word, ws(entry_logit(word))};
+  }
+  __syncthreads();
+  // The masses before each entry: kPerThread consecutive ones a thread.
+  u64 own[kPerThread], m = 0;
+#pragma unroll
+  for (int u = 0; u < kPerThread; ++u) {
+    const int i = tid * kPerThread + u;
+    own[u] = i < n ? s.grouped[i].mass : 0;
+    m += own[u];
+  }
+  const u64 total = m;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const u64 o = __shfl_up(m, off, 64);
+    if (lane >= off) m += o;
+  }
+  if (lane == 63) s.wmass[wave] = m;
+  __syncthreads();
+  u64 wm = lane < wave ? s.wmass[lane & (kSampleWaves - 1)] : 0;
+#pragma unroll
+  for (int off = kSampleWaves / 2; off > 0; off >>= 1) wm += __shfl_xor(wm, off, kSampleWaves);
+  m += __shfl(wm, 0, 64);
+  if (tid == kSampleThreads - 1) s.list_mass = m;
+  m -= total;
+#pragma unroll
+  for (int u = 0; u < kPerThread; ++u) {
+    if (tid * kPerThread + u < n) s.prefix[tid * kPerThread + u] = m;
+    m += own[u];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kPerThread; ++u) {
+    out[u] = {0, 0, 0, -1};
+    const int i = tid + u * kSampleThreads;
+    if (i < n) {
+      const Entry e = s.grouped[i];
+      const int bin = bin_of(e.word), from = bin == 0 ? 0 : s.cursor[bin - 1], to = s.cursor[bin];
+      u64 mass = whole ? s.prefix[from] : s.mass[bin];
+      unsigned cnt = whole ? from : s.cnt[bin];
+#pragma unroll 8
+      for (int j = from; j < to; ++j) {
+        const Entry o = s.grouped[j];
+        if (o.word > e.word) {
+          mass += o.mass;
+          ++cnt;
+        }
+      }
+      out[u] = {cnt, mass, e.mass, entry_index(e.word)};
+    }
+  }
 }
 
 // The listed token at position `pos` (by count, or by mass), into s.at; false: not in the list.
-__device__ __forceinline__ bool find_listed(SampleLds& s, const Listed& l, u64 pos, bool by_mass) {
+__device__ __forceinline__ bool find_listed(SampleLds& s, const Listed (&l)[kPerThread], u64 pos, bool by_mass) {
   if (threadIdx.x == 0) s.found = 0;
   __syncthreads();
-  const u64 before = by_mass ? l.before_mass : l.before_cnt, own = by_mass ? l.mass : 1;
-  if (l.mine && pos >= before && pos - before < own) {
-    s.at = l;
-    s.found = 1;
+#pragma unroll
+  for (int u = 0; u < kPerThread; ++u) {
+    const u64 before = by_mass ? l[u].before_mass : l[u].before_cnt, own = by_mass ? l[u].mass : 1;
+    if (l[u].token >= 0 && pos >= before && pos - before < own) {
+      s.at = l[u];
+      s.found = 1;
+    }
   }
   __syncthreads();
   const bool found = s.found != 0;
@@ -325,25 +385,21 @@ __device__ __forceinline__ u64 draw_position(double uni, u64 kept) {
 // A bound that at least k (1 to 1024) of the threads' values reach: the k-th largest of them, its key cut to 16 bits.
 // Two bits a round, from the top.
 __device__ __forceinline__ float kth_of_threads(SampleLds& s, float mine, int k) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const unsigned key = key32(mine);
   unsigned bound = 0;
 #pragma unroll
-  for (int bit = 30; bit >= 16; bit -= 2) {
+  for (int i = 0; i < kRounds; ++i) {
+    const int bit = 30 - 2 * i;
     // How many reach bound + 1, + 2 and + 3 units of these bits, 16 bits each.
     u64 c = 0;
 #pragma unroll
     for (unsigned d = 1; d < 4; ++d) c |= (u64)__popcll(__ballot(key >= (bound | d << bit))) << (16 * (d - 1));
-    u64* const w = bit & 2 ? s.wmass : s.wmass2;  // a buffer per parity: one barrier a round
-    if (lane == 0) w[wave] = c;
+    if ((threadIdx.x & 63) == 0) atomicAdd(&s.round[i], c);
     __syncthreads();
-    u64 n = 0;
-#pragma unroll
-    for (int i = 0; i < kSampleWaves; ++i) n += w[i];
+    const u64 n = s.round[i];
     const unsigned kk = k, n1 = n & 0xffff, n2 = n >> 16 & 0xffff, n3 = n >> 32;
     bound |= (n3 >= kk ? 3u : n2 >= kk ? 2u : n1 >= kk ? 1u : 0u) << bit;
   }
-  __syncthreads();
   return bound <= key32(kNegInf) ? kNegInf : Key<float>::value(bound);
 }
 
@@ -359,6 +415,8 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
   const double uni = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[b]
                                     : static_cast<double>(static_cast<const float*>(a.uniforms)[b]);
   if (tid < 32) s.exp2_table[tid] = ldexp(exp2(tid / 32.0), a.mass_bits);
+  if (tid < kRounds) s.round[tid] = 0;
+  if (tid < kSums) s.sum[tid] = 0;
   if (tid == 0) s.listed = 0;
 
   // 1. The largest logit, and whether one is NaN (magnitude bits above the infinities').
@@ -397,13 +455,7 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
 
     auto list = [&](int bin, float x, int i) {
       const int at = atomicAdd(&s.listed, 1);
-      if (at < kMaxList) s.list[at].word = entry_word(bin, x, i);
-    };
-    // Sets the list's weights; returns this thread's entry's.
-    auto weigh_list = [&](int n) {
-      const double w = tid < n ? ws.scaled(entry_logit(s.list[tid].word)) : 0.0;
-      if (tid < n) s.list[tid].mass = Weights::mass(w);
-      return w;
+      if (at < kMaxList) s.list[at] = entry_word(bin, x, i);
     };
 
     // 2. A short list: the first k and what ties with their bound, or (without top-k) the tokens near or above min-p's
@@ -418,25 +470,30 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
         bound -= 1e-6f * (fabsf(top) + fabsf(bound));  // the weights decide at the border, not this rounding
         if (top == __builtin_inff()) bound = top;
       }
+      // The bins that place_listed groups by: of the distance from the largest, down to the bound.
+      const float per_unit = (kBins - 1) / fmaxf(top - bound, 1e-30f);
+      auto bin_from = [&](float x) {
+        const float d = x == top ? 0.f : (top - x) * per_unit;
+        return d < kBins - 1 ? static_cast<int>(d) : kBins - 1;
+      };
       u64 all = 0;
       if (!cut_k && cut_p) {
         for_row<4>(row, V, [&](T x, int i) {
           all += ws(static_cast<float>(x));
-          if (static_cast<float>(x) >= bound) list(0, static_cast<float>(x), i);
+          if (static_cast<float>(x) >= bound) list(bin_from(static_cast<float>(x)), static_cast<float>(x), i);
         });
-        all = block_sum(all, s);
+        all = block_sum(all, s, 0);
       } else {
         for_row<8>(row, V, [&](T x, int i) {
-          if (static_cast<float>(x) >= bound) list(0, static_cast<float>(x), i);
+          if (static_cast<float>(x) >= bound) list(bin_from(static_cast<float>(x)), static_cast<float>(x), i);
         });
       }
       __syncthreads();
       const int n = s.listed;
       if (n <= kMaxList) {
-        const double w = weigh_list(n);
-        const u64 sum = block_sum(Weights::mass(w), s);
-        const Listed l = place_listed(s, n, true);
-        u64 kept = sum;
+        Listed l[kPerThread];
+        place_listed(s, n, true, ws, l);
+        u64 kept = s.list_mass;
         if (cut_k && n > top_k) {
           find_listed(s, l, top_k - 1, false);
           kept = s.at.before_mass + s.at.mass;
@@ -445,7 +502,14 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
         // Past the list's end (only without top-k) min-p is the closer cut.
         if (cut_p && find_listed(s, l, top_p_position(top_p, cut_k ? kept : all), true))
           cut = min(cut, s.at.before_mass + s.at.mass);
-        if (cut_m) cut = min(cut, max(block_sum(w >= min_scaled ? Weights::mass(w) : 0, s), one));
+        if (cut_m) {
+          u64 heavy = 0;
+          for (int i = tid; i < n; i += kSampleThreads) {
+            const double w = ws.scaled(entry_logit(s.list[i]));
+            if (w >= min_scaled) heavy += Weights::mass(w);
+          }
+          cut = min(cut, max(block_sum(heavy, s, 1), one));
+        }
         find_listed(s, l, draw_position(uni, cut), true);
         if (tid == 0) a.tokens[b] = s.at.token;
         return;
@@ -473,7 +537,7 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
       if (w >= min_scaled) heavy += m;
     });
     __syncthreads();
-    if (cut_m) heavy = max(block_sum(heavy, s), one);
+    if (cut_m) heavy = max(block_sum(heavy, s, 2), one);
     const int b0 = 2 * tid, b1 = b0 + 1;
     const u64 m0 = s.mass[b0], m1 = s.mass[b1];
     const unsigned c0 = s.cnt[b0], c1 = s.cnt[b1];
@@ -530,9 +594,8 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
     __syncthreads();
     const int n = s.listed;
     if (n <= kMaxList) {
-      weigh_list(n);
-      __syncthreads();
-      const Listed l = place_listed(s, n, false);
+      Listed l[kPerThread];
+      place_listed(s, n, false, ws, l);
       u64 cut = all;
       if (cut_k) {
         find_listed(s, l, top_k - 1, false);
