@@ -102,12 +102,22 @@ struct SampleLds {
   u64 wmass[kSampleWaves];
   unsigned wcnt[kSampleWaves];
   u64 round[kRounds], sum[kSums];  // zero at the start
-  unsigned char flag[kBins];
   int bin;
   u64 before_cnt, before_mass, list_mass;
   int listed, token, found;
   Listed at;
 };
+
+// 2^(i / 32), rounded to fp64.
+__device__ const double kExp2Table[32] = {
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0,
+    0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0, 0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0,
+    0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0, 0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0,
+    0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0,
+    0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0, 0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
 
 // The weights of one row: 2^(y / 32) with y = (x - max) * 32 log2(e) / T.
 struct Weights {
@@ -161,6 +171,33 @@ __device__ __forceinline__ void for_row(const T* row, int V, const F& f) {
   }
   const int t = threadIdx.x, i = t < head ? t : n * VEC + t;
   if (i < V) f(row[i], i);
+}
+
+// act(x, index) for the tokens with pred(x), few of them: the tests of 32 tokens first, then the ones that passed (one
+// copy of act, where a branch per token makes the kernel outgrow the instruction cache).
+template <typename T, typename P, typename A>
+__device__ __forceinline__ void for_row_if(const T* row, int V, const P& pred, const A& act) {
+  constexpr int VEC = 16 / (int)sizeof(T), U = 32 / VEC;
+  typedef T vec __attribute__((ext_vector_type(VEC)));
+  const int head = min((int)(-reinterpret_cast<uintptr_t>(row) & 15) / (int)sizeof(T), V), n = (V - head) / VEC;
+  const vec* const v = reinterpret_cast<const vec*>(row + head);
+  for (int j = threadIdx.x; j < n; j += U * kSampleThreads) {
+    vec x[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = v[min(j + u * kSampleThreads, n - 1)];
+    unsigned hit = 0;
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (u == 0 || j + u * kSampleThreads < n)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) hit |= pred(static_cast<T>(x[u][e])) ? 1u << (u * VEC + e) : 0u;
+    for (; hit != 0; hit &= hit - 1) {
+      const int bit = __ffs(hit) - 1, i = head + (j + bit / VEC * kSampleThreads) * VEC + bit % VEC;
+      act(row[i], i);
+    }
+  }
+  const int t = threadIdx.x, i = t < head ? t : n * VEC + t;
+  if (i < V && pred(row[i])) act(row[i], i);
 }
 
 // The sum over the work-group, each call with a slot of its own (integers: any order gives the same).
@@ -234,24 +271,33 @@ __device__ __forceinline__ void place_listed(SampleLds& s, int n, bool whole, co
     m += own[u];
   }
   __syncthreads();
+  // `share` threads, a power of two within a wavefront, split the walk over an entry's bin; the first of them has it.
+  int share = 64;
+  while (share * n > kSampleThreads && share > 1) share >>= 1;
+  const int part = tid & (share - 1);
 #pragma unroll
   for (int u = 0; u < kPerThread; ++u) {
     out[u] = {0, 0, 0, -1};
-    const int i = tid + u * kSampleThreads;
+    const int i = tid / share + u * kSampleThreads;
     if (i < n) {
       const Entry e = s.grouped[i];
       const int bin = bin_of(e.word), from = bin == 0 ? 0 : s.cursor[bin - 1], to = s.cursor[bin];
-      u64 mass = whole ? s.prefix[from] : s.mass[bin];
-      unsigned cnt = whole ? from : s.cnt[bin];
-#pragma unroll 8
-      for (int j = from; j < to; ++j) {
+      u64 mass = 0;
+      unsigned cnt = 0;
+#pragma unroll 4
+      for (int j = from + part; j < to; j += share) {
         const Entry o = s.grouped[j];
         if (o.word > e.word) {
           mass += o.mass;
           ++cnt;
         }
       }
-      out[u] = {cnt, mass, e.mass, entry_index(e.word)};
+      for (int off = 1; off < share; off <<= 1) {
+        mass += __shfl_xor(mass, off, 64);
+        cnt += __shfl_xor(cnt, off, 64);
+      }
+      if (part == 0)
+        out[u] = {cnt + (whole ? from : s.cnt[bin]), mass + (whole ? s.prefix[from] : s.mass[bin]), e.mass, entry_index(e.word)};
     }
   }
 }
@@ -414,10 +460,10 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
   const double min_p = a.min_p != nullptr ? static_cast<double>(a.min_p[b]) : a.min_p_all;
   const double uni = a.uniforms_f64 ? static_cast<const double*>(a.uniforms)[b]
                                     : static_cast<double>(static_cast<const float*>(a.uniforms)[b]);
-  if (tid < 32) s.exp2_table[tid] = ldexp(exp2(tid / 32.0), a.mass_bits);
+  if (tid < 32) s.exp2_table[tid] = kExp2Table[tid] * static_cast<double>(1ull << a.mass_bits);
   if (tid < kRounds) s.round[tid] = 0;
   if (tid < kSums) s.sum[tid] = 0;
-  if (tid == 0) s.listed = 0;
+  if (tid == 0) s.listed = 0, s.token = V;
 
   // 1. The largest logit, and whether one is NaN (magnitude bits above the infinities').
   float mine = kNegInf;
@@ -439,15 +485,22 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
     if (tid == 0) a.tokens[b] = -1;
     return;
   }
-  unsigned key = Key<T>::of(static_cast<T>(top));
-  u64 nth = 0;
-  if (temp > 0.0) {  // else (0, negative or NaN) the first of the largest logits
+  if (!(temp > 0.0)) {  // 0, negative or NaN: the first of the largest logits
+    for_row_if(row, V, [&](T x) { return static_cast<float>(x) == top; }, [&](T, int i) { atomicMin(&s.token, i); });
+    __syncthreads();
+    if (tid == 0) a.tokens[b] = s.token;
+    return;
+  }
+  unsigned key;
+  u64 nth;
+  {
     Weights ws;
     ws.top = top;
     ws.top64 = static_cast<double>(top);
     ws.c = 32.0 * 1.4426950408889634074 / temp;
     ws.one = static_cast<double>(1ull << a.mass_bits);
-    ws.reach = static_cast<float>(fmin((a.mass_bits + 2) * 32.0 / ws.c, 3.4028234e38));
+    const float temp32 = static_cast<float>(fmin(temp, 1e37));
+    ws.reach = fminf((a.mass_bits + 2) * kLn2 * temp32, 3.4028234e38f);
     ws.table = s.exp2_table;
     const bool cut_k = top_k > 0 && top_k < V, cut_p = top_p < 1.0, cut_m = min_p > 0.0;
     const double min_scaled = min_p * ws.one;
@@ -460,13 +513,15 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
 
     // 2. A short list: the first k and what ties with their bound, or (without top-k) the tokens near or above min-p's
     // bound; top-p then also needs the sum of all weights.
-    if ((cut_k && top_k <= kMaxListK) || (!cut_k && cut_m)) {
+    int n = kMaxList + 1;
+    u64 all = 0, heavy = 0;  // the weights' sum, and min-p's part of it
+    const bool whole = (cut_k && top_k <= kMaxListK) || (!cut_k && cut_m);
+    if (whole) {
       float bound;
       if (cut_k) {
         bound = kth_of_threads(s, mine, top_k);
       } else {
-        const double below = fmax(-log2(min_p), 0.0) * 32.0 / ws.c;
-        bound = top - static_cast<float>(below * 1.00001);
+        bound = top - fmaxf(-log2f(static_cast<float>(min_p)), 0.f) * kLn2 * temp32 * 1.00001f;
         bound -= 1e-6f * (fabsf(top) + fabsf(bound));  // the weights decide at the border, not this rounding
         if (top == __builtin_inff()) bound = top;
       }
@@ -476,158 +531,139 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
         const float d = x == top ? 0.f : (top - x) * per_unit;
         return d < kBins - 1 ? static_cast<int>(d) : kBins - 1;
       };
-      u64 all = 0;
-      if (!cut_k && cut_p) {
-        for_row<4>(row, V, [&](T x, int i) {
-          all += ws(static_cast<float>(x));
-          if (static_cast<float>(x) >= bound) list(bin_from(static_cast<float>(x)), static_cast<float>(x), i);
-        });
-        all = block_sum(all, s, 0);
-      } else {
-        for_row<8>(row, V, [&](T x, int i) {
-          if (static_cast<float>(x) >= bound) list(bin_from(static_cast<float>(x)), static_cast<float>(x), i);
-        });
-      }
+      const bool add_up = !cut_k && cut_p;
+      for_row_if(row, V, [&](T x) {
+        if (add_up) all += ws(static_cast<float>(x));
+        return static_cast<float>(x) >= bound;
+      }, [&](T x, int i) { list(bin_from(static_cast<float>(x)), static_cast<float>(x), i); });
+      if (add_up) all = block_sum(all, s, 0);
       __syncthreads();
-      const int n = s.listed;
-      if (n <= kMaxList) {
-        Listed l[kPerThread];
-        place_listed(s, n, true, ws, l);
-        u64 kept = s.list_mass;
-        if (cut_k && n > top_k) {
-          find_listed(s, l, top_k - 1, false);
-          kept = s.at.before_mass + s.at.mass;
+      n = s.listed;
+      if (n <= kMaxList && cut_m) {
+        for (int i = tid; i < n; i += kSampleThreads) {
+          const double w = ws.scaled(entry_logit(s.list[i]));
+          if (w >= min_scaled) heavy += Weights::mass(w);
         }
-        u64 cut = kept;
-        // Past the list's end (only without top-k) min-p is the closer cut.
-        if (cut_p && find_listed(s, l, top_p_position(top_p, cut_k ? kept : all), true))
-          cut = min(cut, s.at.before_mass + s.at.mass);
-        if (cut_m) {
-          u64 heavy = 0;
-          for (int i = tid; i < n; i += kSampleThreads) {
-            const double w = ws.scaled(entry_logit(s.list[i]));
-            if (w >= min_scaled) heavy += Weights::mass(w);
-          }
-          cut = min(cut, max(block_sum(heavy, s, 1), one));
-        }
-        find_listed(s, l, draw_position(uni, cut), true);
-        if (tid == 0) a.tokens[b] = s.at.token;
-        return;
+        heavy = block_sum(heavy, s, 1);
       }
     }
+    const bool listed = n <= kMaxList;
 
     // 3. Weights by distance from the largest logit, in bins of reach / kBins (the last also holds what has no weight).
-    const float per_bin = kBins / ws.reach;
-    auto bin_of = [&](float x) {
-      const float d = x == top ? 0.f : (top - x) * per_bin;
-      return d < kBins - 1 ? static_cast<int>(d) : kBins - 1;
-    };
-    __syncthreads();
-    for (int i = tid; i < kBins; i += kSampleThreads) s.cnt[i] = 0, s.mass[i] = 0;
-    if (tid == 0) s.listed = 0;
-    __syncthreads();
-    u64 heavy = 0;
-    for_row<4>(row, V, [&](T x, int) {
-      const float f = static_cast<float>(x);
-      const double w = ws.scaled(f);
-      const u64 m = Weights::mass(w);
-      const int bin = bin_of(f);
-      if (cut_k) atomicAdd(&s.cnt[bin], 1u);
-      if (m != 0) atomicAdd(&s.mass[bin], m);
-      if (w >= min_scaled) heavy += m;
-    });
-    __syncthreads();
-    if (cut_m) heavy = max(block_sum(heavy, s, 2), one);
-    const int b0 = 2 * tid, b1 = b0 + 1;
-    const u64 m0 = s.mass[b0], m1 = s.mass[b1];
-    const unsigned c0 = s.cnt[b0], c1 = s.cnt[b1];
-    u64 c_in, m_in;
-    scan_bins(s, b0, b1, c_in, m_in);
-    // What lies before this thread's bins takes their place.
-    const u64 cb1 = c_in - c1, cb0 = cb1 - c0, mb1 = m_in - m1, mb0 = mb1 - m0;
-    __syncthreads();
-    s.mass[b0] = mb0;
-    s.mass[b1] = mb1;
-    s.cnt[b0] = (unsigned)cb0;
-    s.cnt[b1] = (unsigned)cb1;
-    if (tid == kSampleThreads - 1) s.before_mass = m_in;
-    __syncthreads();
-    const u64 all = s.before_mass;
-    __syncthreads();
-    bool f0 = false, f1 = false;
-    // Flags the bins that hold positions lo .. hi by mass (or a position by count); `from` and `to`: the masses before the
-    // first such bin and up to the end of the last.
-    auto flag = [&](bool by_mass, u64 lo, u64 hi, u64& from, u64& to) {
-      const u64 B0 = by_mass ? mb0 : cb0, B1 = by_mass ? mb1 : cb1, E0 = B0 + (by_mass ? m0 : c0), E1 = B1 + (by_mass ? m1 : c1);
-      f0 |= B0 <= hi && lo < E0;
-      f1 |= B1 <= hi && lo < E1;
-      if (B0 <= lo && lo < E0) s.before_mass = mb0;
-      if (B1 <= lo && lo < E1) s.before_mass = mb1;
-      if (B0 <= hi && hi < E0) s.before_cnt = mb0 + m0;
-      if (B1 <= hi && hi < E1) s.before_cnt = mb1 + m1;
+    if (!listed) {
+      const float per_bin = kBins / ws.reach;
+      auto bin_of = [&](float x) {
+        const float d = x == top ? 0.f : (top - x) * per_bin;
+        return d < kBins - 1 ? static_cast<int>(d) : kBins - 1;
+      };
       __syncthreads();
-      from = s.before_mass;
-      to = s.before_cnt;
+      for (int i = tid; i < kBins; i += kSampleThreads) s.cnt[i] = 0, s.mass[i] = 0;
+      if (tid == 0) s.listed = 0;
       __syncthreads();
-    };
-    u64 lo = all, hi = all;  // the kept mass lies in [lo, hi]
-    if (cut_k) flag(false, top_k - 1, top_k - 1, lo, hi);
-    if (cut_p) {
-      u64 p_lo, p_hi;
-      flag(true, top_p_position(top_p, lo), top_p_position(top_p, hi), p_lo, p_hi);
-      lo = min(lo, p_lo);
-      hi = min(hi, p_hi);
+      heavy = 0;
+      for_row<4>(row, V, [&](T x, int) {
+        const float f = static_cast<float>(x);
+        const double w = ws.scaled(f);
+        const u64 m = Weights::mass(w);
+        const int bin = bin_of(f);
+        if (cut_k) atomicAdd(&s.cnt[bin], 1u);
+        if (m != 0) atomicAdd(&s.mass[bin], m);
+        if (w >= min_scaled) heavy += m;
+      });
+      __syncthreads();
+      if (cut_m) heavy = block_sum(heavy, s, 2);
+      const int b0 = 2 * tid, b1 = b0 + 1;
+      const u64 m0 = s.mass[b0], m1 = s.mass[b1];
+      const unsigned c0 = s.cnt[b0], c1 = s.cnt[b1];
+      u64 c_in, m_in;
+      scan_bins(s, b0, b1, c_in, m_in);
+      // What lies before this thread's bins takes their place.
+      const u64 cb1 = c_in - c1, cb0 = cb1 - c0, mb1 = m_in - m1, mb0 = mb1 - m0;
+      __syncthreads();
+      s.mass[b0] = mb0;
+      s.mass[b1] = mb1;
+      s.cnt[b0] = (unsigned)cb0;
+      s.cnt[b1] = (unsigned)cb1;
+      if (tid == kSampleThreads - 1) s.before_mass = m_in;
+      __syncthreads();
+      all = s.before_mass;
+      __syncthreads();
+      // The bins from the one that holds position lo (by mass, or by count) to the one that holds hi; `from` and `to`: the
+      // masses before the first and up to the end of the last.
+      struct Range {
+        int first;
+        unsigned more;
+      };
+      auto range = [&](bool by_mass, u64 lo, u64 hi, u64& from, u64& to) {
+        const u64 B0 = by_mass ? mb0 : cb0, B1 = by_mass ? mb1 : cb1, E0 = B0 + (by_mass ? m0 : c0), E1 = B1 + (by_mass ? m1 : c1);
+        if (B0 <= lo && lo < E0) s.before_mass = mb0, s.bin = b0;
+        if (B1 <= lo && lo < E1) s.before_mass = mb1, s.bin = b1;
+        if (B0 <= hi && hi < E0) s.before_cnt = mb0 + m0, s.found = b0;
+        if (B1 <= hi && hi < E1) s.before_cnt = mb1 + m1, s.found = b1;
+        __syncthreads();
+        from = s.before_mass;
+        to = s.before_cnt;
+        const Range r{s.bin, (unsigned)(s.found - s.bin)};
+        __syncthreads();
+        return r;
+      };
+      u64 lo = all, hi = all;  // the kept mass lies in [lo, hi]
+      Range at_k{0, 0}, at_p{0, 0};
+      if (cut_k) at_k = range(false, top_k - 1, top_k - 1, lo, hi);
+      if (cut_p) {
+        u64 p_lo, p_hi;
+        at_p = range(true, top_p_position(top_p, lo), top_p_position(top_p, hi), p_lo, p_hi);
+        lo = min(lo, p_lo);
+        hi = min(hi, p_hi);
+      }
+      if (cut_m) lo = min(lo, max(heavy, one)), hi = min(hi, max(heavy, one));
+      lo = max(lo, one);  // the first token is always kept
+      hi = max(hi, lo);
+      u64 from, to;
+      const Range at_u = range(true, draw_position(uni, lo), draw_position(uni, hi), from, to);
+      if (!cut_k) at_k = at_u;
+      if (!cut_p) at_p = at_u;
+      for_row_if(row, V, [&](T x) {
+        const int bin = bin_of(static_cast<float>(x));
+        return (unsigned)(bin - at_u.first) <= at_u.more || (unsigned)(bin - at_p.first) <= at_p.more ||
+               (unsigned)(bin - at_k.first) <= at_k.more;
+      }, [&](T x, int i) { list(bin_of(static_cast<float>(x)), static_cast<float>(x), i); });
+      __syncthreads();
+      n = s.listed;
     }
-    if (cut_m) lo = min(lo, heavy), hi = min(hi, heavy);
-    lo = max(lo, one);
-    hi = max(hi, lo);
-    u64 from, to;
-    flag(true, draw_position(uni, lo), draw_position(uni, hi), from, to);
-    s.flag[b0] = f0;
-    s.flag[b1] = f1;
-    __syncthreads();
-    for_row<4>(row, V, [&](T x, int i) {
-      const float f = static_cast<float>(x);
-      const int bin = bin_of(f);
-      if (s.flag[bin]) list(bin, f, i);
-    });
-    __syncthreads();
-    const int n = s.listed;
+    heavy = max(heavy, one);
+
+    // The end of the top-k, the end of the top-p and the draw: `end_at(pos, by_mass, end)` finds a position and the mass up
+    // to the end of its token; false: it has none.  (Top-p without top-k takes its part of all weights, also where the
+    // list holds fewer.)
+    auto resolve = [&](u64 cut, auto end_at) {
+      u64 end;
+      if (cut_k && end_at(top_k - 1, false, end)) cut = end;
+      if (cut_p && end_at(top_p_position(top_p, cut_k ? cut : all), true, end)) cut = min(cut, end);
+      if (cut_m) cut = min(cut, heavy);
+      end_at(draw_position(uni, cut), true, end);
+    };
     if (n <= kMaxList) {
       Listed l[kPerThread];
-      place_listed(s, n, false, ws, l);
-      u64 cut = all;
-      if (cut_k) {
-        find_listed(s, l, top_k - 1, false);
-        cut = s.at.before_mass + s.at.mass;
-      }
-      if (cut_p) {
-        find_listed(s, l, top_p_position(top_p, cut), true);
-        cut = min(cut, s.at.before_mass + s.at.mass);
-      }
-      if (cut_m) cut = min(cut, heavy);
-      find_listed(s, l, draw_position(uni, cut), true);
+      place_listed(s, n, listed, ws, l);
+      resolve(listed ? s.list_mass : all, [&](u64 pos, bool by_mass, u64& end) {
+        // Not in the list: past its end, where min-p is the closer cut.
+        if (!find_listed(s, l, pos, by_mass)) return false;
+        end = s.at.before_mass + s.at.mass;
+        return true;
+      });
       if (tid == 0) a.tokens[b] = s.at.token;
       return;
     }
-
-    // 4. Radix select: the end of the top-k, the end of the top-p, the draw.
-    u64 cut = all;
-#pragma unroll 1
-    for (int step = 0; step < 3; ++step) {
-      if (step == 2 && cut_m) cut = min(cut, heavy);
-      if ((step == 0 && !cut_k) || (step == 1 && !cut_p)) continue;
-      const u64 pos = step == 0 ? top_k - 1 : step == 1 ? top_p_position(top_p, cut) : draw_position(uni, cut);
-      const Place p = locate(s, row, V, pos, step > 0, ws);
+    // 4. By radix select.
+    resolve(all, [&](u64 pos, bool by_mass, u64& end) {
+      const Place p = locate(s, row, V, pos, by_mass, ws);
       const u64 w = ws(Key<T>::value(p.key));
-      const u64 at = step == 0 ? pos - p.before_cnt : (pos - p.before_mass) / w;  // among the tokens of this key
-      if (step < 2) {
-        cut = min(cut, p.before_mass + (at + 1) * w);
-      } else {
-        key = p.key;
-        nth = at;
-      }
-    }
+      nth = by_mass ? (pos - p.before_mass) / w : pos - p.before_cnt;  // among the tokens of this key
+      end = p.before_mass + (nth + 1) * w;
+      key = p.key;
+      return true;
+    });
   }
   const int token = nth_token(s, row, V, key, nth);
   if (tid == 0) a.tokens[b] = token;
