@@ -12,6 +12,10 @@ GELU MLP (4x), residual.  The LM head is tied to the token embedding.
 
 ``attention`` is injectable so tests can run the same model on the CPU with a
 reference attention; the default is the native ``co_alibi_attention``.
+
+Serving: ``GPT.prefill`` and ``GPT.extend`` run new tokens over a ``PagedCache`` and each other, ``PagedCache.accept``
+keeps their keys and values, ``GPT.generate`` samples with them, and ``GPT.speculate`` checks a tree of drafts.  These
+call the native operators (co_alibi_attn/serving.py), on the GPU only.
 """
 from __future__ import annotations
 
@@ -24,6 +28,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .co_alibi_attn import co_alibi_attention, co_alibi_attention_qkv
+from .serving import co_alibi_cache_append, co_alibi_decode_tree, co_alibi_sample
 
 
 @dataclass(frozen=True)
@@ -37,6 +42,53 @@ class GPTConfig:
 
 
 AttentionFn = Callable[..., torch.Tensor]
+
+
+class PagedCache:
+    """Every layer's keys and values of a batch of sequences, in pages under one block table.
+
+    ``capacity`` rows per sequence, all empty at first.  ``dtype`` is the one the model's projections have (the
+    weights' type, or autocast's).  A forward over the cache leaves its new keys and values in ``new``, one
+    (k, v) per layer; ``accept`` writes them.
+    """
+
+    def __init__(self, cfg: GPTConfig, batch: int, capacity: int, dtype: torch.dtype = torch.bfloat16,
+                 device: str | torch.device = "cuda", page_size: int = 64):
+        blocks = -(-capacity // page_size)
+        self.capacity = blocks * page_size
+        shape = (batch * blocks, cfg.n_head, page_size, cfg.d_model // cfg.n_head)
+        self.layers = [(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
+                       for _ in range(cfg.n_layer)]
+        self.block_table = torch.arange(batch * blocks, dtype=torch.int32, device=device).view(batch, blocks)
+        self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.bound = 0  # no sequence is longer; known without reading the device
+        self.new: list[tuple[torch.Tensor, torch.Tensor]] = []
+
+    def room_for(self, tokens: int) -> None:
+        """Raises ValueError where a sequence has no room for this many more rows."""
+        if self.bound + tokens > self.capacity:  # the bound counts every row as accepted: look before refusing
+            self.bound = int(self.seq_lens.max())
+        if self.bound + tokens > self.capacity:
+            raise ValueError(f"{tokens} more rows behind {self.bound} do not fit a cache of {self.capacity}")
+
+    def accept(self, rows: torch.Tensor | None = None, counts: torch.Tensor | None = None) -> None:
+        """Keeps the last forward's new rows: all, the first counts[b], or the rows[b, :counts[b]] (a path of a tree).
+
+        All rows have to fit (ValueError); of ``counts``, which are on the device, what fits is kept.
+        """
+        if not self.new:
+            raise ValueError("no new keys and values: run a forward over this cache first")
+        n = self.new[0][0].shape[2] if rows is None else rows.shape[1]
+        if counts is None:
+            self.room_for(n)
+        for (k_cache, v_cache), (k, v) in zip(self.layers, self.new):
+            co_alibi_cache_append(k, v, k_cache, v_cache, self.seq_lens, self.block_table, rows=rows, counts=counts)
+        if counts is None:
+            self.seq_lens += n
+        else:
+            self.seq_lens += torch.minimum(counts.clamp(0, n), self.capacity - self.seq_lens)
+        self.bound = min(self.bound + n, self.capacity)
+        self.new = []
 
 
 class CausalCoALiBiAttention(nn.Module):
@@ -60,6 +112,18 @@ class CausalCoALiBiAttention(nn.Module):
         y = self.attention(q, k, v, causal=True, bias_max=self.bias_max)
         return self.proj(y.transpose(1, 2).reshape(B, S, C))
 
+    def over_cache(self, x: torch.Tensor, cache: PagedCache, layer: int, parents: torch.Tensor | None,
+                   prefill: bool) -> torch.Tensor:
+        B, T, C = x.shape
+        qkv = self.qkv(x).view(B, T, 3, self.n_head, self.head_dim)
+        q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
+        cache.new.append((k, v))
+        if prefill:
+            return self.proj(co_alibi_attention_qkv(qkv, causal=True, bias_max=self.bias_max).reshape(B, T, C))
+        y = co_alibi_decode_tree(q, k, v, *cache.layers[layer], seq_len=cache.seq_lens, parents=parents,
+                                 block_table=cache.block_table, bias_max=self.bias_max)
+        return self.proj(y.transpose(1, 2).reshape(B, T, C))
+
 
 class Block(nn.Module):
     def __init__(self, cfg: GPTConfig, attention: AttentionFn):
@@ -71,7 +135,9 @@ class Block(nn.Module):
         self.out = nn.Linear(cfg.mlp_ratio * cfg.d_model, cfg.d_model)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        x = x + self.attn(self.ln1(x))
+        return self.mlp(x + self.attn(self.ln1(x)))
+
+    def mlp(self, x: torch.Tensor) -> torch.Tensor:
         return x + self.out(F.gelu(self.fc(self.ln2(x)), approximate="tanh"))
 
 
@@ -106,6 +172,83 @@ class GPT(nn.Module):
             return logits
         loss = F.cross_entropy(logits.float().view(-1, logits.size(-1)), targets.view(-1))
         return logits, loss
+
+    def _over_cache(self, idx: torch.Tensor, cache: PagedCache, parents=None, prefill=False) -> torch.Tensor:
+        cache.new = []
+        x = self.wte(idx)
+        for i, blk in enumerate(self.blocks):
+            x = blk.mlp(x + blk.attn.over_cache(blk.ln1(x), cache, i, parents, prefill))
+        return self.ln_f(x)
+
+    @torch.no_grad()
+    def prefill(self, idx: torch.Tensor, cache: PagedCache, lengths: torch.Tensor | None = None) -> torch.Tensor:
+        """Puts prompts (B, S) into an empty cache; returns the logits (B, vocab) behind each one's last token.
+
+        ``lengths``: integer tensor (B,) with values in [1, S]: sequence b is idx[b, :lengths[b]], the rest padding.
+        """
+        if cache.bound != 0:
+            raise ValueError("prefill needs an empty cache")
+        B, S = idx.shape
+        cache.room_for(S)
+        h = self._over_cache(idx, cache, prefill=True)
+        cache.accept(counts=lengths)
+        h = h[:, -1] if lengths is None else h[torch.arange(B, device=h.device), lengths.long() - 1]
+        return F.linear(h, self.wte.weight)
+
+    @torch.no_grad()
+    def extend(self, idx: torch.Tensor, cache: PagedCache, parents: torch.Tensor | None = None) -> torch.Tensor:
+        """Logits (B, T, vocab) behind each of T <= 64 new tokens idx (B, T), a chain or the tree of ``parents``.
+
+        The cache's rows stay as they are; ``cache.accept`` keeps the new ones.
+        """
+        return F.linear(self._over_cache(idx, cache, parents), self.wte.weight)
+
+    @torch.no_grad()
+    def generate(self, idx: torch.Tensor, lengths: torch.Tensor | None, uniforms: torch.Tensor, cache: PagedCache,
+                 **sampling) -> torch.Tensor:
+        """Tokens (B, n) that follow the prompts (as for ``prefill``), one per uniform number of ``uniforms`` (B, n).
+
+        ``sampling``: the settings of ``co_alibi_sample``.  The last token is not in the cache.
+        """
+        logits = self.prefill(idx, cache, lengths)
+        out = torch.empty(uniforms.shape, dtype=torch.long, device=idx.device)
+        for i in range(uniforms.shape[1]):
+            if i > 0:
+                cache.room_for(1)
+                logits = self.extend(out[:, i - 1:i], cache)[:, 0]
+                cache.accept()
+            out[:, i] = co_alibi_sample(logits, uniforms[:, i], **sampling)
+        return out
+
+    @torch.no_grad()
+    def speculate(self, idx: torch.Tensor, parents: torch.Tensor, uniforms: torch.Tensor, cache: PagedCache, **sampling):
+        """One step over a tree of drafts; returns (rows (B, T), counts (B,), next tokens (B,)).
+
+        idx, parents: (B, T).  Node 0 is the sequence's last token, which the cache does not hold yet, with parent -1; the
+        others are drafts.  Behind every node one token is drawn with that node's number of ``uniforms`` (B, T).  A
+        draft is accepted when its parent is and it is the token drawn there (the first of equal ones), so what
+        is accepted, idx[b, rows[b, 1:counts[b]]], and the next token, drawn behind it, are what drawing token by token
+        gives with those numbers.  The cache keeps the accepted rows.
+        """
+        B, T = idx.shape
+        cache.room_for(T)
+        logits = self.extend(idx, cache, parents)
+        drawn = co_alibi_sample(logits.reshape(B * T, -1), uniforms.reshape(B * T), **sampling).view(B, T)
+        node = torch.arange(T, device=idx.device)
+        up = parents.long().clamp(0, T - 1)
+        ok = (idx == drawn.gather(1, up)) & (parents >= 0) & (parents < node)
+        twin = (parents[:, :, None] == parents[:, None]) & (idx[:, :, None] == idx[:, None]) & (node < node[:, None])
+        ok &= ~twin.any(2)
+        ok[:, 0] = True
+        up[:, 0] = 0
+        for _ in range(T.bit_length()):  # accepted: so are 1, 2, 4, ... ancestors
+            ok &= ok.gather(1, up)
+            up = up.gather(1, up)
+        counts = ok.sum(1, dtype=torch.int32)
+        rows = torch.where(ok, node, T).sort(1).values.int()
+        cache.accept(rows, counts)
+        last = rows.gather(1, counts[:, None].long() - 1).long()
+        return rows, counts, drawn.gather(1, last)[:, 0]
 
     def n_params(self) -> int:
         return sum(p.numel() for p in self.parameters())

@@ -75,6 +75,27 @@ def test_special_rows(dtype):
             check(rows, torch.full((11,), u), **kw)
 
 
+@pytest.mark.parametrize("dtype", (F32, BF16), ids=str)
+def test_cuts_of_many_tokens_and_cuts_together(dtype):
+    x, u = logits_of(6, 50304, dtype, seed=21)
+    for kw in (dict(k=700), dict(k=800), dict(k=801), dict(k=2047), dict(k=2049, p=0.9), dict(k=50303), dict(p=0.999999),
+               dict(p=0.9, m=1e-4), dict(p=0.2, m=1e-4), dict(p=0.999, m=0.3), dict(m=1e-6), dict(m=1e-300), dict(k=30, m=0.2),
+               dict(k=5000, m=1e-3, p=0.7), dict(t=20.0, m=0.5), dict(t=20.0, p=0.5), dict(t=0.05), dict(t=0.02, p=0.5)):
+        print(dtype, kw, flush=True)
+        check(x, u, **kw)
+
+
+def test_temperatures_and_logits_of_any_size():
+    x, u = logits_of(6, 5000, F32, seed=22)
+    wide = x * 1e37  # up to about 1e38
+    tiny = x * 1e-42  # subnormal
+    for rows in (x, wide, tiny):
+        for t in (1e-300, 1e-40, 1e-6, 1e6, 1e40, 1e300, math.inf):
+            for kw in (dict(), dict(k=20), dict(p=0.5), dict(m=0.5), dict(m=1.0)):
+                print(t, kw, flush=True)
+                check(rows, u, t=t, **kw)
+
+
 def test_masked_vocabulary():
     for dtype in DTYPES:
         x, u = logits_of(8, 20011, dtype, seed=5, masked=0.9)

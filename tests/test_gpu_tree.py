@@ -134,6 +134,62 @@ def test_tree_random(seed):
     check(run(*inputs, lens, parents), want, dtype)
 
 
+def few_long(B, long, seed):
+    """Lengths around `long` at a few places, else up to 90, with 0 and 1 among them."""
+    gen = torch.Generator().manual_seed(seed)
+    lens = torch.randint(2, 91, (B,), generator=gen)
+    lens[0], lens[B // 2], lens[B - 1], lens[1], lens[B - 2] = long, long - 37, long // 3, 0, 1
+    return lens.tolist()
+
+
+# Enough sequences and rows that the launch divides its splits by the sequences' own lengths.
+RAGGED = [
+    (16, 8, 8, 2, few_long(16, 2305, 1), 128, 64, BF16),    # 16-row blocks
+    (24, 16, 4, 10, few_long(24, 2900, 2), 128, 16, F16),   # 64
+    (40, 32, 2, 5, few_long(40, 1793, 3), 128, 32, BF16),   # 128, of which 80 rows are used
+    (30, 16, 1, 10, few_long(30, 3000, 4), 64, 64, F16),    # two blocks
+    (100, 2, 1, 1, few_long(100, 4200, 5), 64, 0, BF16),    # more sequences than a wavefront's lanes
+    (20, 4, 4, 3, few_long(20, 1700, 6), 128, 64, F32),
+    (30, 2, 2, 2, few_long(30, 2400, 7), 256, 64, BF16),
+]
+
+
+@pytest.mark.parametrize("case", RAGGED, ids=lambda c: "B{}_Hq{}_Hkv{}_T{}_L{}_D{}_p{}_{}".format(
+    *c[:4], max(c[4]), *c[5:7], NAME[c[7]]))
+def test_tree_ragged_batch(case):
+    B, Hq, Hkv, T, lens, D, page, dtype = case
+    inputs = make(*case[:6], dtype, page, seed=B)
+    parents = random_parents(B, T, torch.Generator().manual_seed(B), absent=T > 4)
+    want = oracle.decode_tree(*inputs[:5], lens, parents, inputs[5], lam_of(Hq, dtype), D ** -0.5)
+    check(run(*inputs, lens, parents), want, dtype)
+    check(run(*inputs, lens, parents, max_seq_len=max(lens)), want, dtype)
+
+
+def test_ragged_batch_with_a_page_outside_the_pool():
+    B, lens = 16, few_long(16, 2305, 8)
+    q, k, v, kc, vc, table = make(B, 8, 8, 2, lens, 128, BF16, 64, seed=8)
+    sound, _ = run(q, k, v, kc, vc, table, lens, None)
+    table[0, 20], table[3, 0] = kc.shape[0], -1
+    got, lse = run(q, k, v, kc, vc, table, lens, None)
+    for b in range(B):
+        if b in (0, 3):
+            assert got[b].isnan().all() and lse[b].isnan().all()
+        else:
+            assert torch.equal(got[b], sound[b])
+
+
+def test_ragged_batches_in_every_order_of_sequences():
+    """The same sequences in another order, or with others' lengths changed: the long one's result moves by rounding only."""
+    B, Hq, Hkv, T, D = 16, 8, 8, 2, 128
+    lens = few_long(B, 2305, 9)
+    q, k, v, kc, vc, table = make(B, Hq, Hkv, T, lens, D, F16, 64, seed=9)
+    want = oracle.decode_tree(q, k, v, kc, vc, lens, None, table, lam_of(Hq, F16), D ** -0.5)
+    for seed in range(3):
+        order = torch.randperm(B, generator=torch.Generator().manual_seed(seed))
+        got = run(q[order], k[order], v[order], kc, vc, table[order], [lens[b] for b in order], None)
+        check(got, tuple(w[order] for w in want), F16)
+
+
 @pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
 @pytest.mark.parametrize("dtype", (BF16, F32), ids=NAME.get)
 def test_unseen_tokens_do_not_reach_a_result(dtype, bad):

@@ -8,6 +8,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 
 import co_alibi_attn as co
 from co_alibi_attn import _native
+from co_alibi_attn.gpt import GPT, GPTConfig, PagedCache
 from oracle import co_alibi_ref as ref
 from oracle import serving as oracle
 
@@ -88,6 +89,50 @@ def test_decode_tree_argument_errors(over, code, msg):
     lib = _native.lib()
     assert _tree(lib, **over) == code
     assert msg in lib.co_alibi_last_error().decode()
+
+
+def test_decode_tree_workspace():
+    """Per sequence and kv head one int, then per (sequence, query head, token, split) three floats and D more, each
+    array rounded up to 256 bytes; nothing with one split."""
+    lib = _native.lib()
+    size = lambda *a: lib.co_alibi_decode_tree_workspace_bytes(*a)  # noqa: E731
+    up = lambda n: -(-n // 256) * 256  # noqa: E731
+    for dtype, B, Hq, Hkv, T, L, D in ((1, 1, 4, 4, 1, 300, 64), (2, 2, 8, 2, 16, 5000, 128), (0, 1, 6, 2, 3, 9000, 32)):
+        n = size(dtype, B, Hq, Hkv, T, L, D)
+        rows = B * Hq * T
+        for splits in range(2, 513):
+            if n == up(4 * B * Hkv) + 3 * up(4 * rows * splits) + 4 * rows * splits * D:
+                break
+        else:
+            raise AssertionError((n, rows))
+        assert splits <= -(-L // 64) + 1
+    assert size(1, 1, 4, 4, 1, 0, 64) == 0  # only the new tokens: one split
+    for bad in ((1, 0, 4, 4, 1, 9, 64), (1, 1, 2, 4, 1, 9, 64), (1, 1, 4, 4, 0, 9, 64), (1, 1, 4, 4, 1, -1, 64)):
+        assert size(*bad) == 0
+    need = size(2, 2, 8, 2, 3, 500, 128)
+    assert need > 0
+    for over, msg in ((dict(ws=None, ws_bytes=need), "workspace is NULL"), (dict(ws=P + 16, ws_bytes=need), "workspace is not 256"),
+                      (dict(lens=P, ws_bytes=need - 1), f"workspace of {need - 1} bytes, need {need}")):
+        args = dict(dtype=2, B=2, Hq=8, Hkv=2, T=3, L=500, D=128)
+        assert _tree(lib, **args, **over) == 1
+        assert msg in lib.co_alibi_last_error().decode()
+
+
+def test_cache_of_the_gpt_without_a_device():
+    cfg = GPTConfig(n_layer=2, n_head=2, d_model=64, vocab=11)
+    cache = PagedCache(cfg, 3, 70, torch.float32, "cpu", page_size=32)
+    assert cache.capacity == 96 and cache.block_table.tolist() == [[0, 1, 2], [3, 4, 5], [6, 7, 8]]
+    assert len(cache.layers) == 2 and cache.layers[0][0].shape == (9, 2, 32, 32)
+    with pytest.raises(ValueError, match="no new keys"):
+        cache.accept()
+    cache.seq_lens += torch.tensor([5, 60, 0])
+    cache.bound = 96
+    cache.room_for(36)
+    assert cache.bound == 60
+    with pytest.raises(ValueError, match="37 more rows behind 60 do not fit a cache of 96"):
+        cache.room_for(37)
+    with pytest.raises(ValueError, match="empty cache"):
+        GPT(cfg).prefill(torch.zeros(3, 4, dtype=torch.long), cache)
 
 
 def _append(lib, **over):
