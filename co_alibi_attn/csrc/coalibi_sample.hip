@@ -499,8 +499,7 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
     ws.top64 = static_cast<double>(top);
     ws.c = 32.0 * 1.4426950408889634074 / temp;
     ws.one = static_cast<double>(1ull << a.mass_bits);
-    const float temp32 = static_cast<float>(fmin(temp, 1e37));
-    ws.reach = fminf((a.mass_bits + 2) * kLn2 * temp32, 3.4028234e38f);
+    ws.reach = fminf((a.mass_bits + 2) * kLn2 * static_cast<float>(temp), 3.4028234e38f);
     ws.table = s.exp2_table;
     const bool cut_k = top_k > 0 && top_k < V, cut_p = top_p < 1.0, cut_m = min_p > 0.0;
     const double min_scaled = min_p * ws.one;
@@ -521,8 +520,9 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
       if (cut_k) {
         bound = kth_of_threads(s, mine, top_k);
       } else {
-        bound = top - fmaxf(-log2f(static_cast<float>(min_p)), 0.f) * kLn2 * temp32 * 1.00001f;
-        bound -= 1e-6f * (fabsf(top) + fabsf(bound));  // the weights decide at the border, not this rounding
+        // At the border the weights decide, not this rounding (to them what is 2^-54 below 1 is 1).
+        bound = top - (fmaxf(-log2f(static_cast<float>(min_p)), 0.f) * (kLn2 * 1.00001f) + 1e-12f) * static_cast<float>(temp);
+        bound -= 1e-6f * (fabsf(top) + fabsf(bound));
         if (top == __builtin_inff()) bound = top;
       }
       // The bins that place_listed groups by: of the distance from the largest, down to the bound.
