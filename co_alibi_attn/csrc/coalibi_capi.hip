@@ -804,7 +804,13 @@ TreePlan tree_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, 
     const int most = static_cast<int>(std::min<long long>({std::max(n, 1ll), chunks, coalibi::kMaxTreeSplits}));
     return (chunks + most - 1) / most;
   };
-  p.cps = walk(few / units);
+  // Few chunks go through one work-group, which needs no merge and no workspace: that saves a second launch, 2 us of a
+  // captured call and 4 us of host time in an eager one, and costs 1.3 us a chunk at 128-byte rows.  12 heads, one token,
+  // us captured / eager, split against whole: 120 keys 10.0 / 17.1 and 8.0 / 13.3, 500 keys (5 chunks) 10.0 / 17.6 and
+  // 12.4 / 13.3, 760 keys 10.0 / 18.1 and 15.3 / 15.6.  At 256-byte rows 250 keys (3 chunks) 11.4 / 18.1 and 11.3 / 13.3; in fp32
+  // 12.0 / 18.2 and 14.5 / 14.8; 64-row blocks 14.3 / 18.7 and 17.9 / 18.2, at 120 keys 14.0 / 18.7 and 14.2 / 14.6.
+  const int whole = row_bytes > 256 || block > 64 ? 1 : block == 64 ? 2 : row_bytes <= 128 && dtype != CO_ALIBI_F32 ? 5 : 3;
+  p.cps = chunks <= whole ? chunks : walk(few / units);
   p.splits = (chunks + p.cps - 1) / p.cps;
   p.share = static_cast<int>(std::max<long long>(slots / heads, 1));
   p.planned = static_cast<int>(std::min<long long>({p.splits * static_cast<long long>(kTreeRaggedSplits), chunks, p.share,

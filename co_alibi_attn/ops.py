@@ -77,9 +77,10 @@ if _MISSING is None:
     fwd_qkv = torch.ops.co_alibi.fwd_qkv
     bwd_qkv = torch.ops.co_alibi.bwd_qkv
     decode = torch.ops.co_alibi.decode
-    decode_tree = torch.ops.co_alibi.decode_tree
-    cache_append = torch.ops.co_alibi.cache_append
-    sample = torch.ops.co_alibi.sample
+    # (Naming the overload saves these short calls its look-up on the host.)
+    decode_tree = torch.ops.co_alibi.decode_tree.default
+    cache_append = torch.ops.co_alibi.cache_append.default
+    sample = torch.ops.co_alibi.sample.default
 else:
     fwd = bwd = bwd_dq = fwd_qkv = bwd_qkv = decode = decode_tree = cache_append = sample = _unavailable
 

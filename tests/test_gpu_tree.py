@@ -97,6 +97,10 @@ CASES = [
     (1, 2, 2, 63, [40], 128, 256),
     (1, 32, 1, 2, [130], 64, 64),           # 32 heads a group
     (1, 40, 1, 1, [130], 32, 16),           # more than the single-token decode takes
+    (1, 4, 4, 1, [1500], 64, 64),           # merged from splits at every head dim
+    (3, 6, 2, 5, [900, 640, 0], 32, 32),
+    (2, 4, 2, 7, [70, 1000], 16, 16),
+    (2, 3, 3, 2, [511, 513], 64, 16),       # five chunks and six
 ]
 
 

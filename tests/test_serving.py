@@ -97,7 +97,7 @@ def test_decode_tree_workspace():
     lib = _native.lib()
     size = lambda *a: lib.co_alibi_decode_tree_workspace_bytes(*a)  # noqa: E731
     up = lambda n: -(-n // 256) * 256  # noqa: E731
-    for dtype, B, Hq, Hkv, T, L, D in ((1, 1, 4, 4, 1, 300, 64), (2, 2, 8, 2, 16, 5000, 128), (0, 1, 6, 2, 3, 9000, 32)):
+    for dtype, B, Hq, Hkv, T, L, D in ((1, 1, 4, 4, 1, 900, 64), (2, 2, 8, 2, 16, 5000, 128), (0, 1, 6, 2, 3, 9000, 32)):
         n = size(dtype, B, Hq, Hkv, T, L, D)
         rows = B * Hq * T
         for splits in range(2, 513):
@@ -106,7 +106,7 @@ def test_decode_tree_workspace():
         else:
             raise AssertionError((n, rows))
         assert splits <= -(-L // 64) + 1
-    assert size(1, 1, 4, 4, 1, 0, 64) == 0  # only the new tokens: one split
+    assert size(1, 1, 4, 4, 1, 0, 64) == 0 and size(1, 1, 4, 4, 1, 300, 64) == 0  # few chunks: one split
     for bad in ((1, 0, 4, 4, 1, 9, 64), (1, 1, 2, 4, 1, 9, 64), (1, 1, 4, 4, 0, 9, 64), (1, 1, 4, 4, 1, -1, 64)):
         assert size(*bad) == 0
     need = size(2, 2, 8, 2, 3, 500, 128)
