@@ -784,8 +784,13 @@ hipError_t tree_dispatch_d(const coalibi::TreeArgs& a, int D, hipStream_t st) {
 
 // How a tree decode is split: equal lengths (or short walks) by the bound, into `splits` runs of `cps` chunks; longer walks
 // over a length per sequence by the kernels' plan, into at most `planned` runs per sequence.
-constexpr int kTreePlanWalk = 4;      // chunks per split from which the plan pays
-constexpr int kTreeRaggedSplits = 4;  // times as many splits as by the bound that a longer sequence may get
+//
+// Chunks per split from which the plan pays: 16 sequences of up to 1024 keys (bf16 D 128, walk 2) 22.1 us with it and 21.7
+// without, of up to 2048 (walk 5) 24.4 and 28.4, of up to 8192 53.9 and 68.4, of 96 rows each 74.5 and 105.7.
+constexpr int kTreePlanWalk = 4;
+// How many times the splits by the bound a long sequence may get.  One sequence of 8000 keys among 15 of 500, at most 1 / 2 /
+// 4 / 8 times: 65.5 / 39.1 / 25.9 / 25.1 us; among 31 66.2 / 66.1 / 39.8 / 31.4.  The workspace grows with it.
+constexpr int kTreeRaggedSplits = 4;
 struct TreePlan {
   int chunk, row_blocks, cps, splits, planned, share;
   bool plans;
@@ -797,14 +802,20 @@ TreePlan tree_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, 
   p.row_blocks = (rows + block - 1) / block;
   const int chunks = static_cast<int>((seq_kv + static_cast<long long>(p.chunk) - 1) / p.chunk) + 1;
   const int row_bytes = head_dim * (dtype == CO_ALIBI_F32 ? 4 : 2), cus = device_cus();
-  const int slots = (row_bytes <= 128 ? 3 : row_bytes <= 256 ? 2 : 1) * cus;
+  // Work-groups that run at once, and the splits share one round of them.  1 / 2 / 3 per CU, us, ragged lengths up to 8192:
+  // D 64 (128-byte rows), 16 query rows 44.9 / 34.7 / 33.1 and 128 rows 83 / 67 / 73; D 32, 128 rows 62 at 2 and 52 at 3;
+  // D 128 55.5 / 53.8 / 56.3, 96 rows 92 / 74 / 80; D 256 64.7 / 74.8 / 93.0.
+  const int slots = (row_bytes <= (block <= 64 ? 128 : 64) ? 3 : row_bytes <= 256 ? 2 : 1) * cus;
+  // Equal lengths over few query rows are bound by the chunk's latency and the merge, so that one round of one per CU is
+  // as fast or faster: 16384 keys, 1 / 2 / 3 per CU: D 128 19.6 / 20.8 / 24.2, 64 rows 24.7 / 27.5 / 31.6, fp32 D 64 25.1 /
+  // 27.0 / 28.7; not so D 64 16.6 / 16.2 / 16.5, nor 96 rows 31.0 / 30.6 / 30.7.
   const int few = block <= 64 && row_bytes > 128 ? cus : slots;
   const long long heads = static_cast<long long>(heads_kv) * p.row_blocks, units = batch * heads;
   auto walk = [&](long long n) {  // chunks per split of n splits
     const int most = static_cast<int>(std::min<long long>({std::max(n, 1ll), chunks, coalibi::kMaxTreeSplits}));
     return (chunks + most - 1) / most;
   };
-  // Few chunks go through one work-group, which needs no merge and no workspace: that saves a second launch, 2 us of a
+  // A few chunks go through one work-group, which needs no merge and no workspace: that saves a second launch, 2 us of a
   // captured call and 4 us of host time in an eager one, and costs 1.3 us a chunk at 128-byte rows.  12 heads, one token,
   // us captured / eager, split against whole: 120 keys 10.0 / 17.1 and 8.0 / 13.3, 500 keys (5 chunks) 10.0 / 17.6 and
   // 12.4 / 13.3, 760 keys 10.0 / 18.1 and 15.3 / 15.6.  At 256-byte rows 250 keys (3 chunks) 11.4 / 18.1 and 11.3 / 13.3; in fp32

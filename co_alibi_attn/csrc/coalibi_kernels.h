@@ -376,9 +376,12 @@ struct CachePlace {
 // (rows, nSplits) and pout (rows, nSplits, D), fp32; a sequence with one split has none.
 constexpr int kMaxTreeTokens = 64;   // a node's ancestors are the bits of one 64-bit mask
 constexpr int kMaxTreeSplits = 512;  // merge weights in LDS
-// Query rows (of the G*T of a kv head) per work-group: one, two or four 32-row tiles.
+// Query rows (of the G*T of a kv head) per work-group: one, two or four 32-row tiles, the fewest that hold them all; more
+// rows go by 128.  Blocks of 32 / 64 / 128, us at bf16 D 128: 32 rows over 8 x 4096 keys 35.1 / 37.3 / 41.7, 64 rows over
+// 16384 keys 26.4 / 24.5 / 28.8, 128 rows over 4 x 32768 keys 185 / 150 / 126, 256 rows 322 / 245 / 215.
 constexpr int tree_block_rows(int rows) { return rows <= 32 ? 32 : rows <= 64 ? 64 : 128; }
-// Keys held in LDS, and keys per chunk: one buffer of 128, or two of 64 where four wavefronts share every tile.
+// Keys held in LDS, and keys per chunk: one buffer of 128, or two of 64 where four wavefronts share every tile (96 rows
+// over 16 sequences of up to 8192 keys: 90 us; with one buffer of 128 and its four barriers 123).
 constexpr int kTreeLdsKeys = 128;
 constexpr int tree_chunk_keys(int block_rows) { return block_rows == 128 ? 64 : 128; }
 struct TreeArgs {

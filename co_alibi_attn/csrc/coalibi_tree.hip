@@ -21,6 +21,13 @@
 // one buffer of 128 keys, each tile's next chunk issued as soon as the tile has been read.  LDS rows are not
 // padded: the 16-byte pieces of a row are stored in an order XORed with its index (the DMA lanes fetch them so), which
 // keeps the operand reads off each other's banks and every DMA lane busy.
+//
+// What bounds it, bf16 or fp16 at D 128, captured: 64 query rows over 8192 keys 19.7 us, latency (the merge 3.8 of it,
+// three chunks in a row the rest); 96 rows over 16 sequences of up to 8192 keys 74 us, issue (their 259 MB are 38 us at
+// the read rate of 6.9 TB/s); 256 rows over 131072 keys 187 us, issue (538 MB: 78 us; 137 Gflop of products: 114).
+//   In the 128-row form VALU (two exponentials, a reciprocal and the suffix sums per score) and MFMA of the two wavefronts of
+// a SIMD hardly overlap: 68 % and 31 % of the cycles before the chunks of far keys were left out (217 us -> 187).
+//   Smaller blocks wait rather than issue, and looking for far chunks made them slower (19.7 -> 20.3 us at 64 rows).
 #include <algorithm>
 #include <type_traits>
 
@@ -34,8 +41,13 @@ namespace {
 constexpr int kTreeWaves = 4;
 constexpr int kTreeThreads = 64 * kTreeWaves;
 // O is rescaled when the weights of a lane's keys of a chunk sum to more than this at the running scale: a weight stays
-// far below fp16's 65504.
+// far below fp16's 65504.  (A maximum per chunk in its place: 77 us against 75, 96 rows over 16 sequences of 8192 keys.)
 constexpr float kTreeRescale = 4096.0f;
+
+// A chunk's keys are left out where they all weigh less than 2^-this of the row's sum: 2^17 of them, were there that many
+// at the bound, would be 2^-23 of it.  fp32, the validation mode, keeps the forward's tail-skip bound.
+template <typename T>
+constexpr float kTreeFar = sizeof(T) == 4 ? 64.0f : 40.0f;
 
 // A partial's sum in the newest split where the row's node is absent.
 constexpr float kAbsent = -1.0f;
@@ -513,53 +525,70 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
         carry += sum;
       }
 
-      // a relative to the row's scale, and its weights.
+      // a relative to the row's scale is at most the largest score less cst, and the row's sum at least 1.  A chunk whose keys
+      // all weigh less than 2^-kTreeFar in every row of the wavefront is left out: its weights, and its V (a NaN or an
+      // infinity among the scores or the sigmas keeps it).
       const float mb = m2 == kNegInf ? 0.f : m2;
+      float cst[NTILE];
 #pragma unroll
-      for (int st = 0; st < NTILE; ++st) {
-        const float cst = mb + lam2 * (after + off[st]);
+      for (int st = 0; st < NTILE; ++st) cst[st] = mb + lam2 * (after + off[st]);
+      bool left_out = false;
+      if constexpr (WR == 4) {
+        bool near = fresh || m2 == kNegInf || !(lam2 >= 0.f);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) sacc[st][r] = fmaf(-lam2, loc[st][r], sacc[st][r] - cst);
+        for (int st = 0; st < NTILE; ++st) {
+          float mt = sacc[st][0];
+#pragma unroll
+          for (int r = 1; r < 16; ++r) mt = fmaxf(mt, sacc[st][r]);
+          near = near || !(mt - cst[st] < -kTreeFar<T>) || !(tot[st] >= 0.f);
+        }
+        left_out = !__any(near);
       }
       V8 pb[NTILE][2];
-      auto weights = [&] {
-        float sum_p = 0.f;
+      if (!left_out) {
 #pragma unroll
         for (int st = 0; st < NTILE; ++st)
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            f32x8 p;
+          for (int r = 0; r < 16; ++r) sacc[st][r] = fmaf(-lam2, loc[st][r], sacc[st][r] - cst[st]);
+        auto weights = [&] {
+          float sum_p = 0.f;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              p[e] = fast_exp2(sacc[st][8 * s + e]);
-              sum_p += p[e];  // before the rounding for the product: the LSE is fp32's
+          for (int st = 0; st < NTILE; ++st)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              f32x8 p;
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                p[e] = fast_exp2(sacc[st][8 * s + e]);
+                sum_p += p[e];  // before the rounding for the product: the LSE is fp32's
+              }
+              pb[st][s] = M::pack(p);
             }
-            pb[st][s] = M::pack(p);
-          }
-        return sum_p;
-      };
-      float sum_p = weights();
-      // The scale follows the maximum where the weights' sum says that it has risen far (or has none yet): no maximum is
-      // taken otherwise.
-      if (__any(m2 == kNegInf || sum_p > kTreeRescale)) {
-        float mt = kNegInf;
+          return sum_p;
+        };
+        float sum_p = weights();
+        // The scale follows the maximum where the weights' sum says that it has risen far (or has none yet): no maximum is
+        // taken otherwise.
+        if (__any(m2 == kNegInf || sum_p > kTreeRescale)) {
+          float mt = kNegInf;
 #pragma unroll
-        for (int st = 0; st < NTILE; ++st)
+          for (int st = 0; st < NTILE; ++st)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sacc[st][r]);
-        mt = fmaxf(mt, other_half(mt));
-        const bool need = mt > (m2 == kNegInf ? kNegInf : 0.f);
-        const float delta = need ? mt : 0.f;
-        const float alpha = need ? (m2 == kNegInf ? 0.f : fast_exp2(-delta)) : 1.f;
-        m2 = need ? mb + delta : m2;
-        lsum *= alpha;
+            for (int r = 0; r < 16; ++r) mt = fmaxf(mt, sacc[st][r]);
+          mt = fmaxf(mt, other_half(mt));
+          const bool need = mt > (m2 == kNegInf ? kNegInf : 0.f);
+          const float delta = need ? mt : 0.f;
+          const float alpha = need ? (m2 == kNegInf ? 0.f : fast_exp2(-delta)) : 1.f;
+          m2 = need ? mb + delta : m2;
+          lsum *= alpha;
 #pragma unroll
-        for (int j = 0; j < C::DT; ++j) acc[j] *= alpha;
+          for (int j = 0; j < C::DT; ++j) acc[j] *= alpha;
 #pragma unroll
-        for (int st = 0; st < NTILE; ++st) sacc[st] -= delta;
-        sum_p = weights();
+          for (int st = 0; st < NTILE; ++st) sacc[st] -= delta;
+          sum_p = weights();
+        }
+        lsum += sum_p;
       }
-      lsum += sum_p;
 
       {
         if constexpr (NBUF == 1) {
@@ -593,6 +622,7 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
         }
       }
       // O^T[d][row] += V^T[d][key] P^T[key][row]; keys 8*s + 16*(l/32) + e of each tile, as in pb.
+      if (!left_out)
 #pragma unroll
       for (int st = 0; st < NTILE; ++st)
 #pragma unroll
@@ -843,7 +873,9 @@ hipError_t launch_tree(const TreeArgs& a, hipStream_t stream) {
     e = launch_split<T, D, 4>(a, stream);
   if (e != hipSuccess || a.nSplits == 1) return e;
   const long long rows = (long long)a.B * a.Hq * a.T;
-  if (rows <= 2048)
+  // Four wavefronts a row against one, whole step in us at D 128: 128 rows 31.5 against 33.3, 512 rows 37.0 against 38.7,
+  // 2048 rows 39.0 against 37.1 (and 62.6 against 61.7), 12288 rows 135 against 124.
+  if (rows <= 1024)
     hipLaunchKernelGGL((coalibi_tree_merge_kernel<T, D, 4>), dim3(static_cast<unsigned>(rows)), dim3(kTreeMergeThreads), 0,
                        stream, a);
   else

@@ -169,6 +169,30 @@ def test_tree_ragged_batch(case):
     check(run(*inputs, lens, parents, max_seq_len=max(lens)), want, dtype)
 
 
+@pytest.mark.parametrize("dtype", (BF16, F16, F32), ids=NAME.get)
+def test_old_keys_of_large_scores_count(dtype):
+    """Old keys fade below what a sum shows and are left out of it, but not one whose score makes up for its age."""
+    B, Hq, Hkv, T, L, D = 1, 8, 1, 12, 5000, 128
+    q, k, v, kc, vc, table = make(B, Hq, Hkv, T, [L], D, dtype, 64, seed=31)
+    lam = lam_of(Hq, dtype)
+
+    def want():
+        return oracle.decode_tree(q, k, v, kc, vc, [L], None, table, lam, D ** -0.5)
+
+    plain = want()
+    check(run(q, k, v, kc, vc, table, [L], None), plain, dtype)
+    for row in (700, 3000):  # as much as nodes 0 and 5 of the flattest head, and of the fourth, can ask for
+        for h, t in ((7, 0), (3, 5)):
+            kc[table[0, row // 64], :, row % 64] = (8 * q[0, h, t].float()).to(dtype)
+            planted = want()
+            check(run(q, k, v, kc, vc, table, [L], None), planted, dtype)
+            if h == 7:
+                assert (planted[0][0, h, t] - plain[0][0, h, t]).abs().max() > 0.01  # ten times what roundings may do here
+    kc[table[0, 1], 0, 3, 5] = math.nan  # a key that every row sees
+    o, lse = run(q, k, v, kc, vc, table, [L], None)
+    assert o.isnan().all() and lse.isnan().all()
+
+
 def test_ragged_batch_with_a_page_outside_the_pool():
     B, lens = 16, few_long(16, 2305, 8)
     q, k, v, kc, vc, table = make(B, 8, 8, 2, lens, 128, BF16, 64, seed=8)
