@@ -7,6 +7,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
+#include <limits>
 #include <mutex>
 #include <string>
 #include <utility>
@@ -925,6 +926,9 @@ int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v,
     a.psig = reinterpret_cast<float*>(ws + 2 * stat_bytes);
     a.pout = reinterpret_cast<float*>(ws + 3 * stat_bytes);
   }
+  // 2^17 keys at the 16-bit types' bound, were there so many, would be 2^-23 of the sum; fp32, the validation mode, has the
+  // forward's.  Without the tail skip no key is far.
+  a.far = g_tail_skip.load() == 0 ? std::numeric_limits<float>::infinity() : dtype == CO_ALIBI_F32 ? 64.f : 40.f;
   a.sc2 = sm_scale * coalibi::kLog2eHost;
   hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e;

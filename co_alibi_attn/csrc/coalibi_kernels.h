@@ -410,6 +410,7 @@ struct TreeArgs {
   int cps;         // chunks per split (with a plan the kernels share the chunks out)
   int share;       // the plan's splits of all sequences together, per kv head and row block
   bool plan;       // splits sized by the lengths in seq_lens
+  float far;       // a chunk's keys are left out where they all weigh less than 2^-far of the row's sum
   float sc2;
 };
 

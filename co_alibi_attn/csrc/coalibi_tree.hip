@@ -44,11 +44,6 @@ constexpr int kTreeThreads = 64 * kTreeWaves;
 // far below fp16's 65504.  (A maximum per chunk in its place: 77 us against 75, 96 rows over 16 sequences of 8192 keys.)
 constexpr float kTreeRescale = 4096.0f;
 
-// A chunk's keys are left out where they all weigh less than 2^-this of the row's sum: 2^17 of them, were there that many
-// at the bound, would be 2^-23 of it.  fp32, the validation mode, keeps the forward's tail-skip bound.
-template <typename T>
-constexpr float kTreeFar = sizeof(T) == 4 ? 64.0f : 40.0f;
-
 // A partial's sum in the newest split where the row's node is absent.
 constexpr float kAbsent = -1.0f;
 
@@ -526,7 +521,7 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
       }
 
       // a relative to the row's scale is at most the largest score less cst, and the row's sum at least 1.  A chunk whose keys
-      // all weigh less than 2^-kTreeFar in every row of the wavefront is left out: its weights, and its V (a NaN or an
+      // all weigh less than 2^-a.far in every row of the wavefront is left out: its weights, and its V (a NaN or an
       // infinity among the scores or the sigmas keeps it).
       const float mb = m2 == kNegInf ? 0.f : m2;
       float cst[NTILE];
@@ -534,13 +529,13 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
       for (int st = 0; st < NTILE; ++st) cst[st] = mb + lam2 * (after + off[st]);
       bool left_out = false;
       if constexpr (WR == 4) {
-        bool near = fresh || m2 == kNegInf || !(lam2 >= 0.f);
+        bool near = row_ok && (fresh || m2 == kNegInf || !(lam2 >= 0.f));
 #pragma unroll
         for (int st = 0; st < NTILE; ++st) {
           float mt = sacc[st][0];
 #pragma unroll
           for (int r = 1; r < 16; ++r) mt = fmaxf(mt, sacc[st][r]);
-          near = near || !(mt - cst[st] < -kTreeFar<T>) || !(tot[st] >= 0.f);
+          near = near || (row_ok && (!(mt - cst[st] < -a.far) || !(tot[st] >= 0.f)));
         }
         left_out = !__any(near);
       }

@@ -113,16 +113,17 @@ class CausalCoALiBiAttention(nn.Module):
         return self.proj(y.transpose(1, 2).reshape(B, S, C))
 
     def over_cache(self, x: torch.Tensor, cache: PagedCache, layer: int, parents: torch.Tensor | None,
-                   prefill: bool) -> torch.Tensor:
+                   prefill: bool) -> tuple[torch.Tensor, tuple[torch.Tensor, torch.Tensor]]:
+        """The attention of new tokens (B, T, C) over one layer of the cache, and their (k, v)."""
         B, T, C = x.shape
         qkv = self.qkv(x).view(B, T, 3, self.n_head, self.head_dim)
         q, k, v = (qkv[:, :, i].transpose(1, 2) for i in range(3))
-        cache.new.append((k, v))
         if prefill:
-            return self.proj(co_alibi_attention_qkv(qkv, causal=True, bias_max=self.bias_max).reshape(B, T, C))
-        y = co_alibi_decode_tree(q, k, v, *cache.layers[layer], seq_len=cache.seq_lens, parents=parents,
-                                 block_table=cache.block_table, bias_max=self.bias_max)
-        return self.proj(y.transpose(1, 2).reshape(B, T, C))
+            y = co_alibi_attention_qkv(qkv, causal=True, bias_max=self.bias_max)
+        else:
+            y = co_alibi_decode_tree(q, k, v, *cache.layers[layer], seq_len=cache.seq_lens, parents=parents,
+                                     block_table=cache.block_table, bias_max=self.bias_max).transpose(1, 2)
+        return self.proj(y.reshape(B, T, C)), (k, v)
 
 
 class Block(nn.Module):
@@ -175,9 +176,13 @@ class GPT(nn.Module):
 
     def _over_cache(self, idx: torch.Tensor, cache: PagedCache, parents=None, prefill=False) -> torch.Tensor:
         cache.new = []
+        new: list[tuple[torch.Tensor, torch.Tensor]] = []
         x = self.wte(idx)
         for i, blk in enumerate(self.blocks):
-            x = blk.mlp(x + blk.attn.over_cache(blk.ln1(x), cache, i, parents, prefill))
+            y, kv = blk.attn.over_cache(blk.ln1(x), cache, i, parents, prefill)
+            x = blk.mlp(x + y)
+            new.append(kv)
+        cache.new = new  # all layers' or none
         return self.ln_f(x)
 
     @torch.no_grad()

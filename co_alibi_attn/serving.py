@@ -65,8 +65,8 @@ def co_alibi_decode_tree(q, k, v, k_cache, v_cache, seq_len=None, parents=None, 
     sees the filled rows and its chain of parents up to itself, in that order, so its result is that of
     ``co_alibi_decode`` with the chain appended to the cache.  Any other value makes the token absent and with
     it every token after it: O = 0 and LSE = -inf there (the padding of a batch of trees).  Keys and values
-    that a token does not see do not reach its result, whatever they hold; cached values that weigh less than 2^-40
-    (fp32: 2^-64) of a row's sum may be left out of it.  A sequence whose filled rows
+    that a token does not see do not reach its result, whatever they hold; cached keys that weigh less than 2^-40
+    (fp32: 2^-64) of a row's sum may be left out of it (the library's tail skip).  A sequence whose filled rows
     lie on a page outside the pool gets NaN.
 
     Inference only: no autograd record.  Returns o (B, Hq, T, D) in q.dtype, and with ``return_lse`` also

@@ -234,7 +234,8 @@ int co_alibi_decode_noalloc(int dtype, const void* q, const void* k_cache, const
  * the chain's keys and values appended to the cache.  Filled rows: seq_lens (B int32 on the device) clamped to
  * [0, seq_kv], or NULL for seq_kv (>= 0).  A sequence whose filled rows lie on a page outside the pool gets
  * NaN.  Rows past the filled ones, pages that hold none, and keys and values of tokens outside a token's chain
- * do not reach its result whatever they hold.  Head dims 16 to 256 (256 in fp16 / bf16 only).  strides: those
+ * do not reach its result whatever they hold.  With the tail skip on, cached keys that weigh less than 2^-40
+ * (fp32: 2^-64) of a row's sum may be left out of it.  Head dims 16 to 256 (256 in fp16 / bf16 only).  strides: those
  * of q, k, v, k_cache and v_cache (15 values) or NULL.  workspace holds
  * co_alibi_decode_tree_workspace_bytes(...) bytes (256-byte aligned; may be NULL when that is 0). */
 size_t co_alibi_decode_tree_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,

@@ -217,6 +217,10 @@ def test_a_full_cache_is_refused(models):
     gpu.prefill(idx[:, :14], cache, torch.tensor([10], device=DEV))
     with pytest.raises(ValueError, match="empty cache"):
         gpu.prefill(idx, cache)
+    with pytest.raises(ValueError, match="at most 64 new tokens"):
+        gpu.extend(idx[:, :1].expand(1, 65), cache)
+    with pytest.raises(ValueError, match="no new keys"):  # of a forward that was refused
+        cache.accept()
     gpu.extend(idx[:, :4], cache)  # 10 rows are filled, 14 were bounded
     cache.accept()
     gpu.extend(idx[:, :3], cache)

@@ -8,7 +8,7 @@ import math
 import pytest
 import torch
 
-from co_alibi_attn import co_alibi_attention, co_alibi_cache_append, co_alibi_decode, co_alibi_decode_tree
+from co_alibi_attn import _native, co_alibi_attention, co_alibi_cache_append, co_alibi_decode, co_alibi_decode_tree
 from oracle import co_alibi_ref as ref
 from oracle import serving as oracle
 
@@ -188,6 +188,8 @@ def test_old_keys_of_large_scores_count(dtype):
             check(run(q, k, v, kc, vc, table, [L], None), planted, dtype)
             if h == 7:
                 assert (planted[0][0, h, t] - plain[0][0, h, t]).abs().max() > 0.01  # ten times what roundings may do here
+    with _native.tail_skip(False):
+        check(run(q, k, v, kc, vc, table, [L], None), planted, dtype)
     kc[table[0, 1], 0, 3, 5] = math.nan  # a key that every row sees
     o, lse = run(q, k, v, kc, vc, table, [L], None)
     assert o.isnan().all() and lse.isnan().all()
