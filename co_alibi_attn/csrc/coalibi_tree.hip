@@ -23,8 +23,9 @@
 // keeps the operand reads off each other's banks and every DMA lane busy.
 //
 // What bounds it, bf16 or fp16 at D 128, captured: 64 query rows over 8192 keys 19.7 us, latency (the merge 3.8 of it,
-// three chunks in a row the rest); 96 rows over 16 sequences of up to 8192 keys 74 us, issue (their 259 MB are 38 us at
-// the read rate of 6.9 TB/s); 256 rows over 131072 keys 187 us, issue (538 MB: 78 us; 137 Gflop of products: 114).
+// three chunks in a row the rest); 96 rows over 16 sequences of up to 8192 keys 74 us, its DMA at 4.5 TB/s with issue
+// beside it (their 259 MB are 38 us at the read rate of 6.9 TB/s); 256 rows over 131072 keys 187 to 196 us from box to
+// box, issue (538 MB: 78 us; 137 Gflop of products: 113).
 //   In the 128-row form VALU (two exponentials, a reciprocal and the suffix sums per score) and MFMA of the two wavefronts of
 // a SIMD hardly overlap: 68 % and 31 % of the cycles before the chunks of far keys were left out (217 us -> 187).
 //   Smaller blocks wait rather than issue, and looking for far chunks made them slower (19.7 -> 20.3 us at 64 rows).

@@ -61,7 +61,9 @@ DECODE_KERNELS = ("coalibi_decode_split_kernel", "coalibi_decode_merge_kernel")
 # the forward kernel; per-launch timings of "coalibi_fwd_kernel" through the C ABI include it.
 FORM_KERNELS = ("coalibi_fwd_split_kernel", "coalibi_bwd_dq_split_kernel", "coalibi_bwd_dkdv_key_kernel",
                 "coalibi_bwd_dkdv_f32_kernel")
-NAMED_KERNELS = KERNELS + STORE_KERNELS[2:] + FORM_KERNELS + DECODE_KERNELS + ("coalibi_key_norm_kernel",)
+SERVING_KERNELS = ("coalibi_tree_split_kernel", "coalibi_tree_merge_kernel", "coalibi_append_kernel",
+                   "coalibi_sample_kernel")
+NAMED_KERNELS = KERNELS + STORE_KERNELS[2:] + FORM_KERNELS + DECODE_KERNELS + SERVING_KERNELS + ("coalibi_key_norm_kernel",)
 # The two --pmc passes of the counter summary: at most 8 SQ and 2 GRBM counters each.
 COUNTER_PASSES = (
     ("SQ_INSTS_VALU", "SQ_INSTS_VALU_TRANS_F32", "SQ_INSTS_MFMA", "SQ_INSTS_LDS", "SQ_INSTS_SALU", "SQ_WAVES",
