@@ -11,7 +11,7 @@ import copy
 import pytest
 import torch
 
-from co_alibi_attn import co_alibi_attention, co_alibi_decode_tree, co_alibi_sample
+from co_alibi_attn import co_alibi_attention, co_alibi_cache_append, co_alibi_decode_tree, co_alibi_sample
 from co_alibi_attn.gpt import GPT, GPTConfig, PagedCache
 from oracle import co_alibi_ref as ref
 
@@ -233,3 +233,47 @@ def test_a_full_cache_is_refused(models):
     o = co_alibi_decode_tree(*(torch.zeros(1, 2, 1, 64, device=DEV) for _ in range(3)), *cache.layers[0],
                              seq_len=cache.seq_lens, block_table=cache.block_table)
     assert torch.isfinite(o).all()
+
+
+def step_inputs():
+    gen = torch.Generator(device=DEV).manual_seed(20)
+    n = lambda *s: torch.randn(*s, generator=gen, device=DEV)  # noqa: E731
+    q, k, v = n(2, 4, 3, 64), n(2, 2, 3, 64), n(2, 2, 3, 64)
+    pools = n(9, 2, 16, 64), n(9, 2, 16, 64)
+    table = torch.arange(8, dtype=torch.int32, device=DEV).view(2, 4)
+    lens = torch.tensor([40, 7], dtype=torch.int32, device=DEV)
+    return q, k, v, *pools, table, lens
+
+
+def test_operators_pass_the_dispatcher_checks():
+    q, k, v, kc, vc, table, lens = step_inputs()
+    slopes = torch.tensor([0.5, 0.25, 0.125, 0.0625], device=DEV)
+    parents = torch.tensor([-1, 0, 0], dtype=torch.int32, device=DEV)
+    op = torch.ops.co_alibi
+    for args in ((q, k, v, kc, vc, slopes, lens, parents, table, 64, 0.125, True), (q, k, v, kc, vc, slopes, None, None, table, 30, 0.125, False)):
+        torch.library.opcheck(op.decode_tree.default, args)
+    counts = torch.tensor([3, 1], dtype=torch.int32, device=DEV)
+    for args in ((k, v, kc, vc, lens, None, None, table), (k, v, kc, vc, lens, counts, torch.tensor([[0, 2], [1, 0]], device=DEV), table)):
+        torch.library.opcheck(op.cache_append.default, args)
+    logits, u = torch.randn(3, 500, device=DEV), torch.rand(3, device=DEV)
+    torch.library.opcheck(op.sample.default, (logits, u, None, None, None, None, 0.9, 20, 0.95, 0.0))
+    torch.library.opcheck(op.sample.default, (logits, u, u, None, u, None, 1.0, 0, 1.0, 0.1))
+
+
+def test_a_compiled_step_is_the_eager_one():
+    head = torch.randn(64, 97, device=DEV)
+
+    def step(q, k, v, kc, vc, table, lens, u):
+        o = co_alibi_decode_tree(q, k, v, kc, vc, seq_len=lens, block_table=table)
+        co_alibi_cache_append(k, v, kc, vc, lens, table)
+        more = co_alibi_decode_tree(q, k, v, kc, vc, seq_len=lens + 3, block_table=table)
+        return o, more, co_alibi_sample((o + more).sum((1, 2)) @ head, u, top_p=0.9)
+
+    u = torch.rand(2, device=DEV)
+    a, b = step_inputs(), step_inputs()
+    want = step(*a, u)
+    got = torch.compile(step, fullgraph=True, backend="aot_eager")(*b, u)
+    for x, y in zip(want, got):
+        assert torch.equal(x, y)
+    assert torch.equal(a[3], b[3]) and torch.equal(a[4], b[4])
+    assert not torch.equal(a[3], step_inputs()[3])
