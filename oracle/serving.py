@@ -1,4 +1,4 @@
-"""Plain float64 forms of the serving step's operators (checker only): tree decode, cache append, sampling.
+"""Plain float64 forms of the serving step's operators (for the tests only): tree decode, cache append, sampling.
 
 Written from the definitions, token by token on the CPU; they share no code with the kernels or with the
 attention oracle.
