@@ -85,6 +85,19 @@ def test_cuts_of_many_tokens_and_cuts_together(dtype):
         check(x, u, **kw)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=str)
+def test_many_tokens_close_together(dtype):
+    """Rows whose tokens crowd into few distances, alone, with masked ones and with one far below."""
+    x, u = logits_of(6, 60000, dtype, seed=23, scale=0.05)
+    masked = x.masked_fill(torch.rand(x.shape, generator=torch.Generator().manual_seed(24)) < 0.3, -math.inf)
+    outlier = x.clone()
+    outlier[:, 777] = -30000.0
+    for rows in (x, masked, outlier, x.abs().clamp(max=0.02)):
+        for kw in (dict(), dict(k=20000, p=0.9), dict(p=0.5, t=1.3), dict(t=0.01), dict(k=59999)):
+            print(dtype, kw, flush=True)
+            check(rows, u, **kw)
+
+
 def test_temperatures_and_logits_of_any_size():
     x, u = logits_of(6, 5000, F32, seed=22)
     wide = x * 1e37  # up to about 1e38
