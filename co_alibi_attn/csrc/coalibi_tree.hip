@@ -289,6 +289,7 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
   __shared__ float sSig[2][WK][WR * 32];
   __shared__ float sMax[WK][WR * 32], sSum[WK][WR * 32], sScale[WK][WR * 32];
   __shared__ unsigned long long sBad;  // new keys whose values hold an infinity or a NaN
+  __shared__ bool sLost[kTreeWaves];   // a wavefront found a filled row on no page of the pool
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hl = lane & 31, hh = lane >> 5;
@@ -339,7 +340,8 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
   const unsigned ldsK = lds_address(smem), ldsV = ldsK + kTreeLdsKeys * C::ROWB;
 
   // This wavefront's keys of chunk c: the unit and the row in it of each run of 16.  `lost`: a filled row lies
-  // on no page of the pool (the pages are then read from unit 0 and the results made NaN at the end).
+  // on no page of the pool (such pages are read from unit 0).  A wavefront looks up only the keys it brings in, which every
+  // wavefront's rows take part in: at the end its `lost` makes all rows of the work-group NaN.
   bool lost = false;
   struct Halves {
     int unit[HALVES], row[HALVES];
@@ -671,8 +673,8 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
   }
 
   // The row's sum over both halves, then over the wavefronts of its keys (in one z frame: the split's own keys).
-  float l = lsum + other_half(lsum);
-  if (lost) l = __builtin_nanf("");
+  const float l = lsum + other_half(lsum);
+  if (lane == 0) sLost[wave] = lost;
   const int rl = wr * 32 + hl;
   if (hh == 0) {
     sMax[wk][rl] = m2;
@@ -690,8 +692,11 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
       sScale[w][tid] = f;
       ls += sMax[w][tid] == kNegInf && sSum[w][tid] == 0.f ? 0.f : f * sSum[w][tid];
     }
+    bool any_lost = false;
+#pragma unroll
+    for (int w = 0; w < kTreeWaves; ++w) any_lost |= sLost[w];
     sMax[0][tid] = m;
-    sSum[0][tid] = ls;
+    sSum[0][tid] = any_lost ? __builtin_nanf("") : ls;
   }
   __syncthreads();
   float* const so = reinterpret_cast<float*>(smem) + (size_t)(wk * WR + wr) * 32 * C::LDO;
