@@ -144,7 +144,7 @@ def lib() -> ctypes.CDLL:
 
 class tail_skip:
     """Context manager over the library's tail-skip setting (co_alibi_set_tail_skip): within
-    ``with tail_skip(False):`` every forward processes every key, as the reference does; the
+    ``with tail_skip(False):`` every forward (and ``co_alibi_decode_tree``) processes every key, as the reference does; the
     previous setting comes back on exit."""
 
     def __init__(self, enabled: bool):

@@ -796,17 +796,21 @@ __global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(T
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor(mx, off, 64));
   const float mref = mx == kNegInf ? 0.f : mx;
+  const float cut = __builtin_isinf(a.far) ? 0.f : 0x1p-64f;
   float l = 0.f;
   for (int s = lane; s < n; s += 64) {  // a lane reads back what it wrote itself
-    const float f = fast_exp2(w[s] - mref);
-    w[s] = f;
-    l = fmaf(f, s == lane ? sum0 : psum[s], l);
+    const float f = fast_exp2(w[s] - mref), sum = s == lane ? sum0 : psum[s];
+    // A split's O is not read where its weights' sum, and with it each of its keys' weights, is below 2^-64 of the row's
+    // (which is at least 1 here): on a steep head all but the newest ones.  (The fp32 tail skip's bound; without the tail
+    // skip all are read.  f alone would not do: a key may weigh kTreeRescale times its split's scale.)  The newest split holds
+    // the new keys, which always count.
+    w[s] = s < n - 1 && f * sum < cut ? -1.f : f;
+    l = fmaf(f, sum, l);
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) l += __shfl_xor(l, off, 64);
   wait_lds();  // the weights are read across lanes below (LDS operations of a wavefront complete in order)
 
-  // A split of weight below 2^-64 is not read: on a steep head all but the newest ones.  (The fp32 tail skip's bound.)
   const int sub = lane / LPS, d = (lane % LPS) * 4;
   const float* const po = a.pout + row * a.nSplits * D + d;
   f32x4 acc[4] = {};
@@ -817,8 +821,8 @@ __global__ __launch_bounds__(kTreeMergeThreads) void coalibi_tree_merge_kernel(T
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int at = s - u * STRIDE;
-      f[u] = at >= 0 ? w[at] : 0.f;
-      x[u] = f[u] >= 0x1p-64f || f[u] != f[u] ? *reinterpret_cast<const f32x4*>(po + (size_t)at * D) : f32x4{};
+      f[u] = at >= 0 ? w[at] : -1.f;
+      x[u] = !(f[u] < 0.f) ? *reinterpret_cast<const f32x4*>(po + (size_t)at * D) : f32x4{};  // NaN is read, too
     }
 #pragma unroll
     for (int u = 0; u < 4; ++u) acc[u] += f[u] * x[u];

@@ -66,7 +66,8 @@ size_t co_alibi_stats_numel(int batch, int heads_q, int seq_q, int seq_kv);
  * call of the process: enabled != 0 (the default) leaves out the keys whose softmax weight is
  * provably below 2^-T of their row's total (above), 0 makes the forward process every key, as
  * the reference does (co_alibi_fwd_kernel.py:66-71), with no key-norm launch and no per-tile
- * test.  The backward follows what its forward recorded.  Returns the previous setting.  No
+ * test.  The backward follows what its forward recorded.  co_alibi_decode_tree, too, leaves out
+ * cached keys only while it is on (its bounds are stated there).  Returns the previous setting.  No
  * counterpart in the reference, which processes every key. */
 int co_alibi_set_tail_skip(int enabled);
 int co_alibi_tail_skip(void);
@@ -235,7 +236,7 @@ int co_alibi_decode_noalloc(int dtype, const void* q, const void* k_cache, const
  * [0, seq_kv], or NULL for seq_kv (>= 0).  A sequence whose filled rows lie on a page outside the pool gets
  * NaN.  Rows past the filled ones, pages that hold none, and keys and values of tokens outside a token's chain
  * do not reach its result whatever they hold.  With the tail skip on, cached keys that weigh less than 2^-40
- * (fp32: 2^-64) of a row's sum may be left out of it.  Head dims 16 to 256 (256 in fp16 / bf16 only).  strides: those
+ * (fp32: 2^-64) of a row's sum may be left out of it; with it off every filled row is read.  Head dims 16 to 256 (256 in fp16 / bf16 only).  strides: those
  * of q, k, v, k_cache and v_cache (15 values) or NULL.  workspace holds
  * co_alibi_decode_tree_workspace_bytes(...) bytes (256-byte aligned; may be NULL when that is 0). */
 size_t co_alibi_decode_tree_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,
