@@ -125,9 +125,11 @@ __device__ const double kExp2Table[32] = {
 
 // The weights of one row: 2^(y / 32) with y = (x - max) * 32 log2(e) / T.
 struct Weights {
-  float top, reach;  // the largest logit; logits further than `reach` below it have weight 0
-  double top64, c;   // c = 32 log2(e) / T
-  double one;        // 2^mass_bits
+  float top;          // the largest logit
+  double top64, c;    // c = 32 log2(e) / T
+  double reach;       // logits further than this below the largest have weight 0; fp64, as fp32 holds neither the
+                      // distance of any two logits nor this at every temperature
+  double one;         // 2^mass_bits
   const double* table;  // 2^mass_bits * 2^(i / 32)
 
   // 2^mass_bits * w, before its rounding to an integer: y = i + r with an integer i and |r| <= 1/2, 2^(r/32) by its
@@ -147,7 +149,7 @@ struct Weights {
     // The table's entry times 2^(i >> 5), through its exponent: the result is normal where it is used.
     const u64 e = __builtin_bit_cast(u64, table[i & 31]) + ((u64)(unsigned)((i >> 5) << 20) << 32);
     const double w = p * __builtin_bit_cast(double, e);
-    return x == top ? one : top - x <= reach ? w : 0.0;  // 0 also for -inf, and for what is below a +inf
+    return x == top ? one : d >= -reach ? w : 0.0;  // 0 also for -inf, and for what is below a +inf
   }
   static __device__ __forceinline__ u64 mass(double scaled) {
     return __builtin_bit_cast(u64, scaled + 4503599627370496.0) & 0xfffffffffffffull;  // + 2^52: scaled <= 2^50
@@ -504,7 +506,7 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
     ws.top64 = static_cast<double>(top);
     ws.c = 32.0 * 1.4426950408889634074 / temp;
     ws.one = static_cast<double>(1ull << a.mass_bits);
-    ws.reach = fminf((a.mass_bits + 2) * kLn2 * static_cast<float>(temp), 3.4028234e38f);
+    ws.reach = fmin((a.mass_bits + 2) * static_cast<double>(kLn2) * temp, 0x1p1023);
     ws.table = s.exp2_table;
     const bool cut_k = top_k > 0 && top_k < V, cut_p = top_p < 1.0, cut_m = min_p > 0.0;
     const double min_scaled = min_p * ws.one;
@@ -569,7 +571,8 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
       for (int off = 32; off > 0; off >>= 1) low = fminf(low, __shfl_xor(low, off, 64));
       if (lane == 0) atomicMin(&s.low, key32(low));
       __syncthreads();
-      const float per_bin = (kBins - 1) * 0.9999f / fminf(ws.reach, top - Key<float>::value(s.low));
+      const float span = fminf(static_cast<float>(fmin(ws.reach, 0x1p127)), top - Key<float>::value(s.low));
+      const float per_bin = (kBins - 1) * 0.9999f / span;
       auto bin_of = [&](float x) {
         const float d = x == top ? 0.f : (top - x) * per_bin;
         return d < kBins - 1 ? static_cast<int>(d) : kBins - 1;
