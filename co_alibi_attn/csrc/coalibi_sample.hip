@@ -527,8 +527,10 @@ __global__ __launch_bounds__(kSampleThreads) void coalibi_sample_kernel(SampleAr
       if (cut_k) {
         bound = kth_of_threads(s, mine, top_k);
       } else {
-        // At the border the weights decide, not this rounding (to them what is 2^-54 below 1 is 1).
-        bound = top - (fmaxf(-log2f(static_cast<float>(min_p)), 0.f) * (kLn2 * 1.00001f) + 1e-12f) * static_cast<float>(temp);
+        // At the border the weights decide, not this rounding (to them what is 2^-54 below 1 is 1).  Below 2^-126 of the
+        // largest no weight is left, and the logarithm stays finite; the product with a temperature of any size is fp64's.
+        const float far = fmaxf(-log2f(fmaxf(static_cast<float>(min_p), 0x1p-126f)), 0.f) * (kLn2 * 1.00001f) + 1e-12f;
+        bound = static_cast<float>(ws.top64 - static_cast<double>(far) * temp);
         bound -= 1e-6f * (fabsf(top) + fabsf(bound));
         if (top == __builtin_inff()) bound = top;
       }

@@ -35,3 +35,16 @@ def test_logits_further_apart_than_the_largest_number(dtype):
             for kw in (dict(), dict(k=3), dict(k=900), dict(p=0.7), dict(m=0.3)):
                 print(x.shape, t, kw, flush=True)
                 check(x, U, t=t, **kw)
+
+
+def test_min_p_and_temperature_both_far_below_fp32():
+    gen = torch.Generator().manual_seed(2)
+    x = torch.randn(6, 5000, generator=gen)
+    ties = torch.randint(0, 3, (6, 3000), generator=gen).float()
+    wide = x * 1e37
+    for rows in (x, ties, wide, x * 1e-42, x.to(torch.bfloat16), x[:, :5]):
+        for t in (5e-324, 1e-300, 1e-46, 1e-40, 1e-6, 1.0, 1e300, math.inf):
+            for m in (5e-324, 1e-300, 1e-46, 1e-39, 1e-20):
+                for p in (1.0, 0.6):
+                    print(rows.shape, t, m, p, flush=True)
+                    check(rows, U, t=t, m=m, p=p)
