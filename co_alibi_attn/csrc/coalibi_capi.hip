@@ -796,6 +796,12 @@ struct TreePlan {
   int chunk, row_blocks, cps, splits, planned, share;
   bool plans;
 };
+// Whether the query rows, and the key chunks of all sequences together (of at least 64 keys each, and the new ones), can be
+// counted in 32 bits, as the plan on the host and the kernels do.
+bool tree_countable(int batch, int heads_q, int tokens, int seq_kv) {
+  return static_cast<double>(batch) * heads_q * tokens <= 2.1e9 && static_cast<double>(batch) * (seq_kv / 64 + 2.0) <= 2.1e9;
+}
+// Of shapes that are countable.
 TreePlan tree_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim) {
   const int rows = heads_q / heads_kv * tokens, block = coalibi::tree_block_rows(rows);
   TreePlan p;
@@ -845,7 +851,10 @@ extern "C" {
 
 size_t co_alibi_decode_tree_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,
                                             int head_dim) {
-  if (batch < 1 || heads_kv < 1 || heads_q < heads_kv || tokens < 1 || seq_kv < 0 || head_dim < 1) return 0;
+  if (batch < 1 || heads_kv < 1 || heads_q < 1 || heads_q % heads_kv != 0 || tokens < 1 ||
+      tokens > coalibi::kMaxTreeTokens || seq_kv < 0 || head_dim < 1 || head_dim > 256 ||
+      !tree_countable(batch, heads_q, tokens, seq_kv))
+    return 0;
   const TreePlan plan = tree_plan(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim);
   return tree_workspace(plan, true, batch, heads_q, heads_kv, tokens, head_dim);
 }
@@ -877,9 +886,10 @@ int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v,
       (rc = check_opt_ptr(fn, "lse", lse, 4)))
     return rc;
   if (!std::isfinite(sm_scale)) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": sm_scale must be finite");
+  if (!tree_countable(batch, heads_q, tokens, seq_kv))
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
   const TreePlan plan = tree_plan(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim);
-  if (static_cast<double>(batch) * heads_kv * plan.row_blocks * (plan.planned + 8.0) > 2.1e9 ||
-      static_cast<double>(batch) * heads_q * tokens > 2.1e9)
+  if (static_cast<double>(batch) * heads_kv * plan.row_blocks * (plan.planned + 8.0) > 2.1e9)
     return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
   const size_t need = tree_workspace(plan, seq_lens != nullptr, batch, heads_q, heads_kv, tokens, head_dim);
   if (workspace_bytes < need)

@@ -238,7 +238,8 @@ int co_alibi_decode_noalloc(int dtype, const void* q, const void* k_cache, const
  * do not reach its result whatever they hold.  With the tail skip on, cached keys that weigh less than 2^-40
  * (fp32: 2^-64) of a row's sum may be left out of it; with it off every filled row is read.  Head dims 16 to 256 (256 in fp16 / bf16 only).  strides: those
  * of q, k, v, k_cache and v_cache (15 values) or NULL.  workspace holds
- * co_alibi_decode_tree_workspace_bytes(...) bytes (256-byte aligned; may be NULL when that is 0). */
+ * co_alibi_decode_tree_workspace_bytes(...) bytes (256-byte aligned; may be NULL when that is 0, as it also is for a
+ * shape that the call refuses). */
 size_t co_alibi_decode_tree_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,
                                             int head_dim);
 int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v, const void* k_cache,
