@@ -242,8 +242,9 @@ class GPT(nn.Module):
         node = torch.arange(T, device=idx.device)
         up = parents.long().clamp(0, T - 1)
         ok = (idx == drawn.gather(1, up)) & (parents >= 0) & (parents < node)
-        twin = (parents[:, :, None] == parents[:, None]) & (idx[:, :, None] == idx[:, None]) & (node < node[:, None])
-        ok &= ~twin.any(2)
+        # (Of nodes that are there: one whose parent comes after it is absent.)
+        same = (parents[:, :, None] == parents[:, None]) & (idx[:, :, None] == idx[:, None])
+        ok &= ~(same & (node < node[:, None]) & ok[:, None]).any(2)
         ok[:, 0] = True
         up[:, 0] = 0
         for _ in range(T.bit_length()):  # accepted: so are 1, 2, 4, ... ancestors

@@ -1,0 +1,81 @@
+"""GPT's serving path on the CPU: the four operators it calls are replaced by the oracles, so what is tested is the
+model's own bookkeeping -- trees, rooms, lengths, and tokens that a draw could not give."""
+import pytest
+import torch
+
+from co_alibi_attn import gpt as gpt_module
+from co_alibi_attn.gpt import GPT, GPTConfig, PagedCache
+from oracle import co_alibi_ref as ref
+from oracle import serving as oracle
+
+CFG = GPTConfig(n_layer=2, n_head=2, d_model=32, vocab=29)
+
+
+def attention(q, k, v, causal=True, sm_scale=None, bias_max=8.0):
+    lam = ref.slopes(q.shape[1], bias_max, dtype=q.dtype).float()
+    return ref.forward_autograd(q.float(), k.float(), v.float(), lam, causal=causal, scale=sm_scale).to(q.dtype)
+
+
+def attention_qkv(qkv, causal=True, bias_max=8.0):
+    return attention(*(qkv[:, :, i].transpose(1, 2) for i in range(3)), causal=causal, bias_max=bias_max).transpose(1, 2)
+
+
+def decode_tree(q, k, v, k_cache, v_cache, seq_len=None, parents=None, block_table=None, bias_max=8.0):
+    page, blocks = k_cache.shape[2], block_table.shape[1]
+    lens = seq_len.clamp(0, page * blocks).tolist()
+    lam = ref.slopes(q.shape[1], bias_max, dtype=q.dtype).float()
+    return oracle.decode_tree(q, k, v, k_cache, v_cache, lens, parents, block_table, lam, q.shape[3] ** -0.5)[0].to(q.dtype)
+
+
+def cache_append(k, v, k_cache, v_cache, seq_lens, block_table=None, rows=None, counts=None):
+    for old, new in zip((k_cache, v_cache), oracle.cache_append(k, v, k_cache, v_cache, seq_lens, block_table, rows, counts)):
+        old.copy_(new)
+
+
+def sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+    B = logits.shape[0]
+    return torch.tensor(oracle.sample(logits, uniforms, [temperature] * B, [top_k] * B, [top_p] * B, [min_p] * B))
+
+
+@pytest.fixture()
+def model(monkeypatch):
+    for name, f in (("co_alibi_attention_qkv", attention_qkv), ("co_alibi_decode_tree", decode_tree),
+                    ("co_alibi_cache_append", cache_append), ("co_alibi_sample", sample)):
+        monkeypatch.setattr(gpt_module, name, f)
+    torch.manual_seed(0)
+    return GPT(CFG, attention=attention)
+
+
+def new_cache(batch, capacity=32):
+    return PagedCache(CFG, batch, capacity, torch.float32, "cpu", page_size=16)
+
+
+def start(model, lengths, drawn, capacity=32, seed=1):
+    """Prompts, `drawn` uniform numbers behind each, and the tokens that drawing one by one gives with them."""
+    gen = torch.Generator().manual_seed(seed)
+    idx = torch.randint(0, CFG.vocab, (len(lengths), max(lengths)), generator=gen)
+    u = torch.rand(len(lengths), drawn, generator=gen)
+    return idx, torch.tensor(lengths), u, model.generate(idx, torch.tensor(lengths), u, new_cache(len(lengths), 64))
+
+
+def test_generate_follows_the_full_forward(model):
+    """(That the replacements stand in for the operators.)"""
+    idx, lengths, u, out = start(model, [5, 1], 6)
+    for b in range(2):
+        seq = idx[b, :lengths[b]].tolist()
+        for i in range(6):
+            with torch.no_grad():
+                logits = model(torch.tensor([seq]))[:, -1]
+            assert sample(logits, u[b:b + 1, i]).tolist() == [out[b, i].item()]
+            seq.append(out[b, i].item())
+
+
+def test_an_absent_node_is_no_earlier_twin(model):
+    """Node 1's parent comes after it, so node 1 is absent; node 3 holds the same token behind the same, valid parent."""
+    idx, lengths, u, truth = start(model, [4], 4)
+    parents = torch.tensor([[-1, 2, 0, 2]])
+    depth = torch.tensor([0, 2, 1, 2])
+    cache = new_cache(1)
+    model.prefill(idx, cache, lengths)
+    rows, counts, after = model.speculate(truth[:, depth], parents, u[:, 1:][:, depth], cache)
+    assert counts.tolist() == [3] and rows[0, :3].tolist() == [0, 2, 3] and after.tolist() == truth[:, 3].tolist()
