@@ -233,10 +233,11 @@ class GPT(nn.Module):
         others are drafts.  Behind every node one token is drawn with that node's number of ``uniforms`` (B, T).  A
         draft is accepted when its parent is and it is the token drawn there (the first of equal ones), so what
         is accepted, idx[b, rows[b, 1:counts[b]]], and the next token, drawn behind it, are what drawing token by token
-        gives with those numbers.  The cache keeps the accepted rows.
+        gives with those numbers.  The cache keeps the accepted rows; of a path that it has no room for, as many as fit are
+        accepted (node 0 has to fit: ValueError).
         """
         B, T = idx.shape
-        cache.room_for(T)
+        cache.room_for(1)
         logits = self.extend(idx, cache, parents)
         drawn = co_alibi_sample(logits.reshape(B * T, -1), uniforms.reshape(B * T), **sampling).view(B, T)
         node = torch.arange(T, device=idx.device)
@@ -250,10 +251,11 @@ class GPT(nn.Module):
         for _ in range(T.bit_length()):  # accepted: so are 1, 2, 4, ... ancestors
             ok &= ok.gather(1, up)
             up = up.gather(1, up)
-        counts = ok.sum(1, dtype=torch.int32)
+        # What is accepted is one path, in the nodes' order: what fits is its beginning.
+        counts = torch.minimum(ok.sum(1, dtype=torch.int32), cache.capacity - cache.seq_lens)
         rows = torch.where(ok, node, T).sort(1).values.int()
         cache.accept(rows, counts)
-        last = rows.gather(1, counts[:, None].long() - 1).long()
+        last = rows.gather(1, counts[:, None].long().clamp(min=1) - 1).long()
         return rows, counts, drawn.gather(1, last)[:, 0]
 
     def n_params(self) -> int:

@@ -79,3 +79,21 @@ def test_an_absent_node_is_no_earlier_twin(model):
     model.prefill(idx, cache, lengths)
     rows, counts, after = model.speculate(truth[:, depth], parents, u[:, 1:][:, depth], cache)
     assert counts.tolist() == [3] and rows[0, :3].tolist() == [0, 2, 3] and after.tolist() == truth[:, 3].tolist()
+
+
+def test_the_last_rows_of_a_cache_take_the_path_that_fits(model):
+    """Room for fewer rows than the tree has nodes: what fits of the accepted path is kept, the next token is drawn behind it."""
+    idx, lengths, u, truth = start(model, [29, 30, 31], 6)
+    parents = torch.tensor([-1, 0, 0, 2, 3, 4]).expand(3, 6).contiguous()
+    depth = torch.tensor([0, 1, 1, 2, 3, 4])
+    tok = truth[:, depth].clone()
+    tok[:, 1] = (tok[:, 1] + 1) % CFG.vocab
+    cache = new_cache(3)
+    model.prefill(idx, cache, lengths)
+    rows, counts, after = model.speculate(tok, parents, u[:, 1:][:, depth], cache)
+    path = [0, 2, 3, 4, 5]
+    assert counts.tolist() == [3, 2, 1] and cache.seq_lens.tolist() == [32, 32, 32]
+    for b, n in enumerate((3, 2, 1)):
+        assert rows[b, :n].tolist() == path[:n] and after[b] == truth[b, n]
+    with pytest.raises(ValueError, match="do not fit"):
+        model.speculate(tok, parents, u[:, 1:][:, depth], cache)
