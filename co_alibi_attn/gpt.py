@@ -177,7 +177,7 @@ class GPT(nn.Module):
     def _over_cache(self, idx: torch.Tensor, cache: PagedCache, parents=None, prefill=False) -> torch.Tensor:
         cache.new = []
         new: list[tuple[torch.Tensor, torch.Tensor]] = []
-        x = self.wte(idx)
+        x = self.wte(idx.clamp(min=0))  # -1, co_alibi_sample's for a row without a token, is no row of the embedding
         for i, blk in enumerate(self.blocks):
             y, kv = blk.attn.over_cache(blk.ln1(x), cache, i, parents, prefill)
             x = blk.mlp(x + y)
@@ -213,7 +213,8 @@ class GPT(nn.Module):
                  **sampling) -> torch.Tensor:
         """Tokens (B, n) that follow the prompts (as for ``prefill``), one per uniform number of ``uniforms`` (B, n).
 
-        ``sampling``: the settings of ``co_alibi_sample``.  The last token is not in the cache.
+        ``sampling``: the settings of ``co_alibi_sample``.  The last token is not in the cache.  A sequence for which no
+        token can be drawn (logits with a NaN) has -1 there and from there on.
         """
         logits = self.prefill(idx, cache, lengths)
         out = torch.empty(uniforms.shape, dtype=torch.long, device=idx.device)
@@ -223,6 +224,8 @@ class GPT(nn.Module):
                 logits = self.extend(out[:, i - 1:i], cache)[:, 0]
                 cache.accept()
             out[:, i] = co_alibi_sample(logits, uniforms[:, i], **sampling)
+            if i > 0:
+                out[:, i].masked_fill_(out[:, i - 1] < 0, -1)
         return out
 
     @torch.no_grad()

@@ -97,3 +97,31 @@ def test_the_last_rows_of_a_cache_take_the_path_that_fits(model):
         assert rows[b, :n].tolist() == path[:n] and after[b] == truth[b, n]
     with pytest.raises(ValueError, match="do not fit"):
         model.speculate(tok, parents, u[:, 1:][:, depth], cache)
+
+
+def test_a_row_without_a_token_stays_without_one(model, monkeypatch):
+    """-1 (a row of NaN, say) is no row of the embedding; what such a sequence would go on with is -1, too."""
+    idx, lengths, u, truth = start(model, [3, 4], 5)
+    calls = []
+
+    def failing(logits, uniforms, **kw):
+        out = sample(logits, uniforms, **kw)
+        calls.append(0)
+        if len(calls) == 2:
+            out[1] = -1
+        return out
+
+    monkeypatch.setattr(gpt_module, "co_alibi_sample", failing)
+    out = model.generate(idx, lengths, u, new_cache(2))
+    assert out[0].tolist() == truth[0].tolist()
+    assert out[1].tolist() == truth[1, :1].tolist() + [-1] * 4
+
+
+def test_tokens_below_0_are_read_as_0(model):
+    """What a caller feeds back after such a draw stays inside the embedding."""
+    cache = new_cache(2)
+    idx = torch.tensor([[3, 4], [5, 6]])
+    assert torch.equal(model.prefill(torch.tensor([[3, 4], [-1, 6]]), cache)[0], model.prefill(idx, new_cache(2))[0])
+    got = model.extend(torch.tensor([[7], [-1]]), cache)
+    want = model.extend(torch.tensor([[7], [0]]), cache)
+    assert torch.equal(got, want) and torch.isfinite(got).all()
