@@ -189,12 +189,16 @@ class GPT(nn.Module):
     def prefill(self, idx: torch.Tensor, cache: PagedCache, lengths: torch.Tensor | None = None) -> torch.Tensor:
         """Puts prompts (B, S) into an empty cache; returns the logits (B, vocab) behind each one's last token.
 
-        ``lengths``: integer tensor (B,) with values in [1, S]: sequence b is idx[b, :lengths[b]], the rest padding.
+        ``lengths``: integer tensor (B,) with values in [1, S], others are clamped: sequence b is idx[b, :lengths[b]], the
+        rest padding.
         """
         if cache.bound != 0:
             raise ValueError("prefill needs an empty cache")
         B, S = idx.shape
+        if S < 1:
+            raise ValueError("a prompt needs at least one token")
         cache.room_for(S)
+        lengths = None if lengths is None else lengths.clamp(1, S)
         h = self._over_cache(idx, cache, prefill=True)
         cache.accept(counts=lengths)
         h = h[:, -1] if lengths is None else h[torch.arange(B, device=h.device), lengths.long() - 1]

@@ -125,3 +125,13 @@ def test_tokens_below_0_are_read_as_0(model):
     got = model.extend(torch.tensor([[7], [-1]]), cache)
     want = model.extend(torch.tensor([[7], [0]]), cache)
     assert torch.equal(got, want) and torch.isfinite(got).all()
+
+
+def test_prompt_lengths_outside_the_prompts_are_clamped(model):
+    idx = torch.randint(0, CFG.vocab, (3, 6), generator=torch.Generator().manual_seed(3))
+    cache, want_cache = new_cache(3), new_cache(3)
+    got = model.prefill(idx, cache, torch.tensor([0, 9, 1 << 40]))
+    want = model.prefill(idx, want_cache, torch.tensor([1, 6, 6]))
+    assert torch.equal(got, want) and cache.seq_lens.tolist() == want_cache.seq_lens.tolist() == [1, 6, 6]
+    with pytest.raises(ValueError, match="at least one token"):
+        model.prefill(idx[:, :0], new_cache(3), torch.tensor([1, 1, 1]))
