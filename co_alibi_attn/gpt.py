@@ -50,6 +50,10 @@ class PagedCache:
     ``capacity`` rows per sequence, all empty at first.  ``dtype`` is the one the model's projections have (the
     weights' type, or autocast's).  A forward over the cache leaves its new keys and values in ``new``, one
     (k, v) per layer; ``accept`` writes them.
+
+    A step with ``accept`` in it may be captured and replayed.  A replay cannot raise: rows without room are dropped
+    and the lengths stay at the capacity.  The host sees no replay, so that from the capture on ``room_for`` reads the lengths
+    from the device (it waits for them): call it between replays to be told of a cache that fills up.
     """
 
     def __init__(self, cfg: GPTConfig, batch: int, capacity: int, dtype: torch.dtype = torch.bfloat16,
@@ -61,12 +65,19 @@ class PagedCache:
                        for _ in range(cfg.n_layer)]
         self.block_table = torch.arange(batch * blocks, dtype=torch.int32, device=device).view(batch, blocks)
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
-        self.bound = 0  # no sequence is longer; known without reading the device
+        self.bound = 0  # no sequence is longer; known without reading the device, but for replays of a captured accept
+        self.captured = False
         self.new: list[tuple[torch.Tensor, torch.Tensor]] = []
 
+    def _capturing(self) -> bool:
+        return self.seq_lens.is_cuda and torch.cuda.is_current_stream_capturing()
+
     def room_for(self, tokens: int) -> None:
-        """Raises ValueError where a sequence has no room for this many more rows."""
-        if self.bound + tokens > self.capacity:  # the bound counts every row as accepted: look before refusing
+        """Raises ValueError where a sequence has no room for this many more rows (not in a capture: see above)."""
+        if self._capturing():
+            return
+        # The bound counts every row as accepted, and no replayed one: look before refusing, or before relying on it.
+        if self.captured or self.bound + tokens > self.capacity:
             self.bound = int(self.seq_lens.max())
         if self.bound + tokens > self.capacity:
             raise ValueError(f"{tokens} more rows behind {self.bound} do not fit a cache of {self.capacity}")
@@ -74,7 +85,7 @@ class PagedCache:
     def accept(self, rows: torch.Tensor | None = None, counts: torch.Tensor | None = None) -> None:
         """Keeps the last forward's new rows: all, the first counts[b], or the rows[b, :counts[b]] (a path of a tree).
 
-        All rows have to fit (ValueError); of ``counts``, which are on the device, what fits is kept.
+        All rows have to fit (ValueError, but in a capture); of ``counts``, which are on the device, what fits is kept.
         """
         if not self.new:
             raise ValueError("no new keys and values: run a forward over this cache first")
@@ -83,10 +94,14 @@ class PagedCache:
             self.room_for(n)
         for (k_cache, v_cache), (k, v) in zip(self.layers, self.new):
             co_alibi_cache_append(k, v, k_cache, v_cache, self.seq_lens, self.block_table, rows=rows, counts=counts)
-        if counts is None:
-            self.seq_lens += n
-        else:
+        if self._capturing():
+            self.captured = True
+        if counts is not None:
             self.seq_lens += torch.minimum(counts.clamp(0, n), self.capacity - self.seq_lens)
+        elif self.captured:
+            self.seq_lens.add_(n).clamp_(max=self.capacity)
+        else:
+            self.seq_lens += n
         self.bound = min(self.bound + n, self.capacity)
         self.new = []
 
@@ -192,11 +207,12 @@ class GPT(nn.Module):
         ``lengths``: integer tensor (B,) with values in [1, S], others are clamped: sequence b is idx[b, :lengths[b]], the
         rest padding.
         """
-        if cache.bound != 0:
-            raise ValueError("prefill needs an empty cache")
         B, S = idx.shape
         if S < 1:
             raise ValueError("a prompt needs at least one token")
+        cache.room_for(0)  # the bound, where replays have moved the lengths
+        if cache.bound != 0:
+            raise ValueError("prefill needs an empty cache")
         cache.room_for(S)
         lengths = None if lengths is None else lengths.clamp(1, S)
         h = self._over_cache(idx, cache, prefill=True)

@@ -135,3 +135,35 @@ def test_prompt_lengths_outside_the_prompts_are_clamped(model):
     assert torch.equal(got, want) and cache.seq_lens.tolist() == want_cache.seq_lens.tolist() == [1, 6, 6]
     with pytest.raises(ValueError, match="at least one token"):
         model.prefill(idx[:, :0], new_cache(3), torch.tensor([1, 1, 1]))
+
+
+def test_replays_of_a_captured_step_are_counted(model, monkeypatch):
+    """A replayed accept moves the lengths without the host: from the capture on the room is read from the device, and a
+    replay that finds none leaves the lengths at the capacity."""
+    cache = new_cache(2)
+    model.prefill(torch.tensor([[1, 2, 3], [4, 5, 6]]), cache)
+    tok = torch.tensor([[7], [8]])
+
+    def step():
+        model.extend(tok, cache)
+        cache.accept()
+
+    monkeypatch.setattr(PagedCache, "_capturing", lambda self: True, raising=False)
+    step()  # stands for the capture, which runs the host's part once ...
+    for _ in range(28):  # ... and for the replays, of which the host sees nothing
+        bound = cache.bound
+        step()
+        cache.bound = bound
+    assert cache.seq_lens.tolist() == [32, 32]
+    step()
+    assert cache.seq_lens.tolist() == [32, 32]
+    monkeypatch.undo()
+    for name, f in (("co_alibi_decode_tree", decode_tree), ("co_alibi_cache_append", cache_append)):
+        monkeypatch.setattr(gpt_module, name, f)
+    with pytest.raises(ValueError, match="1 more rows behind 32 do not fit"):
+        step()
+    with pytest.raises(ValueError, match="empty cache"):
+        model.prefill(torch.tensor([[1], [2]]), cache)
+    cache.seq_lens.zero_()
+    cache.room_for(32)
+    assert cache.bound == 0
