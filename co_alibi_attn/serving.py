@@ -167,5 +167,8 @@ def co_alibi_sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p
     k, k_all = _setting("top_k", top_k, 0, math.inf)
     p, p_all = _setting("top_p", top_p, 0.0, 1.0)
     m, m_all = _setting("min_p", min_p, 0.0, 1.0)
-    return ops.sample(_detached(logits), _detached(uniforms), t, k, p, m, float(t_all), int(min(k_all, _native.MAX_VOCAB)),
+    k_all = min(k_all, _native.MAX_VOCAB)
+    if k_all != int(k_all):
+        raise ValueError(f"top_k must be a whole number, got {k_all}")
+    return ops.sample(_detached(logits), _detached(uniforms), t, k, p, m, float(t_all), int(k_all),
                       float(p_all), float(m_all))
