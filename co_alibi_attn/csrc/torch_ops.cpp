@@ -439,9 +439,10 @@ std::tuple<Tensor, Tensor> decode_tree_hip(const Tensor& q_in, const Tensor& k_i
   Tensor lse = with_lse ? at::empty({batch, heads_q, tokens}, f32) : empty_stats(q_in);
   if (q_in.numel() == 0) return {o, lse};
   const Tensor q = in_place(q_in), k = in_place(k_in), v = in_place(v_in);
-  // A pool without rows is never read; the launch wants an address all the same.
-  const Tensor kc = k_cache.numel() != 0 ? k_cache : k, vc = v_cache.numel() != 0 ? v_cache : v;
-  TORCH_CHECK_VALUE(k_cache.numel() != 0 || max_seq_len == 0, fn, ": the caches hold no rows");
+  // A pool without rows, or behind a table without blocks, is never read; the launch wants an address all the same.
+  const bool none = k_cache.numel() == 0 || c.capacity == 0;
+  const Tensor kc = none ? k : k_cache, vc = none ? v : v_cache;
+  TORCH_CHECK_VALUE(!none || max_seq_len == 0, fn, ": the caches hold no rows");
   const Tensor sl = slopes_f32(slopes, q);
   const size_t ws_bytes = co_alibi_decode_tree_workspace_bytes(code, as_int(fn, "batch", batch), as_int(fn, "heads", heads_q),
                                                                as_int(fn, "heads", heads_kv), as_int(fn, "tokens", tokens),
@@ -450,7 +451,6 @@ std::tuple<Tensor, Tensor> decode_tree_hip(const Tensor& q_in, const Tensor& k_i
   Tensor ws;
   if (ws_bytes != 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
   const auto strides = all_strides<5>({q, k, v, kc, vc});
-  const bool none = k_cache.numel() == 0;
   check(co_alibi_decode_tree(code, q.data_ptr(), k.data_ptr(), v.data_ptr(), kc.data_ptr(), vc.data_ptr(), strides.data(),
                              sl.data_ptr<float>(), data_or_null(lens), data_or_null(par),
                              par.defined() && par.dim() == 2 ? 1 : 0, none ? nullptr : data_or_null(c.table),
@@ -490,7 +490,7 @@ void cache_append_hip(const Tensor& k_in, const Tensor& v_in, const Tensor& k_ca
     idx = index_i32(*rows, k_in);
     new_rows = idx.size(1);
   }
-  if (k_in.numel() == 0 || new_rows == 0 || k_cache.numel() == 0) return;
+  if (k_in.numel() == 0 || new_rows == 0 || k_cache.numel() == 0 || c.capacity == 0) return;
   const Tensor k = in_place(k_in), v = in_place(v_in);
   const auto strides = all_strides<4>({k, v, k_cache, v_cache});
   check(co_alibi_cache_append(code, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), strides.data(),
