@@ -13,9 +13,10 @@
 // fp32 exponentials a border between 50304 tokens would move past the uniform number in one draw of about a
 // thousand.
 //
-// One work-group per row, passes over it from L2 after the first.  What bounds it: 1 row of 50304 fp32 with top-k 14.9 us, the
-// latency of two passes and of the steps between; 64 rows with top-p (bf16) 16.7 us where top-k leaves a list and 40 us by the
-// histogram, the fp64 weights of a row on one CU; 256 rows of 131071 (134 MB, 26 us at a copy's rate) 68 us, the same.
+// One work-group per row, passes over it from L2 after the first.  What bounds it, captured: 1 row of 50304 fp32 with top-k
+// 15.2 us, the latency of two passes and of the steps between; 64 rows (bf16) 16.8 us where top-k leaves a list.  By the
+// histogram a row's fp64 weights and LDS atomics on one CU, whatever the batch: 1 row 36 us, 64 rows 40, 64 rows of 131072 fp32
+// 79, 256 of them 102 (134 MB, 26 us at a copy's rate); with min-p, whose list saves the histogram, 256 rows of 131071 69.
 //   1. the largest logit;
 //   2. short lists: where top-k (or min-p) leaves few tokens, those above a bound are gathered in LDS -- for top-k the
 //      k-th largest of the threads' own maxima, below which no token of the first k lies -- and all positions are

@@ -22,12 +22,14 @@
 // padded: the 16-byte pieces of a row are stored in an order XORed with its index (the DMA lanes fetch them so), which
 // keeps the operand reads off each other's banks and every DMA lane busy.
 //
-// What bounds it, bf16 or fp16 at D 128, captured: 64 query rows over 8192 keys 19.7 us, latency (the merge 3.8 of it,
-// three chunks in a row the rest); 96 rows over 16 sequences of up to 8192 keys 74 us, its DMA at 4.5 TB/s with issue
-// beside it (their 259 MB are 38 us at the read rate of 6.9 TB/s); 256 rows over 131072 keys 187 to 196 us from box to
-// box, issue (538 MB: 78 us; 137 Gflop of products: 113).
-//   In the 128-row form VALU (two exponentials, a reciprocal and the suffix sums per score) and MFMA of the two wavefronts of
-// a SIMD hardly overlap: 68 % and 31 % of the cycles before the chunks of far keys were left out (217 us -> 187).
+// What bounds it, bf16 or fp16 at D 128, captured: 64 query rows over 8192 keys 19.5 us, latency (the merge 4 of it,
+// three chunks in a row the rest; VALU issues in 11 % of the cycles, MFMA in 4 %); 96 rows over 16 sequences of up to 8192
+// keys 75 us, of which the split 68 (265 MB fetched at 3.9 TB/s, VALU 35 %, MFMA 13 %; 259 MB are 38 us at the read rate of 6.9
+// TB/s); 256 rows over 131072 keys 191 to 197 us from box to box (VALU 46 %, MFMA 20 %, 3.0 TB/s; 538 MB are 78 us, 137 Gflop
+// of products 113).
+//   In the 128-row form nothing is saturated: a wavefront's products, two exponentials, a reciprocal and suffix sums per
+// score follow one another behind one barrier per 64 keys, and the two wavefronts of a SIMD run in step.  Leaving out the
+// chunks of far keys took 217 us to 187.
 //   Smaller blocks wait rather than issue, and looking for far chunks made them slower (19.7 -> 20.3 us at 64 rows).
 #include <algorithm>
 #include <type_traits>

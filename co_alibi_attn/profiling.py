@@ -435,7 +435,7 @@ def _mode_split(trace_rows):
 
 
 def cmd_stats(args) -> None:
-    lines = [f"# rocprofv3 kernel statistics: {args.title}", "", "Command (R is the repository root on the GPU box):", "",
+    lines = [f"# rocprofv3 kernel statistics: {args.title}", "", "Command (R is the repository root):", "",
              "```", args.command, "```", "",
              "The summary is written by `python3 co_alibi_attn/profiling.py stats <rocprofv3 output dir>`.", ""]
     traces = glob.glob(os.path.join(args.dir, "**", "*kernel_trace.csv"), recursive=True)
@@ -478,7 +478,7 @@ def _per_dispatch(directory: str, counter: str):
 
 
 def cmd_traffic(args) -> None:
-    lines = [f"# HBM traffic per launch: {args.title}", "", "Commands (R is the repository root on the GPU box):", "",
+    lines = [f"# HBM traffic per launch: {args.title}", "", "Commands (R is the repository root):", "",
              "```", args.command, "```", "",
              f"Each counter is read in KiB per dispatch and scaled by the factor that makes the calibration copy "
              f"(a {CALIBRATION_BYTES >> 20} MiB device-to-device copy, `__amd_rocclr_copyBuffer`, the copy "
@@ -561,7 +561,7 @@ def cmd_counters(args) -> None:
         with open(args.issued) as fh:
             issued = json.load(fh)["k16_per_launch"]
     simds = 4 * MI355X_CUS
-    lines = [f"# Shader counters per launch: {args.title}", "", "Commands (R is the repository root on the GPU box):",
+    lines = [f"# Shader counters per launch: {args.title}", "", "Commands (R is the repository root):",
              "", "```", args.command, "```", "",
              "The summary is written by `python3 co_alibi_attn/profiling.py counters <pass dirs>`. Definitions "
              "(MI355X: 256 CUs = 1024 SIMDs, 8 XCDs; T = GRBM_GUI_ACTIVE / 8, the active cycles of a dispatch):",

@@ -146,11 +146,12 @@ def co_alibi_sample(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p
     and including which more than uniform times the kept weight lies.  ``temperature`` 0 takes the first token
     (the largest logit of the lowest index).
 
-    Each setting is a number or a tensor (B,) with one value per row (top_k integer, the others floating); values
-    on the device cannot be checked: temperatures <= 0 or NaN take the first token, a top_k <= 0, a top_p >= 1 or NaN
+    Each setting is a number or a tensor (B,) with one value per row (top_k integer, the others floating and taken as
+    float32); values on the device cannot be checked: temperatures <= 0 or NaN take the first token, a top_k <= 0, a top_p >= 1 or NaN
     and a min_p <= 0 or NaN keep all, a top_p <= 0 and a min_p > 1 the first only, uniforms outside [0, 1) are
     taken as 0 or as the last kept token.  A row with a NaN, or with no logit above -inf, gives -1; of several
-    +inf logits all have weight 1 and every other token 0.
+    +inf logits all have weight 1 and every other token 0.  Weights below 2^-51 of the largest
+    (2^-43 at 2^20 tokens) count as 0.
 
     logits: float32, float16 or bfloat16; uniforms: (B,) float32 or float64.  Returns int64 tokens (B,).  The
     weights are summed exactly, so the same inputs always give the same tokens.
