@@ -244,9 +244,7 @@ class GPT(nn.Module):
                 logits = self.extend(out[:, i - 1:i], cache)[:, 0]
                 cache.accept()
             out[:, i] = co_alibi_sample(logits, uniforms[:, i], **sampling)
-            if i > 0:
-                out[:, i].masked_fill_(out[:, i - 1] < 0, -1)
-        return out
+        return out.masked_fill_((out < 0).cumsum(1) > 0, -1)
 
     @torch.no_grad()
     def speculate(self, idx: torch.Tensor, parents: torch.Tensor, uniforms: torch.Tensor, cache: PagedCache, **sampling):
