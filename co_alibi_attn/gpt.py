@@ -263,7 +263,7 @@ class GPT(nn.Module):
         drawn = co_alibi_sample(logits.reshape(B * T, -1), uniforms.reshape(B * T), **sampling).view(B, T)
         node = torch.arange(T, device=idx.device)
         up = parents.long().clamp(0, T - 1)
-        ok = (idx == drawn.gather(1, up)) & (parents >= 0) & (parents < node)
+        ok = (idx == drawn.gather(1, up)) & (idx >= 0) & (parents >= 0) & (parents < node)
         # (Of nodes that are there: one whose parent comes after it is absent.)
         same = (parents[:, :, None] == parents[:, None]) & (idx[:, :, None] == idx[:, None])
         ok &= ~(same & (node < node[:, None]) & ok[:, None]).any(2)

@@ -167,3 +167,13 @@ def test_replays_of_a_captured_step_are_counted(model, monkeypatch):
     cache.seq_lens.zero_()
     cache.room_for(32)
     assert cache.bound == 0
+
+
+def test_no_draft_is_accepted_where_no_token_was_drawn(model, monkeypatch):
+    """A draft of -1 behind a node whose draw gave -1 is no token that was drawn."""
+    idx, lengths, u, truth = start(model, [3], 2)
+    monkeypatch.setattr(gpt_module, "co_alibi_sample", lambda logits, uniforms, **kw: torch.full((logits.shape[0],), -1))
+    cache = new_cache(1)
+    model.prefill(idx, cache, lengths)
+    rows, counts, after = model.speculate(torch.tensor([[truth[0, 0], -1]]), torch.tensor([[-1, 0]]), u, cache)
+    assert counts.tolist() == [1] and rows[0, 0] == 0 and after.tolist() == [-1]
