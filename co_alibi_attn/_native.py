@@ -16,6 +16,11 @@ LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "lib
 # Most new tokens per sequence of co_alibi_decode_tree, and most logits per row of co_alibi_sample.
 MAX_TREE_TOKENS = 64
 MAX_VOCAB = 1 << 20
+# Most beams of co_alibi_beam_select and co_alibi_cache_reorder.
+MAX_BEAMS = 64
+# Rows of an 8-bit cache under one scale, and its formats.
+SCALE_ROWS = 16
+FORMAT_CODES = {torch.float8_e4m3fn: 0, torch.int8: 1}
 
 DTYPE_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 SUPPORTED_HEAD_DIMS = (16, 32, 64, 128, 256)
@@ -49,6 +54,13 @@ EXPORTS = (
     "co_alibi_decode_tree",
     "co_alibi_cache_append",
     "co_alibi_sample",
+    "co_alibi_cache_append_8bit",
+    "co_alibi_cache_read_8bit",
+    "co_alibi_decode_tree_8bit_workspace_bytes",
+    "co_alibi_decode_tree_8bit",
+    "co_alibi_beam_select_workspace_bytes",
+    "co_alibi_beam_select",
+    "co_alibi_cache_reorder",
     "co_alibi_probe_mfma",
     "co_alibi_last_error",
     "co_alibi_abi_version",
@@ -59,6 +71,7 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 _Z = ctypes.c_size_t
 _L = ctypes.POINTER(ctypes.c_longlong)
+_PP = ctypes.POINTER(ctypes.c_void_p)
 _LL = ctypes.c_longlong
 _D = ctypes.c_double
 
@@ -106,6 +119,23 @@ _SIGNATURES = {
         [_I, _P, _P, _P, _P, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
     ),
     "co_alibi_sample": (_I, [_I, _P, _LL, _P, _I, _P, _P, _P, _P, _D, _I, _D, _D, _P, _I, _I, _P]),
+    "co_alibi_cache_append_8bit": (
+        _I,
+        [_I, _I, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P, _P, _I, _P, _I, _I, _I, _I, _I, _I, _I, _P],
+    ),
+    "co_alibi_cache_read_8bit": (
+        _I,
+        [_I, _I, _P, _P, _P, _P, _L, _L, _P, _P, _I, _P, _I, _I, _I, _P, _P, _I, _I, _I, _P],
+    ),
+    "co_alibi_decode_tree_8bit_workspace_bytes": (_Z, [_I] * 7),
+    "co_alibi_decode_tree_8bit": (
+        _I,
+        [_I, _I, _P, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P, _P, _I, _P, _I, _I, _I, _P, _P, _P, _Z, _I, _I, _I, _I, _I, _I,
+         _F, _P],
+    ),
+    "co_alibi_beam_select_workspace_bytes": (_Z, [_I] * 4),
+    "co_alibi_beam_select": (_I, [_I, _P, _L, _P, _P, _I, _P, _P, _P, _P, _Z, _I, _I, _I, _I, _P]),
+    "co_alibi_cache_reorder": (_I, [_PP, _L, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "co_alibi_probe_mfma": (_I, [_P, _P, _I, _I, _P]),
     "co_alibi_last_error": (ctypes.c_char_p, []),
     "co_alibi_abi_version": (_I, []),

@@ -1,0 +1,226 @@
+// Key / value caches held in 8 bits, on gfx950: quantising rows as they are written, and reading them back.
+//
+// A value is code * scale, with a scale for each kv head's blocks of 16 rows.  A block that is begun gets the least power of two
+// 2^k, k >= -40, at which none of its new rows passes the format's largest code; a block that has rows keeps its scale, or
+// doubles it as often as the new ones need, and its codes are halved as often.  Scaling by powers of two rounds nothing but the
+// codes, so that however often a block's scale grows its int8 codes stay within one step of their values (half a step for the
+// first rounding, and less than half of the final one's for all later ones together) and its e4m3 codes within the format's own
+// half step, below its smallest normal number within one of its smallest steps.
+//   A new value that is not finite, or too large for the largest scale, makes its block's scale NaN, and with it all that is
+// read from the block, until its first row is written again.
+//
+// Both are copies, bound by HBM for prompts and by the launch for single tokens.
+#include <algorithm>
+
+#include "coalibi_codes.h"
+#include "coalibi_kernels.h"
+
+namespace coalibi {
+
+namespace {
+
+constexpr int kCacheThreads = 256;
+constexpr int kCacheWaves = kCacheThreads / 64;
+
+template <typename T>
+__device__ __forceinline__ f32x8 load8(const T* p) {
+  f32x8 x;
+  const auto v = ld_vec8(p);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = static_cast<float>(v[e]);
+  return x;
+}
+
+// The least k with x <= 2^k times the format's largest code, for finite x >= 0 given as its bits (subnormals as the smallest
+// exponent).
+template <typename F>
+__device__ __forceinline__ int least_exponent(unsigned bits) {
+  // 448 = 1.75 * 2^8, 127 = 1.984375 * 2^6.
+  constexpr int e = __is_same(F, E4M3) ? 8 : 6;
+  constexpr unsigned m = __is_same(F, E4M3) ? 0x600000u : 0x7e0000u;
+  return (int)(bits >> 23) - 127 - e + ((bits & 0x7fffffu) > m ? 1 : 0);
+}
+constexpr int kLeastExponent = -40, kMostExponent = 40;
+
+// One wavefront per block of 16 rows that gets new ones, kv head and cache: 8 elements a lane and piece, a piece's row the
+// block's row.
+template <typename T, typename F, int D>
+__global__ __launch_bounds__(kCacheThreads) void coalibi_append8_kernel(Append8Args a8) {
+  const AppendArgs& a = a8.t;
+  constexpr int PPR = D / 8;                                 // pieces per row
+  constexpr int N = kScaleRows * PPR < 64 ? 1 : kScaleRows * PPR / 64;  // pieces per lane
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long id = (long long)blockIdx.x * kCacheWaves + wave;
+  const int h = (int)(id % a.Hkv);
+  const long long block_no = id / a.Hkv;
+  const bool value = blockIdx.z != 0;
+  const Layout& from = value ? a.vl : a.kl;
+  const Layout& to = value ? a.vcl : a.kcl;
+  for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
+    const long long len = a.seq_lens[b];
+    const int n = a.counts == nullptr ? a.N : min(max(a.counts[b], 0), a.N);
+    // The new rows are cache rows [lo, hi); the block has `had` rows before them.
+    const int lo = (int)min(max(len, 0ll), (long long)a.capacity);
+    const int hi = (int)max(min(len + n, (long long)a.capacity), 0ll);
+    const long long at = (long long)(lo / kScaleRows + block_no) * kScaleRows;
+    if (at >= hi) continue;
+    const int row0 = (int)at, had = max(lo - row0, 0), end = min(hi - row0, kScaleRows);
+    int unit = b, in_unit = row0;
+    if (a.place.table != nullptr) {
+      unit = a.place.table[(size_t)b * a.place.table_stride + (row0 >> a.place.page_shift)];
+      if (unit < 0 || unit >= a.place.units) continue;
+      in_unit = row0 & ((1 << a.place.page_shift) - 1);
+    }
+    const T* const src = static_cast<const T*>(value ? a.v : a.k) + (size_t)b * from.b + (size_t)h * from.h;
+    char* const dst = static_cast<char*>(value ? a.vc : a.kc) + (size_t)unit * to.b + (size_t)h * to.h + (size_t)in_unit * D;
+    float* const scale = (value ? a8.vs + (size_t)unit * a8.vsb + (size_t)h * a8.vsh : a8.ks + (size_t)unit * a8.ksb + (size_t)h * a8.ksh) +
+                         in_unit / kScaleRows;
+
+    // The pieces: new ones (their values), old ones (their codes), others.
+    f32x8 x[N];
+    u32x2 old[N];
+    bool fresh[N], held[N];
+    unsigned top = 0;
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = lane + 64 * i, r = p / PPR, col = p % PPR * 8;
+      held[i] = r < had;
+      fresh[i] = r >= had && r < end;
+      x[i] = f32x8{};
+      old[i] = u32x2{};
+      if (held[i]) {
+        old[i] = *reinterpret_cast<const u32x2*>(dst + r * D + col);
+      } else if (fresh[i]) {
+        const int ni = (int)(row0 + r - len);
+        const int s = a.rows == nullptr ? ni : a.rows[(size_t)b * a.N + ni];
+        fresh[i] = s >= 0 && s < a.T;
+        if (fresh[i]) x[i] = load8(src + (size_t)s * from.r + col);
+      }
+      any |= fresh[i];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = fabsf(x[i][e]);
+        top = max(top, __builtin_bit_cast(unsigned, y));
+      }
+    }
+    if (!__any(any)) continue;
+    const float was = had > 0 ? *scale : 0.f;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, off, 64));
+
+    int grow = 0;  // doublings of the scale that the block had
+    float now;
+    if (had > 0) {
+      const unsigned t = __builtin_bit_cast(unsigned, was * F::kMost);
+      grow = max((int)(top >> 23) - (int)(t >> 23) + ((top & 0x7fffffu) > (t & 0x7fffffu) ? 1 : 0), 0);
+      now = was >= kScaleLeast && was <= kScaleMost ? ldexpf(was, grow) : __builtin_nanf("");
+    } else {
+      const int k = max(least_exponent<F>(top), kLeastExponent);
+      now = k > kMostExponent ? __builtin_nanf("") : ldexpf(1.f, k);
+    }
+    const bool fine = now <= kScaleMost && top < 0x7f800000u;
+    if (!fine) now = __builtin_nanf("");
+    // (A block whose scale is no power of two came from elsewhere.)
+    const bool two = (__builtin_bit_cast(unsigned, now) & 0x7fffffu) == 0;
+    const float inv = 1.f / now, shrink = ldexpf(1.f, -grow);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int p = lane + 64 * i, r = p / PPR, col = p % PPR * 8;
+      f32x8 y{};
+      if (fresh[i]) {
+        if (fine) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = two ? x[i][e] * inv : x[i][e] / now;
+        }
+      } else if (held[i] && fine && grow > 0) {
+        y = from_codes<F>(old[i]) * shrink;
+      } else {
+        continue;
+      }
+      *reinterpret_cast<u32x2*>(dst + r * D + col) = to_codes<F>(y);
+    }
+    if (lane == 0) *scale = now;
+  }
+}
+
+// Rows [first, first + n) of every sequence, 8 elements a thread.
+template <typename T, typename F>
+__global__ __launch_bounds__(kCacheThreads) void coalibi_read8_kernel(Read8Args a) {
+  const int ppr = a.D / 8;
+  const long long per_seq = (long long)a.Hkv * a.N * ppr;
+  const long long at = (long long)blockIdx.x * kCacheThreads + threadIdx.x;
+  if (at >= per_seq) return;
+  const int col = (int)(at % ppr) * 8;
+  const int hr = (int)(at / ppr);  // (h, row): at most 2^31 by the host's check
+  const int h = hr / a.N, i = hr - h * a.N;
+  const bool value = blockIdx.z != 0;
+  const Layout& l = value ? a.vcl : a.kcl;
+  for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
+    const long long row = (a.first == nullptr ? 0 : (long long)a.first[b]) + i;
+    T* const out = static_cast<T*>(value ? a.v : a.k) + (((size_t)b * a.Hkv + h) * a.N + i) * a.D + col;
+    f32x8 x{};
+    if (row >= 0 && row < min(a.seq_lens[b], a.capacity)) {
+      int unit = b, in_unit = (int)row;
+      bool there = true;
+      if (a.place.table != nullptr) {
+        unit = a.place.table[(size_t)b * a.place.table_stride + (in_unit >> a.place.page_shift)];
+        there = unit >= 0 && unit < a.place.units;
+        in_unit &= (1 << a.place.page_shift) - 1;
+      }
+      float s = __builtin_nanf("");
+      if (there) {
+        s = value ? a.vs[(size_t)unit * a.vsb + (size_t)h * a.vsh + in_unit / kScaleRows]
+                  : a.ks[(size_t)unit * a.ksb + (size_t)h * a.ksh + in_unit / kScaleRows];
+        const char* const p = static_cast<const char*>(value ? a.vc : a.kc) + (size_t)unit * l.b + (size_t)h * l.h +
+                              (size_t)in_unit * a.D + col;
+        x = from_codes<F>(*reinterpret_cast<const u32x2*>(p));
+        if (!(s >= kScaleLeast && s <= kScaleMost)) s = __builtin_nanf("");
+      }
+      x *= s;
+    }
+    store8(out, x);
+  }
+}
+
+template <typename T, typename F>
+hipError_t append_d(const Append8Args& a, int D, dim3 grid, hipStream_t st) {
+  switch (D) {
+    case 16: hipLaunchKernelGGL((coalibi_append8_kernel<T, F, 16>), grid, dim3(kCacheThreads), 0, st, a); break;
+    case 32: hipLaunchKernelGGL((coalibi_append8_kernel<T, F, 32>), grid, dim3(kCacheThreads), 0, st, a); break;
+    case 64: hipLaunchKernelGGL((coalibi_append8_kernel<T, F, 64>), grid, dim3(kCacheThreads), 0, st, a); break;
+    case 128: hipLaunchKernelGGL((coalibi_append8_kernel<T, F, 128>), grid, dim3(kCacheThreads), 0, st, a); break;
+    default: hipLaunchKernelGGL((coalibi_append8_kernel<T, F, 256>), grid, dim3(kCacheThreads), 0, st, a); break;
+  }
+  return hipGetLastError();
+}
+
+}  // namespace
+
+template <typename T>
+hipError_t launch_append8(const Append8Args& a, bool e4m3, int D, hipStream_t stream) {
+  // N rows from anywhere in a block touch at most (N + 14) / 16 + 1 blocks.
+  const long long waves = ((a.t.N + kScaleRows - 2ll) / kScaleRows + 1) * a.t.Hkv;
+  const dim3 grid(static_cast<unsigned>((waves + kCacheWaves - 1) / kCacheWaves), static_cast<unsigned>(std::min(a.t.B, 65535)), 2);
+  return e4m3 ? append_d<T, E4M3>(a, D, grid, stream) : append_d<T, I8>(a, D, grid, stream);
+}
+
+template <typename T>
+hipError_t launch_read8(const Read8Args& a, bool e4m3, hipStream_t stream) {
+  const long long per_seq = (long long)a.Hkv * a.N * (a.D / 8);
+  const dim3 grid(static_cast<unsigned>((per_seq + kCacheThreads - 1) / kCacheThreads), static_cast<unsigned>(std::min(a.B, 65535)), 2);
+  if (e4m3)
+    hipLaunchKernelGGL((coalibi_read8_kernel<T, E4M3>), grid, dim3(kCacheThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((coalibi_read8_kernel<T, I8>), grid, dim3(kCacheThreads), 0, stream, a);
+  return hipGetLastError();
+}
+
+#define COALIBI_INST_CACHE8(T)                                                          \
+  template hipError_t launch_append8<T>(const Append8Args&, bool, int, hipStream_t);    \
+  template hipError_t launch_read8<T>(const Read8Args&, bool, hipStream_t);
+COALIBI_INST_CACHE8(_Float16)
+COALIBI_INST_CACHE8(__bf16)
+COALIBI_INST_CACHE8(float)
+
+}  // namespace coalibi

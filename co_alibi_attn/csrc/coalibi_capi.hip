@@ -83,11 +83,12 @@ constexpr long long kMaxRowStride = 1 << 20;
 int check_kv_rows(const char* fn, const coalibi::Layout& k, const coalibi::Layout& v) {
   return k.r == v.r ? CO_ALIBI_OK : fail(CO_ALIBI_EINVAL, std::string(fn) + ": k and v must have the same row stride");
 }
+constexpr int kCodes = -1;  // in place of a dtype: elements of one byte
 int read_layout(const char* fn, const char* name, const long long* strides, int dtype, int H, int S, int D,
                 coalibi::Layout* out) {
   *out = coalibi::contiguous_layout(H, S, D);
   if (strides == nullptr) return CO_ALIBI_OK;
-  const long long per16 = dtype == CO_ALIBI_F32 ? 4 : 8;
+  const long long per16 = dtype == kCodes ? 16 : dtype == CO_ALIBI_F32 ? 4 : 8;
   for (int i = 0; i < 3; ++i)
     if (strides[i] < 0 || strides[i] % per16 != 0)
       return fail(CO_ALIBI_EINVAL, std::string(fn) + ": the strides of " + name + " must be >= 0 and whole 16-byte units");
@@ -845,27 +846,89 @@ size_t tree_workspace(const TreePlan& p, bool ragged, int batch, int heads_q, in
          decode_partials_bytes(static_cast<size_t>(batch) * heads_q * tokens * splits, head_dim);
 }
 
-}  // namespace
 
-extern "C" {
-
-size_t co_alibi_decode_tree_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,
-                                            int head_dim) {
-  if (batch < 1 || heads_kv < 1 || heads_q < 1 || heads_q % heads_kv != 0 || tokens < 1 ||
-      tokens > coalibi::kMaxTreeTokens || seq_kv < 0 || head_dim < 1 || head_dim > 256 ||
-      !tree_countable(batch, heads_q, tokens, seq_kv))
-    return 0;
-  const TreePlan plan = tree_plan(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim);
-  return tree_workspace(plan, true, batch, heads_q, heads_kv, tokens, head_dim);
+// How a decode over an 8-bit cache is split, in chunks of 32 keys for each wavefront of a work-group: as tree_plan.
+TreePlan tree8_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim) {
+  const int rows = heads_q / heads_kv * tokens;
+  TreePlan p;
+  p.chunk = 128;
+  p.row_blocks = (rows + 31) / 32;
+  const int chunks = static_cast<int>((seq_kv + static_cast<long long>(p.chunk) - 1) / p.chunk) + 1;
+  const int row_bytes = head_dim * (dtype == CO_ALIBI_F32 ? 4 : 2), cus = device_cus();
+  const int slots = (row_bytes <= 256 ? 2 : 1) * cus;
+  const long long heads = static_cast<long long>(heads_kv) * p.row_blocks, units = batch * heads;
+  auto walk = [&](long long n) {  // chunks per split of n splits
+    const int most = static_cast<int>(std::min<long long>({std::max(n, 1ll), chunks, coalibi::kMaxTreeSplits}));
+    return (chunks + most - 1) / most;
+  };
+  p.cps = chunks <= 3 ? chunks : walk(slots / units);
+  p.splits = (chunks + p.cps - 1) / p.cps;
+  p.share = static_cast<int>(std::max<long long>(slots / heads, 1));
+  p.planned = static_cast<int>(std::min<long long>({p.splits * static_cast<long long>(kTreeRaggedSplits), chunks, p.share,
+                                                    coalibi::kMaxTreeSplits}));
+  p.planned = std::max({p.planned, p.splits, 2});
+  p.plans = slots / units > 1 && walk(slots / units) >= kTreePlanWalk;
+  return p;
+}
+bool tree_shape_ok(int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim) {
+  return batch >= 1 && heads_kv >= 1 && heads_q >= 1 && heads_q % heads_kv == 0 && tokens >= 1 &&
+         tokens <= coalibi::kMaxTreeTokens && seq_kv >= 0 && head_dim >= 1 && head_dim <= 256 &&
+         tree_countable(batch, heads_q, tokens, seq_kv);
 }
 
-int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v, const void* k_cache,
-                         const void* v_cache, const long long* strides, const float* slopes, const int* seq_lens,
-                         const int* parents, int parents_per_seq, const int* block_table, int blocks_per_seq,
-                         int num_pages, int page_size, void* o, float* lse, void* workspace, size_t workspace_bytes,
-                         int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim, float sm_scale,
-                         void* stream) {
-  const char* fn = "co_alibi_decode_tree";
+int check_format(const char* fn, int format) {
+  return format == CO_ALIBI_E4M3 || format == CO_ALIBI_INT8
+             ? CO_ALIBI_OK
+             : fail(CO_ALIBI_EUNSUPPORTED, std::string(fn) + ": format must be 0 (e4m3) or 1 (int8)");
+}
+
+// An 8-bit cache's rows follow one another.
+int check_dense(const char* fn, const coalibi::Layout& k, const coalibi::Layout& v, int D) {
+  return k.r == D && v.r == D ? CO_ALIBI_OK
+                              : fail(CO_ALIBI_EINVAL, std::string(fn) + ": the rows of an 8-bit cache must be dense (row stride head_dim)");
+}
+
+// The scales' (unit, head) strides, of k_scale then of v_scale, or the contiguous ones.
+int read_scales(const char* fn, const float* k_scale, const float* v_scale, const long long* strides, int heads_kv,
+                int page_size, long long* ksb, long long* ksh, long long* vsb, long long* vsh) {
+  int rc;
+  if ((rc = check_ptr(fn, "k_scale", k_scale, 4)) || (rc = check_ptr(fn, "v_scale", v_scale, 4))) return rc;
+  const long long blocks = (static_cast<long long>(page_size) + coalibi::kScaleRows - 1) / coalibi::kScaleRows;
+  *ksb = *vsb = heads_kv * blocks;
+  *ksh = *vsh = blocks;
+  if (strides == nullptr) return CO_ALIBI_OK;
+  for (int i = 0; i < 4; ++i)
+    if (strides[i] < 0) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": the strides of the scales must be >= 0");
+  *ksb = strides[0];
+  *ksh = strides[1];
+  *vsb = strides[2];
+  *vsh = strides[3];
+  return CO_ALIBI_OK;
+}
+
+template <typename T, typename F>
+hipError_t tree8_dispatch_d(const coalibi::Tree8Args& a, int D, hipStream_t st) {
+  switch (D) {
+    case 16: return coalibi::launch_tree8<T, F, 16>(a, st);
+    case 32: return coalibi::launch_tree8<T, F, 32>(a, st);
+    case 64: return coalibi::launch_tree8<T, F, 64>(a, st);
+    case 256:
+      if constexpr (sizeof(T) == 2) return coalibi::launch_tree8<T, F, 256>(a, st);
+      return hipErrorInvalidValue;
+    default: return coalibi::launch_tree8<T, F, 128>(a, st);
+  }
+}
+template <typename T>
+hipError_t tree8_dispatch(const coalibi::Tree8Args& a, bool e4m3, int D, hipStream_t st) {
+  return e4m3 ? tree8_dispatch_d<T, coalibi::E4M3>(a, D, st) : tree8_dispatch_d<T, coalibi::I8>(a, D, st);
+}
+
+// The arguments of a tree decode (`eight`: over an 8-bit cache), checked, as the kernels take them.
+int tree_args(const char* fn, int dtype, bool eight, const void* q, const void* k, const void* v, const void* k_cache,
+              const void* v_cache, const long long* strides, const float* slopes, const int* seq_lens, const int* parents,
+              int parents_per_seq, const int* block_table, int blocks_per_seq, int num_pages, int page_size, void* o,
+              float* lse, void* workspace, size_t workspace_bytes, int batch, int heads_q, int heads_kv, int tokens,
+              int seq_kv, int head_dim, float sm_scale, coalibi::TreeArgs* out) {
   const Shape s{batch, heads_q, heads_kv, tokens, seq_kv > 0 ? seq_kv : 1, head_dim};
   int rc;
   if ((rc = check_shape(fn, dtype, s))) return rc;
@@ -874,7 +937,7 @@ int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v,
   if (tokens > coalibi::kMaxTreeTokens)
     return fail(CO_ALIBI_EUNSUPPORTED, std::string(fn) + ": at most " + std::to_string(coalibi::kMaxTreeTokens) +
                                            " new tokens per sequence, got " + std::to_string(tokens));
-  coalibi::TreeArgs a{};
+  coalibi::TreeArgs& a = *out;
   long long capacity = 0;
   if ((rc = check_place(fn, block_table, blocks_per_seq, num_pages, page_size, batch, &a.place, &capacity))) return rc;
   if (seq_kv < 0 || seq_kv > capacity)
@@ -888,7 +951,7 @@ int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v,
   if (!std::isfinite(sm_scale)) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": sm_scale must be finite");
   if (!tree_countable(batch, heads_q, tokens, seq_kv))
     return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
-  const TreePlan plan = tree_plan(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim);
+  const TreePlan plan = (eight ? tree8_plan : tree_plan)(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim);
   if (static_cast<double>(batch) * heads_kv * plan.row_blocks * (plan.planned + 8.0) > 2.1e9)
     return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
   const size_t need = tree_workspace(plan, seq_lens != nullptr, batch, heads_q, heads_kv, tokens, head_dim);
@@ -899,8 +962,8 @@ int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v,
   if ((rc = layout_at(fn, "q", strides, 0, dtype, heads_q, tokens, head_dim, &a.ql)) ||
       (rc = layout_at(fn, "k", strides, 1, dtype, heads_kv, tokens, head_dim, &a.kl)) ||
       (rc = layout_at(fn, "v", strides, 2, dtype, heads_kv, tokens, head_dim, &a.vl)) ||
-      (rc = layout_at(fn, "k_cache", strides, 3, dtype, heads_kv, page_size, head_dim, &a.kcl)) ||
-      (rc = layout_at(fn, "v_cache", strides, 4, dtype, heads_kv, page_size, head_dim, &a.vcl)))
+      (rc = layout_at(fn, "k_cache", strides, 3, eight ? kCodes : dtype, heads_kv, page_size, head_dim, &a.kcl)) ||
+      (rc = layout_at(fn, "v_cache", strides, 4, eight ? kCodes : dtype, heads_kv, page_size, head_dim, &a.vcl)))
     return rc;
   a.q = q;
   a.k = k;
@@ -940,32 +1003,24 @@ int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v,
   // forward's.  Without the tail skip no key is far.
   a.far = g_tail_skip.load() == 0 ? std::numeric_limits<float>::infinity() : dtype == CO_ALIBI_F32 ? 64.f : 40.f;
   a.sc2 = sm_scale * coalibi::kLog2eHost;
-  hipStream_t st = static_cast<hipStream_t>(stream);
-  hipError_t e;
-  switch (dtype) {
-    case CO_ALIBI_F16: e = tree_dispatch_d<_Float16>(a, head_dim, st); break;
-    case CO_ALIBI_BF16: e = tree_dispatch_d<__bf16>(a, head_dim, st); break;
-    default: e = tree_dispatch_d<float>(a, head_dim, st); break;
-  }
-  if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
   return CO_ALIBI_OK;
 }
 
-int co_alibi_cache_append(int dtype, const void* k, const void* v, void* k_cache, void* v_cache,
-                          const long long* strides, const int* seq_lens, const int* counts, const int* rows,
-                          int new_rows, const int* block_table, int blocks_per_seq, int num_pages, int page_size,
-                          int batch, int heads_kv, int tokens, int head_dim, void* stream) {
-  const char* fn = "co_alibi_cache_append";
+// The arguments of a cache append (`eight`: to an 8-bit cache), checked, as the kernels take them.
+int append_args(const char* fn, int dtype, bool eight, const void* k, const void* v, void* k_cache, void* v_cache,
+                const long long* strides, const int* seq_lens, const int* counts, const int* rows, int new_rows,
+                const int* block_table, int blocks_per_seq, int num_pages, int page_size, int batch, int heads_kv, int tokens,
+                int head_dim, coalibi::AppendArgs* out) {
   const Shape s{batch, heads_kv, heads_kv, tokens, 1, head_dim};
   int rc;
   if ((rc = check_shape(fn, dtype, s))) return rc;
   if (new_rows < 1) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": new_rows must be >= 1");
   if (rows == nullptr && new_rows > tokens)
     return fail(CO_ALIBI_EINVAL, std::string(fn) + ": new_rows is above tokens and there is no rows array");
-  coalibi::AppendArgs a{};
+  coalibi::AppendArgs& a = *out;
   long long capacity = 0;
   if ((rc = check_place(fn, block_table, blocks_per_seq, num_pages, page_size, batch, &a.place, &capacity))) return rc;
-  const int elem = dtype == CO_ALIBI_F32 ? 4 : 2;
+  const int elem = eight ? 1 : dtype == CO_ALIBI_F32 ? 4 : 2;
   if (static_cast<double>(new_rows) * heads_kv * head_dim * elem / 16 > 1e9 || capacity > (1ll << 30))
     return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
   if ((rc = check_ptr(fn, "k", k, 16)) || (rc = check_ptr(fn, "v", v, 16)) ||
@@ -976,8 +1031,8 @@ int co_alibi_cache_append(int dtype, const void* k, const void* v, void* k_cache
   const int units = block_table != nullptr ? num_pages : batch;
   if ((rc = layout_at(fn, "k", strides, 0, dtype, heads_kv, tokens, head_dim, &a.kl)) ||
       (rc = layout_at(fn, "v", strides, 1, dtype, heads_kv, tokens, head_dim, &a.vl)) ||
-      (rc = layout_at(fn, "k_cache", strides, 2, dtype, heads_kv, page_size, head_dim, &a.kcl)) ||
-      (rc = layout_at(fn, "v_cache", strides, 3, dtype, heads_kv, page_size, head_dim, &a.vcl)) ||
+      (rc = layout_at(fn, "k_cache", strides, 2, eight ? kCodes : dtype, heads_kv, page_size, head_dim, &a.kcl)) ||
+      (rc = layout_at(fn, "v_cache", strides, 3, eight ? kCodes : dtype, heads_kv, page_size, head_dim, &a.vcl)) ||
       (rc = check_output(fn, "k_cache", a.kcl, units, heads_kv, page_size, head_dim)) ||
       (rc = check_output(fn, "v_cache", a.vcl, units, heads_kv, page_size, head_dim)))
     return rc;
@@ -995,8 +1050,320 @@ int co_alibi_cache_append(int dtype, const void* k, const void* v, void* k_cache
   a.capacity = static_cast<int>(capacity);
   a.row_chunks = head_dim * elem / 16;
   a.elem = elem;
+  return CO_ALIBI_OK;
+}
+
+// Beam selection's segments of a row: the longest that give the GPU two work-groups per CU, else the shortest.
+struct SelectPlan {
+  int segments, per_segment;
+};
+SelectPlan select_plan(int batch, int beams, int vocab) {
+  const long long rows = static_cast<long long>(batch) * beams;
+  int per = 8192;
+  while (per > 1024 && rows * ((vocab + per - 1) / per) < 2ll * device_cus()) per /= 2;
+  return {(vocab + per - 1) / per, per};
+}
+bool select_shape_ok(int batch, int beams, int num_beams, int vocab) {
+  return batch >= 1 && beams >= 1 && beams <= coalibi::kMaxBeams && num_beams >= 1 && num_beams <= coalibi::kMaxBeams &&
+         vocab >= 1 && vocab <= coalibi::kMaxVocab && static_cast<double>(batch) * beams <= 1e9;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t co_alibi_decode_tree_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,
+                                            int head_dim) {
+  if (!tree_shape_ok(batch, heads_q, heads_kv, tokens, seq_kv, head_dim)) return 0;
+  const TreePlan plan = tree_plan(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim);
+  return tree_workspace(plan, true, batch, heads_q, heads_kv, tokens, head_dim);
+}
+
+int co_alibi_decode_tree(int dtype, const void* q, const void* k, const void* v, const void* k_cache,
+                         const void* v_cache, const long long* strides, const float* slopes, const int* seq_lens,
+                         const int* parents, int parents_per_seq, const int* block_table, int blocks_per_seq,
+                         int num_pages, int page_size, void* o, float* lse, void* workspace, size_t workspace_bytes,
+                         int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim, float sm_scale,
+                         void* stream) {
+  const char* fn = "co_alibi_decode_tree";
+  coalibi::TreeArgs a{};
+  const int rc = tree_args(fn, dtype, false, q, k, v, k_cache, v_cache, strides, slopes, seq_lens, parents, parents_per_seq,
+                           block_table, blocks_per_seq, num_pages, page_size, o, lse, workspace, workspace_bytes, batch,
+                           heads_q, heads_kv, tokens, seq_kv, head_dim, sm_scale, &a);
+  if (rc) return rc;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e;
+  switch (dtype) {
+    case CO_ALIBI_F16: e = tree_dispatch_d<_Float16>(a, head_dim, st); break;
+    case CO_ALIBI_BF16: e = tree_dispatch_d<__bf16>(a, head_dim, st); break;
+    default: e = tree_dispatch_d<float>(a, head_dim, st); break;
+  }
+  if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+  return CO_ALIBI_OK;
+}
+
+size_t co_alibi_decode_tree_8bit_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,
+                                                 int head_dim) {
+  if (!tree_shape_ok(batch, heads_q, heads_kv, tokens, seq_kv, head_dim)) return 0;
+  const TreePlan plan = tree8_plan(dtype, batch, heads_q, heads_kv, tokens, seq_kv, head_dim);
+  return tree_workspace(plan, true, batch, heads_q, heads_kv, tokens, head_dim);
+}
+
+int co_alibi_decode_tree_8bit(int dtype, int format, const void* q, const void* k, const void* v, const void* k_cache,
+                              const void* v_cache, const float* k_scale, const float* v_scale, const long long* strides,
+                              const long long* scale_strides, const float* slopes, const int* seq_lens, const int* parents,
+                              int parents_per_seq, const int* block_table, int blocks_per_seq, int num_pages, int page_size,
+                              void* o, float* lse, void* workspace, size_t workspace_bytes, int batch, int heads_q,
+                              int heads_kv, int tokens, int seq_kv, int head_dim, float sm_scale, void* stream) {
+  const char* fn = "co_alibi_decode_tree_8bit";
+  int rc;
+  if ((rc = check_format(fn, format))) return rc;
+  coalibi::Tree8Args a{};
+  if ((rc = tree_args(fn, dtype, true, q, k, v, k_cache, v_cache, strides, slopes, seq_lens, parents, parents_per_seq,
+                      block_table, blocks_per_seq, num_pages, page_size, o, lse, workspace, workspace_bytes, batch, heads_q,
+                      heads_kv, tokens, seq_kv, head_dim, sm_scale, &a.t)) ||
+      (rc = check_dense(fn, a.t.kcl, a.t.vcl, head_dim)) ||
+      (rc = read_scales(fn, k_scale, v_scale, scale_strides, heads_kv, page_size, &a.ksb, &a.ksh, &a.vsb, &a.vsh)))
+    return rc;
+  a.ks = k_scale;
+  a.vs = v_scale;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool e4m3 = format == CO_ALIBI_E4M3;
+  hipError_t e;
+  switch (dtype) {
+    case CO_ALIBI_F16: e = tree8_dispatch<_Float16>(a, e4m3, head_dim, st); break;
+    case CO_ALIBI_BF16: e = tree8_dispatch<__bf16>(a, e4m3, head_dim, st); break;
+    default: e = tree8_dispatch<float>(a, e4m3, head_dim, st); break;
+  }
+  if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+  return CO_ALIBI_OK;
+}
+
+int co_alibi_cache_append(int dtype, const void* k, const void* v, void* k_cache, void* v_cache,
+                          const long long* strides, const int* seq_lens, const int* counts, const int* rows,
+                          int new_rows, const int* block_table, int blocks_per_seq, int num_pages, int page_size,
+                          int batch, int heads_kv, int tokens, int head_dim, void* stream) {
+  const char* fn = "co_alibi_cache_append";
+  coalibi::AppendArgs a{};
+  const int rc = append_args(fn, dtype, false, k, v, k_cache, v_cache, strides, seq_lens, counts, rows, new_rows, block_table,
+                             blocks_per_seq, num_pages, page_size, batch, heads_kv, tokens, head_dim, &a);
+  if (rc) return rc;
   const hipError_t e = coalibi::launch_append(a, static_cast<hipStream_t>(stream));
   if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+  return CO_ALIBI_OK;
+}
+
+int co_alibi_cache_append_8bit(int dtype, int format, const void* k, const void* v, void* k_cache, void* v_cache,
+                               float* k_scale, float* v_scale, const long long* strides, const long long* scale_strides,
+                               const int* seq_lens, const int* counts, const int* rows, int new_rows, const int* block_table,
+                               int blocks_per_seq, int num_pages, int page_size, int batch, int heads_kv, int tokens,
+                               int head_dim, void* stream) {
+  const char* fn = "co_alibi_cache_append_8bit";
+  int rc;
+  if ((rc = check_format(fn, format))) return rc;
+  coalibi::Append8Args a{};
+  if ((rc = append_args(fn, dtype, true, k, v, k_cache, v_cache, strides, seq_lens, counts, rows, new_rows, block_table,
+                        blocks_per_seq, num_pages, page_size, batch, heads_kv, tokens, head_dim, &a.t)) ||
+      (rc = check_dense(fn, a.t.kcl, a.t.vcl, head_dim)) ||
+      (rc = read_scales(fn, k_scale, v_scale, scale_strides, heads_kv, page_size, &a.ksb, &a.ksh, &a.vsb, &a.vsh)))
+    return rc;
+  // The scales are written by different work-groups, too.
+  const int units = block_table != nullptr ? num_pages : batch, blocks = (page_size + coalibi::kScaleRows - 1) / coalibi::kScaleRows;
+  if ((rc = check_output(fn, "k_scale", {a.ksb, a.ksh, 1}, units, heads_kv, blocks, 1)) ||
+      (rc = check_output(fn, "v_scale", {a.vsb, a.vsh, 1}, units, heads_kv, blocks, 1)))
+    return rc;
+  a.ks = k_scale;
+  a.vs = v_scale;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool e4m3 = format == CO_ALIBI_E4M3;
+  hipError_t e;
+  switch (dtype) {
+    case CO_ALIBI_F16: e = coalibi::launch_append8<_Float16>(a, e4m3, head_dim, st); break;
+    case CO_ALIBI_BF16: e = coalibi::launch_append8<__bf16>(a, e4m3, head_dim, st); break;
+    default: e = coalibi::launch_append8<float>(a, e4m3, head_dim, st); break;
+  }
+  if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+  return CO_ALIBI_OK;
+}
+
+int co_alibi_cache_read_8bit(int dtype, int format, const void* k_cache, const void* v_cache, const float* k_scale,
+                             const float* v_scale, const long long* strides, const long long* scale_strides,
+                             const int* seq_lens, const int* first, int rows, const int* block_table, int blocks_per_seq,
+                             int num_pages, int page_size, void* k, void* v, int batch, int heads_kv, int head_dim,
+                             void* stream) {
+  const char* fn = "co_alibi_cache_read_8bit";
+  const Shape s{batch, heads_kv, heads_kv, rows, 1, head_dim};
+  int rc;
+  if ((rc = check_format(fn, format)) || (rc = check_shape(fn, dtype, s))) return rc;
+  coalibi::Read8Args a{};
+  long long capacity = 0;
+  if ((rc = check_place(fn, block_table, blocks_per_seq, num_pages, page_size, batch, &a.place, &capacity))) return rc;
+  if (static_cast<double>(rows) * heads_kv * (head_dim / 8) > 1e9 || static_cast<double>(rows) * heads_kv > 2e9 ||
+      capacity > (1ll << 30))
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
+  if ((rc = check_ptr(fn, "k_cache", k_cache, 16)) || (rc = check_ptr(fn, "v_cache", v_cache, 16)) ||
+      (rc = check_ptr(fn, "k", k, 16)) || (rc = check_ptr(fn, "v", v, 16)) || (rc = check_ptr(fn, "seq_lens", seq_lens, 4)) ||
+      (rc = check_opt_ptr(fn, "first", first, 4)) ||
+      (rc = layout_at(fn, "k_cache", strides, 0, kCodes, heads_kv, page_size, head_dim, &a.kcl)) ||
+      (rc = layout_at(fn, "v_cache", strides, 1, kCodes, heads_kv, page_size, head_dim, &a.vcl)) ||
+      (rc = check_dense(fn, a.kcl, a.vcl, head_dim)) ||
+      (rc = read_scales(fn, k_scale, v_scale, scale_strides, heads_kv, page_size, &a.ksb, &a.ksh, &a.vsb, &a.vsh)))
+    return rc;
+  a.kc = k_cache;
+  a.vc = v_cache;
+  a.ks = k_scale;
+  a.vs = v_scale;
+  a.seq_lens = seq_lens;
+  a.first = first;
+  a.k = k;
+  a.v = v;
+  a.B = batch;
+  a.Hkv = heads_kv;
+  a.N = rows;
+  a.D = head_dim;
+  a.capacity = static_cast<int>(capacity);
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  const bool e4m3 = format == CO_ALIBI_E4M3;
+  hipError_t e;
+  switch (dtype) {
+    case CO_ALIBI_F16: e = coalibi::launch_read8<_Float16>(a, e4m3, st); break;
+    case CO_ALIBI_BF16: e = coalibi::launch_read8<__bf16>(a, e4m3, st); break;
+    default: e = coalibi::launch_read8<float>(a, e4m3, st); break;
+  }
+  if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+  return CO_ALIBI_OK;
+}
+
+size_t co_alibi_beam_select_workspace_bytes(int batch, int beams, int num_beams, int vocab) {
+  if (!select_shape_ok(batch, beams, num_beams, vocab)) return 0;
+  const SelectPlan p = select_plan(batch, beams, vocab);
+  const size_t parts = static_cast<size_t>(batch) * beams * p.segments;
+  return round_up(parts * sizeof(double), 256) + round_up(parts * sizeof(float), 256) +
+         2 * round_up(parts * num_beams * sizeof(float), 256);
+}
+
+int co_alibi_beam_select(int dtype, const void* logits, const long long* strides, const float* scores,
+                         const unsigned char* finished, int end_token, float* out_scores, int* parents, long long* tokens,
+                         void* workspace, size_t workspace_bytes, int batch, int beams, int num_beams, int vocab,
+                         void* stream) {
+  const char* fn = "co_alibi_beam_select";
+  if (dtype != CO_ALIBI_F32 && dtype != CO_ALIBI_F16 && dtype != CO_ALIBI_BF16)
+    return fail(CO_ALIBI_EUNSUPPORTED, std::string(fn) + ": dtype must be 0 (fp32), 1 (fp16) or 2 (bf16)");
+  if (batch < 1) return fail(CO_ALIBI_EINVAL, std::string(fn) + ": batch must be >= 1");
+  if (beams < 1 || beams > coalibi::kMaxBeams || num_beams < 1 || num_beams > coalibi::kMaxBeams)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": beams and num_beams must be in [1, " + std::to_string(coalibi::kMaxBeams) + "]");
+  if (vocab < 1 || vocab > coalibi::kMaxVocab)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": vocab must be in [1, " + std::to_string(coalibi::kMaxVocab) + "]");
+  if (!select_shape_ok(batch, beams, num_beams, vocab))
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
+  if (strides != nullptr && (strides[0] < 0 || strides[1] < 0))
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": the strides of logits must be >= 0");
+  if (finished != nullptr && (end_token < 0 || end_token >= vocab))
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": end_token must be in [0, vocab)");
+  int rc;
+  if ((rc = check_ptr(fn, "logits", logits, dtype == CO_ALIBI_F32 ? 4 : 2)) || (rc = check_ptr(fn, "scores", scores, 4)) ||
+      (rc = check_ptr(fn, "out_scores", out_scores, 4)) || (rc = check_ptr(fn, "parents", parents, 4)) ||
+      (rc = check_ptr(fn, "tokens", tokens, 8)))
+    return rc;
+  const size_t need = co_alibi_beam_select_workspace_bytes(batch, beams, num_beams, vocab);
+  if (workspace_bytes < need)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": workspace of " + std::to_string(workspace_bytes) + " bytes, need " +
+                                     std::to_string(need));
+  if ((rc = check_ptr(fn, "workspace", workspace, 256))) return rc;
+  const SelectPlan p = select_plan(batch, beams, vocab);
+  const size_t parts = static_cast<size_t>(batch) * beams * p.segments;
+  coalibi::SelectArgs a{};
+  a.logits = logits;
+  a.batch_stride = strides != nullptr ? strides[0] : static_cast<long long>(beams) * vocab;
+  a.beam_stride = strides != nullptr ? strides[1] : vocab;
+  a.scores = scores;
+  a.finished = finished;
+  a.end_token = end_token;
+  a.out_scores = out_scores;
+  a.out_parents = parents;
+  a.out_tokens = tokens;
+  char* ws = static_cast<char*>(workspace);
+  a.psum = reinterpret_cast<double*>(ws);
+  ws += round_up(parts * sizeof(double), 256);
+  a.pmax = reinterpret_cast<float*>(ws);
+  ws += round_up(parts * sizeof(float), 256);
+  a.pval = reinterpret_cast<float*>(ws);
+  a.ptok = reinterpret_cast<int*>(ws + round_up(parts * num_beams * sizeof(float), 256));
+  a.B = batch;
+  a.W = beams;
+  a.N = num_beams;
+  a.V = vocab;
+  a.segments = p.segments;
+  a.per_segment = p.per_segment;
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e;
+  switch (dtype) {
+    case CO_ALIBI_F16: e = coalibi::launch_select<_Float16>(a, st); break;
+    case CO_ALIBI_BF16: e = coalibi::launch_select<__bf16>(a, st); break;
+    default: e = coalibi::launch_select<float>(a, st); break;
+  }
+  if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+  return CO_ALIBI_OK;
+}
+
+int co_alibi_cache_reorder(void* const* pools, const long long* shapes, int num_pools, const int* block_table,
+                           const int* pages, const int* seq_lens, const int* parents, int* out_table, int* out_lens,
+                           int batch, int beams, int blocks_per_seq, int num_pages, int page_size, void* stream) {
+  const char* fn = "co_alibi_cache_reorder";
+  if (batch < 1 || blocks_per_seq < 1 || num_pages < 1)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": batch, blocks_per_seq and num_pages must be >= 1");
+  if (beams < 1 || beams > coalibi::kMaxBeams)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": beams must be in [1, " + std::to_string(coalibi::kMaxBeams) + "]");
+  if (page_size < 16 || (page_size & (page_size - 1)) != 0)
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": page_size must be a power of two >= 16, got " + std::to_string(page_size));
+  if (static_cast<double>(batch) * beams * blocks_per_seq > 2.1e9 || static_cast<double>(blocks_per_seq) * page_size > (1 << 30))
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
+  if (num_pools < 0 || (num_pools > 0 && (pools == nullptr || shapes == nullptr)))
+    return fail(CO_ALIBI_EINVAL, std::string(fn) + ": pools or shapes is NULL");
+  int rc;
+  if ((rc = check_ptr(fn, "block_table", block_table, 4)) || (rc = check_ptr(fn, "pages", pages, 4)) ||
+      (rc = check_ptr(fn, "seq_lens", seq_lens, 4)) || (rc = check_ptr(fn, "parents", parents, 4)) ||
+      (rc = check_ptr(fn, "out_table", out_table, 4)) || (rc = check_ptr(fn, "out_lens", out_lens, 4)))
+    return rc;
+  coalibi::ReorderArgs a{};
+  a.table = block_table;
+  a.pages = pages;
+  a.lens = seq_lens;
+  a.parents = parents;
+  a.out_table = out_table;
+  a.out_lens = out_lens;
+  a.B = batch;
+  a.W = beams;
+  a.J = blocks_per_seq;
+  a.page = page_size;
+  a.num_pages = num_pages;
+  a.page_shift = 4;
+  while ((1 << a.page_shift) < page_size) ++a.page_shift;
+  for (int i = 0; i < num_pools; ++i) {  // page stride, head stride, heads, entries, bytes of an entry
+    const long long* const s = shapes + 5 * i;
+    const std::string name = "pool " + std::to_string(i);
+    if ((rc = check_ptr(fn, name.c_str(), pools[i], 4))) return rc;
+    if (s[2] < 1 || s[3] < 1 || s[3] > page_size || page_size % s[3] != 0 || s[4] < 1 || s[4] > (1 << 24) || s[4] % 4 != 0)
+      return fail(CO_ALIBI_EINVAL, std::string(fn) + ": " + name + " must have heads, entries that divide a page's rows, and entries of whole 4 bytes");
+    if (s[0] % 4 != 0 || s[1] % 4 != 0 || s[1] < 0 || (s[2] > 1 && s[1] < s[3] * s[4]) ||
+        (num_pages > 1 && s[0] < (s[2] - 1) * s[1] + s[3] * s[4]))
+      return fail(CO_ALIBI_EINVAL, std::string(fn) + ": " + name + " must have heads and pages that do not overlap, whole 4 bytes apart");
+    if (static_cast<double>(s[2]) * s[3] * s[4] > 1e9)
+      return fail(CO_ALIBI_EINVAL, std::string(fn) + ": problem too large for one launch");
+  }
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  for (int first = 0; first == 0 || first < num_pools; first += coalibi::kMaxPools) {
+    a.pools = std::min(num_pools - first, coalibi::kMaxPools);
+    a.tables = first == 0;
+    for (int i = 0; i < a.pools; ++i) {
+      const long long* const s = shapes + 5 * (first + i);
+      const bool wide = aligned(pools[first + i], 16) && s[0] % 16 == 0 && s[1] % 16 == 0 && s[4] % 16 == 0;
+      a.pool[i] = {static_cast<char*>(pools[first + i]), s[0], s[1], static_cast<int>(s[2]), static_cast<int>(s[3]),
+                   static_cast<int>(s[4]), wide};
+    }
+    const hipError_t e = coalibi::launch_reorder(a, st);
+    if (e != hipSuccess) return fail(CO_ALIBI_ELAUNCH, std::string(fn) + ": launch failed: " + hipGetErrorString(e));
+  }
   return CO_ALIBI_OK;
 }
 

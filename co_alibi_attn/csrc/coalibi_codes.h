@@ -1,0 +1,67 @@
+// Codes of 8 bits (e4m3, or int8 in [-127, 127]) from and to fp32, eight at a time.
+#pragma once
+#include "coalibi_common.h"
+#include "coalibi_kernels.h"
+
+namespace coalibi {
+
+namespace {
+
+template <typename F>
+__device__ __forceinline__ f32x8 from_codes(u32x2 c) {
+  f32x8 x;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (__is_same(F, E4M3)) {
+      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c[i], true);
+      x[4 * i] = lo[0];
+      x[4 * i + 1] = lo[1];
+      x[4 * i + 2] = hi[0];
+      x[4 * i + 3] = hi[1];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[4 * i + e] = static_cast<float>(static_cast<signed char>(c[i] >> 8 * e));
+    }
+  }
+  return x;
+}
+
+// The nearest codes, ties to even; values past the largest code become it.
+template <typename F>
+__device__ __forceinline__ u32x2 to_codes(f32x8 x) {
+  u32x2 c;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      y[e] = x[4 * i + e];
+      y[e] = y[e] > F::kMost ? F::kMost : y[e] < -F::kMost ? -F::kMost : y[e];  // (a NaN stays one)
+    }
+    if constexpr (__is_same(F, E4M3)) {
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+      c[i] = (unsigned)w;
+    } else {
+      unsigned w = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w |= ((unsigned)(int)rintf(y[e]) & 255u) << 8 * e;
+      c[i] = w;
+    }
+  }
+  return c;
+}
+
+template <typename T>
+__device__ __forceinline__ void store8(T* p, f32x8 x) {
+  if constexpr (sizeof(T) == 4) {
+    reinterpret_cast<f32x4*>(p)[0] = f32x4{x[0], x[1], x[2], x[3]};
+    reinterpret_cast<f32x4*>(p)[1] = f32x4{x[4], x[5], x[6], x[7]};
+  } else {
+    *reinterpret_cast<typename Mfma<T>::vec8*>(p) = Mfma<T>::pack(x);
+  }
+}
+
+}  // namespace
+
+}  // namespace coalibi

@@ -414,6 +414,26 @@ struct TreeArgs {
   float sc2;
 };
 
+// An 8-bit cache: a code per element, dense rows, and a scale (fp32) for each kv head's blocks of kScaleRows rows of a unit.
+// A format's largest code, and the scales that codes may have: rows read with another one make a sequence NaN.
+struct E4M3 {
+  static constexpr float kMost = 448.f;
+};
+struct I8 {
+  static constexpr float kMost = 127.f;
+};
+constexpr int kScaleRows = 16;
+constexpr float kScaleLeast = 0x1p-40f, kScaleMost = 0x1p40f;
+
+// Tree decode over an 8-bit cache: t.kc and t.vc hold codes, t.kcl and t.vcl their strides; ks / vs the scales, (unit, head)
+// strides in elements.
+struct Tree8Args {
+  TreeArgs t;
+  const float* ks;
+  const float* vs;
+  long long ksb, ksh, vsb, vsh;
+};
+
 // Cache append: row i of sequence b, new row rows[b][i] (or i) of k / v, goes to cache row lens[b] + i, for
 // i < counts[b] (or N).
 struct AppendArgs {
@@ -430,6 +450,73 @@ struct AppendArgs {
   int capacity;    // cache rows a sequence has room for
   int row_chunks;  // 16-byte chunks per row
   int elem;        // bytes per element
+};
+
+// Append to an 8-bit cache: t's caches hold codes (their strides and `elem` in bytes); ks / vs the scales, (unit, head) strides
+// in elements.
+struct Append8Args {
+  AppendArgs t;
+  float* ks;
+  float* vs;
+  long long ksb, ksh, vsb, vsh;
+};
+
+// Reading an 8-bit cache: rows [first[b], first[b] + N) of every sequence into k / v (B, Hkv, N, D); zeros where a row is not
+// filled, NaN where its page or its scale is none.
+struct Read8Args {
+  Layout kcl, vcl;
+  const void* kc;
+  const void* vc;
+  const float* ks;
+  const float* vs;
+  long long ksb, ksh, vsb, vsh;
+  CachePlace place;
+  const int* seq_lens;  // (B,)
+  const int* first;     // (B,) or NULL: 0
+  void* k;
+  void* v;
+  int B, Hkv, N, D, capacity;
+};
+
+// Beam selection: the N best of score[b][w] + log_softmax(logits[b][w])[t] over (w, t), rows (B, W) of V logits.
+// Workspace, per row and segment: pmax / psum of its weights and the N best logits (value, token), best first.
+constexpr int kMaxBeams = 64;
+struct SelectArgs {
+  const void* logits;
+  long long batch_stride, beam_stride;
+  const float* scores;             // (B, W)
+  const unsigned char* finished;   // (B, W) or NULL
+  int end_token;
+  float* out_scores;     // (B, N)
+  int* out_parents;      // (B, N)
+  long long* out_tokens; // (B, N)
+  float* pmax;           // (B*W, segments)
+  double* psum;
+  float* pval;  // (B*W, segments, N)
+  int* ptok;
+  int B, W, N, V;
+  int segments, per_segment;
+};
+
+// Reordering a paged cache: sequence (g, i) of B groups of W takes over the rows of sequence (g, parents[g][i]).
+constexpr int kMaxPools = 64;
+struct PoolDesc {
+  char* p;
+  long long page_stride, head_stride;  // bytes
+  int heads, entries, entry_bytes;     // entries per page and head, consecutive
+  bool wide;                           // all of it in whole, aligned 16 bytes (else 4)
+};
+struct ReorderArgs {
+  PoolDesc pool[kMaxPools];
+  int pools;
+  const int* table;    // (B*W, J)
+  const int* pages;    // (B*W, J): the pages that a group's column owns
+  const int* lens;     // (B*W)
+  const int* parents;  // (B, W)
+  int* out_table;
+  int* out_lens;
+  int B, W, J, page, page_shift, num_pages;
+  bool tables;  // write the tables, too
 };
 
 // Sampling: one token per row of logits (B, V), rows row_stride elements apart.  A setting's array holds
@@ -458,8 +545,24 @@ hipError_t launch_bwd(const BwdArgs& a, int stages, hipStream_t stream);
 
 template <typename T, int D>
 hipError_t launch_tree(const TreeArgs& a, hipStream_t stream);
+// O and LSE of the sequences with more than one split, from their partials.
+template <typename T, int D>
+hipError_t launch_tree_merge(const TreeArgs& a, hipStream_t stream);
+
+template <typename T, typename F, int D>
+hipError_t launch_tree8(const Tree8Args& a, hipStream_t stream);
 
 hipError_t launch_append(const AppendArgs& a, hipStream_t stream);
+
+template <typename T>
+hipError_t launch_append8(const Append8Args& a, bool e4m3, int D, hipStream_t stream);
+template <typename T>
+hipError_t launch_read8(const Read8Args& a, bool e4m3, hipStream_t stream);
+
+template <typename T>
+hipError_t launch_select(const SelectArgs& a, hipStream_t stream);
+
+hipError_t launch_reorder(const ReorderArgs& a, hipStream_t stream);
 
 template <typename T>
 hipError_t launch_sample(const SampleArgs& a, hipStream_t stream);

@@ -1,0 +1,512 @@
+// Co-ALiBi attention of a step's new tokens over a key / value cache held in 8 bits, and each other, on gfx950.
+//
+// The definition is the tree decode's (coalibi_tree.hip) with cached keys ks * kc and values vs * vc: codes kc, vc (e4m3 or
+// int8) and a scale for each kv head's block of 16 rows.  A code is a 16-bit type's own value, so the codes go into the
+// products as they are and the scales outside of them:
+//   t_j = sm_scale*log2(e) * ks * (q.kc_j),   a_j = t_j - slope*log2(e) * z_j,   a'_j = a_j + log2 vs,
+//   O   = sum_j 2^(a'_j - m) vc_j / l,   l = sum_j 2^(a'_j - m) / vs,   LSE = (m + log2 l) * ln 2.
+// The lane of a score holds the 16 keys of a block, so ks is a factor of its scores' one multiplication, log2 vs a part of
+// the one term that all of its exponents subtract, and 1 / vs one multiplication for their sum.
+//
+// A wavefront takes 32 query rows over a run of 32-key tiles, newest first, by itself: S^T = K Q^T and O^T += V^T P^T on MFMA,
+// the operands straight from memory into registers.
+//   K: a lane reads 16 bytes of its key's row, the codes of two k16 steps; Q is laid out to match.
+//   V: a lane reads D / 32 consecutive codes of each of its half's 16 keys; output row R of tile j is d = (D / 32) * R + j, so
+// they are one element of each tile's operand.  Two keys' codes are interleaved by byte permutes and converted as pairs.
+// There are no barriers and no LDS in the loop.  The four wavefronts of a work-group take four runs of a split's tiles and are
+// joined at its end, each one's maximum shifted by the sigmas of the keys after it, as splits are in the merge.
+#include <algorithm>
+
+#include "coalibi_tree.h"
+
+namespace coalibi {
+
+namespace {
+
+constexpr int kTree8Waves = 4;
+constexpr int kTree8Threads = 64 * kTree8Waves;
+
+typedef unsigned short u16;
+
+// Pair HI (bytes 0 and 1, or 2 and 3) of the codes in x, as two T.
+template <typename T, typename F, bool HI>
+__device__ __forceinline__ void code_pair(unsigned x, T* out) {
+  if constexpr (__is_same(F, E4M3)) {
+    if constexpr (__is_same(T, __bf16)) {
+      const auto p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, HI);
+      out[0] = p[0];
+      out[1] = p[1];
+    } else if constexpr (__is_same(T, _Float16)) {
+      const auto p = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, HI);
+      out[0] = p[0];
+      out[1] = p[1];
+    } else {
+      const auto p = __builtin_amdgcn_cvt_pk_f32_fp8(x, HI);
+      out[0] = p[0];
+      out[1] = p[1];
+    }
+  } else if constexpr (__is_same(T, _Float16)) {
+    // The byte plus 128 in the last bits of 1024: exact, and so is the difference.
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const unsigned h = __builtin_amdgcn_perm(0x64646464u, x ^ 0x80808080u, HI ? 0x05030402u : 0x05010400u);
+    const f16x2 p = __builtin_bit_cast(f16x2, h) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f};
+    out[0] = p[0];
+    out[1] = p[1];
+  } else {
+    out[0] = static_cast<T>(static_cast<float>(static_cast<signed char>(x >> (HI ? 16 : 0))));
+    out[1] = static_cast<T>(static_cast<float>(static_cast<signed char>(x >> (HI ? 24 : 8))));
+  }
+}
+
+// D / 32 consecutive codes, at least one.
+template <int DT>
+struct Run {
+  static constexpr int W = DT > 4 ? DT / 4 : 1;
+  unsigned w[W];
+  __device__ __forceinline__ void load(const char* p) {
+    if constexpr (DT == 8) {
+      const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+      w[0] = x[0];
+      w[1] = x[1];
+    } else if constexpr (DT == 4) {
+      w[0] = *reinterpret_cast<const unsigned*>(p);
+    } else if constexpr (DT == 2) {
+      w[0] = *reinterpret_cast<const u16*>(p);
+    } else {
+      w[0] = *reinterpret_cast<const unsigned char*>(p);
+    }
+  }
+};
+
+// A tile's codes as a lane holds them, and its half's scales.
+template <int D>
+struct Tile8 {
+  static constexpr int KL = D < 32 ? 1 : D / 32;  // 16-byte pieces of a key (D 16: 8 bytes)
+  static constexpr int DT = D < 32 ? 1 : D / 32;
+  u32x4 k[KL];
+  Run<DT> v[16];
+  float ks, vs;
+};
+
+template <typename T, int D>
+struct Tree8Cfg {
+  static constexpr int KS = D / 16;
+  static constexpr int DT = D < 32 ? 1 : D / 32;
+  static constexpr int LDO = D + 4;  // a wavefront's O rows in LDS, 16 bytes apart from a power of two
+  static constexpr int LDS_BYTES = kTree8Waves * 32 * LDO * 4;
+  static constexpr int WGS_PER_CU = D * sizeof(T) <= 256 ? 2 : 1;
+};
+
+// Whether a scale is one that the formulas hold for: from the smallest to the largest (a NaN is not).
+__device__ __forceinline__ bool scale_ok(float s) { return s >= kScaleLeast && s <= kScaleMost; }
+
+template <typename T, typename F, int D>
+__global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void coalibi_tree8_kernel(Tree8Args a8) {
+  using C = Tree8Cfg<T, D>;
+  using M = Mfma<T>;
+  using V8 = typename M::vec8;
+  constexpr int DT = C::DT;
+  const TreeArgs& a = a8.t;
+  __shared__ __align__(16) char smem[C::LDS_BYTES];
+  __shared__ float sMax[kTree8Waves][32], sSum[kTree8Waves][32], sSig[kTree8Waves][32], sScale[kTree8Waves][32];
+  __shared__ bool sLost[kTree8Waves];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int hl = lane & 31, hh = lane >> 5;
+  // Ids: the row blocks of an item (split, sequence, kv head) 8 apart, so that they share an XCD and its L2.
+  const int RB = a.row_blocks, id = blockIdx.x;
+  const int rb = (id >> 3) % RB, item = (id / (8 * RB)) * 8 + (id & 7);
+  const int nS = a.nSplits;
+  int cps = a.cps;
+  TreeItem it{item / nS, item % nS};
+  if (a.plan) {
+    cps = plan_cps(a, lane);
+    it = plan_item(a, cps, item, lane);
+    if (it.bhk < 0) return;
+  } else if (it.bhk >= a.B * a.Hkv) {
+    return;
+  }
+  const int bhk = __builtin_amdgcn_readfirstlane(it.bhk), split = __builtin_amdgcn_readfirstlane(it.split);
+  const int b = __builtin_amdgcn_readfirstlane(bhk / a.Hkv), hkv = bhk - b * a.Hkv;
+  const int L = __builtin_amdgcn_readfirstlane(filled_rows(a, b));
+  const int chunks = __builtin_amdgcn_readfirstlane(chunks_of(a, L));
+  TreeSplits sp = splits_of(a, cps, chunks);
+  sp = {__builtin_amdgcn_readfirstlane(sp.cps), __builtin_amdgcn_readfirstlane(sp.used)};
+  if (split >= sp.used) return;
+  const bool newest = split == sp.used - 1;
+
+  // The split's tiles: of the filled rows, then (in the newest) of the new keys, shared out over the wavefronts in order.
+  const int cache_tiles = (L + 31) >> 5, fresh_tiles = (a.T + 31) >> 5, per_chunk = a.chunk >> 5;
+  const int t0 = min(split * sp.cps * per_chunk, cache_tiles);
+  const int t1 = newest ? cache_tiles + fresh_tiles : min((split + 1) * sp.cps * per_chunk, cache_tiles);
+  const int per = (t1 - t0 + kTree8Waves - 1) / kTree8Waves;
+  const int t_first = min(t0 + wave * per, t1), t_end = min(t_first + per, t1);
+
+  const int R = a.G * a.T, row = rb * 32 + hl;
+  const bool row_ok = row < R;
+  const int rsafe = row_ok ? row : 0;
+  const int g = rsafe / a.T, t = rsafe - g * a.T, h = hkv * a.G + g;
+  const float lam2 = a.slopes[h] * kLog2e;
+
+  unsigned long long sees = 0;
+  if (newest) {
+    if (tid == 0 && nS > 1) a.used[bhk] = sp.used;
+    const unsigned long long all = ancestors(a, b, lane);
+    sees = (unsigned long long)__shfl((unsigned)(all >> 32), t, 64) << 32 | __shfl((unsigned)all, t, 64);
+  }
+
+  const T* const kn = head_at(static_cast<const T*>(a.k), a.kl, b, hkv);
+  const T* const vn = head_at(static_cast<const T*>(a.v), a.vl, b, hkv);
+  const char* const kc = static_cast<const char*>(a.kc) + (size_t)hkv * a.kcl.h;
+  const char* const vc = static_cast<const char*>(a.vc) + (size_t)hkv * a.vcl.h;
+  const float* const ksc = a8.ks + (size_t)hkv * a8.ksh;
+  const float* const vsc = a8.vs + (size_t)hkv * a8.vsh;
+  const int page_mask = a.place.table != nullptr ? (1 << a.place.page_shift) - 1 : 0x7fffffff;
+
+  // The units of a tile's two blocks of 16 rows, -1 for a block on no page of the pool (its rows are read from unit 0).
+  struct Units {
+    int u[2];
+  };
+  auto find = [&](int tile) {
+    Units f{{b, b}};
+    if (a.place.table != nullptr) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int r = min(tile * 32 + 16 * i, L - 1);
+        const int u = scalar_load(a.place.table + (size_t)b * a.place.table_stride + (r >> a.place.page_shift));
+        f.u[i] = u >= 0 && u < a.place.units ? u : -1;
+      }
+    }
+    return f;
+  };
+  bool lost = false;
+  // A cached tile's loads.  Rows past the filled ones are read from the last of them: their scores are masked.
+  auto load = [&](int tile, const Units& f) {
+    Tile8<D> x;
+    lost |= (f.u[0] | f.u[1]) < 0;
+    const int u0 = max(f.u[0], 0), u1 = max(f.u[1], 0);
+    const int key0 = tile * 32;
+    {
+      const int key = min(key0 + kRowOfReg(hl), L - 1);
+      const char* const base0 = kc + (size_t)u0 * a.kcl.b;
+      const char* const base1 = kc + (size_t)u1 * a.kcl.b;
+      const char* const p = (kRowOfReg(hl) >= 16 ? base1 : base0) + (size_t)(key & page_mask) * D;
+      if constexpr (D < 32) {
+        const u32x2 lo = *reinterpret_cast<const u32x2*>(p + hh * 8);
+        x.k[0] = u32x4{lo[0], lo[1], 0, 0};
+      } else {
+#pragma unroll
+        for (int i = 0; i < Tile8<D>::KL; ++i) x.k[i] = ld16(p + 32 * i + 16 * hh);
+      }
+    }
+    const int first = min(key0 + 16 * hh, L - 1);  // the half's first key
+    const int u = hh ? u1 : u0;
+    {
+      const size_t at = (first & page_mask) >> 4;
+      x.ks = ksc[(size_t)u * a8.ksb + at];
+      x.vs = vsc[(size_t)u * a8.vsb + at];
+    }
+    const char* const p = vc + (size_t)u * a.vcl.b + (size_t)(first & page_mask) * D + (D < 32 ? hl & 15 : DT * hl);
+    if (key0 + 32 <= L) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x.v[i].load(p + i * D);
+    } else {
+      const int left = L - 1 - first;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x.v[i].load(p + min(i, left) * D);
+    }
+    return x;
+  };
+
+  // Q^T fragments in the order of K's: step 2 i + s holds the elements 32 i + 16 (l / 32) + 8 s + e of the row (D 16: 8 (l / 32)
+  // + e).  Zero past R.
+  V8 qf[C::KS];
+  {
+    const T* const q = head_at(static_cast<const T*>(a.q), a.ql, b, h) + (size_t)t * a.ql.r;
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks)
+      qf[ks] = row_ok ? ld_vec8(q + (D < 32 ? 8 * hh : (ks >> 1) * 32 + 16 * hh + (ks & 1) * 8)) : zero_vec8<T>();
+  }
+
+  // State of the lane's row: scale, this half's share of the sum, O^T, and the sigma of the keys after the current ones.
+  float m2 = kNegInf, lsum = 0.f, carry = 0.f;
+  f32x16 acc[DT];
+#pragma unroll
+  for (int j = 0; j < DT; ++j) acc[j] = f32x16{};
+
+  // From a tile's scores (log2 units; -inf where the row does not see the key) to its weights, in the order of P^T.
+  auto weigh = [&](f32x16 s, float vs, V8 (&pb)[2]) {
+    float loc[16], run = 0.f;
+#pragma unroll
+    for (int r = 15; r >= 0; --r) {
+      run += sigmoid_log2(s[r]);
+      loc[r] = run;
+    }
+    const float oth = other_half(run);
+    const float mb = m2 == kNegInf ? 0.f : m2;
+    const float cst = mb + lam2 * (carry + (hh ? 0.f : oth)) - __builtin_amdgcn_logf(vs);
+    carry += hh ? run + oth : oth + run;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = fmaf(-lam2, loc[r], s[r] - cst);
+    auto weights = [&] {
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f32x8 p;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          p[e] = fast_exp2(s[8 * i + e]);
+          sum += p[e];  // before the rounding for the product: the LSE is fp32's
+        }
+        pb[i] = M::pack(p);
+      }
+      return sum;
+    };
+    float sum = weights();
+    if (__any(m2 == kNegInf || sum > kTreeRescale)) {
+      float mt = kNegInf;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[r]);
+      mt = fmaxf(mt, other_half(mt));
+      const bool need = mt > (m2 == kNegInf ? kNegInf : 0.f);
+      const float delta = need ? mt : 0.f;
+      const float alpha = need ? (m2 == kNegInf ? 0.f : fast_exp2(-delta)) : 1.f;
+      m2 = need ? mb + delta : m2;
+      lsum *= alpha;
+#pragma unroll
+      for (int j = 0; j < DT; ++j) acc[j] *= alpha;
+      s -= delta;
+      sum = weights();
+    }
+    lsum = fmaf(sum, fast_rcp(vs), lsum);
+  };
+
+  int tile = t_end - 1;
+  // The new keys' tiles.
+  for (; tile >= t_first && tile >= cache_tiles; --tile) {
+    const int key0 = (tile - cache_tiles) * 32;
+    f32x16 s{};
+    {
+      const T* const k = kn + (size_t)min(key0 + kRowOfReg(hl), a.T - 1) * a.kl.r;
+#pragma unroll
+      for (int ks = 0; ks < C::KS; ++ks)
+        s = M::k16(ld_vec8(k + (D < 32 ? 8 * hh : (ks >> 1) * 32 + 16 * hh + (ks & 1) * 8)), qf[ks], s);
+    }
+    const unsigned ok = (unsigned)(sees >> (key0 + 16 * hh));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = ok >> r & 1 ? s[r] * a.sc2 : kNegInf;
+    V8 pb[2];
+    weigh(s, 1.0f, pb);
+    // A product with a weight of 0 would carry an infinity or a NaN of a value to rows that do not see it: such values are 0
+    // here and added to the rows that do below.
+    unsigned bad = 0;
+#pragma unroll
+    for (int st = 0; st < 2; ++st)
+#pragma unroll
+      for (int j = 0; j < DT; ++j) {
+        V8 va;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int key = 16 * hh + 8 * st + e;
+          T x = vn[(size_t)min(key0 + key, a.T - 1) * a.vl.r + (D < 32 ? hl & 15 : DT * hl + j)];
+          if (not_finite(x)) {
+            x = T(0);
+            bad |= 1u << key;
+          }
+          va[e] = x;
+        }
+        acc[j] = M::k16(va, pb[st], acc[j]);
+      }
+    if (__any(bad != 0)) {
+      for (int key = 0; key < min(a.T - key0, 32); ++key) {
+        if (!__any(bad >> key & 1)) continue;
+        if (sees >> (key0 + key) & 1) {
+#pragma unroll
+          for (int j = 0; j < DT; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+              const int d = DT * ((r >> 2) * 8 + hh * 4 + (r & 3)) + j;
+              if (d >= D) continue;
+              const T x = vn[(size_t)(key0 + key) * a.vl.r + d];
+              if (not_finite(x)) acc[j][r] += static_cast<float>(x);
+            }
+        }
+      }
+    }
+  }
+
+  // The cache's tiles, each one's codes loaded while the one before is worked on, and its units another one before.
+  if (tile >= t_first) {
+    Units units = find(tile);
+    Tile8<D> cur = load(tile, units);
+    units = find(max(tile - 1, t_first));
+    for (; tile >= t_first; --tile) {
+      Tile8<D> next;
+      if (tile > t_first) {
+        next = load(tile - 1, units);
+        units = find(max(tile - 2, t_first));
+      }
+      f32x16 s{};
+#pragma unroll
+      for (int ks = 0; ks < C::KS; ++ks) {
+        T x[8];
+        const unsigned lo = cur.k[ks >> 1][2 * (ks & 1)], hi = cur.k[ks >> 1][2 * (ks & 1) + 1];
+        code_pair<T, F, false>(lo, x);
+        code_pair<T, F, true>(lo, x + 2);
+        code_pair<T, F, false>(hi, x + 4);
+        code_pair<T, F, true>(hi, x + 6);
+        s = M::k16(V8{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]}, qf[ks], s);
+      }
+      const bool fine = scale_ok(cur.ks) && scale_ok(cur.vs);
+      lost |= !fine;
+      const float vs = fine ? cur.vs : 1.f, sc = a.sc2 * cur.ks;
+      const int left = L - tile * 32 - 16 * hh;
+      if (tile * 32 + 32 > L) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = r < left ? s[r] * sc : kNegInf;
+      } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= sc;
+      }
+      V8 pb[2];
+      weigh(s, vs, pb);
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+#pragma unroll
+        for (int jj = 0; jj < (DT + 1) / 2; ++jj) {
+          T x[2][8];
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            // Keys e and e + 1 of the step: [d, d, d + 1, d + 1].
+            const unsigned w = __builtin_amdgcn_perm(cur.v[8 * st + e + 1].w[jj >> 1], cur.v[8 * st + e].w[jj >> 1],
+                                                     jj & 1 ? 0x07030602u : 0x05010400u);
+            code_pair<T, F, false>(w, &x[0][e]);
+            if constexpr (DT > 1) code_pair<T, F, true>(w, &x[1][e]);
+          }
+#pragma unroll
+          for (int i = 0; i < (DT > 1 ? 2 : 1); ++i)
+            acc[2 * jj + i] = M::k16(V8{x[i][0], x[i][1], x[i][2], x[i][3], x[i][4], x[i][5], x[i][6], x[i][7]}, pb[st],
+                                     acc[2 * jj + i]);
+        }
+      }
+      cur = next;
+    }
+  }
+
+  // The wavefronts joined: each one's maximum shifted by the sigmas of the later ones' keys.
+  const float l = lsum + other_half(lsum);
+  const bool any_lost = __any(lost);
+  if (lane == 0) sLost[wave] = any_lost;
+  if (hh == 0) {
+    sMax[wave][hl] = m2;
+    sSum[wave][hl] = l;
+    sSig[wave][hl] = carry;
+  }
+  __syncthreads();
+  if (tid < 32) {  // lane tid holds row tid
+    float after = 0.f, m = kNegInf, mw[kTree8Waves];
+    bool gone = false;
+#pragma unroll
+    for (int w = kTree8Waves - 1; w >= 0; --w) {
+      mw[w] = sMax[w][tid] - lam2 * after;
+      after += sSig[w][tid];
+      m = fmaxf(m, mw[w]);
+      gone |= sLost[w];
+    }
+    float ls = 0.f, f[kTree8Waves];
+#pragma unroll
+    for (int w = 0; w < kTree8Waves; ++w) {
+      const bool none = mw[w] == kNegInf;
+      f[w] = none ? 0.f : fast_exp2(mw[w] - m);
+      ls += none && sSum[w][tid] == 0.f ? 0.f : f[w] * sSum[w][tid];
+    }
+    // The sum to [1, 2): the merge takes it for at least 1, and the scales of V have moved it.
+    const int e = ls > 0.f && ls < __builtin_inff() ? __builtin_amdgcn_frexp_expf(ls) - 1 : 0;
+#pragma unroll
+    for (int w = 0; w < kTree8Waves; ++w) sScale[w][tid] = ldexpf(f[w], -e);
+    sMax[0][tid] = m + static_cast<float>(e);
+    sSum[0][tid] = gone ? __builtin_nanf("") : ldexpf(ls, -e);
+    sSig[0][tid] = after;
+  }
+  __syncthreads();
+  float* const so = reinterpret_cast<float*>(smem) + (size_t)wave * 32 * C::LDO + hl * C::LDO;
+  const float f = sScale[wave][hl];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int d = DT * ((r >> 2) * 8 + hh * 4 + (r & 3));
+    if (d < D) {
+#pragma unroll
+      for (int j = 0; j < DT; ++j) so[d + j] = acc[j][r] * f;
+    }
+  }
+  const size_t row0 = (size_t)bhk * R + rb * 32;  // the block's first row in o, lse and the partials
+  const int rows = min(R - rb * 32, 32);
+  const bool direct = sp.used == 1;
+  if (wave == 0 && hh == 0 && row_ok) {
+    const bool absent = newest && sees == 0;
+    if (direct) {
+      const float ls = sSum[0][hl];
+      if (a.lse != nullptr) a.lse[row0 + hl] = absent ? kNegInf : (sMax[0][hl] + log2f(ls)) * kLn2;
+      sSig[1][hl] = absent ? 0.f : 1.f / ls;
+      sMax[1][hl] = absent ? 0.f : 1.f;
+    } else {
+      const size_t pi = (row0 + hl) * nS + split;
+      a.pmax[pi] = sMax[0][hl];
+      a.psum[pi] = absent ? kAbsent : sSum[0][hl];
+      a.psig[pi] = sSig[0][hl];
+    }
+  }
+  __syncthreads();
+  for (int i = tid; i < rows * (D / 4); i += kTree8Threads) {
+    const int r = i / (D / 4), d = (i - r * (D / 4)) * 4;
+    f32x4 s = f32x4{};
+#pragma unroll
+    for (int w = 0; w < kTree8Waves; ++w)
+      s += *reinterpret_cast<const f32x4*>(reinterpret_cast<float*>(smem) + ((size_t)w * 32 + r) * C::LDO + d);
+    if (direct) {
+      typedef T out4 __attribute__((ext_vector_type(4)));
+      const bool there = sMax[1][r] != 0.f;
+      const float inv = sSig[1][r];
+      out4 v;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = static_cast<T>(there ? s[e] * inv : 0.f);
+      *reinterpret_cast<out4*>(static_cast<T*>(a.o) + (row0 + r) * D + d) = v;
+    } else {
+      *reinterpret_cast<f32x4*>(a.pout + ((row0 + r) * nS + split) * D + d) = s;
+    }
+  }
+}
+
+}  // namespace
+
+template <typename T, typename F, int D>
+hipError_t launch_tree8(const Tree8Args& a8, hipStream_t stream) {
+  const TreeArgs& a = a8.t;
+  // Under a plan at most one round of work-groups and a rounded-up split per sequence.
+  const long long even = (long long)a.B * a.Hkv * a.nSplits;
+  const long long items = a.plan ? std::min<long long>(even, ((long long)a.share + a.B) * a.Hkv) : even;
+  const dim3 grid(static_cast<unsigned>((items + 7) / 8 * 8 * a.row_blocks));
+  hipLaunchKernelGGL((coalibi_tree8_kernel<T, F, D>), grid, dim3(kTree8Threads), 0, stream, a8);
+  const hipError_t e = hipGetLastError();
+  return e != hipSuccess || a.nSplits == 1 ? e : launch_tree_merge<T, D>(a, stream);
+}
+
+#define COALIBI_INST_TREE8(T, D)                                                 \
+  template hipError_t launch_tree8<T, E4M3, D>(const Tree8Args&, hipStream_t);   \
+  template hipError_t launch_tree8<T, I8, D>(const Tree8Args&, hipStream_t);
+COALIBI_INST_TREE8(_Float16, 16)
+COALIBI_INST_TREE8(_Float16, 32)
+COALIBI_INST_TREE8(_Float16, 64)
+COALIBI_INST_TREE8(_Float16, 128)
+COALIBI_INST_TREE8(_Float16, 256)
+COALIBI_INST_TREE8(__bf16, 16)
+COALIBI_INST_TREE8(__bf16, 32)
+COALIBI_INST_TREE8(__bf16, 64)
+COALIBI_INST_TREE8(__bf16, 128)
+COALIBI_INST_TREE8(__bf16, 256)
+COALIBI_INST_TREE8(float, 16)
+COALIBI_INST_TREE8(float, 32)
+COALIBI_INST_TREE8(float, 64)
+COALIBI_INST_TREE8(float, 128)
+
+}  // namespace coalibi

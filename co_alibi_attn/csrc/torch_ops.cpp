@@ -10,6 +10,12 @@
 //                         with_lse) -> (o, lse)
 //   co_alibi::cache_append(k, v, k_cache!, v_cache!, seq_lens, counts, rows, block_table) -> ()
 //   co_alibi::sample(logits, uniforms, temperature, top_k, top_p, min_p, their four values for every row) -> tokens
+//   co_alibi::decode_tree_8bit(q, k, v, k_cache, v_cache, k_scale, v_scale, slopes, seq_lens, parents, block_table, max_seq_len,
+//                              sm_scale, with_lse) -> (o, lse)
+//   co_alibi::cache_append_8bit(k, v, k_cache!, v_cache!, k_scale!, v_scale!, seq_lens, counts, rows, block_table) -> ()
+//   co_alibi::cache_read_8bit(k_cache, v_cache, k_scale, v_scale, seq_lens, first, block_table, rows, dtype) -> (k, v)
+//   co_alibi::beam_select(logits, scores, finished, num_beams, end_token) -> (scores, parents, tokens)
+//   co_alibi::cache_reorder(caches!, block_table, pages, seq_lens, parents, page_size) -> (block_table, seq_lens)
 //
 // They replace the reference's two Triton launches with their buffer set-up
 // (co_alibi_attn/co_alibi_attn.py:35-57 and :83-133); decode and the operators after it have no counterpart there.  Each
@@ -36,6 +42,7 @@
 #include <cstdint>
 #include <cstdlib>
 #include <tuple>
+#include <vector>
 
 #include "../../include/co_alibi.h"
 
@@ -361,11 +368,11 @@ struct Caches {
   int64_t blocks = 0, units = 0, page = 0, capacity = 0;
 };
 Caches check_caches(const char* fn, const Tensor& like, int64_t batch, const Tensor& k_cache, const Tensor& v_cache,
-                    const c10::optional<Tensor>& block_table) {
+                    const c10::optional<Tensor>& block_table, bool eight = false) {
   TORCH_CHECK_VALUE(k_cache.dim() == 4 && v_cache.sizes() == k_cache.sizes(), fn,
                     ": k_cache and v_cache must be 4-dimensional and of one shape, got ", k_cache.sizes(), " and ",
                     v_cache.sizes());
-  TORCH_CHECK_TYPE(k_cache.scalar_type() == like.scalar_type() && v_cache.scalar_type() == like.scalar_type(), fn,
+  TORCH_CHECK_TYPE(eight || (k_cache.scalar_type() == like.scalar_type() && v_cache.scalar_type() == like.scalar_type()), fn,
                    ": the caches' dtype must be the new tokens', ", like.scalar_type(), ", got ", k_cache.scalar_type(),
                    " and ", v_cache.scalar_type());
   TORCH_CHECK_VALUE(k_cache.device() == like.device() && v_cache.device() == like.device(), fn,
@@ -397,12 +404,16 @@ int as_int(const char* fn, const char* name, int64_t x) {
   return static_cast<int>(x);
 }
 
-std::tuple<Tensor, Tensor> decode_tree_hip(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
-                                           const Tensor& k_cache, const Tensor& v_cache, const Tensor& slopes,
-                                           const c10::optional<Tensor>& seq_lens, const c10::optional<Tensor>& parents,
-                                           const c10::optional<Tensor>& block_table, int64_t max_seq_len, double sm_scale,
-                                           bool with_lse) {
-  const char* fn = "co_alibi::decode_tree";
+// What the tree decodes check of their inputs, and the index arrays as the kernels read them.
+struct TreeInputs {
+  int code;
+  Caches caches;
+  Tensor lens, parents;
+};
+TreeInputs check_tree(const char* fn, const Tensor& q_in, const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache,
+                      const Tensor& v_cache, const Tensor& slopes, const c10::optional<Tensor>& seq_lens,
+                      const c10::optional<Tensor>& parents, const c10::optional<Tensor>& block_table, int64_t max_seq_len,
+                      bool eight) {
   TORCH_CHECK_VALUE(q_in.dim() == 4 && k_in.dim() == 4 && v_in.sizes() == k_in.sizes(), fn,
                     ": q must be (B, Hq, T, D) and k, v (B, Hkv, T, D), got ", q_in.sizes(), ", ", k_in.sizes(), " and ",
                     v_in.sizes());
@@ -414,26 +425,41 @@ std::tuple<Tensor, Tensor> decode_tree_hip(const Tensor& q_in, const Tensor& k_i
                    ": q, k and v must share one dtype");
   TORCH_CHECK_VALUE(k_in.device() == q_in.device() && v_in.device() == q_in.device(), fn,
                     ": q, k and v must be on one device");
-  const int code = dtype_code(q_in.scalar_type());
+  TreeInputs in;
+  in.code = dtype_code(q_in.scalar_type());
   c10::hip::HIPGuard guard(q_in.device().index());
-  const Caches c = check_caches(fn, q_in, batch, k_cache, v_cache, block_table);
+  in.caches = check_caches(fn, q_in, batch, k_cache, v_cache, block_table, eight);
+  const Caches& c = in.caches;
   TORCH_CHECK_VALUE(k_cache.size(1) == heads_kv && k_cache.size(3) == head_dim, fn,
                     ": the caches must have k's heads and head dim, got ", k_cache.sizes(), " for ", k_in.sizes());
   TORCH_CHECK_VALUE(slopes.dim() == 1 && slopes.size(0) == heads_q, fn, ": slopes must be (", heads_q, ",), got ", slopes.sizes());
   TORCH_CHECK_VALUE(max_seq_len >= 0 && max_seq_len <= c.capacity, fn, ": max_seq_len must be in [0, ", c.capacity, "], got ",
                     max_seq_len);
-  Tensor lens, par;
   if (given(seq_lens)) {
     TORCH_CHECK_VALUE(seq_lens->dim() == 1 && seq_lens->size(0) == batch, fn, ": seq_lens must be (", batch, ",), got ",
                       seq_lens->sizes());
-    lens = index_i32(*seq_lens, q_in);
+    in.lens = index_i32(*seq_lens, q_in);
   }
   if (given(parents)) {
     const bool one = parents->dim() == 1 && parents->size(0) == tokens;
     TORCH_CHECK_VALUE(one || (parents->dim() == 2 && parents->size(0) == batch && parents->size(1) == tokens), fn,
                       ": parents must be (", tokens, ",) or (", batch, ", ", tokens, "), got ", parents->sizes());
-    par = index_i32(*parents, q_in);
+    in.parents = index_i32(*parents, q_in);
   }
+  return in;
+}
+
+std::tuple<Tensor, Tensor> decode_tree_hip(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
+                                           const Tensor& k_cache, const Tensor& v_cache, const Tensor& slopes,
+                                           const c10::optional<Tensor>& seq_lens, const c10::optional<Tensor>& parents,
+                                           const c10::optional<Tensor>& block_table, int64_t max_seq_len, double sm_scale,
+                                           bool with_lse) {
+  const char* fn = "co_alibi::decode_tree";
+  const auto [code, c, lens, par] =
+      check_tree(fn, q_in, k_in, v_in, k_cache, v_cache, slopes, seq_lens, parents, block_table, max_seq_len, false);
+  c10::hip::HIPGuard guard(q_in.device().index());
+  const int64_t batch = q_in.size(0), heads_q = q_in.size(1), tokens = q_in.size(2), head_dim = q_in.size(3);
+  const int64_t heads_kv = k_in.size(1);
   const auto f32 = q_in.options().dtype(at::kFloat);
   Tensor o = at::empty(q_in.sizes(), q_in.options());
   Tensor lse = with_lse ? at::empty({batch, heads_q, tokens}, f32) : empty_stats(q_in);
@@ -461,35 +487,52 @@ std::tuple<Tensor, Tensor> decode_tree_hip(const Tensor& q_in, const Tensor& k_i
   return {o, lse};
 }
 
-void cache_append_hip(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache, const Tensor& v_cache,
-                      const Tensor& seq_lens, const c10::optional<Tensor>& counts, const c10::optional<Tensor>& rows,
-                      const c10::optional<Tensor>& block_table) {
-  const char* fn = "co_alibi::cache_append";
+// What the appends check of their inputs, and the index arrays as the kernels read them.
+struct AppendInputs {
+  int code;
+  Caches caches;
+  Tensor lens, counts, rows;
+  int64_t new_rows;
+};
+AppendInputs check_append(const char* fn, const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache, const Tensor& v_cache,
+                          const Tensor& seq_lens, const c10::optional<Tensor>& counts, const c10::optional<Tensor>& rows,
+                          const c10::optional<Tensor>& block_table, bool eight) {
   TORCH_CHECK_VALUE(k_in.dim() == 4 && v_in.sizes() == k_in.sizes(), fn, ": k and v must be (B, Hkv, T, D), got ",
                     k_in.sizes(), " and ", v_in.sizes());
   TORCH_CHECK_TYPE(v_in.scalar_type() == k_in.scalar_type(), fn, ": k and v must share one dtype");
   TORCH_CHECK_VALUE(v_in.device() == k_in.device(), fn, ": k and v must be on one device");
   const int64_t batch = k_in.size(0), heads_kv = k_in.size(1), tokens = k_in.size(2), head_dim = k_in.size(3);
-  const int code = dtype_code(k_in.scalar_type());
+  AppendInputs in;
+  in.code = dtype_code(k_in.scalar_type());
   c10::hip::HIPGuard guard(k_in.device().index());
-  const Caches c = check_caches(fn, k_in, batch, k_cache, v_cache, block_table);
+  in.caches = check_caches(fn, k_in, batch, k_cache, v_cache, block_table, eight);
   TORCH_CHECK_VALUE(k_cache.size(1) == heads_kv && k_cache.size(3) == head_dim, fn,
                     ": the caches must have k's heads and head dim, got ", k_cache.sizes(), " for ", k_in.sizes());
   TORCH_CHECK_VALUE(seq_lens.dim() == 1 && seq_lens.size(0) == batch, fn, ": seq_lens must be (", batch, ",), got ",
                     seq_lens.sizes());
-  const Tensor lens = index_i32(seq_lens, k_in);
-  Tensor cnt, idx;
+  in.lens = index_i32(seq_lens, k_in);
   if (given(counts)) {
     TORCH_CHECK_VALUE(counts->dim() == 1 && counts->size(0) == batch, fn, ": counts must be (", batch, ",), got ",
                       counts->sizes());
-    cnt = index_i32(*counts, k_in);
+    in.counts = index_i32(*counts, k_in);
   }
-  int64_t new_rows = tokens;
+  in.new_rows = tokens;
   if (given(rows)) {
     TORCH_CHECK_VALUE(rows->dim() == 2 && rows->size(0) == batch, fn, ": rows must be (", batch, ", n), got ", rows->sizes());
-    idx = index_i32(*rows, k_in);
-    new_rows = idx.size(1);
+    in.rows = index_i32(*rows, k_in);
+    in.new_rows = in.rows.size(1);
   }
+  return in;
+}
+
+void cache_append_hip(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache, const Tensor& v_cache,
+                      const Tensor& seq_lens, const c10::optional<Tensor>& counts, const c10::optional<Tensor>& rows,
+                      const c10::optional<Tensor>& block_table) {
+  const char* fn = "co_alibi::cache_append";
+  const auto [code, c, lens, cnt, idx, new_rows] =
+      check_append(fn, k_in, v_in, k_cache, v_cache, seq_lens, counts, rows, block_table, false);
+  c10::hip::HIPGuard guard(k_in.device().index());
+  const int64_t batch = k_in.size(0), heads_kv = k_in.size(1), tokens = k_in.size(2), head_dim = k_in.size(3);
   if (k_in.numel() == 0 || new_rows == 0 || k_cache.numel() == 0 || c.capacity == 0) return;
   const Tensor k = in_place(k_in), v = in_place(v_in);
   const auto strides = all_strides<4>({k, v, k_cache, v_cache});
@@ -500,6 +543,222 @@ void cache_append_hip(const Tensor& k_in, const Tensor& v_in, const Tensor& k_ca
                               as_int(fn, "tokens", tokens), as_int(fn, "head_dim", head_dim), current_stream(k)));
   for (const Tensor* t : {&k_cache, &v_cache})  // autograd's record of a write in place
     if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+// An 8-bit cache: its format, and the scales beside its codes, read and written in place, too.
+int format_code(const char* fn, const Tensor& k_cache, const Tensor& v_cache) {
+  const auto t = k_cache.scalar_type();
+  TORCH_CHECK_TYPE((t == at::kFloat8_e4m3fn || t == at::kChar) && v_cache.scalar_type() == t, fn,
+                   ": the caches must both be float8_e4m3fn or int8, got ", t, " and ", v_cache.scalar_type());
+  return t == at::kChar ? CO_ALIBI_INT8 : CO_ALIBI_E4M3;
+}
+struct Scales {
+  std::array<long long, 4> strides;  // (unit, head) of k's, then of v's
+};
+Scales check_scales(const char* fn, const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale, const Tensor& v_scale) {
+  const std::array<int64_t, 3> want{k_cache.size(0), k_cache.size(1), (k_cache.size(2) + 15) / 16};
+  for (const Tensor* t : {&k_scale, &v_scale}) {
+    TORCH_CHECK_VALUE(t->sizes() == at::IntArrayRef(want), fn, ": the scales must be ", at::IntArrayRef(want), ", got ", t->sizes());
+    TORCH_CHECK_TYPE(t->scalar_type() == at::kFloat, fn, ": the scales must be float32, got ", t->scalar_type());
+    TORCH_CHECK_VALUE(t->device() == k_cache.device(), fn, ": the scales must be on the caches' device");
+    TORCH_CHECK_VALUE(t->size(2) <= 1 || t->stride(2) == 1, fn, ": a head's scales must follow one another");
+  }
+  for (const Tensor* t : {&k_cache, &v_cache})
+    TORCH_CHECK_VALUE(t->numel() == 0 || t->size(2) == 1 || t->stride(2) == t->size(3), fn,
+                      ": the rows of an 8-bit cache must be dense");
+  return {{k_scale.stride(0), k_scale.stride(1), v_scale.stride(0), v_scale.stride(1)}};
+}
+
+std::tuple<Tensor, Tensor> decode_tree_8bit_hip(const Tensor& q_in, const Tensor& k_in, const Tensor& v_in,
+                                                const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
+                                                const Tensor& v_scale, const Tensor& slopes,
+                                                const c10::optional<Tensor>& seq_lens, const c10::optional<Tensor>& parents,
+                                                const c10::optional<Tensor>& block_table, int64_t max_seq_len,
+                                                double sm_scale, bool with_lse) {
+  const char* fn = "co_alibi::decode_tree_8bit";
+  const TreeInputs in = check_tree(fn, q_in, k_in, v_in, k_cache, v_cache, slopes, seq_lens, parents, block_table, max_seq_len, true);
+  const int format = format_code(fn, k_cache, v_cache);
+  const Scales sc = check_scales(fn, k_cache, v_cache, k_scale, v_scale);
+  c10::hip::HIPGuard guard(q_in.device().index());
+  const int64_t batch = q_in.size(0), heads_q = q_in.size(1), tokens = q_in.size(2), head_dim = q_in.size(3);
+  const int64_t heads_kv = k_in.size(1);
+  Tensor o = at::empty(q_in.sizes(), q_in.options());
+  Tensor lse = with_lse ? at::empty({batch, heads_q, tokens}, q_in.options().dtype(at::kFloat)) : empty_stats(q_in);
+  if (q_in.numel() == 0) return {o, lse};
+  const Tensor q = in_place(q_in), k = in_place(k_in), v = in_place(v_in);
+  // A pool without rows, or behind a table without blocks, is never read; the launch wants addresses all the same.
+  const bool none = k_cache.numel() == 0 || in.caches.capacity == 0;
+  TORCH_CHECK_VALUE(!none || max_seq_len == 0, fn, ": the caches hold no rows");
+  const Tensor sl = slopes_f32(slopes, q);
+  const size_t ws_bytes = co_alibi_decode_tree_8bit_workspace_bytes(
+      in.code, as_int(fn, "batch", batch), as_int(fn, "heads", heads_q), as_int(fn, "heads", heads_kv),
+      as_int(fn, "tokens", tokens), as_int(fn, "max_seq_len", max_seq_len), as_int(fn, "head_dim", head_dim));
+  Tensor ws;
+  if (ws_bytes != 0) ws = at::empty({static_cast<int64_t>(ws_bytes)}, q.options().dtype(at::kByte));
+  const auto new_strides = all_strides<3>({q, k, v});
+  std::array<long long, 15> strides{};
+  std::copy(new_strides.begin(), new_strides.end(), strides.begin());
+  strides[11] = strides[14] = head_dim;
+  if (!none) {
+    const auto cache_strides = all_strides<2>({k_cache, v_cache});
+    std::copy(cache_strides.begin(), cache_strides.end(), strides.begin() + 9);
+  }
+  const void* const spare = k.data_ptr();
+  check(co_alibi_decode_tree_8bit(
+      in.code, format, q.data_ptr(), k.data_ptr(), v.data_ptr(), none ? spare : k_cache.data_ptr(),
+      none ? spare : v_cache.data_ptr(), none ? static_cast<const float*>(spare) : k_scale.data_ptr<float>(),
+      none ? static_cast<const float*>(spare) : v_scale.data_ptr<float>(), strides.data(), sc.strides.data(),
+      sl.data_ptr<float>(), data_or_null(in.lens), data_or_null(in.parents),
+      in.parents.defined() && in.parents.dim() == 2 ? 1 : 0, none ? nullptr : data_or_null(in.caches.table),
+      as_int(fn, "blocks", in.caches.blocks), as_int(fn, "pages", in.caches.units),
+      none ? 1 : as_int(fn, "page", in.caches.page), o.data_ptr(), with_lse ? lse.data_ptr<float>() : nullptr,
+      ws.defined() ? ws.data_ptr() : nullptr, ws_bytes, batch, heads_q, heads_kv, tokens, max_seq_len, head_dim,
+      static_cast<float>(sm_scale), current_stream(q)));
+  return {o, lse};
+}
+
+void cache_append_8bit_hip(const Tensor& k_in, const Tensor& v_in, const Tensor& k_cache, const Tensor& v_cache,
+                           const Tensor& k_scale, const Tensor& v_scale, const Tensor& seq_lens,
+                           const c10::optional<Tensor>& counts, const c10::optional<Tensor>& rows,
+                           const c10::optional<Tensor>& block_table) {
+  const char* fn = "co_alibi::cache_append_8bit";
+  const AppendInputs in = check_append(fn, k_in, v_in, k_cache, v_cache, seq_lens, counts, rows, block_table, true);
+  const int format = format_code(fn, k_cache, v_cache);
+  const Scales sc = check_scales(fn, k_cache, v_cache, k_scale, v_scale);
+  c10::hip::HIPGuard guard(k_in.device().index());
+  if (k_in.numel() == 0 || in.new_rows == 0 || k_cache.numel() == 0 || in.caches.capacity == 0) return;
+  const Tensor k = in_place(k_in), v = in_place(v_in);
+  const auto strides = all_strides<4>({k, v, k_cache, v_cache});
+  check(co_alibi_cache_append_8bit(in.code, format, k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                   k_scale.data_ptr<float>(), v_scale.data_ptr<float>(), strides.data(), sc.strides.data(),
+                                   in.lens.data_ptr<int>(), data_or_null(in.counts), data_or_null(in.rows),
+                                   as_int(fn, "rows", in.new_rows), data_or_null(in.caches.table),
+                                   as_int(fn, "blocks", in.caches.blocks), as_int(fn, "pages", in.caches.units),
+                                   as_int(fn, "page", in.caches.page), as_int(fn, "batch", k_in.size(0)),
+                                   as_int(fn, "heads", k_in.size(1)), as_int(fn, "tokens", k_in.size(2)),
+                                   as_int(fn, "head_dim", k_in.size(3)), current_stream(k)));
+  for (const Tensor* t : {&k_cache, &v_cache, &k_scale, &v_scale})
+    if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
+std::tuple<Tensor, Tensor> cache_read_8bit_hip(const Tensor& k_cache, const Tensor& v_cache, const Tensor& k_scale,
+                                               const Tensor& v_scale, const Tensor& seq_lens,
+                                               const c10::optional<Tensor>& first, const c10::optional<Tensor>& block_table,
+                                               int64_t rows, at::ScalarType dtype) {
+  const char* fn = "co_alibi::cache_read_8bit";
+  TORCH_CHECK_VALUE(seq_lens.dim() == 1, fn, ": seq_lens must be (B,), got ", seq_lens.sizes());
+  const int64_t batch = seq_lens.size(0);
+  const int code = dtype_code(dtype), format = format_code(fn, k_cache, v_cache);
+  c10::hip::HIPGuard guard(k_cache.device().index());
+  const Caches c = check_caches(fn, k_cache, batch, k_cache, v_cache, block_table, true);
+  const Scales sc = check_scales(fn, k_cache, v_cache, k_scale, v_scale);
+  const Tensor lens = index_i32(seq_lens, k_cache);
+  Tensor from;
+  if (given(first)) {
+    TORCH_CHECK_VALUE(first->dim() == 1 && first->size(0) == batch, fn, ": first must be (", batch, ",), got ", first->sizes());
+    from = index_i32(*first, k_cache);
+  }
+  TORCH_CHECK_VALUE(rows >= 0, fn, ": rows must be >= 0, got ", rows);
+  const int64_t heads = k_cache.size(1), head_dim = k_cache.size(3);
+  const auto options = k_cache.options().dtype(dtype);
+  if (k_cache.numel() == 0 || c.capacity == 0)
+    return {at::zeros({batch, heads, rows, head_dim}, options), at::zeros({batch, heads, rows, head_dim}, options)};
+  Tensor k = at::empty({batch, heads, rows, head_dim}, options), v = at::empty_like(k);
+  if (k.numel() == 0) return {k, v};
+  const auto strides = all_strides<2>({k_cache, v_cache});
+  check(co_alibi_cache_read_8bit(code, format, k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr<float>(),
+                                 v_scale.data_ptr<float>(), strides.data(), sc.strides.data(), lens.data_ptr<int>(),
+                                 data_or_null(from), as_int(fn, "rows", rows), data_or_null(c.table),
+                                 as_int(fn, "blocks", c.blocks), as_int(fn, "pages", c.units), as_int(fn, "page", c.page),
+                                 k.data_ptr(), v.data_ptr(), as_int(fn, "batch", batch), as_int(fn, "heads", heads),
+                                 as_int(fn, "head_dim", head_dim), current_stream(k_cache)));
+  return {k, v};
+}
+
+std::tuple<Tensor, Tensor, Tensor> beam_select_hip(const Tensor& logits_in, const Tensor& scores_in,
+                                                   const c10::optional<Tensor>& finished, int64_t num_beams,
+                                                   int64_t end_token) {
+  const char* fn = "co_alibi::beam_select";
+  TORCH_CHECK_VALUE(logits_in.dim() == 3, fn, ": logits must be (B, W, V), got ", logits_in.sizes());
+  const int64_t batch = logits_in.size(0), beams = logits_in.size(1), vocab = logits_in.size(2);
+  const int code = dtype_code(logits_in.scalar_type());
+  TORCH_CHECK_VALUE(scores_in.dim() == 2 && scores_in.size(0) == batch && scores_in.size(1) == beams, fn, ": scores must be (",
+                    batch, ", ", beams, "), got ", scores_in.sizes());
+  TORCH_CHECK_TYPE(scores_in.scalar_type() == at::kFloat, fn, ": scores must be float32, got ", scores_in.scalar_type());
+  c10::hip::HIPGuard guard(logits_in.device().index());
+  Tensor done;
+  if (given(finished)) {
+    TORCH_CHECK_VALUE(finished->sizes() == scores_in.sizes(), fn, ": finished must be (", batch, ", ", beams, "), got ",
+                      finished->sizes());
+    TORCH_CHECK_TYPE(finished->scalar_type() == at::kBool, fn, ": finished must be bool, got ", finished->scalar_type());
+    done = finished->to(logits_in.device()).contiguous();
+  }
+  Tensor scores = at::empty({batch, num_beams}, logits_in.options().dtype(at::kFloat));
+  Tensor parents = at::empty({batch, num_beams}, logits_in.options().dtype(at::kInt));
+  Tensor tokens = at::empty({batch, num_beams}, logits_in.options().dtype(at::kLong));
+  if (batch == 0) return {scores, parents, tokens};
+  const Tensor logits = logits_in.stride(2) == 1 || vocab == 1 ? logits_in : logits_in.contiguous();
+  const Tensor from = scores_in.to(logits.device()).contiguous();
+  const size_t ws_bytes = co_alibi_beam_select_workspace_bytes(as_int(fn, "batch", batch), as_int(fn, "beams", beams),
+                                                               as_int(fn, "num_beams", num_beams), as_int(fn, "vocab", vocab));
+  Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, logits.options().dtype(at::kByte));
+  const std::array<long long, 2> strides{batch == 1 ? beams * vocab : logits.stride(0), beams == 1 ? vocab : logits.stride(1)};
+  check(co_alibi_beam_select(code, logits.data_ptr(), strides.data(), from.data_ptr<float>(),
+                             done.defined() ? reinterpret_cast<const unsigned char*>(done.data_ptr<bool>()) : nullptr,
+                             as_int(fn, "end_token", end_token), scores.data_ptr<float>(), parents.data_ptr<int>(),
+                             reinterpret_cast<long long*>(tokens.data_ptr<int64_t>()), ws.data_ptr(), ws_bytes, batch, beams,
+                             num_beams, vocab, current_stream(logits)));
+  return {scores, parents, tokens};
+}
+
+std::tuple<Tensor, Tensor> cache_reorder_hip(at::TensorList caches, const Tensor& block_table, const Tensor& pages,
+                                             const Tensor& seq_lens, const Tensor& parents, int64_t page_size) {
+  const char* fn = "co_alibi::cache_reorder";
+  TORCH_CHECK_VALUE(parents.dim() == 2, fn, ": parents must be (B, W), got ", parents.sizes());
+  const int64_t batch = parents.size(0), beams = parents.size(1);
+  TORCH_CHECK_VALUE(block_table.dim() == 2 && block_table.size(0) == batch * beams && pages.sizes() == block_table.sizes(), fn,
+                    ": block_table and pages must be (", batch * beams, ", blocks), got ", block_table.sizes(), " and ",
+                    pages.sizes());
+  TORCH_CHECK_VALUE(seq_lens.dim() == 1 && seq_lens.size(0) == batch * beams, fn, ": seq_lens must be (", batch * beams,
+                    ",), got ", seq_lens.sizes());
+  TORCH_CHECK_VALUE(!caches.empty(), fn, ": there are no caches");
+  const Tensor& like = caches[0];
+  c10::hip::HIPGuard guard(like.device().index());
+  std::vector<void*> pools;
+  std::vector<long long> shapes;
+  const int64_t num_pages = like.size(0);
+  for (const Tensor& t : caches) {
+    TORCH_CHECK_VALUE(t.dim() >= 3 && t.size(0) == num_pages, fn, ": the caches must be (", num_pages,
+                      " pages, heads, rows of a page, ...), got ", t.sizes());
+    TORCH_CHECK_VALUE(t.device() == like.device() && t.device().is_cuda(), fn, ": the caches must be on one CUDA device");
+    int64_t entry = t.element_size();
+    for (int64_t d = t.dim() - 1; d >= 3; --d) {
+      TORCH_CHECK_VALUE(t.size(d) == 1 || t.stride(d) * t.element_size() == entry, fn, ": the rows of a page's head must be dense");
+      entry *= t.size(d);
+    }
+    TORCH_CHECK_VALUE(t.size(2) == 1 || t.stride(2) * t.element_size() == entry, fn, ": the rows of a page's head must be dense");
+    if (t.numel() == 0) continue;
+    pools.push_back(t.data_ptr());
+    for (long long x : {static_cast<long long>(t.stride(0) * t.element_size()), static_cast<long long>(t.stride(1) * t.element_size()),
+                        static_cast<long long>(t.size(1)), static_cast<long long>(t.size(2)), static_cast<long long>(entry)})
+      shapes.push_back(x);
+  }
+  const Tensor table = index_i32(block_table, like), home = index_i32(pages, like), lens = index_i32(seq_lens, like),
+               par = index_i32(parents, like);
+  Tensor out_table = at::empty(table.sizes(), table.options()), out_lens = at::empty(lens.sizes(), lens.options());
+  if (table.numel() == 0) {
+    TORCH_CHECK_VALUE(lens.numel() == 0, fn, ": the block table has no blocks");
+    return {out_table, out_lens};
+  }
+  TORCH_CHECK_VALUE(!pools.empty(), fn, ": the caches are empty");
+  check(co_alibi_cache_reorder(pools.data(), shapes.data(), static_cast<int>(pools.size()), table.data_ptr<int>(),
+                               home.data_ptr<int>(), lens.data_ptr<int>(), par.data_ptr<int>(), out_table.data_ptr<int>(),
+                               out_lens.data_ptr<int>(), as_int(fn, "batch", batch), as_int(fn, "beams", beams),
+                               as_int(fn, "blocks", table.size(1)), as_int(fn, "pages", num_pages),
+                               as_int(fn, "page_size", page_size), current_stream(like)));
+  for (const Tensor& t : caches)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return {out_table, out_lens};
 }
 
 // A setting with one value per row, as the kernel reads it.
@@ -675,6 +934,17 @@ TORCH_LIBRARY(co_alibi, m) {
         "Tensor? rows, Tensor? block_table) -> ()");
   m.def("sample(Tensor logits, Tensor uniforms, Tensor? temperature, Tensor? top_k, Tensor? top_p, Tensor? min_p, "
         "float temperature_all, SymInt top_k_all, float top_p_all, float min_p_all) -> Tensor");
+  m.def("decode_tree_8bit(Tensor q, Tensor k, Tensor v, Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, "
+        "Tensor slopes, Tensor? seq_lens, Tensor? parents, Tensor? block_table, SymInt max_seq_len, float sm_scale, "
+        "bool with_lse) -> (Tensor, Tensor)");
+  m.def("cache_append_8bit(Tensor k, Tensor v, Tensor(a!) k_cache, Tensor(b!) v_cache, Tensor(c!) k_scale, "
+        "Tensor(d!) v_scale, Tensor seq_lens, Tensor? counts, Tensor? rows, Tensor? block_table) -> ()");
+  m.def("cache_read_8bit(Tensor k_cache, Tensor v_cache, Tensor k_scale, Tensor v_scale, Tensor seq_lens, Tensor? first, "
+        "Tensor? block_table, SymInt rows, ScalarType dtype) -> (Tensor, Tensor)");
+  m.def("beam_select(Tensor logits, Tensor scores, Tensor? finished, SymInt num_beams, SymInt end_token) -> "
+        "(Tensor, Tensor, Tensor)");
+  m.def("cache_reorder(Tensor(a!)[] caches, Tensor block_table, Tensor pages, Tensor seq_lens, Tensor parents, "
+        "SymInt page_size) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(co_alibi, CUDA, m) {
@@ -687,6 +957,11 @@ TORCH_LIBRARY_IMPL(co_alibi, CUDA, m) {
   m.impl("decode_tree", &decode_tree_hip);
   m.impl("cache_append", &cache_append_hip);
   m.impl("sample", &sample_hip);
+  m.impl("decode_tree_8bit", &decode_tree_8bit_hip);
+  m.impl("cache_append_8bit", &cache_append_8bit_hip);
+  m.impl("cache_read_8bit", &cache_read_8bit_hip);
+  m.impl("beam_select", &beam_select_hip);
+  m.impl("cache_reorder", &cache_reorder_hip);
 }
 
 TORCH_LIBRARY_IMPL(co_alibi, Autograd, m) {

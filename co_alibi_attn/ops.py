@@ -1,6 +1,8 @@
 """PyTorch operators over the native library: ``co_alibi::fwd``, ``co_alibi::bwd``, ``co_alibi::bwd_dq``,
 ``co_alibi::fwd_qkv``, ``co_alibi::bwd_qkv``, ``co_alibi::decode``, ``co_alibi::decode_tree``,
-``co_alibi::cache_append``, ``co_alibi::sample``.
+``co_alibi::cache_append``, ``co_alibi::sample``; over 8-bit caches ``co_alibi::decode_tree_8bit``,
+``co_alibi::cache_append_8bit``, ``co_alibi::cache_read_8bit``; for beam search ``co_alibi::beam_select``,
+``co_alibi::cache_reorder``.
 
 The operators are defined in C++ (``csrc/torch_ops.cpp``, built into
 ``_lib/libco_alibi_torch.so`` and loaded here): each one is one C-ABI launch
@@ -17,8 +19,9 @@ They replace the reference's two Triton launches with their buffer set-up:
 ``_co_alibi_fwd_kernel[grid](...)`` with the O / LSE / RowSigTotal allocations
 (co_alibi_attn/co_alibi_attn.py:35-57) and ``_co_alibi_bwd_kernel[grid](...)`` with its
 dK / dV partial buffers and their reduction (:83-133).  ``co_alibi::decode`` has no
-counterpart in the reference (its forward with Sq = 1 over a cache), nor have the three after it.
-``co_alibi::cache_append`` writes its two cache operands in place.
+counterpart in the reference (its forward with Sq = 1 over a cache), nor have the ones after it.
+``co_alibi::cache_append`` writes its two cache operands in place, ``co_alibi::cache_append_8bit`` the caches and their scales,
+``co_alibi::cache_reorder`` all of its caches.
 
 Operands are (B, H, S, D) tensors as in include/co_alibi.h.  The forward, and the backward on
 its score-store path, read them in place in any layout whose rows are consecutive and 16-byte
@@ -35,7 +38,8 @@ from torch import Tensor
 from . import _native
 
 __all__ = ["fwd", "bwd", "bwd_dq", "fwd_qkv", "bwd_qkv", "backward_for", "decode", "decode_tree",
-           "cache_append", "sample", "stats_numel", "TORCH_LIB_PATH"]
+           "cache_append", "sample", "decode_tree_8bit", "cache_append_8bit", "cache_read_8bit", "beam_select",
+           "cache_reorder", "stats_numel", "TORCH_LIB_PATH"]
 
 TORCH_LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "_lib", "libco_alibi_torch.so")
 
@@ -44,7 +48,7 @@ def _load() -> str | None:
     """Load the C++ operators (once); returns why they are unavailable, or None.  There is
     no Python fallback: without them every operator raises (so the package still imports,
     as the build itself needs)."""
-    if hasattr(torch.ops.co_alibi, "fwd"):
+    if hasattr(torch.ops.co_alibi, "cache_reorder"):
         return None
     if not os.path.exists(TORCH_LIB_PATH):
         return (f"co_alibi_attn: torch operator library {TORCH_LIB_PATH} is not built; "
@@ -54,6 +58,9 @@ def _load() -> str | None:
     except RuntimeError as e:
         return str(e)
     torch.ops.load_library(TORCH_LIB_PATH)
+    if not hasattr(torch.ops.co_alibi, "cache_reorder"):  # built before the newest operators
+        return (f"co_alibi_attn: torch operator library {TORCH_LIB_PATH} is older than the package; "
+                "run `python -m co_alibi_attn._build`")
     return None
 
 
@@ -81,8 +88,14 @@ if _MISSING is None:
     decode_tree = torch.ops.co_alibi.decode_tree.default
     cache_append = torch.ops.co_alibi.cache_append.default
     sample = torch.ops.co_alibi.sample.default
+    decode_tree_8bit = torch.ops.co_alibi.decode_tree_8bit.default
+    cache_append_8bit = torch.ops.co_alibi.cache_append_8bit.default
+    cache_read_8bit = torch.ops.co_alibi.cache_read_8bit.default
+    beam_select = torch.ops.co_alibi.beam_select.default
+    cache_reorder = torch.ops.co_alibi.cache_reorder.default
 else:
     fwd = bwd = bwd_dq = fwd_qkv = bwd_qkv = decode = decode_tree = cache_append = sample = _unavailable
+    decode_tree_8bit = cache_append_8bit = cache_read_8bit = beam_select = cache_reorder = _unavailable
 
 
 def stats_numel(batch: int, heads_q: int, seq_q: int, seq_kv: int) -> int:
@@ -179,6 +192,35 @@ def _register_fakes() -> None:
     def _sample_fake(logits, uniforms, temperature, top_k, top_p, min_p, temperature_all, top_k_all, top_p_all, min_p_all):
         """One int64 token per row of logits."""
         return logits.new_empty(logits.shape[:1], dtype=torch.int64)
+
+    @torch.library.register_fake("co_alibi::decode_tree_8bit")
+    def _decode_tree_8bit_fake(q, k, v, k_cache, v_cache, k_scale, v_scale, slopes, seq_lens, parents, block_table,
+                               max_seq_len, sm_scale, with_lse):
+        """co_alibi::decode_tree's."""
+        o = torch.empty_like(q, memory_format=torch.contiguous_format)
+        return o, q.new_empty(q.shape[:3], dtype=torch.float32) if with_lse else _empty_stats(q)
+
+    @torch.library.register_fake("co_alibi::cache_append_8bit")
+    def _cache_append_8bit_fake(k, v, k_cache, v_cache, k_scale, v_scale, seq_lens, counts, rows, block_table):
+        """Nothing: the caches and their scales are written in place."""
+
+    @torch.library.register_fake("co_alibi::cache_read_8bit")
+    def _cache_read_8bit_fake(k_cache, v_cache, k_scale, v_scale, seq_lens, first, block_table, rows, dtype):
+        """k and v (B, Hkv, rows, D) in dtype."""
+        shape = (seq_lens.shape[0], k_cache.shape[1], rows, k_cache.shape[3])
+        return k_cache.new_empty(shape, dtype=dtype), k_cache.new_empty(shape, dtype=dtype)
+
+    @torch.library.register_fake("co_alibi::beam_select")
+    def _beam_select_fake(logits, scores, finished, num_beams, end_token):
+        """Scores (fp32), parents (int32) and tokens (int64), each (B, num_beams)."""
+        shape = (logits.shape[0], num_beams)
+        return (logits.new_empty(shape, dtype=torch.float32), logits.new_empty(shape, dtype=torch.int32),
+                logits.new_empty(shape, dtype=torch.int64))
+
+    @torch.library.register_fake("co_alibi::cache_reorder")
+    def _cache_reorder_fake(caches, block_table, pages, seq_lens, parents, page_size):
+        """The new block table and lengths (int32); the caches are written in place."""
+        return block_table.new_empty(block_table.shape, dtype=torch.int32), seq_lens.new_empty(seq_lens.shape, dtype=torch.int32)
 
 
 if _MISSING is None:

@@ -15,7 +15,10 @@
  * with Sq = 1 over a key / value cache, as one split-K pass over the cache;
  * and the rest of a serving step around it, without counterparts there either:
  * co_alibi_decode_tree (several new tokens, paged caches), co_alibi_cache_append
- * and co_alibi_sample.
+ * and co_alibi_sample; the same over caches held in 8 bits
+ * (co_alibi_decode_tree_8bit, co_alibi_cache_append_8bit,
+ * co_alibi_cache_read_8bit); and beam search (co_alibi_beam_select,
+ * co_alibi_cache_reorder).
  *
  * Tensor layout (except the _strided calls): contiguous row-major, q / o / dout / dq are (B, Hq, Sq, D),
  * k / v / dk / dv are (B, Hkv, Skv, D); query head h attends key/value head
@@ -276,6 +279,73 @@ int co_alibi_sample(int dtype, const void* logits, long long row_stride, const v
                     const float* temperature, const int* top_k, const float* top_p, const float* min_p,
                     double temperature_all, int top_k_all, double top_p_all, double min_p_all, long long* tokens,
                     int batch, int vocab, void* stream);
+
+/* Caches held in 8 bits: an element is a code (format CO_ALIBI_E4M3: e4m3 without infinities, largest 448; CO_ALIBI_INT8: a
+ * two's complement byte, written in [-127, 127]) and its value code * scale, with one fp32 scale for each kv head's blocks of 16
+ * rows: k_scale and v_scale are (num_pages, heads_kv, page_size / 16), or (batch, heads_kv, ceil(page_size / 16)) without a
+ * block_table.  scale_strides holds their strides from page (sequence) to page and head to head, k_scale's then v_scale's, or is
+ * NULL: contiguous; a head's scales follow one another.  Cache strides are in elements, whole 16-byte units, with the row stride
+ * head_dim.  Scales must lie in [2^-40, 2^40]; a block with another one (a NaN among them) reads as NaN. */
+enum co_alibi_format { CO_ALIBI_E4M3 = 0, CO_ALIBI_INT8 = 1 };
+
+/* co_alibi_cache_append to an 8-bit cache.  A block that is begun gets the least power of two from 2^-40 on at which no new
+ * value's code passes the largest; a block that holds rows before seq_lens[b] keeps its scale, doubled as often as the new values
+ * need, and the codes of those rows are halved as often.  Codes are rounded to the nearest, ties to even.  A new value that is not
+ * finite, or needs a scale past 2^40, makes its block's scale NaN, until the block's first row is written again.  No two
+ * sequences may write one page's same block.  strides: those of k, v, k_cache and v_cache (12 values) or NULL. */
+int co_alibi_cache_append_8bit(int dtype, int format, const void* k, const void* v, void* k_cache, void* v_cache,
+                               float* k_scale, float* v_scale, const long long* strides, const long long* scale_strides,
+                               const int* seq_lens, const int* counts, const int* rows, int new_rows, const int* block_table,
+                               int blocks_per_seq, int num_pages, int page_size, int batch, int heads_kv, int tokens,
+                               int head_dim, void* stream);
+
+/* Rows of an 8-bit cache as values of `dtype`: k and v (batch, heads_kv, rows, D), contiguous, get cache row first[b] + i
+ * (batch int32, or NULL: i) of sequence b in row i: zeros where it is not below seq_lens[b], NaN on a page outside the pool.
+ * strides: those of k_cache and v_cache (6 values) or NULL. */
+int co_alibi_cache_read_8bit(int dtype, int format, const void* k_cache, const void* v_cache, const float* k_scale,
+                             const float* v_scale, const long long* strides, const long long* scale_strides,
+                             const int* seq_lens, const int* first, int rows, const int* block_table, int blocks_per_seq,
+                             int num_pages, int page_size, void* k, void* v, int batch, int heads_kv, int head_dim,
+                             void* stream);
+
+/* co_alibi_decode_tree over an 8-bit cache: q, k, v and o stay in `dtype`, the cached keys and values are code * scale in fp32.
+ * A sequence with a filled block whose scale is not in [2^-40, 2^40] gets NaN. */
+size_t co_alibi_decode_tree_8bit_workspace_bytes(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv,
+                                                 int head_dim);
+int co_alibi_decode_tree_8bit(int dtype, int format, const void* q, const void* k, const void* v, const void* k_cache,
+                              const void* v_cache, const float* k_scale, const float* v_scale, const long long* strides,
+                              const long long* scale_strides, const float* slopes, const int* seq_lens, const int* parents,
+                              int parents_per_seq, const int* block_table, int blocks_per_seq, int num_pages, int page_size,
+                              void* o, float* lse, void* workspace, size_t workspace_bytes, int batch, int heads_q,
+                              int heads_kv, int tokens, int seq_kv, int head_dim, float sm_scale, void* stream);
+
+/* Beam selection: of every sequence's candidates (w, t), beam w < beams continued with token t < vocab, the num_beams with the
+ * largest score, scores[b][w] + log_softmax(logits[b][w])[t], best first; equal scores go by beam, then by logit, then by token.
+ * logits: (batch, beams, vocab) in `dtype`, strides its batch and beam strides in elements (2 values) or NULL: contiguous.
+ * scores: (batch, beams) fp32.  A beam with finished[b][w] != 0 (batch x beams bytes, or NULL) has one candidate, end_token at its
+ * score as it is, and its logits are not read.  A beam whose score is not finite, whose logits hold a NaN or none above -inf
+ * has no candidates, and a logit of -inf is none; of +inf logits all weigh the same and every other one nothing.  Results, each
+ * (batch, num_beams): out_scores, parents (the beam) and tokens; places without a candidate get -inf, 0 and -1.  At most 64 beams in
+ * and out, vocab <= 2^20.  workspace holds co_alibi_beam_select_workspace_bytes(...) bytes (256-byte aligned). */
+size_t co_alibi_beam_select_workspace_bytes(int batch, int beams, int num_beams, int vocab);
+int co_alibi_beam_select(int dtype, const void* logits, const long long* strides, const float* scores,
+                         const unsigned char* finished, int end_token, float* out_scores, int* parents, long long* tokens,
+                         void* workspace, size_t workspace_bytes, int batch, int beams, int num_beams, int vocab,
+                         void* stream);
+
+/* Cache reorder: sequence g * beams + i of a paged cache takes over the rows of sequence g * beams + parents[g][i] (batch x beams
+ * int32, clamped to [0, beams)).  block_table and pages are (batch * beams, blocks_per_seq): the pages in use, and the ones that
+ * each sequence owns, every page of the pool at most once among them; the entries of a group's column in block_table are
+ * entries of that column in pages.  Full pages are shared.  A page that is filled in part stays with its first heir and is copied
+ * for the others, its filled rows only, into pages of the group's column that nobody holds; columns behind the filled rows
+ * get such pages, too.  So a page that is filled in part belongs to one sequence, which co_alibi_cache_append needs.
+ * out_table and out_lens (batch * beams) receive the new table and lengths (they must not overlap the inputs); the pools, num_pools
+ * of them, are written in place.  shapes has five values for each: bytes from page to page, and head to head, heads, entries per
+ * page and head, bytes of an entry; entries follow one another and stand for page_size / entries rows each.  Everything is in
+ * whole 4 bytes.  Copies to or from a page outside [0, num_pages) are left out.  At most 64 beams. */
+int co_alibi_cache_reorder(void* const* pools, const long long* shapes, int num_pools, const int* block_table,
+                           const int* pages, const int* seq_lens, const int* parents, int* out_table, int* out_lens,
+                           int batch, int beams, int blocks_per_seq, int num_pages, int page_size, void* stream);
 
 /* Measurement helper with no counterpart in the reference: `blocks` work-groups of 256
  * threads each issue `iters` rounds of four independent fp16 32x32x16 MFMAs per
