@@ -133,7 +133,7 @@ _SIGNATURES = {
         [_I, _I, _P, _P, _P, _P, _P, _P, _P, _L, _L, _P, _P, _P, _I, _P, _I, _I, _I, _P, _P, _P, _Z, _I, _I, _I, _I, _I, _I,
          _F, _P],
     ),
-    "co_alibi_beam_select_workspace_bytes": (_Z, [_I] * 4),
+    "co_alibi_beam_select_workspace_bytes": (_Z, [_I] * 5),
     "co_alibi_beam_select": (_I, [_I, _P, _L, _P, _P, _I, _P, _P, _P, _P, _Z, _I, _I, _I, _I, _P]),
     "co_alibi_cache_reorder": (_I, [_PP, _L, _I, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "co_alibi_probe_mfma": (_I, [_P, _P, _I, _I, _P]),

@@ -6,9 +6,9 @@
 // Within a row the order is the logits', so that each segment of a row yields its maximum, its sum and its N largest logits in
 // one read (its elements stay in registers), and a second launch ranks those of a sequence's beams.  Exponentials are fp32's,
 // summed in fp64 over the threads; scores are fp64 until they are written.
-//   The N largest of a segment: the N-th largest of the 256 threads' maxima is at most the N-th largest element, and few others
-// are above it.  Those at or above it are listed and ranked by counting.  Where equal logits make the list overflow, N rounds
-// of a search for the next one take its place.
+//   The N largest of a segment: a wavefront's N-th largest of its lanes' maxima is at most the N-th largest element.  Those at or
+// above the largest such bound -- of N lanes of each wavefront at most -- are listed and ranked by counting.  A logit and its
+// token are one 64-bit key, so that equal logits are in order, too.
 //
 // Reordering: a group of W beams owns W pages in every column of its block table.  Pages that are full are shared by all that
 // descend from them; one in use stays with the first of its heirs, and the others get free pages of its column and copies of
@@ -24,180 +24,265 @@ namespace coalibi {
 namespace {
 
 constexpr int kSelectThreads = 256;
-constexpr int kListed = 1024;  // candidates of a list that are ranked by counting
+constexpr int kSelectWaves = kSelectThreads / 64;
+typedef unsigned long long u64;
 
-__device__ __forceinline__ bool better(float xa, int ia, float xb, int ib) { return xa > xb || (xa == xb && ia < ib); }
+// A float as a number of the same order.
+__device__ __forceinline__ unsigned ordered(float x) {
+  x += 0.f;  // -0 is 0
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  return u ^ ((unsigned)((int)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered(unsigned k) { return __builtin_bit_cast(float, k ^ ((k >> 31) - 1u | 0x80000000u)); }
+// A logit and its token as one number: larger logits first, of equal ones the lower token.  0 is none.
+__device__ __forceinline__ u64 logit_key(float x, int token) { return (u64)ordered(x) << 32 | (unsigned)~token; }
+__device__ __forceinline__ float key_logit(u64 k) { return unordered((unsigned)(k >> 32)); }
+__device__ __forceinline__ int key_token(u64 k) { return (int)~(unsigned)k; }
 
-// The best of the work-group's (value, place) pairs, in every thread; a place below 0 is none.
-template <typename X, typename Better>
-__device__ __forceinline__ void best_of_block(X& x, int& at, X* sx, int* si, Better better) {
+// The number of a lane's partner in step S of six that join 1, 2, 4, ..., 32 lanes, of which those of a group hold the same.
+template <int S>
+__device__ __forceinline__ unsigned partner(unsigned x) {
+  if constexpr (S < 4) {  // quad_perm [1, 0, 3, 2] and [2, 3, 0, 1], row_half_mirror, row_mirror
+    constexpr int ctrl = S == 0 ? 0xb1 : S == 1 ? 0x4e : S == 2 ? 0x141 : 0x140;
+    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, false);
+  } else if constexpr (S == 4) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return threadIdx.x & 16 ? r[0] : r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    return threadIdx.x & 32 ? r[0] : r[1];
+  }
+}
+template <int S>
+__device__ __forceinline__ u64 partner(u64 x) {
+  return (u64)partner<S>((unsigned)(x >> 32)) << 32 | partner<S>((unsigned)x);
+}
+template <int S>
+__device__ __forceinline__ float partner(float x) {
+  return __builtin_bit_cast(float, partner<S>(__builtin_bit_cast(unsigned, x)));
+}
+template <int S>
+__device__ __forceinline__ double partner(double x) {
+  return __builtin_bit_cast(double, partner<S>(__builtin_bit_cast(u64, x)));
+}
+template <int S = 0, typename X>
+__device__ __forceinline__ X wave_max(X x) {
+  if constexpr (S == 6) {
+    return x;
+  } else {
+    const X y = partner<S>(x);
+    return wave_max<S + 1>(y > x ? y : x);
+  }
+}
+template <int S = 0>
+__device__ __forceinline__ double wave_sum(double x) {
+  if constexpr (S == 6)
+    return x;
+  else
+    return wave_sum<S + 1>(x + partner<S>(x));
+}
+__device__ __forceinline__ unsigned lane_of(unsigned x, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)x, lane); }
+__device__ __forceinline__ u64 lane_of(u64 x, int lane) {
+  return (u64)lane_of((unsigned)(x >> 32), lane) << 32 | lane_of((unsigned)x, lane);
+}
+// The n-th largest (1 <= n <= 64) of a wavefront's numbers.
+template <typename X>
+__device__ __forceinline__ X nth_of_wave(X x, int n) {
+  int larger = 0;
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    const X ox = __shfl_xor(x, off, 64);
-    const int oi = __shfl_xor(at, off, 64);
-    if (oi >= 0 && (at < 0 || better(ox, oi, x, at))) {
-      x = ox;
-      at = oi;
-    }
-  }
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) {
-    sx[threadIdx.x >> 6] = x;
-    si[threadIdx.x >> 6] = at;
-  }
-  __syncthreads();
-  for (int w = 0; w < kSelectThreads / 64; ++w)
-    if (si[w] >= 0 && (at < 0 || better(sx[w], si[w], x, at))) {
-      x = sx[w];
-      at = si[w];
-    }
+  for (int i = 0; i < 64; ++i) larger += lane_of(x, i) > x ? 1 : 0;
+  u64 is;
+  do is = __ballot(larger == --n);  // (equal ones have the first one's count)
+  while (is == 0);
+  return lane_of(x, __builtin_amdgcn_readfirstlane(__ffsll(is) - 1));
 }
 
-// E: elements of a segment per thread.
-template <typename T, int E>
+constexpr int kListed = 256;  // keys of a wavefront's list, which are ranked by counting
+
+// The lanes' place behind n others, of those for which `is`, and how many they are.
+__device__ __forceinline__ int place_of(u64 is) { return __builtin_amdgcn_mbcnt_hi((unsigned)(is >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)is, 0)); }
+
+// C: 16-byte chunks of a segment per thread.  A row is read in whole chunks from its first 16-byte boundary on; the elements
+// before it go with the first segment and those behind the last whole chunk with the last one, one per thread.
+template <typename T, int C>
 __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(SelectArgs a) {
-  __shared__ float sx[kListed];
-  __shared__ int si[kListed];
-  __shared__ float wx[kSelectThreads / 64];
-  __shared__ int wi[kSelectThreads / 64];
-  __shared__ double ws[kSelectThreads / 64];
-  __shared__ int count;
-  __shared__ float cut;
-  const int tid = threadIdx.x, seg = blockIdx.x;
+  constexpr int PER = 16 / sizeof(T), E = C * PER + 1;
+  typedef T chunk_t __attribute__((ext_vector_type(PER)));
+  __shared__ u64 list[kSelectWaves][kListed];
+  __shared__ int listed[kSelectWaves];
+  __shared__ u64 wnext[kSelectWaves];
+  __shared__ unsigned wcut[kSelectWaves];
+  __shared__ float wmax[kSelectWaves];
+  __shared__ double wsum[kSelectWaves];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = blockIdx.x;
   const long long row = blockIdx.y + (long long)blockIdx.z * gridDim.y;
   if (row >= (long long)a.B * a.W) return;
   if (a.finished != nullptr && a.finished[row] != 0) return;
   const int b = (int)(row / a.W), w = (int)(row - (long long)b * a.W);
   const T* const x = static_cast<const T*>(a.logits) + (size_t)b * a.batch_stride + (size_t)w * a.beam_stride;
-  const int first = seg * a.per_segment, n = min(a.V - first, a.per_segment);
+  const int head = min((int)(-(long long)((size_t)x / sizeof(T)) & (PER - 1)), a.V);
+  const int chunks = (a.V - head) / PER, tail = a.V - head - chunks * PER;
+
   float v[E];
-  bool nan = false;
-  float top = kNegInf;
+  int where = -1;  // the single element's token
+  if (seg == 0 && tid < head) where = tid;
+  if (seg == a.segments - 1 && tid >= 64 && tid - 64 < tail) where = a.V - tail + (tid - 64);
+  v[E - 1] = where >= 0 ? static_cast<float>(x[where]) : kNegInf;
+  const int first = seg * (C * kSelectThreads) + tid;  // the thread's first chunk
+  if (chunks > 0) {
+    chunk_t y[C];
 #pragma unroll
-  for (int e = 0; e < E; ++e) {
-    const int i = tid + e * kSelectThreads;
-    v[e] = i < n ? static_cast<float>(x[first + i]) : kNegInf;
-    nan |= v[e] != v[e];
-    top = fmaxf(top, v[e]);
+    for (int c = 0; c < C; ++c)
+      y[c] = *reinterpret_cast<const chunk_t*>(x + head + (size_t)min(first + c * kSelectThreads, chunks - 1) * PER);
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+      for (int e = 0; e < PER; ++e) v[c * PER + e] = first + c * kSelectThreads < chunks ? static_cast<float>(y[c][e]) : kNegInf;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E - 1; ++e) v[e] = kNegInf;
   }
-  const size_t part = (size_t)row * a.segments + seg;
-  float* const oval = a.pval + part * a.N;
-  int* const otok = a.ptok + part * a.N;
-  // The segment's maximum (a NaN: none), then its sum.
-  float m = top;
-  int at = __any(nan) ? -1 : tid;
-  {
-    // A wavefront with a NaN says so by a place below 0.
-    float wm = m;
+  auto token = [&](int e) { return e == E - 1 ? where : head + (first + e / PER * kSelectThreads) * PER + e % PER; };
+
+  // The segment's maximum, and a bound that its N-th largest logit is not below.
+  float top = v[E - 1];
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) wm = fmaxf(wm, __shfl_xor(wm, off, 64));
-    if ((tid & 63) == 0) {
-      wx[tid >> 6] = wm;
-      wi[tid >> 6] = at;
-    }
-    if (tid == 0) count = 0;
-    __syncthreads();
-    m = wx[0];
-    for (int i = 1; i < kSelectThreads / 64; ++i) m = fmaxf(m, wx[i]);
-    nan = false;
-    for (int i = 0; i < kSelectThreads / 64; ++i) nan |= wi[i] < 0;
+  for (int e = 0; e < E - 1; ++e) top = fmaxf(top, v[e]);
+  const unsigned cut = nth_of_wave(ordered(top), a.N);
+  float m = wave_max(top);
+  if (lane == 0) {
+    wmax[wave] = m;
+    wcut[wave] = cut;
   }
-  float sum = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) sum += v[e] == m ? (m == kNegInf ? 0.f : 1.f) : fast_exp2((v[e] - m) * kLog2e);
-  double total = sum;
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) total += __shfl_xor(total, off, 64);
-  if ((tid & 63) == 0) ws[tid >> 6] = total;
-  sx[tid] = top;
   __syncthreads();
+  unsigned least = 0;
+#pragma unroll
+  for (int i = 0; i < kSelectWaves; ++i) {
+    m = fmaxf(m, wmax[i]);
+    least = max(least, wcut[i]);
+  }
+  // The weights' sum: NaN where there is a NaN.
+  float sum = 0.f;
+  const float ref = m > kNegInf ? m : 0.f;
+  if (m < __builtin_inff()) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += fast_exp2((v[e] - ref) * kLog2e);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += v[e] == m ? 1.f : v[e] == v[e] ? 0.f : v[e];
+  }
+  const float low = unordered(least);
+  int mine = 0;
+  if (__any(top >= low)) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      if (!__any(v[e] >= low)) continue;
+      const bool in = v[e] >= low && v[e] > kNegInf;
+      const u64 is = __ballot(in);
+      const int p = mine + place_of(is);
+      if (in && p < kListed) list[wave][p] = logit_key(v[e], token(e));
+      mine += __popcll(is);
+    }
+  }
+  if (lane == 0) listed[wave] = mine;
+  const double total = wave_sum((double)sum);
+  if (lane == 0) wsum[wave] = total;
+  __syncthreads();
+  const size_t part = (size_t)row * a.segments + seg;
+  const double all = (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
+  const bool nan = all != all;
   if (tid == 0) {
     a.pmax[part] = nan ? __builtin_nanf("") : m;
-    a.psum[part] = (ws[0] + ws[1]) + (ws[2] + ws[3]);
+    a.psum[part] = all;
   }
   if (nan) return;
-  // The N-th largest of the threads' maxima.
-  {
-    int rank = 0;
-    for (int i = 0; i < kSelectThreads; i += 4) {
-      const f32x4 y = *reinterpret_cast<const f32x4*>(sx + i);
+  u64* const out = a.pkey + part * a.N;
+  int c = 0;
+  bool fits = true;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) rank += y[e] > top || (y[e] == top && i + e < tid) ? 1 : 0;
-    }
-    if (rank == a.N - 1) cut = top;
+  for (int i = 0; i < kSelectWaves; ++i) {
+    c += listed[i];
+    fits = fits && listed[i] <= kListed;
   }
-  __syncthreads();
-  const float least = cut;
+  if (c <= 64) {  // one each for the first wavefront's lanes
+    if (wave == 0) {
+      int at = lane, from = 0;
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (v[e] >= least && v[e] > kNegInf) {
-      const int p = atomicAdd(&count, 1);
-      if (p < kListed) {
-        sx[p] = v[e];
-        si[p] = first + tid + e * kSelectThreads;
-      }
-    }
-  __syncthreads();
-  const int c = count;
-  if (c <= kListed) {
-    for (int i = tid; i < c; i += kSelectThreads) {
-      const float xi = sx[i];
-      const int ti = si[i];
-      int rank = 0;
-      for (int j = 0; j < c; ++j) rank += better(sx[j], si[j], xi, ti) ? 1 : 0;
-      if (rank < a.N) {
-        oval[rank] = xi;
-        otok[rank] = ti;
-      }
-    }
-    for (int i = c + tid; i < a.N; i += kSelectThreads) otok[i] = -1;
-  } else {
-    float last = __builtin_inff();
-    int last_at = -1;
-    for (int k = 0; k < a.N; ++k) {
-      float best = kNegInf;
-      int best_at = -1;
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const int i = first + tid + e * kSelectThreads;
-        if (v[e] > kNegInf && (k == 0 || better(last, last_at, v[e], i)) && (best_at < 0 || better(v[e], i, best, best_at))) {
-          best = v[e];
-          best_at = i;
+      for (int i = 0; i < kSelectWaves - 1; ++i)
+        if (from == i && at >= listed[i]) {
+          at -= listed[i];
+          ++from;
         }
-      }
-      best_of_block(best, best_at, wx, wi, [](float xa, int ia, float xb, int ib) { return better(xa, ia, xb, ib); });
-      last = best;
-      last_at = best_at;
-      if (tid == 0) {
-        oval[k] = best;
-        otok[k] = best_at;
-      }
-      if (best_at < 0) {  // fewer than N logits above -inf
-        for (int i = k + 1 + tid; i < a.N; i += kSelectThreads) otok[i] = -1;
-        break;
-      }
+      const u64 k = lane < c ? list[from][at] : 0;
+      int rank = 0;
+      for (int j = 0; j < c; ++j) rank += lane_of(k, j) > k ? 1 : 0;
+      if (lane >= c) rank = lane;
+      if (rank < a.N) out[rank] = k;
+    }
+  } else if (fits) {
+    for (int i = lane; i < mine; i += 64) {
+      const u64 k = list[wave][i];
+      int rank = 0;
+      for (int w = 0; w < kSelectWaves; ++w)
+        for (int j = 0; j < listed[w]; ++j) rank += list[w][j] > k ? 1 : 0;
+      if (rank < a.N) out[rank] = k;
+    }
+    for (int i = c + tid; i < a.N; i += kSelectThreads) out[i] = 0;
+  } else {
+    // Too many to list (threads with many of the largest): the next one, N times.
+    u64 last = ~0ull;
+    for (int n = 0; n < a.N; ++n) {
+      u64 k = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (v[e] > kNegInf) {
+          const u64 y = logit_key(v[e], token(e));
+          if (y < last && y > k) k = y;
+        }
+      k = wave_max(k);
+      __syncthreads();
+      if (lane == 0) wnext[wave] = k;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kSelectWaves; ++i) k = wnext[i] > k ? wnext[i] : k;
+      if (tid == 0) out[n] = k;
+      last = k;
     }
   }
 }
 
-// The N best of a sequence's candidates, which stand in the order (beam, segment, rank).
+// A score as a number of the same order, above 0.
+__device__ __forceinline__ u64 score_key(double x) {
+  x += 0.0;
+  const u64 u = __builtin_bit_cast(u64, x);
+  return u ^ ((u64)((long long)u >> 63) | 1ull << 63);
+}
+__device__ __forceinline__ double key_score(u64 k) {
+  const u64 u = k ^ ((k >> 63) - 1 | 1ull << 63);
+  return __builtin_bit_cast(double, u);
+}
+
+constexpr int kRound = 8;  // candidates of a thread and round
+
+// The N best of a sequence's candidates, kRound per thread at a time, with the N best so far.  The list has room for all of a
+// round's, and few are on it, as in the segments.
 __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(SelectArgs a) {
+  constexpr int kMost = 64 * (kRound + 1);
+  // Candidates: keys of score and logit, and the beam.  Equal scores go by beam, then by the logit's key.
   __shared__ double sbase[kMaxBeams];  // score - log S, or NaN for a beam without candidates
   __shared__ float smax[kMaxBeams];
-  __shared__ double sx[kListed];
-  __shared__ int si[kListed];
-  __shared__ double cut;
-  __shared__ int cut_at, count;
-  __shared__ double wx[kSelectThreads / 64];
-  __shared__ int wi[kSelectThreads / 64];
+  __shared__ bool sdone[kMaxBeams];
+  __shared__ u64 lscore[kSelectWaves][kMost], llogit[kSelectWaves][kMost], kscore[kMaxBeams], klogit[kMaxBeams];
+  __shared__ int lbeam[kSelectWaves][kMost], kbeam[kMaxBeams];
+  __shared__ u64 wcut[kSelectWaves];
+  __shared__ int listed[kSelectWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
   const long long row0 = (long long)b * a.W;
   const int per_beam = a.segments * a.N, total = a.W * per_beam;
-  if (tid == 0) {
-    count = 0;
-    cut_at = -1;
-  }
-  for (int w = wave; w < a.W; w += kSelectThreads / 64) {
+  u64 keys[kRound];  // of the first round, on their way meanwhile
+#pragma unroll
+  for (int r = 0; r < kRound; ++r) keys[r] = a.pkey[(size_t)row0 * per_beam + min(r * kSelectThreads + tid, total - 1)];
+  for (int w = wave; w < a.W; w += kSelectWaves) {
     const long long row = row0 + w;
     const float score = a.scores[row];
     const bool done = a.finished != nullptr && a.finished[row] != 0;
@@ -206,120 +291,145 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
     if (!done) {
       const float* const pm = a.pmax + row * a.segments;
       const double* const ps = a.psum + row * a.segments;
-      bool nan = false;
-      m = kNegInf;
-      for (int s = lane; s < a.segments; s += 64) {
+      const float m0 = lane < a.segments ? pm[lane] : kNegInf;
+      const double s0 = lane < a.segments ? ps[lane] : 0.0;
+      bool nan = m0 != m0;
+      m = fmaxf(m0, kNegInf);
+      for (int s = lane + 64; s < a.segments; s += 64) {
         nan |= pm[s] != pm[s];
         m = fmaxf(m, pm[s]);
       }
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-      double sum = 0.0;
-      for (int s = lane; s < a.segments; s += 64) sum += pm[s] == m ? ps[s] : ps[s] * exp((double)pm[s] - (double)m);
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+      m = wave_max(m);
+      // (A segment's factor in fp32, as its weights are.)
+      double sum = s0 * (m0 == m ? 1.f : fast_exp2((m0 - m) * kLog2e));
+      for (int s = lane + 64; s < a.segments; s += 64) sum += ps[s] * (pm[s] == m ? 1.f : fast_exp2((pm[s] - m) * kLog2e));
+      sum = wave_sum(sum);
       if (!__any(nan) && m > kNegInf) base = (double)score - log(sum);
     }
     if (lane == 0) {
       sbase[w] = score > kNegInf && score < __builtin_inff() ? base : __builtin_nan("");
       smax[w] = m;
+      sdone[w] = done;
     }
   }
-  __syncthreads();
-  // Candidate i: its score, NaN for none.
-  auto candidate = [&](int i) -> double {
-    const int w = i / per_beam, k = i - w * per_beam;
-    const double base = sbase[w];
-    if (base != base) return base;
-    if (a.finished != nullptr && a.finished[row0 + w] != 0) return k == 0 ? base : __builtin_nan("");
-    const size_t at = (size_t)(row0 + w) * per_beam + k;
-    if (a.ptok[at] < 0) return __builtin_nan("");
-    const float x = a.pval[at], m = smax[w];
-    // Of +inf logits all weigh 1, and every other one nothing.
-    return x == m ? base : m == __builtin_inff() ? __builtin_nan("") : base + ((double)x - (double)m);
-  };
-  // Equal scores go by beam, then by logit, then by token.  (Logits that differ may score the same in 64 bits, where they are
-  // far smaller than the row's largest.)
-  auto better = [&](double xa, int ia, double xb, int ib) {
-    if (xa != xb) return xa > xb;
-    const int wa = ia / per_beam, wb = ib / per_beam;
-    if (wa != wb || ia == ib || (a.finished != nullptr && a.finished[row0 + wa] != 0)) return ia < ib;
-    const size_t pa = (size_t)row0 * per_beam + ia, pb = (size_t)row0 * per_beam + ib;
-    return a.pval[pa] > a.pval[pb] || (a.pval[pa] == a.pval[pb] && a.ptok[pa] < a.ptok[pb]);
-  };
-  // As for the segments: the N-th best of the threads' best ones bounds what can be selected.
-  double best = 0.0;
-  int best_at = -1;
-  for (int i = tid; i < total; i += kSelectThreads) {
-    const double x = candidate(i);
-    if (x == x && (best_at < 0 || better(x, i, best, best_at))) {
-      best = x;
-      best_at = i;
-    }
-  }
-  sx[tid] = best;
-  si[tid] = best_at;
-  __syncthreads();
-  if (best_at >= 0) {
-    int rank = 0;
-    for (int j = 0; j < kSelectThreads; ++j) rank += si[j] >= 0 && better(sx[j], si[j], best, best_at) ? 1 : 0;
-    if (rank == a.N - 1) {
-      cut = best;
-      cut_at = best_at;
-    }
+  if (tid < a.N) {
+    kscore[tid] = klogit[tid] = 0;
+    kbeam[tid] = 0;
   }
   __syncthreads();
-  const double least = cut;
-  const int least_at = cut_at;  // below 0: fewer than N threads have any, and all are listed
-  for (int i = tid; i < total; i += kSelectThreads) {
-    const double x = candidate(i);
-    if (x == x && (least_at < 0 || !better(least, least_at, x, i))) {
-      const int p = atomicAdd(&count, 1);
-      if (p < kListed) {
-        sx[p] = x;
-        si[p] = i;
-      }
-    }
-  }
-  __syncthreads();
-  const int c = count;
-  auto write = [&](int k, double x, int i) {
-    const int w = i < 0 ? 0 : i / per_beam;
-    const size_t o = (size_t)b * a.N + k;
-    a.out_scores[o] = i < 0 ? kNegInf : (float)x;
-    a.out_parents[o] = w;
-    a.out_tokens[o] = i < 0 ? -1
-                      : a.finished != nullptr && a.finished[row0 + w] != 0
-                          ? a.end_token
-                          : a.ptok[(size_t)(row0 + w) * per_beam + (i - w * per_beam)];
-  };
-  if (c <= kListed) {
-    for (int i = tid; i < c; i += kSelectThreads) {
-      const double xi = sx[i];
-      const int ti = si[i];
-      int rank = 0;
-      for (int j = 0; j < c; ++j) rank += better(sx[j], si[j], xi, ti) ? 1 : 0;
-      if (rank < a.N) write(rank, xi, ti);
-    }
-    for (int i = c + tid; i < a.N; i += kSelectThreads) write(i, 0.0, -1);
-  } else {
-    double last = 0.0;
-    int last_at = -1;
-    for (int k = 0; k < a.N; ++k) {
-      double x = 0.0;
-      int at = -1;
-      for (int i = tid; i < total; i += kSelectThreads) {
-        const double y = candidate(i);
-        if (y == y && (k == 0 || better(last, last_at, y, i)) && (at < 0 || better(y, i, x, at))) {
-          x = y;
-          at = i;
+  for (int first = 0; first < total; first += kRound * kSelectThreads) {
+    u64 score[kRound + 1], logit[kRound + 1];
+    int beam[kRound + 1];
+#pragma unroll
+    for (int r = 0; r < kRound; ++r) {
+      const int i = first + r * kSelectThreads + tid;
+      score[r] = logit[r] = 0;
+      beam[r] = 0;
+      if (i < total) {
+        const int w = (unsigned)i / (unsigned)per_beam;
+        const double base = sbase[w];
+        const bool done = sdone[w];
+        u64 k = keys[r];
+        const float x = key_logit(k), m = smax[w];
+        if (done) k = i == w * per_beam ? logit_key(0.f, a.end_token) : 0;
+        // Of +inf logits all weigh 1, and every other one nothing.
+        if (base == base && k != 0 && (done || x == m || m < __builtin_inff())) {
+          score[r] = score_key(done || x == m ? base : base + ((double)x - (double)m));
+          logit[r] = k;
+          beam[r] = w;
         }
       }
-      best_of_block(x, at, wx, wi, better);
-      last = x;
-      last_at = at;
-      if (tid == 0) write(k, x, at);
     }
+    score[kRound] = tid < a.N ? kscore[tid] : 0;
+    logit[kRound] = tid < a.N ? klogit[tid] : 0;
+    beam[kRound] = tid < a.N ? kbeam[tid] : 0;
+    if (first + kRound * kSelectThreads < total) {
+#pragma unroll
+      for (int r = 0; r < kRound; ++r)
+        keys[r] = a.pkey[(size_t)row0 * per_beam + min(first + (kRound + r) * kSelectThreads + tid, total - 1)];
+    }
+    u64 best = 0;
+#pragma unroll
+    for (int r = 0; r <= kRound; ++r) best = score[r] > best ? score[r] : best;
+    const u64 cut = nth_of_wave(best, a.N);
+    if (lane == 0) wcut[wave] = cut;
+    __syncthreads();
+    u64 least = 1;
+#pragma unroll
+    for (int i = 0; i < kSelectWaves; ++i) least = wcut[i] > least ? wcut[i] : least;
+    int mine = 0;
+#pragma unroll
+    for (int r = 0; r <= kRound; ++r) {
+      const u64 is = __ballot(score[r] >= least);
+      if (is == 0) continue;
+      const int p = mine + place_of(is);
+      if (score[r] >= least) {
+        lscore[wave][p] = score[r];
+        llogit[wave][p] = logit[r];
+        lbeam[wave][p] = beam[r];
+      }
+      mine += __popcll(is);
+    }
+    if (lane == 0) listed[wave] = mine;
+    __syncthreads();
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < kSelectWaves; ++w) n += listed[w];
+    if (tid < a.N && tid >= n) {
+      kscore[tid] = klogit[tid] = 0;
+      kbeam[tid] = 0;
+    }
+    if (n <= 64) {  // one each for the first wavefront's lanes
+      if (wave == 0) {
+        int at = lane, from = 0;
+#pragma unroll
+        for (int i = 0; i < kSelectWaves - 1; ++i)
+          if (from == i && at >= listed[i]) {
+            at -= listed[i];
+            ++from;
+          }
+        const bool is = lane < n;
+        const u64 x = is ? lscore[from][at] : 0, xl = is ? llogit[from][at] : 0;
+        const int xb = is ? lbeam[from][at] : 0;
+        int rank = 0;
+        for (int j = 0; j < n; ++j) {
+          const u64 y = lane_of(x, j);
+          const int yb = __builtin_amdgcn_readlane(xb, j);
+          rank += y > x || (y == x && (yb < xb || (yb == xb && lane_of(xl, j) > xl))) ? 1 : 0;
+        }
+        if (is && rank < a.N) {
+          kscore[rank] = x;
+          klogit[rank] = xl;
+          kbeam[rank] = xb;
+        }
+      }
+    } else
+    for (int i = lane; i < mine; i += 64) {
+      const u64 x = lscore[wave][i], xl = llogit[wave][i];
+      const int xb = lbeam[wave][i];
+      int rank = 0;
+      for (int w = 0; w < kSelectWaves; ++w)
+        for (int j = 0; j < listed[w]; ++j) {
+          const u64 y = lscore[w][j];
+          if (y > x)
+            ++rank;
+          else if (y == x)
+            rank += lbeam[w][j] < xb || (lbeam[w][j] == xb && llogit[w][j] > xl) ? 1 : 0;
+        }
+      if (rank < a.N) {
+        kscore[rank] = x;
+        klogit[rank] = xl;
+        kbeam[rank] = xb;
+      }
+    }
+    __syncthreads();
+  }
+  if (tid < a.N) {
+    const u64 x = kscore[tid];
+    const size_t o = (size_t)b * a.N + tid;
+    a.out_scores[o] = x == 0 ? kNegInf : (float)key_score(x);
+    a.out_parents[o] = kbeam[tid];
+    a.out_tokens[o] = x == 0 ? -1 : key_token(klogit[tid]);
   }
 }
 
@@ -423,11 +533,10 @@ hipError_t launch_select(const SelectArgs& a, hipStream_t stream) {
   const long long rows = (long long)a.B * a.W;
   const unsigned y = static_cast<unsigned>(std::min<long long>(rows, 32768));
   const dim3 grid(static_cast<unsigned>(a.segments), y, static_cast<unsigned>((rows + y - 1) / y));
-  switch (a.per_segment / kSelectThreads) {
-    case 4: hipLaunchKernelGGL((coalibi_select_rows_kernel<T, 4>), grid, dim3(kSelectThreads), 0, stream, a); break;
-    case 8: hipLaunchKernelGGL((coalibi_select_rows_kernel<T, 8>), grid, dim3(kSelectThreads), 0, stream, a); break;
-    case 16: hipLaunchKernelGGL((coalibi_select_rows_kernel<T, 16>), grid, dim3(kSelectThreads), 0, stream, a); break;
-    default: hipLaunchKernelGGL((coalibi_select_rows_kernel<T, 32>), grid, dim3(kSelectThreads), 0, stream, a); break;
+  switch (a.chunks) {
+    case 1: hipLaunchKernelGGL((coalibi_select_rows_kernel<T, 1>), grid, dim3(kSelectThreads), 0, stream, a); break;
+    case 2: hipLaunchKernelGGL((coalibi_select_rows_kernel<T, 2>), grid, dim3(kSelectThreads), 0, stream, a); break;
+    default: hipLaunchKernelGGL((coalibi_select_rows_kernel<T, 4>), grid, dim3(kSelectThreads), 0, stream, a); break;
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return e;

@@ -1055,13 +1055,17 @@ int append_args(const char* fn, int dtype, bool eight, const void* k, const void
 
 // Beam selection's segments of a row: the longest that give the GPU two work-groups per CU, else the shortest.
 struct SelectPlan {
-  int segments, per_segment;
+  int segments, chunks;
 };
-SelectPlan select_plan(int batch, int beams, int vocab) {
+SelectPlan select_plan(int dtype, int batch, int beams, int vocab) {
   const long long rows = static_cast<long long>(batch) * beams;
-  int per = 8192;
-  while (per > 1024 && rows * ((vocab + per - 1) / per) < 2ll * device_cus()) per /= 2;
-  return {(vocab + per - 1) / per, per};
+  int chunks = 4;
+  auto segments = [&] {
+    const int per = 256 * chunks * (dtype == CO_ALIBI_F32 ? 4 : 8);
+    return (vocab + per - 1) / per;
+  };
+  while (chunks > 1 && rows * segments() < 2ll * device_cus()) chunks /= 2;
+  return {segments(), chunks};
 }
 bool select_shape_ok(int batch, int beams, int num_beams, int vocab) {
   return batch >= 1 && beams >= 1 && beams <= coalibi::kMaxBeams && num_beams >= 1 && num_beams <= coalibi::kMaxBeams &&
@@ -1234,12 +1238,12 @@ int co_alibi_cache_read_8bit(int dtype, int format, const void* k_cache, const v
   return CO_ALIBI_OK;
 }
 
-size_t co_alibi_beam_select_workspace_bytes(int batch, int beams, int num_beams, int vocab) {
+size_t co_alibi_beam_select_workspace_bytes(int dtype, int batch, int beams, int num_beams, int vocab) {
   if (!select_shape_ok(batch, beams, num_beams, vocab)) return 0;
-  const SelectPlan p = select_plan(batch, beams, vocab);
+  const SelectPlan p = select_plan(dtype, batch, beams, vocab);
   const size_t parts = static_cast<size_t>(batch) * beams * p.segments;
   return round_up(parts * sizeof(double), 256) + round_up(parts * sizeof(float), 256) +
-         2 * round_up(parts * num_beams * sizeof(float), 256);
+         round_up(parts * num_beams * sizeof(unsigned long long), 256);
 }
 
 int co_alibi_beam_select(int dtype, const void* logits, const long long* strides, const float* scores,
@@ -1265,12 +1269,12 @@ int co_alibi_beam_select(int dtype, const void* logits, const long long* strides
       (rc = check_ptr(fn, "out_scores", out_scores, 4)) || (rc = check_ptr(fn, "parents", parents, 4)) ||
       (rc = check_ptr(fn, "tokens", tokens, 8)))
     return rc;
-  const size_t need = co_alibi_beam_select_workspace_bytes(batch, beams, num_beams, vocab);
+  const size_t need = co_alibi_beam_select_workspace_bytes(dtype, batch, beams, num_beams, vocab);
   if (workspace_bytes < need)
     return fail(CO_ALIBI_EINVAL, std::string(fn) + ": workspace of " + std::to_string(workspace_bytes) + " bytes, need " +
                                      std::to_string(need));
   if ((rc = check_ptr(fn, "workspace", workspace, 256))) return rc;
-  const SelectPlan p = select_plan(batch, beams, vocab);
+  const SelectPlan p = select_plan(dtype, batch, beams, vocab);
   const size_t parts = static_cast<size_t>(batch) * beams * p.segments;
   coalibi::SelectArgs a{};
   a.logits = logits;
@@ -1286,15 +1290,13 @@ int co_alibi_beam_select(int dtype, const void* logits, const long long* strides
   a.psum = reinterpret_cast<double*>(ws);
   ws += round_up(parts * sizeof(double), 256);
   a.pmax = reinterpret_cast<float*>(ws);
-  ws += round_up(parts * sizeof(float), 256);
-  a.pval = reinterpret_cast<float*>(ws);
-  a.ptok = reinterpret_cast<int*>(ws + round_up(parts * num_beams * sizeof(float), 256));
+  a.pkey = reinterpret_cast<unsigned long long*>(ws + round_up(parts * sizeof(float), 256));
   a.B = batch;
   a.W = beams;
   a.N = num_beams;
   a.V = vocab;
   a.segments = p.segments;
-  a.per_segment = p.per_segment;
+  a.chunks = p.chunks;
   hipStream_t st = static_cast<hipStream_t>(stream);
   hipError_t e;
   switch (dtype) {

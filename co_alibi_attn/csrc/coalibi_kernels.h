@@ -479,7 +479,7 @@ struct Read8Args {
 };
 
 // Beam selection: the N best of score[b][w] + log_softmax(logits[b][w])[t] over (w, t), rows (B, W) of V logits.
-// Workspace, per row and segment: pmax / psum of its weights and the N best logits (value, token), best first.
+// Workspace, per row and segment: pmax / psum of its weights and the N best logits with their tokens, best first, 0 for none.
 constexpr int kMaxBeams = 64;
 struct SelectArgs {
   const void* logits;
@@ -492,10 +492,9 @@ struct SelectArgs {
   long long* out_tokens; // (B, N)
   float* pmax;           // (B*W, segments)
   double* psum;
-  float* pval;  // (B*W, segments, N)
-  int* ptok;
+  unsigned long long* pkey;  // (B*W, segments, N)
   int B, W, N, V;
-  int segments, per_segment;
+  int segments, chunks;  // a segment has `chunks` 16-byte chunks for each of a work-group's 256 threads
 };
 
 // Reordering a paged cache: sequence (g, i) of B groups of W takes over the rows of sequence (g, parents[g][i]).

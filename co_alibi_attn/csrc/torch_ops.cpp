@@ -699,7 +699,7 @@ std::tuple<Tensor, Tensor, Tensor> beam_select_hip(const Tensor& logits_in, cons
   if (batch == 0) return {scores, parents, tokens};
   const Tensor logits = logits_in.stride(2) == 1 || vocab == 1 ? logits_in : logits_in.contiguous();
   const Tensor from = scores_in.to(logits.device()).contiguous();
-  const size_t ws_bytes = co_alibi_beam_select_workspace_bytes(as_int(fn, "batch", batch), as_int(fn, "beams", beams),
+  const size_t ws_bytes = co_alibi_beam_select_workspace_bytes(code, as_int(fn, "batch", batch), as_int(fn, "beams", beams),
                                                                as_int(fn, "num_beams", num_beams), as_int(fn, "vocab", vocab));
   Tensor ws = at::empty({static_cast<int64_t>(ws_bytes)}, logits.options().dtype(at::kByte));
   const std::array<long long, 2> strides{batch == 1 ? beams * vocab : logits.stride(0), beams == 1 ? vocab : logits.stride(1)};

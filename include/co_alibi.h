@@ -327,7 +327,7 @@ int co_alibi_decode_tree_8bit(int dtype, int format, const void* q, const void* 
  * has no candidates, and a logit of -inf is none; of +inf logits all weigh the same and every other one nothing.  Results, each
  * (batch, num_beams): out_scores, parents (the beam) and tokens; places without a candidate get -inf, 0 and -1.  At most 64 beams in
  * and out, vocab <= 2^20.  workspace holds co_alibi_beam_select_workspace_bytes(...) bytes (256-byte aligned). */
-size_t co_alibi_beam_select_workspace_bytes(int batch, int beams, int num_beams, int vocab);
+size_t co_alibi_beam_select_workspace_bytes(int dtype, int batch, int beams, int num_beams, int vocab);
 int co_alibi_beam_select(int dtype, const void* logits, const long long* strides, const float* scores,
                          const unsigned char* finished, int end_token, float* out_scores, int* parents, long long* tokens,
                          void* workspace, size_t workspace_bytes, int batch, int beams, int num_beams, int vocab,

@@ -170,9 +170,9 @@ def test_select_argument_errors(over, code, msg):
 
 def test_select_workspace():
     size = _native.lib().co_alibi_beam_select_workspace_bytes
-    assert size(0, 1, 1, 9) == size(1, 65, 1, 9) == size(1, 1, 65, 9) == size(1, 1, 1, 0) == 0
-    for B, W, N, V in ((1, 1, 1, 1), (1, 4, 4, 50304), (16, 8, 8, 131071)):
-        assert 4 * 256 <= size(B, W, N, V) <= B * W * (-(-V // 1024) * (12 + 8 * N)) + 4 * 256
+    assert size(1, 0, 1, 1, 9) == size(1, 1, 65, 1, 9) == size(1, 1, 1, 65, 9) == size(1, 1, 1, 1, 0) == 0
+    for dtype, B, W, N, V in ((0, 1, 1, 1, 1), (0, 1, 4, 4, 50304), (2, 16, 8, 8, 131071)):
+        assert 3 * 256 <= size(dtype, B, W, N, V) <= B * W * (-(-V // 1024) * (12 + 8 * N)) + 3 * 256
 
 
 def _reorder(**over):
