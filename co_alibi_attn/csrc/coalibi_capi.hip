@@ -847,7 +847,9 @@ size_t tree_workspace(const TreePlan& p, bool ragged, int batch, int heads_q, in
 }
 
 
-// How a decode over an 8-bit cache is split, in chunks of 32 keys for each wavefront of a work-group: as tree_plan.
+int envi(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
+const int kR = envi("T8_ROUNDS", 1), kS = envi("T8_SPLITS", 8), kW = envi("T8_WHOLE", 3);
+// How a decode over an 8-bit cache is split, in chunks of 128 keys, 32 for each wavefront of a work-group: as tree_plan.
 TreePlan tree8_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim) {
   const int rows = heads_q / heads_kv * tokens;
   TreePlan p;
@@ -861,13 +863,13 @@ TreePlan tree8_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens,
     const int most = static_cast<int>(std::min<long long>({std::max(n, 1ll), chunks, coalibi::kMaxTreeSplits}));
     return (chunks + most - 1) / most;
   };
-  p.cps = chunks <= 3 ? chunks : walk(slots / units);
+  p.cps = chunks <= kW ? chunks : walk(slots / units);
   p.splits = (chunks + p.cps - 1) / p.cps;
-  p.share = static_cast<int>(std::max<long long>(slots / heads, 1));
-  p.planned = static_cast<int>(std::min<long long>({p.splits * static_cast<long long>(kTreeRaggedSplits), chunks, p.share,
+  p.share = static_cast<int>(std::max<long long>(kR * slots / heads, 1));
+  p.planned = static_cast<int>(std::min<long long>({std::max(p.splits * static_cast<long long>(kTreeRaggedSplits), (long long)kS), chunks, std::max(p.share, 2),
                                                     coalibi::kMaxTreeSplits}));
   p.planned = std::max({p.planned, p.splits, 2});
-  p.plans = slots / units > 1 && walk(slots / units) >= kTreePlanWalk;
+  p.plans = batch > 1 && chunks >= 8 && p.share > batch;
   return p;
 }
 bool tree_shape_ok(int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim) {

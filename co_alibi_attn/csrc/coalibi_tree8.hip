@@ -16,6 +16,7 @@
 // There are no barriers and no LDS in the loop.  The four wavefronts of a work-group take four runs of a split's tiles and are
 // joined at its end, each one's maximum shifted by the sigmas of the keys after it, as splits are in the merge.
 #include <algorithm>
+#include <type_traits>
 
 #include "coalibi_tree.h"
 
@@ -28,33 +29,66 @@ constexpr int kTree8Threads = 64 * kTree8Waves;
 
 typedef unsigned short u16;
 
-// Pair HI (bytes 0 and 1, or 2 and 3) of the codes in x, as two T.
+// Byte N of x, an int8, as a float: one conversion that picks the byte.  (A shift and a cast took two instructions for odd bytes.)
+template <int N>
+__device__ __forceinline__ float signed_byte(unsigned x) {
+  return static_cast<float>((int)__builtin_amdgcn_sbfe((int)x, 8 * N, 8));
+}
+
+// Two floats of at most 8 significant bits as two bfloat16.
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+  return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, hi), __builtin_bit_cast(unsigned, lo), 0x07060302u);
+}
+// Pair HI (bytes 0 and 1, or 2 and 3) of the codes in x, as the bits of two 16-bit T.
 template <typename T, typename F, bool HI>
-__device__ __forceinline__ void code_pair(unsigned x, T* out) {
-  if constexpr (__is_same(F, E4M3)) {
-    if constexpr (__is_same(T, __bf16)) {
-      const auto p = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, HI);
-      out[0] = p[0];
-      out[1] = p[1];
-    } else if constexpr (__is_same(T, _Float16)) {
-      const auto p = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, HI);
-      out[0] = p[0];
-      out[1] = p[1];
-    } else {
-      const auto p = __builtin_amdgcn_cvt_pk_f32_fp8(x, HI);
-      out[0] = p[0];
-      out[1] = p[1];
-    }
+__device__ __forceinline__ unsigned code_pair(unsigned x) {
+  if constexpr (__is_same(F, E4M3) && __is_same(T, __bf16)) {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, HI));
+  } else if constexpr (__is_same(F, E4M3)) {
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, HI));
   } else if constexpr (__is_same(T, _Float16)) {
     // The byte plus 128 in the last bits of 1024: exact, and so is the difference.
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     const unsigned h = __builtin_amdgcn_perm(0x64646464u, x ^ 0x80808080u, HI ? 0x05030402u : 0x05010400u);
-    const f16x2 p = __builtin_bit_cast(f16x2, h) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f};
-    out[0] = p[0];
-    out[1] = p[1];
+    return __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, h) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f});
   } else {
-    out[0] = static_cast<T>(static_cast<float>(static_cast<signed char>(x >> (HI ? 16 : 0))));
-    out[1] = static_cast<T>(static_cast<float>(static_cast<signed char>(x >> (HI ? 24 : 8))));
+    return pack_bf16(signed_byte<HI ? 2 : 0>(x), signed_byte<HI ? 3 : 1>(x));
+  }
+}
+// Byte N of x, a code, as a float.
+template <typename F, int N>
+__device__ __forceinline__ float code_float(unsigned x) {
+  if constexpr (__is_same(F, E4M3)) return __builtin_amdgcn_cvt_f32_fp8((int)x, N);
+  return signed_byte<N>(x);
+}
+// Eight codes, four of lo and four of hi, as a product's operand.
+template <typename T, typename F>
+__device__ __forceinline__ typename Mfma<T>::vec8 code_vec8(unsigned lo, unsigned hi) {
+  if constexpr (sizeof(T) == 2)
+    return __builtin_bit_cast(typename Mfma<T>::vec8, u32x4{code_pair<T, F, false>(lo), code_pair<T, F, true>(lo),
+                                                            code_pair<T, F, false>(hi), code_pair<T, F, true>(hi)});
+  else
+    return f32x8{code_float<F, 0>(lo), code_float<F, 1>(lo), code_float<F, 2>(lo), code_float<F, 3>(lo),
+                 code_float<F, 0>(hi), code_float<F, 1>(hi), code_float<F, 2>(hi), code_float<F, 3>(hi)};
+}
+// Byte N of eight words as an operand.  Of two words at a time, the byte of both as a pair.
+template <typename T, typename F, int N>
+__device__ __forceinline__ typename Mfma<T>::vec8 byte_vec8(const unsigned (&w)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    f32x8 x;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = code_float<F, N>(w[e]);
+    return x;
+  } else {
+    u32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (__is_same(F, I8) && __is_same(T, __bf16))
+        x[e] = pack_bf16(signed_byte<N>(w[2 * e]), signed_byte<N>(w[2 * e + 1]));
+      else  // (the permute serves the next byte, too)
+        x[e] = code_pair<T, F, (N & 1) != 0>(__builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], N & 2 ? 0x07030602u : 0x05010400u));
+    }
+    return __builtin_bit_cast(typename Mfma<T>::vec8, x);
   }
 }
 
@@ -78,13 +112,11 @@ struct Run {
   }
 };
 
-// A tile's codes as a lane holds them, and its half's scales.
+// A tile's keys as a lane holds them, and its half's scales.
 template <int D>
-struct Tile8 {
+struct Keys8 {
   static constexpr int KL = D < 32 ? 1 : D / 32;  // 16-byte pieces of a key (D 16: 8 bytes)
-  static constexpr int DT = D < 32 ? 1 : D / 32;
   u32x4 k[KL];
-  Run<DT> v[16];
   float ks, vs;
 };
 
@@ -150,7 +182,7 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
 
   unsigned long long sees = 0;
   if (newest) {
-    if (tid == 0 && nS > 1) a.used[bhk] = sp.used;
+    if (tid == 0 && nS > 1) a.used[bhk] = sp.used;  // every row block writes the same
     const unsigned long long all = ancestors(a, b, lane);
     sees = (unsigned long long)__shfl((unsigned)(all >> 32), t, 64) << 32 | __shfl((unsigned)all, t, 64);
   }
@@ -163,89 +195,99 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
   const float* const vsc = a8.vs + (size_t)hkv * a8.vsh;
   const int page_mask = a.place.table != nullptr ? (1 << a.place.page_shift) - 1 : 0x7fffffff;
 
-  // The units of a tile's two blocks of 16 rows, -1 for a block on no page of the pool (its rows are read from unit 0).
+  // The table entries of a tile's two blocks of 16 rows (of the last filled row past it).  They are looked at when they are used:
+  // an entry outside the pool is read as unit 0, and makes the sequence NaN.
   struct Units {
     int u[2];
   };
+  const int* const table = a.place.table + (size_t)b * a.place.table_stride;
   auto find = [&](int tile) {
     Units f{{b, b}};
     if (a.place.table != nullptr) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int r = min(tile * 32 + 16 * i, L - 1);
-        const int u = scalar_load(a.place.table + (size_t)b * a.place.table_stride + (r >> a.place.page_shift));
-        f.u[i] = u >= 0 && u < a.place.units ? u : -1;
-      }
+      for (int i = 0; i < 2; ++i) f.u[i] = scalar_load(table + (min(tile * 32 + 16 * i, L - 1) >> a.place.page_shift));
     }
     return f;
   };
   bool lost = false;
-  // A cached tile's loads.  Rows past the filled ones are read from the last of them: their scores are masked.
-  auto load = [&](int tile, const Units& f) {
-    Tile8<D> x;
-    lost |= (f.u[0] | f.u[1]) < 0;
-    const int u0 = max(f.u[0], 0), u1 = max(f.u[1], 0);
-    const int key0 = tile * 32;
-    {
-      const int key = min(key0 + kRowOfReg(hl), L - 1);
-      const char* const base0 = kc + (size_t)u0 * a.kcl.b;
-      const char* const base1 = kc + (size_t)u1 * a.kcl.b;
-      const char* const p = (kRowOfReg(hl) >= 16 ? base1 : base0) + (size_t)(key & page_mask) * D;
-      if constexpr (D < 32) {
-        const u32x2 lo = *reinterpret_cast<const u32x2*>(p + hh * 8);
-        x.k[0] = u32x4{lo[0], lo[1], 0, 0};
-      } else {
+  auto check = [&](Units& f) {
+    if (a.place.table != nullptr) {
 #pragma unroll
-        for (int i = 0; i < Tile8<D>::KL; ++i) x.k[i] = ld16(p + 32 * i + 16 * hh);
+      for (int i = 0; i < 2; ++i) {
+        const bool in = (unsigned)f.u[i] < (unsigned)a.place.units;
+        lost |= !in;
+        f.u[i] = in ? f.u[i] : 0;
       }
     }
-    const int first = min(key0 + 16 * hh, L - 1);  // the half's first key
-    const int u = hh ? u1 : u0;
-    {
-      const size_t at = (first & page_mask) >> 4;
-      x.ks = ksc[(size_t)u * a8.ksb + at];
-      x.vs = vsc[(size_t)u * a8.vsb + at];
-    }
-    const char* const p = vc + (size_t)u * a.vcl.b + (size_t)(first & page_mask) * D + (D < 32 ? hl & 15 : DT * hl);
-    if (key0 + 32 <= L) {
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x.v[i].load(p + i * D);
-    } else {
-      const int left = L - 1 - first;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x.v[i].load(p + min(i, left) * D);
-    }
-    return x;
   };
+  // A cached tile's loads.  CLAMP: rows past the filled ones are read from the last of them (their scores are masked).  Every lane
+  // reads from one of the tile's two blocks: their addresses are the wavefront's, and a lane picks.
+  const int krow = kRowOfReg(hl);
+  auto pick = [](bool second, const auto* p0, const auto* p1) {
+    const auto a0 = (unsigned long long)p0, a1 = (unsigned long long)p1;
+    const unsigned lo = second ? (unsigned)a1 : (unsigned)a0, hi = second ? (unsigned)(a1 >> 32) : (unsigned)(a0 >> 32);
+    return (decltype(p0))((unsigned long long)hi << 32 | lo);
+  };
+  auto load_keys = [&](auto clamp, int tile, const Units& f, Keys8<D>& x) {
+    const int key0 = tile * 32;
+    const int key = decltype(clamp)::value ? min(key0 + krow, L - 1) : key0 + krow;
+    const char* const p = pick(krow >= 16, kc + (size_t)f.u[0] * a.kcl.b, kc + (size_t)f.u[1] * a.kcl.b) +
+                          (size_t)(key & page_mask) * D + hh * (D < 32 ? 8 : 16);
+    if constexpr (D < 32) {
+      const u32x2 lo = *reinterpret_cast<const u32x2*>(p);
+      x.k[0] = u32x4{lo[0], lo[1], 0, 0};
+    } else {
+#pragma unroll
+      for (int i = 0; i < Keys8<D>::KL; ++i) x.k[i] = ld16(p + 32 * i);
+    }
+    const int r1 = decltype(clamp)::value ? min(key0 + 16, L - 1) : key0 + 16;
+    const int at0 = (key0 & page_mask) >> 4, at1 = (r1 & page_mask) >> 4;
+    x.ks = *pick(hh != 0, ksc + (size_t)f.u[0] * a8.ksb + at0, ksc + (size_t)f.u[1] * a8.ksb + at1);
+    x.vs = *pick(hh != 0, vsc + (size_t)f.u[0] * a8.vsb + at0, vsc + (size_t)f.u[1] * a8.vsb + at1);
+  };
+  auto load_values = [&](auto clamp, int tile, const Units& f, Run<DT> (&v)[16]) {
+    const int r0 = tile * 32, r1 = decltype(clamp)::value ? min(r0 + 16, L - 1) : r0 + 16;
+    const char* const p = pick(hh != 0, vc + (size_t)f.u[0] * a.vcl.b + (size_t)(r0 & page_mask) * D,
+                               vc + (size_t)f.u[1] * a.vcl.b + (size_t)(r1 & page_mask) * D) +
+                          (D < 32 ? hl & 15 : DT * hl);
+    const int left = L - 1 - (hh ? r1 : r0);  // (clamped)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i].load(p + (decltype(clamp)::value ? min(i, left) : i) * D);
+  };
+  using Inside = std::false_type;
+  using Clamped = std::true_type;
 
   // Q^T fragments in the order of K's: step 2 i + s holds the elements 32 i + 16 (l / 32) + 8 s + e of the row (D 16: 8 (l / 32)
-  // + e).  Zero past R.
+  // + e).  Past R they are the first row's, and come to nothing.
   V8 qf[C::KS];
   {
     const T* const q = head_at(static_cast<const T*>(a.q), a.ql, b, h) + (size_t)t * a.ql.r;
 #pragma unroll
     for (int ks = 0; ks < C::KS; ++ks)
-      qf[ks] = row_ok ? ld_vec8(q + (D < 32 ? 8 * hh : (ks >> 1) * 32 + 16 * hh + (ks & 1) * 8)) : zero_vec8<T>();
+      qf[ks] = ld_vec8(q + (D < 32 ? 8 * hh : (ks >> 1) * 32 + 16 * hh + (ks & 1) * 8));
   }
 
   // State of the lane's row: scale, this half's share of the sum, O^T, and the sigma of the keys after the current ones.
   float m2 = kNegInf, lsum = 0.f, carry = 0.f;
+  V8 pb[2];  // weights of the last tile
   f32x16 acc[DT];
 #pragma unroll
   for (int j = 0; j < DT; ++j) acc[j] = f32x16{};
 
-  // From a tile's scores (log2 units; -inf where the row does not see the key) to its weights, in the order of P^T.
-  auto weigh = [&](f32x16 s, float vs, V8 (&pb)[2]) {
+  // From a tile's scores (log2 units; -inf where the row does not see the key) to its weights, in the order of P^T; without `near`
+  // only its sigmas count.
+  auto weigh_or_pass = [&](f32x16 s, float vs, bool near) {
     float loc[16], run = 0.f;
 #pragma unroll
     for (int r = 15; r >= 0; --r) {
       run += sigmoid_log2(s[r]);
       loc[r] = run;
     }
-    const float oth = other_half(run);
-    const float mb = m2 == kNegInf ? 0.f : m2;
-    const float cst = mb + lam2 * (carry + (hh ? 0.f : oth)) - __builtin_amdgcn_logf(vs);
+    const float oth = other_half(run), before = carry;
     carry += hh ? run + oth : oth + run;
+    if (!near) return;
+    const float mb = m2 == kNegInf ? 0.f : m2;
+    const float cst = mb + lam2 * (before + (hh ? 0.f : oth)) - __builtin_amdgcn_logf(vs);
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = fmaf(-lam2, loc[r], s[r] - cst);
     auto weights = [&] {
@@ -280,14 +322,61 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
     }
     lsum = fmaf(sum, fast_rcp(vs), lsum);
   };
+  auto weigh = [&](f32x16 s, float vs) { weigh_or_pass(s, vs, true); };
+
+  // The scores of a tile of cached keys, in log2 units.
+  auto scores = [&](const Keys8<D>& x) {
+    f32x16 s{};
+#pragma unroll
+    for (int ks = 0; ks < C::KS; ++ks) {
+      const unsigned lo = x.k[ks >> 1][2 * (ks & 1)], hi = x.k[ks >> 1][2 * (ks & 1) + 1];
+      s = M::k16(code_vec8<T, F>(lo, hi), qf[ks], s);
+    }
+    const float sc = a.sc2 * x.ks;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= sc;
+    return s;
+  };
+  auto scale_of = [&](const Keys8<D>& x) {
+    const bool fine = scale_ok(x.ks) && scale_ok(x.vs);
+    lost |= !fine;
+    return fine ? x.vs : 1.f;
+  };
+  auto add_values = [&](const Run<DT> (&v)[16], const V8 (&pb)[2]) {
+#pragma unroll
+    for (int st = 0; st < 2; ++st) {
+#pragma unroll
+      for (int q4 = 0; q4 < (DT + 3) / 4; ++q4) {
+        unsigned w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = v[8 * st + e].w[q4];
+        acc[4 * q4] = M::k16(byte_vec8<T, F, 0>(w), pb[st], acc[4 * q4]);
+        if constexpr (DT > 1) acc[4 * q4 + 1] = M::k16(byte_vec8<T, F, 1>(w), pb[st], acc[4 * q4 + 1]);
+        if constexpr (DT > 2) {
+          acc[4 * q4 + 2] = M::k16(byte_vec8<T, F, 2>(w), pb[st], acc[4 * q4 + 2]);
+          acc[4 * q4 + 3] = M::k16(byte_vec8<T, F, 3>(w), pb[st], acc[4 * q4 + 3]);
+        }
+      }
+    }
+  };
 
   int tile = t_end - 1;
+  const int whole = min(t_end, L >> 5) - 1;  // the newest tile of filled rows alone
+  Keys8<D> ka, kb;
+  Run<DT> v[16];
+  Units ua{}, ub{};
+  if (whole >= t_first) {
+    ua = find(whole);
+    check(ua);
+    load_keys(Inside{}, whole, ua, ka);
+    ub = find(max(whole - 1, t_first));
+  }
   // The new keys' tiles.
   for (; tile >= t_first && tile >= cache_tiles; --tile) {
     const int key0 = (tile - cache_tiles) * 32;
     f32x16 s{};
     {
-      const T* const k = kn + (size_t)min(key0 + kRowOfReg(hl), a.T - 1) * a.kl.r;
+      const T* const k = kn + (size_t)min(key0 + krow, a.T - 1) * a.kl.r;
 #pragma unroll
       for (int ks = 0; ks < C::KS; ++ks)
         s = M::k16(ld_vec8(k + (D < 32 ? 8 * hh : (ks >> 1) * 32 + 16 * hh + (ks & 1) * 8)), qf[ks], s);
@@ -295,28 +384,33 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
     const unsigned ok = (unsigned)(sees >> (key0 + 16 * hh));
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = ok >> r & 1 ? s[r] * a.sc2 : kNegInf;
-    V8 pb[2];
-    weigh(s, 1.0f, pb);
+    weigh(s, 1.0f);
     // A product with a weight of 0 would carry an infinity or a NaN of a value to rows that do not see it: such values are 0
     // here and added to the rows that do below.
     unsigned bad = 0;
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
+    for (int st = 0; st < 2; ++st) {
+      typedef T row_t __attribute__((ext_vector_type(DT)));
+      row_t x[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        x[e] = *reinterpret_cast<const row_t*>(vn + (size_t)min(key0 + 16 * hh + 8 * st + e, a.T - 1) * a.vl.r +
+                                               (D < 32 ? hl & 15 : DT * hl));
 #pragma unroll
       for (int j = 0; j < DT; ++j) {
         V8 va;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const int key = 16 * hh + 8 * st + e;
-          T x = vn[(size_t)min(key0 + key, a.T - 1) * a.vl.r + (D < 32 ? hl & 15 : DT * hl + j)];
-          if (not_finite(x)) {
-            x = T(0);
-            bad |= 1u << key;
+          T y = x[e][j];
+          if (not_finite(y)) {
+            y = T(0);
+            bad |= 1u << (16 * hh + 8 * st + e);
           }
-          va[e] = x;
+          va[e] = y;
         }
         acc[j] = M::k16(va, pb[st], acc[j]);
       }
+    }
     if (__any(bad != 0)) {
       for (int key = 0; key < min(a.T - key0, 32); ++key) {
         if (!__any(bad >> key & 1)) continue;
@@ -334,64 +428,49 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
       }
     }
   }
-
-  // The cache's tiles, each one's codes loaded while the one before is worked on, and its units another one before.
-  if (tile >= t_first) {
-    Units units = find(tile);
-    Tile8<D> cur = load(tile, units);
-    units = find(max(tile - 1, t_first));
-    for (; tile >= t_first; --tile) {
-      Tile8<D> next;
-      if (tile > t_first) {
-        next = load(tile - 1, units);
-        units = find(max(tile - 2, t_first));
-      }
-      f32x16 s{};
+  // The tile that the filled rows end in.
+  if (tile > whole && tile >= t_first) {
+    Units f = find(tile);
+    check(f);
+    load_keys(Clamped{}, tile, f, kb);
+    load_values(Clamped{}, tile, f, v);
+    f32x16 s = scores(kb);
+    const int left = L - tile * 32 - 16 * hh;
 #pragma unroll
-      for (int ks = 0; ks < C::KS; ++ks) {
-        T x[8];
-        const unsigned lo = cur.k[ks >> 1][2 * (ks & 1)], hi = cur.k[ks >> 1][2 * (ks & 1) + 1];
-        code_pair<T, F, false>(lo, x);
-        code_pair<T, F, true>(lo, x + 2);
-        code_pair<T, F, false>(hi, x + 4);
-        code_pair<T, F, true>(hi, x + 6);
-        s = M::k16(V8{x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]}, qf[ks], s);
-      }
-      const bool fine = scale_ok(cur.ks) && scale_ok(cur.vs);
-      lost |= !fine;
-      const float vs = fine ? cur.vs : 1.f, sc = a.sc2 * cur.ks;
-      const int left = L - tile * 32 - 16 * hh;
-      if (tile * 32 + 32 > L) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = r < left ? s[r] * sc : kNegInf;
-      } else {
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= sc;
-      }
-      V8 pb[2];
-      weigh(s, vs, pb);
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-#pragma unroll
-        for (int jj = 0; jj < (DT + 1) / 2; ++jj) {
-          T x[2][8];
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            // Keys e and e + 1 of the step: [d, d, d + 1, d + 1].
-            const unsigned w = __builtin_amdgcn_perm(cur.v[8 * st + e + 1].w[jj >> 1], cur.v[8 * st + e].w[jj >> 1],
-                                                     jj & 1 ? 0x07030602u : 0x05010400u);
-            code_pair<T, F, false>(w, &x[0][e]);
-            if constexpr (DT > 1) code_pair<T, F, true>(w, &x[1][e]);
-          }
-#pragma unroll
-          for (int i = 0; i < (DT > 1 ? 2 : 1); ++i)
-            acc[2 * jj + i] = M::k16(V8{x[i][0], x[i][1], x[i][2], x[i][3], x[i][4], x[i][5], x[i][6], x[i][7]}, pb[st],
-                                     acc[2 * jj + i]);
-        }
-      }
-      cur = next;
-    }
+    for (int r = 0; r < 16; ++r) s[r] = r < left ? s[r] : kNegInf;
+    weigh(s, scale_of(kb));
+    add_values(v, pb);
+    --tile;
   }
+  // The others.  Keys come in a tile ahead and table entries two; a tile's values while it is weighed and the next one's scores
+  // are taken, which is when its own product with the weights follows.
+  bool held = false;  // such a product is due
+  auto step = [&](Keys8<D>& x, Keys8<D>& next) {
+    const Units f = ua;
+    if (tile > t_first) {
+      ua = ub;
+      check(ua);
+      load_keys(Inside{}, tile - 1, ua, next);
+      ub = find(max(tile - 2, t_first));
+    }
+    f32x16 s = scores(x);
+    if (held) add_values(v, pb);
+    // A tile whose keys all weigh less than 2^-a.far of their row's sum, as far as it is known, is left out but for its sigmas: a_j
+    // is at most its score less the sigmas after the tile.  (A NaN keeps it.)
+    float mt = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
+    held = __any(row_ok && !(lam2 >= 0.f && mt - lam2 * carry - m2 < __builtin_amdgcn_logf(lsum) - a.far));
+    if (held) load_values(Inside{}, tile, f, v);
+    weigh_or_pass(s, scale_of(x), held);
+    --tile;
+  };
+  while (tile >= t_first) {
+    step(ka, kb);
+    if (tile < t_first) break;
+    step(kb, ka);
+  }
+  if (held) add_values(v, pb);
 
   // The wavefronts joined: each one's maximum shifted by the sigmas of the later ones' keys.
   const float l = lsum + other_half(lsum);
