@@ -847,9 +847,13 @@ size_t tree_workspace(const TreePlan& p, bool ragged, int batch, int heads_q, in
 }
 
 
-int envi(const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; }
-const int kR = envi("T8_ROUNDS", 1), kS = envi("T8_SPLITS", 8), kW = envi("T8_WHOLE", 3);
-// How a decode over an 8-bit cache is split, in chunks of 128 keys, 32 for each wavefront of a work-group: as tree_plan.
+// How a decode over an 8-bit cache is split, in chunks of 128 keys, 32 for each wavefront of a work-group: as tree_plan, but for:
+//   The plan is made wherever lengths may differ, and shares the chunks out over two rounds of work-groups where a kv head has more than one
+// row block: those launches are bound by their instructions, and a second round evens out what one leaves idle.  16 sequences of up to
+// 8192 keys, us, 1 / 2 / 3 rounds: 96 rows 94.5 / 86 / 88; 4 rows over 32 sequences, bound by HBM, 67 / 70 / 75.
+//   A long sequence gets at most 4 times the splits by the bound: 4 / 8 / 16 of them 86 / 91 / 93 (the merge grows).
+//   Three chunks go through one work-group: 12 heads, 500 keys (5 chunks) 9.2 us split, 9.3 whole.
+constexpr int kTree8Whole = 3, kTree8RaggedChunks = 8;
 TreePlan tree8_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim) {
   const int rows = heads_q / heads_kv * tokens;
   TreePlan p;
@@ -863,13 +867,13 @@ TreePlan tree8_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens,
     const int most = static_cast<int>(std::min<long long>({std::max(n, 1ll), chunks, coalibi::kMaxTreeSplits}));
     return (chunks + most - 1) / most;
   };
-  p.cps = chunks <= kW ? chunks : walk(slots / units);
+  p.cps = chunks <= kTree8Whole ? chunks : walk(slots / units);
   p.splits = (chunks + p.cps - 1) / p.cps;
-  p.share = static_cast<int>(std::max<long long>(kR * slots / heads, 1));
-  p.planned = static_cast<int>(std::min<long long>({std::max(p.splits * static_cast<long long>(kTreeRaggedSplits), (long long)kS), chunks, std::max(p.share, 2),
-                                                    coalibi::kMaxTreeSplits}));
+  p.share = static_cast<int>(std::max<long long>((p.row_blocks > 1 ? 2 : 1) * slots / heads, 1));
+  p.planned = static_cast<int>(std::min<long long>({p.splits * static_cast<long long>(kTreeRaggedSplits), chunks,
+                                                    std::max(p.share, 2), coalibi::kMaxTreeSplits}));
   p.planned = std::max({p.planned, p.splits, 2});
-  p.plans = batch > 1 && chunks >= 8 && p.share > batch;
+  p.plans = batch > 1 && chunks >= kTree8RaggedChunks && p.share > batch;
   return p;
 }
 bool tree_shape_ok(int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim) {
