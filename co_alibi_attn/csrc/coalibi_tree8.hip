@@ -132,6 +132,28 @@ struct Tree8Cfg {
 // Whether a scale is one that the formulas hold for: from the smallest to the largest (a NaN is not).
 __device__ __forceinline__ bool scale_ok(float s) { return s >= kScaleLeast && s <= kScaleMost; }
 
+// As plan_item, but by kv head, the last head first: its slopes are the flattest where their number is a power of two, and the tiles
+// of flat heads, of which few are left out, take the longest.
+__device__ __forceinline__ TreeItem head_item(const TreeArgs& a, int cps, int id, int lane) {
+  auto splits = [&](int b) { return b < a.B ? splits_of(a, cps, chunks_of(a, filled_rows(a, b))).used : 0; };
+  int total = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) total += wave_total(splits(b0 + lane));
+  const int head = id / total;
+  if (head >= a.Hkv) return {-1, 0};
+  const int at = id - head * total;
+  int before = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    const int n = splits(b0 + lane), incl = wave_prefix(n);
+    const unsigned long long in = __ballot(at < before + incl);
+    if (in != 0) {
+      const int l = __ffsll(in) - 1;
+      return {(b0 + l) * a.Hkv + a.Hkv - 1 - head, at - before - (__shfl(incl, l, 64) - __shfl(n, l, 64))};
+    }
+    before += __builtin_amdgcn_readlane(incl, 63);
+  }
+  return {-1, 0};
+}
+
 template <typename T, typename F, int D>
 __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void coalibi_tree8_kernel(Tree8Args a8) {
   using C = Tree8Cfg<T, D>;
@@ -150,15 +172,16 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
   const int rb = (id >> 3) % RB, item = (id / (8 * RB)) * 8 + (id & 7);
   const int nS = a.nSplits;
   int cps = a.cps;
-  TreeItem it{item / nS, item % nS};
+  TreeItem it;
   if (a.plan) {
     cps = plan_cps(a, lane);
-    it = plan_item(a, cps, item, lane);
-    if (it.bhk < 0) return;
-  } else if (it.bhk >= a.B * a.Hkv) {
-    return;
+    it = head_item(a, cps, item, lane);
+  } else {
+    const int per_head = a.B * nS, head = item / per_head, at = item - head * per_head;
+    it = head < a.Hkv ? TreeItem{at / nS * a.Hkv + a.Hkv - 1 - head, at % nS} : TreeItem{-1, 0};
   }
   const int bhk = __builtin_amdgcn_readfirstlane(it.bhk), split = __builtin_amdgcn_readfirstlane(it.split);
+  if (bhk < 0) return;
   const int b = __builtin_amdgcn_readfirstlane(bhk / a.Hkv), hkv = bhk - b * a.Hkv;
   const int L = __builtin_amdgcn_readfirstlane(filled_rows(a, b));
   const int chunks = __builtin_amdgcn_readfirstlane(chunks_of(a, L));
