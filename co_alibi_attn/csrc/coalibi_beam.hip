@@ -12,12 +12,13 @@
 //
 // Reordering: a group of W beams owns W pages in every column of its block table.  Pages that are full are shared by all that
 // descend from them; one in use stays with the first of its heirs, and the others get free pages of its column and copies of
-// its rows.  That many are free, as no more than W are in use.  Every wavefront works out its column's W beams by itself, a lane
-// each, so that tables and copies are one launch.
+// its rows.  That many are free, as no more than W are in use.  A wavefront works out a column's W beams by itself, a lane
+// each, for the tables and again for every copy, so that all is one launch.
 #include <algorithm>
 
 #include "coalibi_common.h"
 #include "coalibi_kernels.h"
+#include "coalibi_wave.h"
 
 namespace coalibi {
 
@@ -25,7 +26,6 @@ namespace {
 
 constexpr int kSelectThreads = 256;
 constexpr int kSelectWaves = kSelectThreads / 64;
-typedef unsigned long long u64;
 
 // A float as a number of the same order.
 __device__ __forceinline__ unsigned ordered(float x) {
@@ -39,48 +39,6 @@ __device__ __forceinline__ u64 logit_key(float x, int token) { return (u64)order
 __device__ __forceinline__ float key_logit(u64 k) { return unordered((unsigned)(k >> 32)); }
 __device__ __forceinline__ int key_token(u64 k) { return (int)~(unsigned)k; }
 
-// The number of a lane's partner in step S of six that join 1, 2, 4, ..., 32 lanes, of which those of a group hold the same.
-template <int S>
-__device__ __forceinline__ unsigned partner(unsigned x) {
-  if constexpr (S < 4) {  // quad_perm [1, 0, 3, 2] and [2, 3, 0, 1], row_half_mirror, row_mirror
-    constexpr int ctrl = S == 0 ? 0xb1 : S == 1 ? 0x4e : S == 2 ? 0x141 : 0x140;
-    return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, ctrl, 0xf, 0xf, false);
-  } else if constexpr (S == 4) {
-    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    return threadIdx.x & 16 ? r[0] : r[1];
-  } else {
-    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    return threadIdx.x & 32 ? r[0] : r[1];
-  }
-}
-template <int S>
-__device__ __forceinline__ u64 partner(u64 x) {
-  return (u64)partner<S>((unsigned)(x >> 32)) << 32 | partner<S>((unsigned)x);
-}
-template <int S>
-__device__ __forceinline__ float partner(float x) {
-  return __builtin_bit_cast(float, partner<S>(__builtin_bit_cast(unsigned, x)));
-}
-template <int S>
-__device__ __forceinline__ double partner(double x) {
-  return __builtin_bit_cast(double, partner<S>(__builtin_bit_cast(u64, x)));
-}
-template <int S = 0, typename X>
-__device__ __forceinline__ X wave_max(X x) {
-  if constexpr (S == 6) {
-    return x;
-  } else {
-    const X y = partner<S>(x);
-    return wave_max<S + 1>(y > x ? y : x);
-  }
-}
-template <int S = 0>
-__device__ __forceinline__ double wave_sum(double x) {
-  if constexpr (S == 6)
-    return x;
-  else
-    return wave_sum<S + 1>(x + partner<S>(x));
-}
 __device__ __forceinline__ unsigned lane_of(unsigned x, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)x, lane); }
 __device__ __forceinline__ u64 lane_of(u64 x, int lane) {
   return (u64)lane_of((unsigned)(x >> 32), lane) << 32 | lane_of((unsigned)x, lane);
@@ -440,14 +398,21 @@ struct Column {
   int len;
   bool copies;
 };
-__device__ __forceinline__ Column column(const ReorderArgs& a, int g, int j, int lane, int* free_pages) {
+// A group's parents and its beams' new lengths, a lane each.
+struct Heirs {
+  int parent, len;
+};
+__device__ __forceinline__ Heirs heirs(const ReorderArgs& a, int g, int lane) {
+  const size_t mine = (size_t)g * a.W + (lane < a.W ? lane : 0);
+  const int parent = min(max(a.parents[mine], 0), a.W - 1);
+  return {parent, __shfl(a.lens[mine], parent, 64)};
+}
+__device__ __forceinline__ Column column(const ReorderArgs& a, const Heirs& x, int g, int j, int lane, int* free_pages) {
   const bool is = lane < a.W;
   const size_t mine = (size_t)g * a.W + (is ? lane : 0);
-  const int par = min(max(a.parents[mine], 0), a.W - 1);
-  const size_t of = (size_t)g * a.W + par;
   Column c;
-  c.len = a.lens[of];
-  c.from = a.table[of * a.J + j];
+  c.len = x.len;
+  c.from = __shfl(a.table[mine * a.J + j], x.parent, 64);
   const int home = a.pages[mine * a.J + j];
   c.rows = (int)min(max((long long)c.len - (long long)j * a.page, 0ll), (long long)a.page);
   const bool full = is && c.rows == a.page, part = is && c.rows > 0 && !full;
@@ -475,8 +440,23 @@ __device__ __forceinline__ Column column(const ReorderArgs& a, int g, int j, int
 
 constexpr int kReorderThreads = 256;
 
+template <typename V>
+__device__ __forceinline__ void copy_wave(char* dst, const char* src, int bytes, int lane) {
+  constexpr int N = 8;
+  const int n = bytes / (int)sizeof(V);
+  for (int i = lane; i < n; i += 64 * N) {
+    V x[N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) x[e] = reinterpret_cast<const V*>(src)[min(i + 64 * e, n - 1)];
+#pragma unroll
+    for (int e = 0; e < N; ++e)
+      if (i + 64 * e < n) reinterpret_cast<V*>(dst)[i + 64 * e] = x[e];
+  }
+}
+
 __global__ __launch_bounds__(kReorderThreads) void coalibi_reorder_kernel(ReorderArgs a) {
   __shared__ int sfree[kReorderThreads / 64][64];
+  __shared__ int smove[3];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int beams = a.B * a.W;
   if (blockIdx.y == (unsigned)a.pools) {  // the tables: a wavefront per group and column
@@ -484,7 +464,7 @@ __global__ __launch_bounds__(kReorderThreads) void coalibi_reorder_kernel(Reorde
     for (long long at = (long long)blockIdx.x * (kReorderThreads / 64) + wave; at < columns;
          at += (long long)gridDim.x * (kReorderThreads / 64)) {
       const int g = (int)(at / a.J), j = (int)(at - (long long)g * a.J);
-      const Column c = column(a, g, j, lane, sfree[wave]);
+      const Column c = column(a, heirs(a, g, lane), g, j, lane, sfree[wave]);
       if (lane < a.W) {
         a.out_table[((size_t)g * a.W + lane) * a.J + j] = c.to;
         if (j == 0) a.out_lens[(size_t)g * a.W + lane] = c.len;
@@ -492,36 +472,41 @@ __global__ __launch_bounds__(kReorderThreads) void coalibi_reorder_kernel(Reorde
     }
     return;
   }
-  // A beam's copies in one pool.  Every wavefront works out the column.
+  // A beam's copies in one pool.
   const PoolDesc& p = a.pool[blockIdx.y];
   for (int i = blockIdx.x; i < beams; i += gridDim.x) {
     const int g = i / a.W, w = i - g * a.W;
-    const int par = min(max(a.parents[i], 0), a.W - 1);
-    const int len = a.lens[(size_t)g * a.W + par];
-    if (len <= 0) continue;
-    const int j = len >> a.page_shift;
-    if (j >= a.J || (len & (a.page - 1)) == 0) continue;  // no page that is in use
-    const Column c = column(a, g, j, lane, sfree[wave]);
-    if (!(__ballot(c.copies) >> w & 1)) continue;
-    const int from = __shfl(c.from, w, 64), to = __shfl(c.to, w, 64), rows = __shfl(c.rows, w, 64);
-    if (from < 0 || from >= a.num_pages || to < 0 || to >= a.num_pages) continue;
+    if (wave == 0) {
+      const Heirs x = heirs(a, g, lane);
+      const int len = __shfl(x.len, w, 64), j = len >> a.page_shift;
+      int from = -1, to = -1, rows = 0;
+      if (len > 0 && j < a.J && (len & (a.page - 1)) != 0) {  // there is a page in use
+        const Column c = column(a, x, g, j, lane, sfree[0]);
+        rows = __ballot(c.copies) >> w & 1 ? __shfl(c.rows, w, 64) : 0;
+        from = __shfl(c.from, w, 64);
+        to = __shfl(c.to, w, 64);
+      }
+      if (lane == 0) {
+        const bool in = from >= 0 && from < a.num_pages && to >= 0 && to < a.num_pages;
+        smove[0] = from;
+        smove[1] = to;
+        smove[2] = in ? rows : 0;
+      }
+    }
+    __syncthreads();
+    const int from = smove[0], to = smove[1], rows = smove[2];
+    __syncthreads();
+    if (rows == 0) continue;
     const int bytes = (int)(((long long)rows * p.entries + a.page - 1) / a.page) * p.entry_bytes;  // of each head
     const char* const src = p.p + (size_t)from * p.page_stride;
     char* const dst = p.p + (size_t)to * p.page_stride;
-    if (p.wide) {
-      const int n = bytes / 16;
-      for (int t = tid; t < n * p.heads; t += kReorderThreads) {
-        const int h = t / n, o = t - h * n;
-        const size_t at = (size_t)h * p.head_stride + (size_t)o * 16;
-        *reinterpret_cast<uint4*>(dst + at) = *reinterpret_cast<const uint4*>(src + at);
-      }
-    } else {
-      const int n = bytes / 4;
-      for (int t = tid; t < n * p.heads; t += kReorderThreads) {
-        const int h = t / n, o = t - h * n;
-        const size_t at = (size_t)h * p.head_stride + (size_t)o * 4;
-        *reinterpret_cast<unsigned*>(dst + at) = *reinterpret_cast<const unsigned*>(src + at);
-      }
+    // A wavefront per head, eight pieces a lane on their way at once.
+    for (int h = wave; h < p.heads; h += kReorderThreads / 64) {
+      const size_t at = (size_t)h * p.head_stride;
+      if (p.wide)
+        copy_wave<u32x4>(dst + at, src + at, bytes, lane);
+      else
+        copy_wave<unsigned>(dst + at, src + at, bytes, lane);
     }
   }
 }

@@ -14,6 +14,7 @@
 
 #include "coalibi_codes.h"
 #include "coalibi_kernels.h"
+#include "coalibi_wave.h"
 
 namespace coalibi {
 
@@ -106,8 +107,7 @@ __global__ __launch_bounds__(kCacheThreads) void coalibi_append8_kernel(Append8A
     }
     if (!__any(any)) continue;
     const float was = had > 0 ? *scale : 0.f;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) top = max(top, (unsigned)__shfl_xor((int)top, off, 64));
+    top = wave_max(top);
 
     int grow = 0;  // doublings of the scale that the block had
     float now;
@@ -144,42 +144,59 @@ __global__ __launch_bounds__(kCacheThreads) void coalibi_append8_kernel(Append8A
   }
 }
 
-// Rows [first, first + n) of every sequence, 8 elements a thread.
-template <typename T, typename F>
+// Rows [first, first + n) of every sequence: a wavefront per block of 16 rows, kv head and cache, whose page and scale are then its
+// own, and 16 codes a lane and piece.
+template <typename T, typename F, int D>
 __global__ __launch_bounds__(kCacheThreads) void coalibi_read8_kernel(Read8Args a) {
-  const int ppr = a.D / 8;
-  const long long per_seq = (long long)a.Hkv * a.N * ppr;
-  const long long at = (long long)blockIdx.x * kCacheThreads + threadIdx.x;
-  if (at >= per_seq) return;
-  const int col = (int)(at % ppr) * 8;
-  const int hr = (int)(at / ppr);  // (h, row): at most 2^31 by the host's check
-  const int h = hr / a.N, i = hr - h * a.N;
+  constexpr int PPR = D / 16, N = PPR * kScaleRows < 64 ? 1 : PPR * kScaleRows / 64;  // pieces per row, and per lane
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const long long id = (long long)blockIdx.x * kCacheWaves + wave;
+  const int block = __builtin_amdgcn_readfirstlane((int)(id / a.Hkv)), h = (int)(id - (long long)block * a.Hkv);
   const bool value = blockIdx.z != 0;
   const Layout& l = value ? a.vcl : a.kcl;
   for (int b = blockIdx.y; b < a.B; b += gridDim.y) {
-    const long long row = (a.first == nullptr ? 0 : (long long)a.first[b]) + i;
-    T* const out = static_cast<T*>(value ? a.v : a.k) + (((size_t)b * a.Hkv + h) * a.N + i) * a.D + col;
-    f32x8 x{};
-    if (row >= 0 && row < min(a.seq_lens[b], a.capacity)) {
-      int unit = b, in_unit = (int)row;
+    const long long first = a.first == nullptr ? 0 : a.first[b];
+    const long long at = (first & ~(long long)(kScaleRows - 1)) + (long long)block * kScaleRows;  // (rounded down, below 0 too)
+    if (at >= first + a.N) continue;
+    const int filled = min(a.seq_lens[b], a.capacity);
+    T* const out = static_cast<T*>(value ? a.v : a.k) + ((size_t)b * a.Hkv + h) * a.N * D;
+    float s = 0.f;
+    const char* p = nullptr;
+    if (at >= 0 && at < filled) {
+      int unit = b, in_unit = (int)at;
       bool there = true;
       if (a.place.table != nullptr) {
         unit = a.place.table[(size_t)b * a.place.table_stride + (in_unit >> a.place.page_shift)];
         there = unit >= 0 && unit < a.place.units;
         in_unit &= (1 << a.place.page_shift) - 1;
       }
-      float s = __builtin_nanf("");
       if (there) {
-        s = value ? a.vs[(size_t)unit * a.vsb + (size_t)h * a.vsh + in_unit / kScaleRows]
-                  : a.ks[(size_t)unit * a.ksb + (size_t)h * a.ksh + in_unit / kScaleRows];
-        const char* const p = static_cast<const char*>(value ? a.vc : a.kc) + (size_t)unit * l.b + (size_t)h * l.h +
-                              (size_t)in_unit * a.D + col;
-        x = from_codes<F>(*reinterpret_cast<const u32x2*>(p));
-        if (!(s >= kScaleLeast && s <= kScaleMost)) s = __builtin_nanf("");
+        const float x = value ? a.vs[(size_t)unit * a.vsb + (size_t)h * a.vsh + in_unit / kScaleRows]
+                              : a.ks[(size_t)unit * a.ksb + (size_t)h * a.ksh + in_unit / kScaleRows];
+        s = x >= kScaleLeast && x <= kScaleMost ? x : __builtin_nanf("");
+        p = static_cast<const char*>(value ? a.vc : a.kc) + (size_t)unit * l.b + (size_t)h * l.h + (size_t)in_unit * D;
+      } else {
+        s = __builtin_nanf("");
       }
-      x *= s;
     }
-    store8(out, x);
+    const int left = p == nullptr ? 0 : (int)min(filled - at, (long long)kScaleRows);  // rows that are read
+    u32x4 c[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int piece = lane + 64 * i, r = piece / PPR;
+      c[i] = u32x4{};
+      if (r < left) c[i] = ld16(p + piece * 16);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int piece = lane + 64 * i, r = piece / PPR;
+      const long long row = at + r - first;
+      if (r >= kScaleRows || row < 0 || row >= a.N) continue;
+      const float f = at + r < filled ? s : 0.f;
+      f32x8 x[2] = {from_codes<F>(u32x2{c[i][0], c[i][1]}), from_codes<F>(u32x2{c[i][2], c[i][3]})};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) store8(out + row * D + piece % PPR * 16 + 8 * j, x[j] * f);
+    }
   }
 }
 
@@ -191,6 +208,18 @@ hipError_t append_d(const Append8Args& a, int D, dim3 grid, hipStream_t st) {
     case 64: hipLaunchKernelGGL((coalibi_append8_kernel<T, F, 64>), grid, dim3(kCacheThreads), 0, st, a); break;
     case 128: hipLaunchKernelGGL((coalibi_append8_kernel<T, F, 128>), grid, dim3(kCacheThreads), 0, st, a); break;
     default: hipLaunchKernelGGL((coalibi_append8_kernel<T, F, 256>), grid, dim3(kCacheThreads), 0, st, a); break;
+  }
+  return hipGetLastError();
+}
+
+template <typename T, typename F>
+hipError_t read_d(const Read8Args& a, dim3 grid, hipStream_t st) {
+  switch (a.D) {
+    case 16: hipLaunchKernelGGL((coalibi_read8_kernel<T, F, 16>), grid, dim3(kCacheThreads), 0, st, a); break;
+    case 32: hipLaunchKernelGGL((coalibi_read8_kernel<T, F, 32>), grid, dim3(kCacheThreads), 0, st, a); break;
+    case 64: hipLaunchKernelGGL((coalibi_read8_kernel<T, F, 64>), grid, dim3(kCacheThreads), 0, st, a); break;
+    case 128: hipLaunchKernelGGL((coalibi_read8_kernel<T, F, 128>), grid, dim3(kCacheThreads), 0, st, a); break;
+    default: hipLaunchKernelGGL((coalibi_read8_kernel<T, F, 256>), grid, dim3(kCacheThreads), 0, st, a); break;
   }
   return hipGetLastError();
 }
@@ -207,13 +236,9 @@ hipError_t launch_append8(const Append8Args& a, bool e4m3, int D, hipStream_t st
 
 template <typename T>
 hipError_t launch_read8(const Read8Args& a, bool e4m3, hipStream_t stream) {
-  const long long per_seq = (long long)a.Hkv * a.N * (a.D / 8);
-  const dim3 grid(static_cast<unsigned>((per_seq + kCacheThreads - 1) / kCacheThreads), static_cast<unsigned>(std::min(a.B, 65535)), 2);
-  if (e4m3)
-    hipLaunchKernelGGL((coalibi_read8_kernel<T, E4M3>), grid, dim3(kCacheThreads), 0, stream, a);
-  else
-    hipLaunchKernelGGL((coalibi_read8_kernel<T, I8>), grid, dim3(kCacheThreads), 0, stream, a);
-  return hipGetLastError();
+  const long long waves = ((a.N + kScaleRows - 2ll) / kScaleRows + 1) * a.Hkv;
+  const dim3 grid(static_cast<unsigned>((waves + kCacheWaves - 1) / kCacheWaves), static_cast<unsigned>(std::min(a.B, 65535)), 2);
+  return e4m3 ? read_d<T, E4M3>(a, grid, stream) : read_d<T, I8>(a, grid, stream);
 }
 
 #define COALIBI_INST_CACHE8(T)                                                          \

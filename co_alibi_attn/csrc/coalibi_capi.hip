@@ -852,8 +852,11 @@ size_t tree_workspace(const TreePlan& p, bool ragged, int batch, int heads_q, in
 // row block: those launches are bound by their instructions, and a second round evens out what one leaves idle.  16 sequences of up to
 // 8192 keys, us, 1 / 2 / 3 rounds: 96 rows 94.5 / 86 / 88; 4 rows over 32 sequences, bound by HBM, 67 / 70 / 75.
 //   A long sequence gets at most 4 times the splits by the bound: 4 / 8 / 16 of them 86 / 91 / 93 (the merge grows).
-//   Three chunks go through one work-group: 12 heads, 500 keys (5 chunks) 9.2 us split, 9.3 whole.
-constexpr int kTree8Whole = 3, kTree8RaggedChunks = 8;
+//   A few chunks go through one work-group, which saves a launch and a workspace.  One token, us captured / eager, split against whole: D
+// 64 380 keys 9.1 / 19.6 and 8.4 / 15.8, 500 keys (5 chunks) 9.3 / 19.6 and 9.5 / 15.9, 630 9.1 / 19.7 and 10.5 / 15.9; D 128 500 keys
+// 10.2 / 19.6 and 10.9 / 15.9; D 256 250 keys (3) 12.3 / 19.7 and 12.9 / 15.9, 500 12.3 / 19.7 and 15.7 / 16.0; fp32 D 64 250 keys 11.7 /
+// 19.6 and 14.2 / 15.8, 380 11.7 / 19.6 and 17.3 / 17.3.
+constexpr int kTree8RaggedChunks = 8;
 TreePlan tree8_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens, int seq_kv, int head_dim) {
   const int rows = heads_q / heads_kv * tokens;
   TreePlan p;
@@ -867,7 +870,7 @@ TreePlan tree8_plan(int dtype, int batch, int heads_q, int heads_kv, int tokens,
     const int most = static_cast<int>(std::min<long long>({std::max(n, 1ll), chunks, coalibi::kMaxTreeSplits}));
     return (chunks + most - 1) / most;
   };
-  p.cps = chunks <= kTree8Whole ? chunks : walk(slots / units);
+  p.cps = chunks <= (dtype == CO_ALIBI_F32 || row_bytes > 256 ? 3 : 5) ? chunks : walk(slots / units);
   p.splits = (chunks + p.cps - 1) / p.cps;
   p.share = static_cast<int>(std::max<long long>((p.row_blocks > 1 ? 2 : 1) * slots / heads, 1));
   p.planned = static_cast<int>(std::min<long long>({p.splits * static_cast<long long>(kTreeRaggedSplits), chunks,

@@ -26,27 +26,26 @@ __device__ __forceinline__ f32x8 from_codes(u32x2 c) {
   return x;
 }
 
-// The nearest codes, ties to even; values past the largest code become it.
+// The nearest codes, ties to even, of values that no more than a rounding puts past the largest code: such ones become it.
 template <typename F>
 __device__ __forceinline__ u32x2 to_codes(f32x8 x) {
   u32x2 c;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    float y[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      y[e] = x[4 * i + e];
-      y[e] = y[e] > F::kMost ? F::kMost : y[e] < -F::kMost ? -F::kMost : y[e];  // (a NaN stays one)
-    }
     if constexpr (__is_same(F, E4M3)) {
-      int w = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], 0, false);
-      w = __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], w, true);
+      int w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i], x[4 * i + 1], 0, false);
+      w = __builtin_amdgcn_cvt_pk_fp8_f32(x[4 * i + 2], x[4 * i + 3], w, true);
       c[i] = (unsigned)w;
     } else {
-      unsigned w = 0;
+      // In the last byte of 1.5 * 2^23 + x.
+      unsigned w[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w |= ((unsigned)(int)rintf(y[e]) & 255u) << 8 * e;
-      c[i] = w;
+      for (int e = 0; e < 4; ++e) {
+        const float y = __builtin_amdgcn_fmed3f(x[4 * i + e], -F::kMost, F::kMost) + 0x1.8p23f;
+        w[e] = __builtin_bit_cast(unsigned, y);
+      }
+      const unsigned lo = __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(w[3], w[2], 0x04000c0cu);
+      c[i] = lo | hi;
     }
   }
   return c;

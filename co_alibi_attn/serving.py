@@ -127,17 +127,18 @@ def _decode_tree(q, k, v, caches, scales, seq_len, parents, block_table, sm_scal
 
 
 def _check_8bit(k_cache, v_cache, k_scale, v_scale) -> None:
-    for t in (k_cache, v_cache, k_scale, v_scale):
-        if not t.is_cuda:
-            raise AssertionError("Inputs must be CUDA tensors")
-    if k_cache.dtype not in _native.FORMAT_CODES or v_cache.dtype != k_cache.dtype:
-        raise TypeError(f"the caches must both be float8_e4m3fn or int8, got {k_cache.dtype} and {v_cache.dtype}")
+    if not (k_cache.is_cuda and v_cache.is_cuda and k_scale.is_cuda and v_scale.is_cuda):
+        raise AssertionError("Inputs must be CUDA tensors")
+    fmt = k_cache.dtype
+    if fmt not in _native.FORMAT_CODES or v_cache.dtype != fmt:
+        raise TypeError(f"the caches must both be float8_e4m3fn or int8, got {fmt} and {v_cache.dtype}")
     if k_scale.dtype != torch.float32 or v_scale.dtype != torch.float32:
         raise TypeError(f"the scales must be float32, got {k_scale.dtype} and {v_scale.dtype}")
-    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape:
-        raise ValueError(f"k_cache and v_cache must be 4-dimensional and of one shape, got {tuple(k_cache.shape)} and "
+    shape = k_cache.shape
+    if len(shape) != 4 or v_cache.shape != shape:
+        raise ValueError(f"k_cache and v_cache must be 4-dimensional and of one shape, got {tuple(shape)} and "
                          f"{tuple(v_cache.shape)}")
-    want = (*k_cache.shape[:2], -(-k_cache.shape[2] // _native.SCALE_ROWS))
+    want = (shape[0], shape[1], (shape[2] + _native.SCALE_ROWS - 1) // _native.SCALE_ROWS)
     if k_scale.shape != want or v_scale.shape != want:
         raise ValueError(f"the scales must be {want}, got {tuple(k_scale.shape)} and {tuple(v_scale.shape)}")
 
@@ -268,13 +269,16 @@ def co_alibi_cache_reorder(caches, seq_lens, parents, block_table, pages, page_s
     """
     if parents.dim() != 2 or not 1 <= parents.shape[1] <= _native.MAX_BEAMS:
         raise ValueError(f"parents must be (B, W) with 1 <= W <= {_native.MAX_BEAMS}, got {tuple(parents.shape)}")
-    if len(caches) == 0 or any(t.dim() < 3 for t in caches):
+    if len(caches) == 0 or caches[0].dim() < 3:
         raise ValueError("caches must be pools (num_pages, heads, rows, ...)")
-    if not all(t.is_cuda for t in (*caches, seq_lens, parents, block_table, pages)):
+    for t in caches:
+        if not t.is_cuda:
+            raise AssertionError("Inputs must be CUDA tensors")
+        if t.requires_grad:
+            raise ValueError("the caches are written in place and cannot require gradients")
+    if not (seq_lens.is_cuda and parents.is_cuda and block_table.is_cuda and pages.is_cuda):
         raise AssertionError("Inputs must be CUDA tensors")
-    if any(t.requires_grad for t in caches):
-        raise ValueError("the caches are written in place and cannot require gradients")
-    return ops.cache_reorder(list(caches), block_table, pages, seq_lens, parents,
+    return ops.cache_reorder(caches, block_table, pages, seq_lens, parents,
                              caches[0].shape[2] if page_size is None else int(page_size))
 
 

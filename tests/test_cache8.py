@@ -103,8 +103,8 @@ def _strides(n, row=128):
     (dict(D=256, dtype=0), 2, "head_dim 256 needs fp16 or bf16"),
     (dict(dtype=3), 2, "dtype must be"),
     (dict(scale=float("nan")), 1, "sm_scale must be finite"),
-    (dict(L=500, T=3, lens=P, ws_bytes=0), 1, "workspace of 0 bytes, need"),
-    (dict(L=500, T=3, lens=P, ws=None), 1, "workspace is NULL"),
+    (dict(L=900, page=1024, T=3, lens=P, ws_bytes=0), 1, "workspace of 0 bytes, need"),
+    (dict(L=900, page=1024, T=3, lens=P, ws=None), 1, "workspace is NULL"),
     (dict(B=1 << 20, Hq=1 << 10, T=64), 1, "problem too large"),
 ])
 def test_decode_tree_argument_errors(over, code, msg):
