@@ -14,11 +14,13 @@ GELU MLP (4x), residual.  The LM head is tied to the token embedding.
 reference attention; the default is the native ``co_alibi_attention``.
 
 Serving: ``GPT.prefill`` and ``GPT.extend`` run new tokens over a ``PagedCache`` and each other, ``PagedCache.accept``
-keeps their keys and values, ``GPT.generate`` samples with them, and ``GPT.speculate`` checks a tree of drafts.  These
+keeps their keys and values, ``GPT.generate`` samples with them, ``GPT.speculate`` checks a tree of drafts, and
+``GPT.beam_search`` keeps the likeliest continuations.  A cache may hold 8 bits per element.  These
 call the native operators (co_alibi_attn/serving.py), on the GPU only.
 """
 from __future__ import annotations
 
+import copy
 import math
 from dataclasses import dataclass
 from typing import Callable
@@ -28,7 +30,8 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .co_alibi_attn import co_alibi_attention, co_alibi_attention_qkv
-from .serving import co_alibi_cache_append, co_alibi_decode_tree, co_alibi_sample
+from .serving import (co_alibi_beam_select, co_alibi_cache_append, co_alibi_cache_append_8bit, co_alibi_cache_read_8bit,
+                      co_alibi_cache_reorder, co_alibi_decode_tree, co_alibi_decode_tree_8bit, co_alibi_sample)
 
 
 @dataclass(frozen=True)
@@ -48,7 +51,8 @@ class PagedCache:
     """Every layer's keys and values of a batch of sequences, in pages under one block table.
 
     ``capacity`` rows per sequence, all empty at first.  ``dtype`` is the one the model's projections have (the
-    weights' type, or autocast's).  A forward over the cache leaves its new keys and values in ``new``, one
+    weights' type, or autocast's), or float8_e4m3fn or int8: then ``layers`` holds codes and ``scales`` their scales, and
+    the model's type is free.  A forward over the cache leaves its new keys and values in ``new``, one
     (k, v) per layer; ``accept`` writes them.
 
     A step with ``accept`` in it may be captured and replayed.  A replay cannot raise: rows without room are dropped
@@ -60,10 +64,17 @@ class PagedCache:
                  device: str | torch.device = "cuda", page_size: int = 64):
         blocks = -(-capacity // page_size)
         self.capacity = blocks * page_size
+        self.page_size = page_size
         shape = (batch * blocks, cfg.n_head, page_size, cfg.d_model // cfg.n_head)
         self.layers = [(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device))
                        for _ in range(cfg.n_layer)]
-        self.block_table = torch.arange(batch * blocks, dtype=torch.int32, device=device).view(batch, blocks)
+        self.scales: list[tuple[torch.Tensor, torch.Tensor]] = []
+        if dtype in (torch.float8_e4m3fn, torch.int8):
+            per_block = (*shape[:2], page_size // 16)  # co_alibi_cache_append_8bit's blocks of 16 rows
+            self.scales = [(torch.zeros(per_block, device=device), torch.zeros(per_block, device=device))
+                           for _ in range(cfg.n_layer)]
+        self.pages = torch.arange(batch * blocks, dtype=torch.int32, device=device).view(batch, blocks)  # owned, not in use
+        self.block_table = self.pages.clone()
         self.seq_lens = torch.zeros(batch, dtype=torch.int32, device=device)
         self.bound = 0  # no sequence is longer; known without reading the device, but for replays of a captured accept
         self.captured = False
@@ -92,8 +103,12 @@ class PagedCache:
         n = self.new[0][0].shape[2] if rows is None else rows.shape[1]
         if counts is None:
             self.room_for(n)
-        for (k_cache, v_cache), (k, v) in zip(self.layers, self.new):
-            co_alibi_cache_append(k, v, k_cache, v_cache, self.seq_lens, self.block_table, rows=rows, counts=counts)
+        for i, (k, v) in enumerate(self.new):
+            if self.scales:
+                co_alibi_cache_append_8bit(k, v, *self.layers[i], *self.scales[i], self.seq_lens, self.block_table, rows=rows,
+                                           counts=counts)
+            else:
+                co_alibi_cache_append(k, v, *self.layers[i], self.seq_lens, self.block_table, rows=rows, counts=counts)
         if self._capturing():
             self.captured = True
         if counts is not None:
@@ -104,6 +119,52 @@ class PagedCache:
             self.seq_lens += n
         self.bound = min(self.bound + n, self.capacity)
         self.new = []
+
+    def clear(self) -> None:
+        """Empties the cache; every sequence holds its own pages again."""
+        self.block_table.copy_(self.pages)
+        self.seq_lens.zero_()
+        self.bound = 0
+        self.new = []
+
+    def every(self, n: int) -> PagedCache:
+        """A cache of every n-th sequence that shares this one's memory and lengths.
+
+        Its ``bound`` is its own: what is accepted there this cache has to be told.
+        """
+        part = copy.copy(self)
+        part.pages, part.block_table, part.seq_lens = self.pages[::n], self.block_table[::n], self.seq_lens[::n]
+        part.new = []
+        return part
+
+    def reorder(self, parents: torch.Tensor) -> None:
+        """Sequence g * W + i goes on from what sequence g * W + parents[g, i] holds; ``parents``: integer tensor (groups, W).
+
+        ``co_alibi_cache_reorder`` over all layers: full pages are shared, ones filled in part are copied.  The table and the
+        lengths are updated in place, as a captured step needs them.  A sequence that shared pages must not be shortened to write
+        into them again; ``clear`` gives each its own back.
+        """
+        if parents.dim() != 2 or parents.numel() != self.seq_lens.shape[0]:
+            raise ValueError(f"parents must be (groups, beams) of {self.seq_lens.shape[0]} sequences, got {tuple(parents.shape)}")
+        pools = [t for pair in self.layers + self.scales for t in pair]
+        table, lens = co_alibi_cache_reorder(pools, self.seq_lens, parents, self.block_table, self.pages, self.page_size)
+        self.block_table.copy_(table)
+        self.seq_lens.copy_(lens)
+        self.new = []
+
+    def read(self, layer: int, dtype: torch.dtype = torch.bfloat16, rows: int | None = None,
+             first: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """A layer's keys and values (batch, heads, rows, D) from an 8-bit cache, zeros behind each sequence's last.
+
+        ``rows``: how many from row ``first`` (integer tensor (batch,); default 0) on; default: as many as the longest may have.
+        """
+        if not self.scales:
+            raise ValueError("read is for 8-bit caches: layers holds the keys and values themselves")
+        if rows is None:
+            self.room_for(0)
+            rows = self.capacity if self._capturing() else self.bound
+        return co_alibi_cache_read_8bit(*self.layers[layer], *self.scales[layer], self.seq_lens, rows, dtype, self.block_table,
+                                        first)
 
 
 class CausalCoALiBiAttention(nn.Module):
@@ -136,8 +197,12 @@ class CausalCoALiBiAttention(nn.Module):
         if prefill:
             y = co_alibi_attention_qkv(qkv, causal=True, bias_max=self.bias_max)
         else:
-            y = co_alibi_decode_tree(q, k, v, *cache.layers[layer], seq_len=cache.seq_lens, parents=parents,
-                                     block_table=cache.block_table, bias_max=self.bias_max).transpose(1, 2)
+            over = dict(seq_len=cache.seq_lens, parents=parents, block_table=cache.block_table, bias_max=self.bias_max)
+            if cache.scales:
+                y = co_alibi_decode_tree_8bit(q, k, v, *cache.layers[layer], *cache.scales[layer], **over)
+            else:
+                y = co_alibi_decode_tree(q, k, v, *cache.layers[layer], **over)
+            y = y.transpose(1, 2)
         return self.proj(y.reshape(B, T, C)), (k, v)
 
 
@@ -278,6 +343,49 @@ class GPT(nn.Module):
         cache.accept(rows, counts)
         last = rows.gather(1, counts[:, None].long().clamp(min=1) - 1).long()
         return rows, counts, drawn.gather(1, last)[:, 0]
+
+    @torch.no_grad()
+    def beam_search(self, idx: torch.Tensor, lengths: torch.Tensor | None, n: int, num_beams: int, cache: PagedCache,
+                    end_token: int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+        """The continuations of n tokens that a search with W = ``num_beams`` beams keeps: (tokens (B, W, n), scores (B, W)).
+
+        idx, lengths: B prompts, as for ``prefill``; ``cache``: empty, of B * W sequences, of which b * W + i holds beam i of
+        prompt b in the end (without its last token).  A score is the sum of its tokens' log probabilities, best first.
+        A beam that drew ``end_token`` is finished: it keeps its score, and end tokens follow.  Where there are fewer than W
+        continuations the last beams score -inf, with tokens of -1.  ``co_alibi_beam_select`` says how equal scores go.
+        """
+        B, S = idx.shape
+        if n < 1:
+            raise ValueError(f"a search needs at least one token, got {n}")
+        if not 1 <= num_beams <= 64 or cache.seq_lens.shape[0] != B * num_beams:
+            raise ValueError(f"{B} prompts with {num_beams} beams (1 to 64) need a cache of as many sequences, got "
+                             f"{cache.seq_lens.shape[0]}")
+        if end_token is not None and not 0 <= end_token < self.cfg.vocab:
+            raise ValueError(f"end_token must be in [0, {self.cfg.vocab}), got {end_token}")
+        leaders = cache.every(num_beams)
+        logits = self.prefill(idx, leaders, lengths)[:, None]
+        cache.bound, cache.captured = leaders.bound, leaders.captured
+        scores = torch.zeros(B, 1, device=idx.device)
+        finished = None
+        steps = []
+        for i in range(n):
+            if i > 0:
+                cache.room_for(1)
+                logits = self.extend(tokens.view(B * num_beams, 1), cache).view(B, num_beams, -1)
+                cache.accept()
+            scores, parents, tokens = co_alibi_beam_select(logits, scores, num_beams, finished, end_token or 0)
+            cache.reorder(parents)  # the first one is the fork: all parents are 0, the leader
+            parents = parents.long()
+            steps.append((parents, tokens))
+            if end_token is not None:
+                finished = tokens == end_token if finished is None else finished.gather(1, parents) | (tokens == end_token)
+        out = torch.empty(B, num_beams, n, dtype=torch.long, device=idx.device)
+        beam = torch.arange(num_beams, device=idx.device).expand(B, num_beams)
+        for i in reversed(range(n)):
+            parents, tokens = steps[i]
+            out[:, :, i] = tokens.gather(1, beam)
+            beam = parents.gather(1, beam)
+        return out.masked_fill_(scores[:, :, None] == -math.inf, -1), scores
 
     def n_params(self) -> int:
         return sum(p.numel() for p in self.parameters())

@@ -217,3 +217,34 @@ def reorder(caches, table, pages, lens, parents, page):
             if 0 <= a < old.shape[0] and 0 <= b < old.shape[0]:
                 new[b, :, :-(-rows // per)] = old[a, :, :-(-rows // per)]
     return out, out_table, out_lens
+
+
+def check_search(logits_after, b, prompt, tokens, scores, steps, tol, end_token=None):
+    """Asserts that a beam search did what it says.  ``steps``: its (scores, parents, tokens), batch entry ``b`` of which is checked.
+
+    Every step's beams are the best of what ``logits_after(tokens)`` gives behind the step before's, up to ``tol`` on either side of
+    a log probability (a logit's own and the sum's), and the result (tokens (W, n), scores (W,)) is the way back from the last.
+    """
+    W = tokens.shape[0]
+    beams = [(0.0, [], False)]
+    for s, p, t in steps:
+        found = {}
+        for w, (score, seq, done) in enumerate(beams):
+            if done:
+                found[w, end_token] = score
+            elif math.isfinite(score):
+                logp = torch.log_softmax(logits_after(prompt + seq), 0)
+                found.update({(w, i): score + logp[i].item() for i in range(len(logp))})
+        keys = [(p[b, i].item(), t[b, i].item()) for i in range(W) if s[b, i] > -math.inf]
+        assert len(keys) == min(W, len(found)) == len(set(keys))
+        got = s[b, :len(keys)].tolist()
+        assert got == sorted(got, reverse=True)
+        for key, score in zip(keys, got):
+            assert abs(found[key] - score) <= 2 * tol + 2.0 ** -24 * abs(score)
+        left = [f for key, f in found.items() if key not in keys]
+        assert max(left, default=-math.inf) <= got[-1] + 2 * tol + 2.0 ** -24 * abs(got[-1])
+        beams = [(score, beams[w][1] + [i], beams[w][2] or i == end_token) for (w, i), score in zip(keys, got)]
+        beams += [(-math.inf, [], False)] * (W - len(beams))
+    for i, (score, seq, _) in enumerate(beams):
+        assert scores[i].item() == score
+        assert tokens[i].tolist() == (seq if score > -math.inf else [-1] * len(steps))
