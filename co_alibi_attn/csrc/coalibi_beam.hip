@@ -6,9 +6,9 @@
 // Within a row the order is the logits', so that each segment of a row yields its maximum, its sum and its N largest logits in
 // one read (its elements stay in registers), and a second launch ranks those of a sequence's beams.  Exponentials are fp32's,
 // summed in fp64 over the threads; scores are fp64 until they are written.
-//   The N largest of a segment: a wavefront's N-th largest of its lanes' maxima is at most the N-th largest element.  Those at or
-// above the largest such bound -- of N lanes of each wavefront at most -- are listed and ranked by counting.  A logit and its
-// token are one 64-bit key, so that equal logits are in order, too.
+//   The N largest of a segment: the least of at least N groups' maxima is at most the N-th largest element, and few elements are
+// above it: about N log N.  They are listed and ranked by counting.  A logit and its token are one 64-bit key, so that equal
+// logits are in order, too.
 //
 // Reordering: a group of W beams owns W pages in every column of its block table.  Pages that are full are shared by all that
 // descend from them; one in use stays with the first of its heirs, and the others get free pages of its column and copies of
@@ -43,9 +43,42 @@ __device__ __forceinline__ unsigned lane_of(unsigned x, int lane) { return (unsi
 __device__ __forceinline__ u64 lane_of(u64 x, int lane) {
   return (u64)lane_of((unsigned)(x >> 32), lane) << 32 | lane_of((unsigned)x, lane);
 }
+// Of the largest of groups of a wavefront's numbers, interleaved ones, the least: 2^low groups for `wave`, and 2^max(low - 2, 0)
+// for `part`; `top` is the largest of all.  At least 2^low numbers are not below `wave`, and as many of a work-group's not
+// below the least of its four wavefronts' `part`.
+struct Bounds {
+  unsigned wave, part, top;
+};
+template <int S = 5>
+__device__ __forceinline__ void larger_down_to(unsigned& x, int low, int from) {
+  if constexpr (S >= 0) {
+    if (S >= low && S < from) x = max(x, partner<S>(x));
+    larger_down_to<S - 1>(x, low, from);
+  }
+}
+template <int S = 0>
+__device__ __forceinline__ void smaller_up_to(unsigned& x, int end) {
+  if constexpr (S < 6) {
+    if (S < end) x = min(x, partner<S>(x));
+    smaller_up_to<S + 1>(x, end);
+  }
+}
+__device__ __forceinline__ Bounds bounds(unsigned x, int low) {
+  Bounds r;
+  const int fewer = max(low - 2, 0);
+  larger_down_to(x, low, 6);
+  r.wave = x;
+  smaller_up_to(r.wave, low);
+  larger_down_to(x, fewer, low);
+  r.part = x;
+  smaller_up_to(r.part, fewer);
+  larger_down_to(x, 0, fewer);
+  r.top = x;
+  return r;
+}
+
 // The n-th largest (1 <= n <= 64) of a wavefront's numbers.
-template <typename X>
-__device__ __forceinline__ X nth_of_wave(X x, int n) {
+__device__ __forceinline__ unsigned nth_of_wave(unsigned x, int n) {
   int larger = 0;
 #pragma unroll
   for (int i = 0; i < 64; ++i) larger += lane_of(x, i) > x ? 1 : 0;
@@ -69,7 +102,7 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
   __shared__ u64 list[kSelectWaves][kListed];
   __shared__ int listed[kSelectWaves];
   __shared__ u64 wnext[kSelectWaves];
-  __shared__ unsigned wcut[kSelectWaves];
+  __shared__ unsigned wcut[kSelectWaves], wpart[kSelectWaves];
   __shared__ float wmax[kSelectWaves];
   __shared__ double wsum[kSelectWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = blockIdx.x;
@@ -106,19 +139,22 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
   float top = v[E - 1];
 #pragma unroll
   for (int e = 0; e < E - 1; ++e) top = fmaxf(top, v[e]);
-  const unsigned cut = nth_of_wave(ordered(top), a.N);
-  float m = wave_max(top);
+  const Bounds cut = bounds(ordered(fmaxf(top, kNegInf)), a.log2_n);
   if (lane == 0) {
-    wmax[wave] = m;
-    wcut[wave] = cut;
+    wcut[wave] = cut.wave;
+    wpart[wave] = cut.part;
+    wmax[wave] = unordered(cut.top);
   }
   __syncthreads();
-  unsigned least = 0;
+  unsigned least = 0, part_least = ~0u;
+  float m = kNegInf;
 #pragma unroll
   for (int i = 0; i < kSelectWaves; ++i) {
     m = fmaxf(m, wmax[i]);
     least = max(least, wcut[i]);
+    part_least = min(part_least, wpart[i]);
   }
+  least = max(least, part_least);
   // The weights' sum: NaN where there is a NaN.
   float sum = 0.f;
   const float ref = m > kNegInf ? m : 0.f;
@@ -232,7 +268,7 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
   __shared__ bool sdone[kMaxBeams];
   __shared__ u64 lscore[kSelectWaves][kMost], llogit[kSelectWaves][kMost], kscore[kMaxBeams], klogit[kMaxBeams];
   __shared__ int lbeam[kSelectWaves][kMost], kbeam[kMaxBeams];
-  __shared__ u64 wcut[kSelectWaves];
+  __shared__ unsigned wcut[kSelectWaves];
   __shared__ int listed[kSelectWaves];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
   const long long row0 = (long long)b * a.W;
@@ -309,12 +345,14 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
     u64 best = 0;
 #pragma unroll
     for (int r = 0; r <= kRound; ++r) best = score[r] > best ? score[r] : best;
-    const u64 cut = nth_of_wave(best, a.N);
+    // A wavefront's N-th largest lane, by the scores' first halves, is no more than the N-th largest candidate.  (Segments' lists are
+    // in order, so that groups as in the segments would each hold the first ones or the last ones.)
+    const unsigned cut = nth_of_wave((unsigned)(best >> 32), a.N);
     if (lane == 0) wcut[wave] = cut;
     __syncthreads();
     u64 least = 1;
 #pragma unroll
-    for (int i = 0; i < kSelectWaves; ++i) least = wcut[i] > least ? wcut[i] : least;
+    for (int i = 0; i < kSelectWaves; ++i) least = max(least, (u64)wcut[i] << 32);
     int mine = 0;
 #pragma unroll
     for (int r = 0; r <= kRound; ++r) {
@@ -440,17 +478,23 @@ __device__ __forceinline__ Column column(const ReorderArgs& a, const Heirs& x, i
 
 constexpr int kReorderThreads = 256;
 
+// The first bytes of each head of a page, eight pieces a thread on their way at once.
 template <typename V>
-__device__ __forceinline__ void copy_wave(char* dst, const char* src, int bytes, int lane) {
+__device__ __forceinline__ void copy_heads(char* dst, const char* src, int bytes, int heads, long long stride, int tid) {
   constexpr int N = 8;
-  const int n = bytes / (int)sizeof(V);
-  for (int i = lane; i < n; i += 64 * N) {
+  const unsigned n = (unsigned)bytes / (unsigned)sizeof(V), all = n * (unsigned)heads;
+  for (unsigned i = tid; i < all; i += kReorderThreads * N) {
     V x[N];
+    long long at[N];
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = reinterpret_cast<const V*>(src)[min(i + 64 * e, n - 1)];
+    for (int e = 0; e < N; ++e) {
+      const unsigned j = min(i + kReorderThreads * e, all - 1), h = j / n;
+      at[e] = (long long)h * stride + (long long)(j - h * n) * (int)sizeof(V);
+      x[e] = *reinterpret_cast<const V*>(src + at[e]);
+    }
 #pragma unroll
     for (int e = 0; e < N; ++e)
-      if (i + 64 * e < n) reinterpret_cast<V*>(dst)[i + 64 * e] = x[e];
+      if (i + kReorderThreads * e < all) *reinterpret_cast<V*>(dst + at[e]) = x[e];
   }
 }
 
@@ -500,14 +544,10 @@ __global__ __launch_bounds__(kReorderThreads) void coalibi_reorder_kernel(Reorde
     const int bytes = (int)(((long long)rows * p.entries + a.page - 1) / a.page) * p.entry_bytes;  // of each head
     const char* const src = p.p + (size_t)from * p.page_stride;
     char* const dst = p.p + (size_t)to * p.page_stride;
-    // A wavefront per head, eight pieces a lane on their way at once.
-    for (int h = wave; h < p.heads; h += kReorderThreads / 64) {
-      const size_t at = (size_t)h * p.head_stride;
-      if (p.wide)
-        copy_wave<u32x4>(dst + at, src + at, bytes, lane);
-      else
-        copy_wave<unsigned>(dst + at, src + at, bytes, lane);
-    }
+    if (p.wide)
+      copy_heads<u32x4>(dst, src, bytes, p.heads, p.head_stride, tid);
+    else
+      copy_heads<unsigned>(dst, src, bytes, p.heads, p.head_stride, tid);
   }
 }
 
