@@ -731,6 +731,7 @@ std::tuple<Tensor, Tensor> cache_reorder_hip(at::TensorList caches, const Tensor
     TORCH_CHECK_VALUE(t.dim() >= 3 && t.size(0) == num_pages, fn, ": the caches must be (", num_pages,
                       " pages, heads, rows of a page, ...), got ", t.sizes());
     TORCH_CHECK_VALUE(t.device() == like.device() && t.device().is_cuda(), fn, ": the caches must be on one CUDA device");
+    TORCH_CHECK_VALUE(!t.requires_grad(), fn, ": the caches are written in place and cannot require gradients");
     int64_t entry = t.element_size();
     for (int64_t d = t.dim() - 1; d >= 3; --d) {
       TORCH_CHECK_VALUE(t.size(d) == 1 || t.stride(d) * t.element_size() == entry, fn, ": the rows of a page's head must be dense");

@@ -271,13 +271,11 @@ def co_alibi_cache_reorder(caches, seq_lens, parents, block_table, pages, page_s
         raise ValueError(f"parents must be (B, W) with 1 <= W <= {_native.MAX_BEAMS}, got {tuple(parents.shape)}")
     if len(caches) == 0 or caches[0].dim() < 3:
         raise ValueError("caches must be pools (num_pages, heads, rows, ...)")
-    for t in caches:
-        if not t.is_cuda:
-            raise AssertionError("Inputs must be CUDA tensors")
-        if t.requires_grad:
-            raise ValueError("the caches are written in place and cannot require gradients")
-    if not (seq_lens.is_cuda and parents.is_cuda and block_table.is_cuda and pages.is_cuda):
+    # (The operator looks at the other pools: there may be a hundred.)
+    if not (caches[0].is_cuda and seq_lens.is_cuda and parents.is_cuda and block_table.is_cuda and pages.is_cuda):
         raise AssertionError("Inputs must be CUDA tensors")
+    if caches[0].requires_grad:
+        raise ValueError("the caches are written in place and cannot require gradients")
     return ops.cache_reorder(caches, block_table, pages, seq_lens, parents,
                              caches[0].shape[2] if page_size is None else int(page_size))
 

@@ -285,3 +285,11 @@ def test_reorder_captured():
         hl += 5
         assert torch.equal(table.cpu(), ht) and torch.equal(lens.cpu(), hl)
         assert all(torch.equal(raw(a), raw(b)) for a, b in zip(dc, caches))
+
+
+def test_every_pool_is_looked_at():
+    pool, par = torch.zeros(4, 2, 16, 64, device=DEV), torch.zeros(1, 2, dtype=torch.int32, device=DEV)
+    table, lens = torch.arange(4, dtype=torch.int32, device=DEV).view(2, 2), torch.tensor([5, 0], dtype=torch.int32, device=DEV)
+    for bad in (pool.clone().requires_grad_(), pool.cpu(), pool[:3], pool.transpose(2, 3)):
+        with pytest.raises(ValueError):
+            co_alibi_cache_reorder([pool, bad], lens, par, table, table)
