@@ -62,7 +62,9 @@ DECODE_KERNELS = ("coalibi_decode_split_kernel", "coalibi_decode_merge_kernel")
 FORM_KERNELS = ("coalibi_fwd_split_kernel", "coalibi_bwd_dq_split_kernel", "coalibi_bwd_dkdv_key_kernel",
                 "coalibi_bwd_dkdv_f32_kernel")
 SERVING_KERNELS = ("coalibi_tree_split_kernel", "coalibi_tree_merge_kernel", "coalibi_append_kernel",
-                   "coalibi_sample_kernel")
+                   "coalibi_sample_kernel",
+                   "coalibi_tree8_kernel", "coalibi_append8_kernel", "coalibi_read8_kernel", "coalibi_select_rows_kernel",
+                   "coalibi_select_beams_kernel", "coalibi_reorder_kernel")
 NAMED_KERNELS = KERNELS + STORE_KERNELS[2:] + FORM_KERNELS + DECODE_KERNELS + SERVING_KERNELS + ("coalibi_key_norm_kernel",)
 # The two --pmc passes of the counter summary: at most 8 SQ and 2 GRBM counters each.
 COUNTER_PASSES = (
