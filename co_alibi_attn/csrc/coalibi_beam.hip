@@ -14,6 +14,14 @@
 // descend from them; one in use stays with the first of its heirs, and the others get free pages of its column and copies of
 // its rows.  That many are free, as no more than W are in use.  A wavefront works out a column's W beams by itself, a lane
 // each, for the tables and again for every copy, so that all is one launch.
+//
+// Measured in replayed graphs.  Selection, 8 beams of 16 sequences over 131071 bf16 logits, a third of them finished: 20 us, of which
+// the segments take 12.8 (22.5 MB, which a read takes 4 us for: a segment's loads, its bound, its weights and its list follow one
+// another) and the ranking 7.4, loads and steps of one work-group per sequence in a row.  Lists counted by one wavefront took 13.8
+// and 9.4, a bound by counting 64 lanes in the segments 14.4.  4 beams over 50304: 9.3 us.
+// Reordering, 4 beams, 24 pools: 4.3 us.  8 beams of 16 sequences, 8 pools of codes and 8 of scales: 11.5 us for 21 MB, which a copy
+// takes 4.3 for: 2176 work-groups, of which most find nothing to copy (as many again take 3.5 us more), and three dependent
+// reads before a copy's first.  Several pools to a work-group took 12.3, heads over two of them 14.8.
 #include <algorithm>
 
 #include "coalibi_common.h"
@@ -100,12 +108,12 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
   constexpr int PER = 16 / sizeof(T), E = C * PER + 1;
   typedef T chunk_t __attribute__((ext_vector_type(PER)));
   __shared__ u64 list[kSelectWaves][kListed];
-  __shared__ int listed[kSelectWaves];
+  __shared__ int listed[kSelectWaves], count[kSelectWaves][64];
   __shared__ u64 wnext[kSelectWaves];
   __shared__ unsigned wcut[kSelectWaves], wpart[kSelectWaves];
   __shared__ float wmax[kSelectWaves];
   __shared__ double wsum[kSelectWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, seg = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), seg = blockIdx.x;
   const long long row = blockIdx.y + (long long)blockIdx.z * gridDim.y;
   if (row >= (long long)a.B * a.W) return;
   if (a.finished != nullptr && a.finished[row] != 0) return;
@@ -198,18 +206,23 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
     c += listed[i];
     fits = fits && listed[i] <= kListed;
   }
-  if (c <= 64) {  // one each for the first wavefront's lanes
-    if (wave == 0) {
-      int at = lane, from = 0;
+  if (c <= 64) {  // one each for the lanes; every wavefront counts its share of the larger ones
+    int at = lane, from = 0;
 #pragma unroll
-      for (int i = 0; i < kSelectWaves - 1; ++i)
-        if (from == i && at >= listed[i]) {
-          at -= listed[i];
-          ++from;
-        }
-      const u64 k = lane < c ? list[from][at] : 0;
+    for (int i = 0; i < kSelectWaves - 1; ++i)
+      if (from == i && at >= listed[i]) {
+        at -= listed[i];
+        ++from;
+      }
+    const u64 k = lane < c ? list[from][at] : 0;
+    int larger = 0;
+    for (int j = wave; j < c; j += kSelectWaves) larger += lane_of(k, j) > k ? 1 : 0;
+    count[wave][lane] = larger;
+    __syncthreads();
+    if (wave == 0) {
       int rank = 0;
-      for (int j = 0; j < c; ++j) rank += lane_of(k, j) > k ? 1 : 0;
+#pragma unroll
+      for (int i = 0; i < kSelectWaves; ++i) rank += count[i][lane];
       if (lane >= c) rank = lane;
       if (rank < a.N) out[rank] = k;
     }
@@ -269,8 +282,8 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
   __shared__ u64 lscore[kSelectWaves][kMost], llogit[kSelectWaves][kMost], kscore[kMaxBeams], klogit[kMaxBeams];
   __shared__ int lbeam[kSelectWaves][kMost], kbeam[kMaxBeams];
   __shared__ unsigned wcut[kSelectWaves];
-  __shared__ int listed[kSelectWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, b = blockIdx.x;
+  __shared__ int listed[kSelectWaves], count[kSelectWaves][64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), b = blockIdx.x;
   const long long row0 = (long long)b * a.W;
   const int per_beam = a.segments * a.N, total = a.W * per_beam;
   u64 keys[kRound];  // of the first round, on their way meanwhile
@@ -375,24 +388,29 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
       kscore[tid] = klogit[tid] = 0;
       kbeam[tid] = 0;
     }
-    if (n <= 64) {  // one each for the first wavefront's lanes
-      if (wave == 0) {
-        int at = lane, from = 0;
+    if (n <= 64) {  // one each for the lanes; every wavefront counts its share of the larger ones
+      int at = lane, from = 0;
 #pragma unroll
-        for (int i = 0; i < kSelectWaves - 1; ++i)
-          if (from == i && at >= listed[i]) {
-            at -= listed[i];
-            ++from;
-          }
-        const bool is = lane < n;
-        const u64 x = is ? lscore[from][at] : 0, xl = is ? llogit[from][at] : 0;
-        const int xb = is ? lbeam[from][at] : 0;
-        int rank = 0;
-        for (int j = 0; j < n; ++j) {
-          const u64 y = lane_of(x, j);
-          const int yb = __builtin_amdgcn_readlane(xb, j);
-          rank += y > x || (y == x && (yb < xb || (yb == xb && lane_of(xl, j) > xl))) ? 1 : 0;
+      for (int i = 0; i < kSelectWaves - 1; ++i)
+        if (from == i && at >= listed[i]) {
+          at -= listed[i];
+          ++from;
         }
+      const bool is = lane < n;
+      const u64 x = is ? lscore[from][at] : 0, xl = is ? llogit[from][at] : 0;
+      const int xb = is ? lbeam[from][at] : 0;
+      int larger = 0;
+      for (int j = wave; j < n; j += kSelectWaves) {
+        const u64 y = lane_of(x, j);
+        const int yb = __builtin_amdgcn_readlane(xb, j);
+        larger += y > x || (y == x && (yb < xb || (yb == xb && lane_of(xl, j) > xl))) ? 1 : 0;
+      }
+      count[wave][lane] = larger;
+      __syncthreads();
+      if (wave == 0) {
+        int rank = 0;
+#pragma unroll
+        for (int i = 0; i < kSelectWaves; ++i) rank += count[i][lane];
         if (is && rank < a.N) {
           kscore[rank] = x;
           klogit[rank] = xl;

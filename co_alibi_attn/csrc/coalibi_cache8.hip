@@ -4,12 +4,19 @@
 // 2^k, k >= -40, at which none of its new rows passes the format's largest code; a block that has rows keeps its scale, or
 // doubles it as often as the new ones need, and its codes are halved as often.  Scaling by powers of two rounds nothing but the
 // codes, so that however often a block's scale grows its int8 codes stay within one step of their values (half a step for the
-// first rounding, and less than half of the final one's for all later ones together) and its e4m3 codes within the format's own
-// half step, below its smallest normal number within one of its smallest steps.
+// last rounding, and less than another half for all earlier ones together, whose steps were a half, a quarter, ... of it) and its
+// e4m3 codes within the format's own half step, below its smallest normal number within one of its smallest steps.
 //   A new value that is not finite, or too large for the largest scale, makes its block's scale NaN, and with it all that is
 // read from the block, until its first row is written again.
 //
-// Both are copies, bound by HBM for prompts and by the launch for single tokens.
+// Both are copies, a wavefront per block, kv head and cache: its table entry, page and scale are looked up once, the largest new
+// value is found and applied without leaving the wavefront, and no two wavefronts write one scale.  Measured in a replayed graph:
+//   append, 8 prompts of 14730 rows together (8 kv heads, D 128, bf16 to int8): 17.4 us for 60.3 MB, 3.5 TB/s (a copy reaches 4.9:
+//     12.4 us); the loads have to arrive before the first code is known, and a wavefront has one block's in flight;
+//   append, one token for each of 16 sequences: 4.1 us, of which an empty kernel takes 2.1;
+//   read, 8 sequences of up to 4096 rows (8 kv heads, D 128, e4m3 to bf16): 34.6 us for 178 MB, 5.2 TB/s; one wavefront per 64
+//     pieces without blocks, with a table entry and a scale for each lane, took 54;
+//   read, 500 rows of 12 heads to fp32: 3.9 us.
 #include <algorithm>
 
 #include "coalibi_codes.h"

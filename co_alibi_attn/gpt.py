@@ -371,7 +371,7 @@ class GPT(nn.Module):
         for i in range(n):
             if i > 0:
                 cache.room_for(1)
-                logits = self.extend(tokens.view(B * num_beams, 1), cache).view(B, num_beams, -1)
+                logits = self.extend(tokens.view(B * num_beams, 1), cache).view(B, num_beams, self.cfg.vocab)
                 cache.accept()
             scores, parents, tokens = co_alibi_beam_select(logits, scores, num_beams, finished, end_token or 0)
             cache.reorder(parents)  # the first one is the fork: all parents are 0, the leader

@@ -293,3 +293,28 @@ def test_every_pool_is_looked_at():
     for bad in (pool.clone().requires_grad_(), pool.cpu(), pool[:3], pool.transpose(2, 3)):
         with pytest.raises(ValueError):
             co_alibi_cache_reorder([pool, bad], lens, par, table, table)
+
+
+def test_pools_and_logits_past_32_bits():
+    page, H, D = 64, 8, 128
+    pages = (1 << 32) // (page * H * D) + 8
+    pool = torch.zeros(pages, H, page, D, dtype=torch.int8, device=DEV)
+    gen = torch.Generator(device=DEV).manual_seed(7)
+    table = torch.arange(pages - 4, pages, dtype=torch.int32, device=DEV).view(2, 2)
+    tail = torch.randint(-127, 128, (4, H, page, D), generator=gen, device=DEV, dtype=torch.int8)
+    pool[-4:] = tail
+    lens = torch.tensor([70, 3], dtype=torch.int32, device=DEV)
+    new, n = co_alibi_cache_reorder([pool], lens, torch.zeros(1, 2, dtype=torch.int32, device=DEV), table, table)
+    assert n.tolist() == [70, 70] and new.tolist() == [[pages - 4, pages - 3], [pages - 4, pages - 1]]
+    assert torch.equal(pool[-1, :, :6], tail[1, :, :6]) and torch.equal(pool[-1, :, 6:], tail[3, :, 6:])
+    assert torch.equal(pool[-4:-1], tail[:3]) and not pool[:4].any() and not pool[-8:-4].any()
+    del pool
+    W, V = 64, 1 << 20
+    logits = torch.zeros(35, W, V, dtype=BF16, device=DEV)
+    logits[-1] = torch.randn(W, V, generator=gen, device=DEV).to(BF16)
+    scores = torch.randn(35, W, generator=gen, device=DEV)
+    got = co_alibi_beam_select(logits, scores, 5)
+    want = co_alibi_beam_select(logits[-1:].clone(), scores[-1:].clone(), 5)
+    for x, y in zip(got, want):
+        assert torch.equal(x[-1:], y)
+    assert got[2][0].tolist() == [0, 1, 2, 3, 4]

@@ -265,3 +265,37 @@ def test_a_compiled_step_is_the_eager_one(fmt):
         x, y = (t.view(torch.uint8) if t.dtype != torch.float32 else t for t in (x, y))
         assert torch.equal(x, y)
     assert torch.isfinite(want[1]).all()
+
+
+@pytest.mark.parametrize("fmt", (torch.float32, torch.int8))
+def test_inference_mode_and_an_empty_batch(models, fmt):
+    _, gpu = models
+    idx = prompts([18, 18], 8).to(DEV)
+    want = gpu.beam_search(idx, None, 4, 3, PagedCache(CFG, 6, 32, fmt, DEV, page_size=16))
+    with torch.inference_mode():
+        got = gpu.beam_search(idx, None, 4, 3, PagedCache(CFG, 6, 32, fmt, DEV, page_size=16))
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    tokens, scores = gpu.beam_search(idx[:0], None, 4, 3, PagedCache(CFG, 0, 32, fmt, DEV, page_size=16))
+    assert tokens.shape == (0, 3, 4) and scores.shape == (0, 3)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_generation_and_drafts_over_8_bits(models, fmt):
+    """A tree of one node is generate's step: the same cache, and so the same tokens."""
+    _, gpu = models
+    lengths = torch.tensor([20, 3], device=DEV)
+    idx = prompts([20, 3], 9).to(DEV)
+    u = torch.rand(2, 8, generator=torch.Generator().manual_seed(10)).to(DEV)
+    cache = PagedCache(CFG, 2, 48, fmt, DEV, page_size=16)
+    truth = gpu.generate(idx, lengths, u, cache)
+    assert ((truth >= 0) & (truth < CFG.vocab)).all() and cache.seq_lens.tolist() == [27, 10]
+    cache.clear()
+    gpu.prefill(idx, cache, lengths)
+    parents = torch.tensor([[-1], [-1]], device=DEV)
+    for i in range(7):  # trees of one node: the draw of generate
+        rows, counts, after = gpu.speculate(truth[:, i:i + 1], parents, u[:, i + 1:i + 2], cache)
+        assert counts.tolist() == [1, 1] and torch.equal(after, truth[:, i + 1])
+    wrong = (truth[:, :1] + 1) % CFG.vocab
+    rows, counts, after = gpu.speculate(torch.cat([truth[:, 7:], wrong], 1), torch.tensor([[-1, 0], [-1, 0]], device=DEV),
+                                        torch.zeros(2, 2, device=DEV), cache)
+    assert ((counts == 1) | (after >= 0)).all() and cache.seq_lens.tolist() == [27 + counts[0], 10 + counts[1]]
