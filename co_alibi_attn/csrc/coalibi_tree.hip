@@ -170,8 +170,9 @@ __global__ __launch_bounds__(kTreeThreads, (TreeCfg<T, D>::WGS_PER_CU)) void coa
   int cps = a.cps;
   TreeItem it{item / nS, item % nS};
   if (a.plan) {
-    cps = plan_cps(a, lane);
-    it = plan_item(a, cps, item, lane);
+    const int first = lane_chunks(a, lane);
+    cps = plan_cps(a, lane, first);
+    it = plan_item(a, cps, item, lane, first);
     if (it.bhk < 0) return;
   } else if (it.bhk >= a.B * a.Hkv) {
     return;

@@ -146,16 +146,19 @@ __device__ __forceinline__ bool scale_ok(float s) { return s >= kScaleLeast && s
 
 // As plan_item, but by kv head, the last head first: its slopes are the flattest where their number is a power of two, and the tiles
 // of flat heads, of which few are left out, take the longest.
-__device__ __forceinline__ TreeItem head_item(const TreeArgs& a, int cps, int id, int lane) {
-  auto splits = [&](int b) { return b < a.B ? splits_of(a, cps, chunks_of(a, filled_rows(a, b))).used : 0; };
+__device__ __forceinline__ TreeItem head_item(const TreeArgs& a, int cps, int id, int lane, int first) {
+  auto splits = [&](int b0) {
+    const int chunks = lane_chunks(a, b0, lane, first);
+    return chunks == 0 ? 0 : splits_of(a, cps, chunks).used;
+  };
   int total = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 64) total += wave_total(splits(b0 + lane));
+  for (int b0 = 0; b0 < a.B; b0 += 64) total += wave_total(splits(b0));
   const int head = id / total;
   if (head >= a.Hkv) return {-1, 0};
   const int at = id - head * total;
   int before = 0;
   for (int b0 = 0; b0 < a.B; b0 += 64) {
-    const int n = splits(b0 + lane), incl = wave_prefix(n);
+    const int n = splits(b0), incl = wave_prefix(n);
     const unsigned long long in = __ballot(at < before + incl);
     if (in != 0) {
       const int l = __ffsll(in) - 1;
@@ -186,8 +189,9 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
   int cps = a.cps;
   TreeItem it;
   if (a.plan) {
-    cps = plan_cps(a, lane);
-    it = head_item(a, cps, item, lane);
+    const int first = lane_chunks(a, lane);
+    cps = plan_cps(a, lane, first);
+    it = head_item(a, cps, item, lane, first);
   } else {
     const int per_head = a.B * nS, head = item / per_head, at = item - head * per_head;
     it = head < a.Hkv ? TreeItem{at / nS * a.Hkv + a.Hkv - 1 - head, at % nS} : TreeItem{-1, 0};
