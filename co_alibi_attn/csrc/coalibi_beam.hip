@@ -16,7 +16,7 @@
 // each, for the tables and again for every copy, so that all is one launch.
 //
 // Measured in replayed graphs.  Selection, 8 beams of 16 sequences over 131071 bf16 logits, a third of them finished: 20 us, of which
-// the segments take 12.8 (22.5 MB, which a read takes 4 us for: a segment's loads, its bound, its weights and its list follow one
+// the segments take 12 to 12.8 (22.5 MB, which a read takes 4 us for: a segment's loads, its bound, its weights and its list follow one
 // another) and the ranking 7.4, loads and steps of one work-group per sequence in a row.  Lists counted by one wavefront took 13.8
 // and 9.4, a bound by counting 64 lanes in the segments 14.4.  4 beams over 50304: 9.3 us.
 // Reordering, 4 beams, 24 pools: 4.3 us.  8 beams of 16 sequences, 8 pools of codes and 8 of scales: 11.5 us for 21 MB, which a copy
