@@ -26,7 +26,7 @@
 // Taken step by step for the 32 sequences, the drafts and the long one: keys and values loaded where they are used 71, 115 and 64
 // us; keys a tile ahead, values while a tile is weighed, their product with the weights a tile late 67, 117 and 57; plans by the
 // batch's own lengths, two rounds of work-groups where several row blocks share keys: drafts 86; splits by kv head, the
-// flattest first 64, 84 and 56; conversions without clamps: drafts 82.
+// flattest first 64, 84 and 56; a plan's lengths read once: drafts 82.  Keys two tiles ahead: 63 in place of 64, but D 256 spills.
 #include <algorithm>
 #include <type_traits>
 
