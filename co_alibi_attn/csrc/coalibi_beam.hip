@@ -15,10 +15,11 @@
 // its rows.  That many are free, as no more than W are in use.  A wavefront works out a column's W beams by itself, a lane
 // each, for the tables and again for every copy, so that all is one launch.
 //
-// Measured in replayed graphs.  Selection, 8 beams of 16 sequences over 131071 bf16 logits, a third of them finished: 20 us, of which
-// the segments take 12 to 12.8 (22.5 MB, which a read takes 4 us for: a segment's loads, its bound, its weights and its list follow one
+// Measured in replayed graphs.  Selection, 8 beams of 16 sequences over 131071 bf16 logits, a third of them finished: 19 us, of which
+// the segments take 11.9 (22.5 MB, which a read takes 4 us for: a segment's loads, its bound, its weights and its list follow one
 // another) and the ranking 7.4, loads and steps of one work-group per sequence in a row.  Lists counted by one wavefront took 13.8
-// and 9.4, a bound by counting 64 lanes in the segments 14.4.  4 beams over 50304: 9.3 us.
+// and 9.4, a bound by counting 64 lanes in the segments 14.4, weights against the work-group's maximum 12.9.  4
+// beams over 50304: 9.1 us.
 // Reordering, 4 beams, 24 pools: 4.3 us.  8 beams of 16 sequences, 8 pools of codes and 8 of scales: 11.5 us for 21 MB, which a copy
 // takes 4.3 for: 2176 work-groups, of which most find nothing to copy (as many again take 3.5 us more), and three dependent
 // reads before a copy's first.  Several pools to a work-group took 12.3, heads over two of them 14.8.
@@ -136,7 +137,15 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
-      for (int e = 0; e < PER; ++e) v[c * PER + e] = first + c * kSelectThreads < chunks ? static_cast<float>(y[c][e]) : kNegInf;
+      for (int e = 0; e < PER; ++e) v[c * PER + e] = static_cast<float>(y[c][e]);
+    if ((seg + 1) * (C * kSelectThreads) > chunks) {  // the last segment's own
+#pragma unroll
+      for (int c = 0; c < C; ++c)
+        if (first + c * kSelectThreads >= chunks) {
+#pragma unroll
+          for (int e = 0; e < PER; ++e) v[c * PER + e] = kNegInf;
+        }
+    }
   } else {
 #pragma unroll
     for (int e = 0; e < E - 1; ++e) v[e] = kNegInf;
@@ -148,6 +157,17 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
 #pragma unroll
   for (int e = 0; e < E - 1; ++e) top = fmaxf(top, v[e]);
   const Bounds cut = bounds(ordered(fmaxf(top, kNegInf)), a.log2_n);
+  // The weights' sum, against the wavefront's maximum (the others' are on their way): NaN where there is a NaN.
+  float sum = 0.f;
+  const float wm = unordered(cut.top);
+  const float ref = wm > kNegInf ? wm : 0.f;
+  if (wm < __builtin_inff()) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += fast_exp2((v[e] - ref) * kLog2e);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += v[e] == wm ? 1.f : v[e] == v[e] ? 0.f : v[e];
+  }
   if (lane == 0) {
     wcut[wave] = cut.wave;
     wpart[wave] = cut.part;
@@ -163,16 +183,6 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
     part_least = min(part_least, wpart[i]);
   }
   least = max(least, part_least);
-  // The weights' sum: NaN where there is a NaN.
-  float sum = 0.f;
-  const float ref = m > kNegInf ? m : 0.f;
-  if (m < __builtin_inff()) {
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum += fast_exp2((v[e] - ref) * kLog2e);
-  } else {
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum += v[e] == m ? 1.f : v[e] == v[e] ? 0.f : v[e];
-  }
   const float low = unordered(least);
   int mine = 0;
   if (__any(top >= low)) {
@@ -187,7 +197,7 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
     }
   }
   if (lane == 0) listed[wave] = mine;
-  const double total = wave_sum((double)sum);
+  const double total = wave_sum((double)sum) * (wm == m ? 1.f : fast_exp2((wm - m) * kLog2e));
   if (lane == 0) wsum[wave] = total;
   __syncthreads();
   const size_t part = (size_t)row * a.segments + seg;
