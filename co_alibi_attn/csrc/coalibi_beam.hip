@@ -6,9 +6,10 @@
 // Within a row the order is the logits', so that each segment of a row yields its maximum, its sum and its N largest logits in
 // one read (its elements stay in registers), and a second launch ranks those of a sequence's beams.  Exponentials are fp32's,
 // summed in fp64 over the threads; scores are fp64 until they are written.
-//   The N largest of a segment: the least of at least N groups' maxima is at most the N-th largest element, and few elements are
-// above it: about N log N.  They are listed and ranked by counting.  A logit and its token are one 64-bit key, so that equal
-// logits are in order, too.
+//   The N largest of a segment: a bound that N elements reach leaves few above it, which are listed and ranked by counting.  For N up
+// to 8 it is the least of N groups of lanes' maxima (about N log N above it), for more the least of the four wavefronts' N / 4-th
+// largest lane (about 2 N; but 64 comparisons each).  A logit and its token are one 64-bit key, so that equal logits are in order, too.
+//   The ranking takes the lists' first ones first, and stops when every list has come to what is below the N-th best.
 //
 // Reordering: a group of W beams owns W pages in every column of its block table.  Pages that are full are shared by all that
 // descend from them; one in use stays with the first of its heirs, and the others get free pages of its column and copies of
@@ -19,7 +20,8 @@
 // the segments take 11.9 (22.5 MB, which a read takes 4 us for: a segment's loads, its bound, its weights and its list follow one
 // another) and the ranking 7.4, loads and steps of one work-group per sequence in a row.  Lists counted by one wavefront took 13.8
 // and 9.4, a bound by counting 64 lanes in the segments 14.4, weights against the work-group's maximum 12.9.  4
-// beams over 50304: 9.1 us.
+// beams over 50304: 9.5 us.  16 beams of 8 sequences over 50304, 16 and 32 kept: 20 and 35 us; with groups' bounds for all N and lists
+// one after the other 31 and 85, and 32 of 16 beams over 131072 fp32 198 instead of 33.
 // Reordering, 4 beams, 24 pools: 4.3 us.  8 beams of 16 sequences, 8 pools of codes and 8 of scales: 11.5 us for 21 MB, which a copy
 // takes 4.3 for: 2176 work-groups, of which most find nothing to copy (as many again take 3.5 us more), and three dependent
 // reads before a copy's first.  Several pools to a work-group took 12.3, heads over two of them 14.8.
@@ -86,11 +88,14 @@ __device__ __forceinline__ Bounds bounds(unsigned x, int low) {
   return r;
 }
 
-// The n-th largest (1 <= n <= 64) of a wavefront's numbers.
-__device__ __forceinline__ unsigned nth_of_wave(unsigned x, int n) {
+// How many of a wavefront's numbers are larger than a lane's, and the n-th largest (1 <= n <= 64) of them.
+__device__ __forceinline__ int larger_lanes(unsigned x) {
   int larger = 0;
 #pragma unroll
   for (int i = 0; i < 64; ++i) larger += lane_of(x, i) > x ? 1 : 0;
+  return larger;
+}
+__device__ __forceinline__ unsigned nth_of_wave(unsigned x, int larger, int n) {
   u64 is;
   do is = __ballot(larger == --n);  // (equal ones have the first one's count)
   while (is == 0);
@@ -123,6 +128,7 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
   const int head = min((int)(-(long long)((size_t)x / sizeof(T)) & (PER - 1)), a.V);
   const int chunks = (a.V - head) / PER, tail = a.V - head - chunks * PER;
 
+  const bool ragged = (seg + 1) * (C * kSelectThreads) > chunks;  // not every thread has all of its chunks
   float v[E];
   int where = -1;  // the single element's token
   if (seg == 0 && tid < head) where = tid;
@@ -138,7 +144,7 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
     for (int c = 0; c < C; ++c)
 #pragma unroll
       for (int e = 0; e < PER; ++e) v[c * PER + e] = static_cast<float>(y[c][e]);
-    if ((seg + 1) * (C * kSelectThreads) > chunks) {  // the last segment's own
+    if (ragged) {
 #pragma unroll
       for (int c = 0; c < C; ++c)
         if (first + c * kSelectThreads >= chunks) {
@@ -156,10 +162,24 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
   float top = v[E - 1];
 #pragma unroll
   for (int e = 0; e < E - 1; ++e) top = fmaxf(top, v[e]);
-  const Bounds cut = bounds(ordered(fmaxf(top, kNegInf)), a.log2_n);
+  // A bound from all four wavefronts, and one from each alone (where the others may have few elements).
+  const unsigned none = ordered(kNegInf), key = ordered(fmaxf(top, kNegInf));
+  const int quarter = (a.N + kSelectWaves - 1) / kSelectWaves;
+  unsigned most = 0, fourth = none, single = none;
+  if (a.N <= 8) {
+    const Bounds x = bounds(key, a.N > 4 ? 3 : a.N > 2 ? 2 : a.N - 1);
+    most = x.top;
+    fourth = x.part;
+    single = x.wave;
+  } else {
+    const int larger = larger_lanes(key);
+    most = nth_of_wave(key, larger, 1);
+    fourth = nth_of_wave(key, larger, quarter);
+    if (ragged) single = nth_of_wave(key, larger, a.N);
+  }
   // The weights' sum, against the wavefront's maximum (the others' are on their way): NaN where there is a NaN.
   float sum = 0.f;
-  const float wm = unordered(cut.top);
+  const float wm = unordered(most);
   const float ref = wm > kNegInf ? wm : 0.f;
   if (wm < __builtin_inff()) {
 #pragma unroll
@@ -169,9 +189,9 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
     for (int e = 0; e < E; ++e) sum += v[e] == wm ? 1.f : v[e] == v[e] ? 0.f : v[e];
   }
   if (lane == 0) {
-    wcut[wave] = cut.wave;
-    wpart[wave] = cut.part;
-    wmax[wave] = unordered(cut.top);
+    wcut[wave] = single;
+    wpart[wave] = fourth;
+    wmax[wave] = wm;
   }
   __syncthreads();
   unsigned least = 0, part_least = ~0u;
@@ -291,14 +311,37 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
   __shared__ bool sdone[kMaxBeams];
   __shared__ u64 lscore[kSelectWaves][kMost], llogit[kSelectWaves][kMost], kscore[kMaxBeams], klogit[kMaxBeams];
   __shared__ int lbeam[kSelectWaves][kMost], kbeam[kMaxBeams];
-  __shared__ unsigned wcut[kSelectWaves];
+  __shared__ unsigned wcut[kSelectWaves], wpart[kSelectWaves], wbest[kSelectWaves];
   __shared__ int listed[kSelectWaves], count[kSelectWaves][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), b = blockIdx.x;
   const long long row0 = (long long)b * a.W;
-  const int per_beam = a.segments * a.N, total = a.W * per_beam;
+  // Candidate i is the i / lists-th of list i % lists (a beam's segment), so that each thread has lists' first ones to begin with.
+  const int lists = a.W * a.segments, total = lists * a.N;
+  const u64* const from = a.pkey + (size_t)row0 * a.segments * a.N;
+  const int by_n = (unsigned)kSelectThreads / (unsigned)lists, by_list = kSelectThreads - by_n * lists;
+  struct Place {
+    int n, list;
+  };
+  auto place_at = [&](int first) {
+    const unsigned i = (unsigned)(first + tid), n = i / (unsigned)lists;
+    return Place{(int)n, (int)(i - n * (unsigned)lists)};
+  };
+  auto next = [&](Place& p) {  // kSelectThreads later
+    p.n += by_n;
+    p.list += by_list;
+    if (p.list >= lists) {
+      p.list -= lists;
+      ++p.n;
+    }
+  };
   u64 keys[kRound];  // of the first round, on their way meanwhile
+  auto load_keys = [&](int first) {
+    Place p = place_at(first);
 #pragma unroll
-  for (int r = 0; r < kRound; ++r) keys[r] = a.pkey[(size_t)row0 * per_beam + min(r * kSelectThreads + tid, total - 1)];
+    for (int r = 0; r < kRound; ++r, next(p)) keys[r] = from[(size_t)p.list * a.N + min(p.n, a.N - 1)];
+  };
+  load_keys(0);
+  const float per_segment = 1.f / a.segments;  // (a quotient below 64, half a segment from the next: no rounding reaches it)
   for (int w = wave; w < a.W; w += kSelectWaves) {
     const long long row = row0 + w;
     const float score = a.scores[row];
@@ -337,18 +380,18 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
   for (int first = 0; first < total; first += kRound * kSelectThreads) {
     u64 score[kRound + 1], logit[kRound + 1];
     int beam[kRound + 1];
+    Place p = place_at(first);
 #pragma unroll
-    for (int r = 0; r < kRound; ++r) {
-      const int i = first + r * kSelectThreads + tid;
+    for (int r = 0; r < kRound; ++r, next(p)) {
       score[r] = logit[r] = 0;
       beam[r] = 0;
-      if (i < total) {
-        const int w = (unsigned)i / (unsigned)per_beam;
+      if (p.n < a.N) {
+        const int w = (int)(((float)p.list + 0.5f) * per_segment);
         const double base = sbase[w];
         const bool done = sdone[w];
         u64 k = keys[r];
         const float x = key_logit(k), m = smax[w];
-        if (done) k = i == w * per_beam ? logit_key(0.f, a.end_token) : 0;
+        if (done) k = p.n == 0 && p.list == w * a.segments ? logit_key(0.f, a.end_token) : 0;
         // Of +inf logits all weigh 1, and every other one nothing.
         if (base == base && k != 0 && (done || x == m || m < __builtin_inff())) {
           score[r] = score_key(done || x == m ? base : base + ((double)x - (double)m));
@@ -360,22 +403,32 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
     score[kRound] = tid < a.N ? kscore[tid] : 0;
     logit[kRound] = tid < a.N ? klogit[tid] : 0;
     beam[kRound] = tid < a.N ? kbeam[tid] : 0;
-    if (first + kRound * kSelectThreads < total) {
-#pragma unroll
-      for (int r = 0; r < kRound; ++r)
-        keys[r] = a.pkey[(size_t)row0 * per_beam + min(first + (kRound + r) * kSelectThreads + tid, total - 1)];
-    }
+    if (first + kRound * kSelectThreads < total) load_keys(first + kRound * kSelectThreads);
     u64 best = 0;
 #pragma unroll
-    for (int r = 0; r <= kRound; ++r) best = score[r] > best ? score[r] : best;
-    // A wavefront's N-th largest lane, by the scores' first halves, is no more than the N-th largest candidate.  (Segments' lists are
-    // in order, so that groups as in the segments would each hold the first ones or the last ones.)
-    const unsigned cut = nth_of_wave((unsigned)(best >> 32), a.N);
-    if (lane == 0) wcut[wave] = cut;
+    for (int r = 0; r < kRound; ++r) best = score[r] > best ? score[r] : best;
+    // No more than the N-th largest candidate: the N-th of those before; a wavefront's N-th largest lane, by the scores' first halves;
+    // and the least of four wavefronts' N / 4-th.
+    const unsigned lead = (unsigned)(best >> 32);
+    const int larger = larger_lanes(lead);
+    const unsigned cut = nth_of_wave(lead, larger, a.N), part = nth_of_wave(lead, larger, (a.N + kSelectWaves - 1) / kSelectWaves);
+    if (lane == 0) {
+      wcut[wave] = cut;
+      wpart[wave] = part;
+      wbest[wave] = 0;
+    }
+    u64 least = max(kscore[a.N - 1], 1ull);
+    if (first > 0 && __any(best >= least) && lane == 0) wbest[wave] = 1;
     __syncthreads();
-    u64 least = 1;
+    // A round in which every list is below the N-th already: so is what follows of each.
+    if (first > 0 && lists <= kRound * kSelectThreads && (wbest[0] | wbest[1] | wbest[2] | wbest[3]) == 0) break;
+    unsigned part_least = ~0u;
 #pragma unroll
-    for (int i = 0; i < kSelectWaves; ++i) least = max(least, (u64)wcut[i] << 32);
+    for (int i = 0; i < kSelectWaves; ++i) {
+      least = max(least, (u64)wcut[i] << 32);
+      part_least = min(part_least, wpart[i]);
+    }
+    least = max(least, (u64)part_least << 32);
     int mine = 0;
 #pragma unroll
     for (int r = 0; r <= kRound; ++r) {

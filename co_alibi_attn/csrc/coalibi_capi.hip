@@ -1305,7 +1305,6 @@ int co_alibi_beam_select(int dtype, const void* logits, const long long* strides
   a.W = beams;
   a.N = num_beams;
   a.V = vocab;
-  while ((1 << a.log2_n) < num_beams) ++a.log2_n;
   a.segments = p.segments;
   a.chunks = p.chunks;
   hipStream_t st = static_cast<hipStream_t>(stream);

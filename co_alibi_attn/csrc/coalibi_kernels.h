@@ -494,7 +494,6 @@ struct SelectArgs {
   double* psum;
   unsigned long long* pkey;  // (B*W, segments, N)
   int B, W, N, V;
-  int log2_n;            // the least power of two from N on
   int segments, chunks;  // a segment has `chunks` 16-byte chunks for each of a work-group's 256 threads
 };
 

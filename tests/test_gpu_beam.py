@@ -318,3 +318,20 @@ def test_pools_and_logits_past_32_bits():
     for x, y in zip(got, want):
         assert torch.equal(x[-1:], y)
     assert got[2][0].tolist() == [0, 1, 2, 3, 4]
+
+
+@pytest.mark.parametrize("B,W,N,V,dtype", [(2, 16, 32, 50304, BF16), (1, 16, 31, 9000, F32), (3, 5, 17, 20000, F16), (1, 3, 64, 1000, F32),
+                                           (1, 64, 40, 262144, BF16)])
+def test_many_of_many(B, W, N, V, dtype):
+    """Rounds of the ranking, and the end of them; the last one has more lists than a round."""
+    logits, scores, _ = draw(B, W, V, dtype, seed=9)
+    check(logits, scores * 0.05, N)
+
+
+@pytest.mark.parametrize("N", (9, 32, 64))
+def test_ties_among_many(N):
+    """A few different logits, and beams of equal scores: every order but the scores' counts."""
+    logits = torch.randint(0, 3, (2, 8, 20000), generator=torch.Generator().manual_seed(N)).float()
+    logits[:, 1::2] = logits[:, ::2]
+    check(logits, torch.zeros(2, 8), N)
+    check(logits.flip(2).to(BF16), torch.zeros(2, 8), N)
