@@ -107,12 +107,13 @@ constexpr int kListed = 256;  // keys of a wavefront's list, which are ranked by
 // The lanes' place behind n others, of those for which `is`, and how many they are.
 __device__ __forceinline__ int place_of(u64 is) { return __builtin_amdgcn_mbcnt_hi((unsigned)(is >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)is, 0)); }
 
-// C: 16-byte chunks of a segment per thread.  A row is read in whole chunks from its first 16-byte boundary on; the elements
-// before it go with the first segment and those behind the last whole chunk with the last one, one per thread.
+// C: 16-byte chunks of a segment per thread.  A row's chunks begin with its first token wherever it lies (loads need only an element's
+// alignment), so that equal rows are added in the same order and get the same bits: their scores tie.  The tokens behind the last whole
+// chunk go with the last segment, one per thread.
 template <typename T, int C>
 __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(SelectArgs a) {
   constexpr int PER = 16 / sizeof(T), E = C * PER + 1;
-  typedef T chunk_t __attribute__((ext_vector_type(PER)));
+  typedef T chunk_t __attribute__((ext_vector_type(PER), aligned(sizeof(T))));
   __shared__ u64 list[kSelectWaves][kListed];
   __shared__ int listed[kSelectWaves], count[kSelectWaves][64];
   __shared__ u64 wnext[kSelectWaves];
@@ -125,21 +126,19 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
   if (a.finished != nullptr && a.finished[row] != 0) return;
   const int b = (int)(row / a.W), w = (int)(row - (long long)b * a.W);
   const T* const x = static_cast<const T*>(a.logits) + (size_t)b * a.batch_stride + (size_t)w * a.beam_stride;
-  const int head = min((int)(-(long long)((size_t)x / sizeof(T)) & (PER - 1)), a.V);
-  const int chunks = (a.V - head) / PER, tail = a.V - head - chunks * PER;
+  const int chunks = a.V / PER, tail = a.V - chunks * PER;
 
   const bool ragged = (seg + 1) * (C * kSelectThreads) > chunks;  // not every thread has all of its chunks
   float v[E];
   int where = -1;  // the single element's token
-  if (seg == 0 && tid < head) where = tid;
-  if (seg == a.segments - 1 && tid >= 64 && tid - 64 < tail) where = a.V - tail + (tid - 64);
+  if (seg == a.segments - 1 && tid < tail) where = a.V - tail + tid;
   v[E - 1] = where >= 0 ? static_cast<float>(x[where]) : kNegInf;
   const int first = seg * (C * kSelectThreads) + tid;  // the thread's first chunk
   if (chunks > 0) {
     chunk_t y[C];
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      y[c] = *reinterpret_cast<const chunk_t*>(x + head + (size_t)min(first + c * kSelectThreads, chunks - 1) * PER);
+      y[c] = *reinterpret_cast<const chunk_t*>(x + (size_t)min(first + c * kSelectThreads, chunks - 1) * PER);
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
@@ -156,7 +155,7 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
 #pragma unroll
     for (int e = 0; e < E - 1; ++e) v[e] = kNegInf;
   }
-  auto token = [&](int e) { return e == E - 1 ? where : head + (first + e / PER * kSelectThreads) * PER + e % PER; };
+  auto token = [&](int e) { return e == E - 1 ? where : (first + e / PER * kSelectThreads) * PER + e % PER; };
 
   // The segment's maximum, and a bound that its N-th largest logit is not below.
   float top = v[E - 1];
