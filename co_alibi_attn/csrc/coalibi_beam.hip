@@ -4,8 +4,8 @@
 // Selection: with M_w and S_w a row's largest logit and sum_t exp(x_t - M_w), candidate (w, t) scores
 //   score_w + (x_t - M_w) - log S_w.
 // Within a row the order is the logits', so that each segment of a row yields its maximum, its sum and its N largest logits in
-// one read (its elements stay in registers), and a second launch ranks those of a sequence's beams.  Exponentials are fp32's,
-// summed in fp64 over the threads; scores are fp64 until they are written.
+// one read (its elements stay in registers), and a second launch ranks those of a sequence's beams.  Exponentials are fp32's, each
+// within 2^-22 of itself whatever its argument, and their sums fp64's, as scores are until they are written.
 //   The N largest of a segment: a bound that N elements reach leaves few above it, which are listed and ranked by counting.  For N up
 // to 8 it is the least of N groups of lanes' maxima (about N log N above it), for more the least of the four wavefronts' N / 4-th
 // largest lane (about 2 N; but 64 comparisons each).  A logit and its token are one 64-bit key, so that equal logits are in order, too.
@@ -102,6 +102,37 @@ __device__ __forceinline__ unsigned nth_of_wave(unsigned x, int larger, int n) {
   return lane_of(x, __builtin_amdgcn_readfirstlane(__ffsll(is) - 1));
 }
 
+// Sums of exp(x), as a factor of 2^reference(m) for the largest x, m: a whole number, so that sums of parts are brought to one
+// reference exactly, or m log2 e itself where that is no number of a few digits.
+constexpr float kOrdinary = 0x1p20f;
+constexpr double kLog2e64 = 0x1.71547652b82fep0, kLn2_64 = 0x1.62e42fefa39efp-1;
+constexpr float kLog2eRest = (float)(kLog2e64 - (double)kLog2e);
+__device__ __forceinline__ float whole_reference(float m) { return rintf(m * kLog2e); }
+__device__ __forceinline__ double reference(float m) {
+  return fabsf(m) < kOrdinary ? (double)whole_reference(m) : (double)m * kLog2e64;
+}
+// A sum against `from` as one against `to`, which is not less.
+__device__ __forceinline__ double rescaled(double sum, float from, float to) {
+  if (from == to) return sum;  // (infinities, too)
+  if (fabsf(from) < kOrdinary && fabsf(to) < kOrdinary) return ldexp(sum, (int)(whole_reference(from) - whole_reference(to)));
+  return sum * exp2(reference(from) - reference(to));
+}
+// exp(x) against the reference of an ordinary m, for x <= m, or NaN.  x log2 e is split into a whole number and a rest in [-1/2, 1/2]
+// that is off by 2^-25: the rest's power is off by 2^-23 of itself (one step of v_exp_f32) and 2^-25.5, whatever x is.  (A product
+// that is rounded as a whole, 17 for a logit that 2^20 of make as heavy as the largest, is off by 2^-20.)  What is below 2^-126
+// of the largest may come to 0.
+struct Weights {
+  float least, magic;
+  __device__ __forceinline__ Weights(float m) : least(m - 128.f), magic(0x1.8p23f - whole_reference(m)) {}
+  __device__ __forceinline__ double operator()(float x) const {
+    x = x < least ? least : x;
+    const float t = fmaf(x, kLog2e, magic);  // the whole number in its last bits: t lies in [2^23, 2^24)
+    const float k = t - magic;
+    const float rest = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -k));
+    return (double)ldexpf(fast_exp2(rest), __builtin_bit_cast(int, t) - __builtin_bit_cast(int, 0x1.8p23f));
+  }
+};
+
 constexpr int kListed = 256;  // keys of a wavefront's list, which are ranked by counting
 
 // The lanes' place behind n others, of those for which `is`, and how many they are.
@@ -177,15 +208,21 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
     if (ragged) single = nth_of_wave(key, larger, a.N);
   }
   // The weights' sum, against the wavefront's maximum (the others' are on their way): NaN where there is a NaN.
-  float sum = 0.f;
   const float wm = unordered(most);
-  const float ref = wm > kNegInf ? wm : 0.f;
-  if (wm < __builtin_inff()) {
+  double sum = 0.0;
+  if (fabsf(wm) < kOrdinary) {
+    const Weights of(wm);
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum += fast_exp2((v[e] - ref) * kLog2e);
+    for (int e = 0; e < E; ++e) sum += of(v[e]);
+  } else if (fabsf(wm) < __builtin_inff()) {
+    const Weights of(0.f);  // (exact for every logit that counts)
+#pragma unroll
+    for (int e = 0; e < E; ++e) sum += of(v[e] - wm);
   } else {
+    float n = 0.f;
 #pragma unroll
-    for (int e = 0; e < E; ++e) sum += v[e] == wm ? 1.f : v[e] == v[e] ? 0.f : v[e];
+    for (int e = 0; e < E; ++e) n += v[e] != v[e] ? v[e] : v[e] == __builtin_inff() ? 1.f : 0.f;
+    sum = n;
   }
   if (lane == 0) {
     wcut[wave] = single;
@@ -216,7 +253,7 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_rows_kernel(Sel
     }
   }
   if (lane == 0) listed[wave] = mine;
-  const double total = wave_sum((double)sum) * (wm == m ? 1.f : fast_exp2((wm - m) * kLog2e));
+  const double total = rescaled(wave_sum(sum), wm, m);
   if (lane == 0) wsum[wave] = total;
   __syncthreads();
   const size_t part = (size_t)row * a.segments + seg;
@@ -359,11 +396,12 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
         m = fmaxf(m, pm[s]);
       }
       m = wave_max(m);
-      // (A segment's factor in fp32, as its weights are.)
-      double sum = s0 * (m0 == m ? 1.f : fast_exp2((m0 - m) * kLog2e));
-      for (int s = lane + 64; s < a.segments; s += 64) sum += ps[s] * (pm[s] == m ? 1.f : fast_exp2((pm[s] - m) * kLog2e));
+      double sum = rescaled(s0, m0, m);
+      for (int s = lane + 64; s < a.segments; s += 64) sum += rescaled(ps[s], pm[s], m);
       sum = wave_sum(sum);
-      if (!__any(nan) && m > kNegInf) base = (double)score - log(sum);
+      // (What the reference is more than m goes with the sum, so that a logit counts by its distance to m.)
+      const double more = fabsf(m) < kOrdinary ? (double)whole_reference(m) * kLn2_64 - (double)m : 0.0;
+      if (!__any(nan) && m > kNegInf) base = (double)score - (log(sum) + more);
     }
     if (lane == 0) {
       sbase[w] = score > kNegInf && score < __builtin_inff() ? base : __builtin_nan("");

@@ -232,7 +232,8 @@ def co_alibi_beam_select(logits, scores, num_beams=None, finished=None, end_toke
     of several +inf logits all weigh the same and the others nothing.  Places without a candidate get score -inf, parent 0 and
     token -1: no row of an embedding.
 
-    Returns scores (float32; sums in float64, each rounded once), parents (int32) and tokens (int64).
+    Returns scores (float32), parents (int32) and tokens (int64).  Scores are worked out and compared in float64, from exponentials of
+    float32's accuracy (so log_softmax is within 2^-22, and the same for the same logits wherever they lie), and rounded once.
     """
     if logits.dim() != 3 or not 1 <= logits.shape[2] <= _native.MAX_VOCAB or not 1 <= logits.shape[1] <= _native.MAX_BEAMS:
         raise ValueError(f"logits must be (B, W, V) with 1 <= W <= {_native.MAX_BEAMS} and 1 <= V <= {_native.MAX_VOCAB}, got "

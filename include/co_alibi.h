@@ -321,6 +321,7 @@ int co_alibi_decode_tree_8bit(int dtype, int format, const void* q, const void* 
 
 /* Beam selection: of every sequence's candidates (w, t), beam w < beams continued with token t < vocab, the num_beams with the
  * largest score, scores[b][w] + log_softmax(logits[b][w])[t], best first; equal scores go by beam, then by logit, then by token.
+ * Scores are compared in fp64 and rounded once; log_softmax is within 2^-22, and the same for the same logits wherever they lie.
  * logits: (batch, beams, vocab) in `dtype`, strides its batch and beam strides in elements (2 values) or NULL: contiguous.
  * scores: (batch, beams) fp32.  A beam with finished[b][w] != 0 (batch x beams bytes, or NULL) has one candidate, end_token at its
  * score as it is, and its logits are not read.  A beam whose score is not finite, whose logits hold a NaN or none above -inf
