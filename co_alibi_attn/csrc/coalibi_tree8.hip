@@ -495,10 +495,11 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
     f32x16 s = scores(x);
     if (held) add_values(v, pb);
     // A tile whose keys all weigh less than 2^-a.far of their row's sum, as far as it is known, is left out but for its sigmas: a_j
-    // is at most its score less the sigmas after the tile.  (A NaN keeps it.)
+    // is at most its score less the sigmas after the tile.  A NaN keeps it: the largest score is NaN if one is (v_maximum3; fmaxf
+    // takes the other operand).
     float mt = s[0];
 #pragma unroll
-    for (int r = 1; r < 16; ++r) mt = fmaxf(mt, s[r]);
+    for (int r = 1; r < 16; ++r) mt = __builtin_elementwise_maximum(mt, s[r]);
     held = __any(row_ok && !(lam2 >= 0.f && mt - lam2 * carry - m2 < __builtin_amdgcn_logf(lsum) - a.far));
     if (held) load_values(Inside{}, tile, f, v);
     weigh_or_pass(s, scale_of(x), held);
