@@ -6,7 +6,8 @@
 //   t_j = sm_scale*log2(e) * ks * (q.kc_j),   a_j = t_j - slope*log2(e) * z_j,   a'_j = a_j + log2 vs,
 //   O   = sum_j 2^(a'_j - m) vc_j / l,   l = sum_j 2^(a'_j - m) / vs,   LSE = (m + log2 l) * ln 2.
 // The lane of a score holds the 16 keys of a block, so ks is a factor of its scores' one multiplication, log2 vs a part of
-// the one term that all of its exponents subtract, and 1 / vs one multiplication for their sum.
+// the one term that all of its exponents subtract, and 1 / vs one multiplication for their sum.  (With fp16 weights the codes take the
+// powers of two of vs instead, which leaves the weights their bits: no slower.)
 //
 // A wavefront takes 32 query rows over a run of 32-key tiles, newest first, by itself: S^T = K Q^T and O^T += V^T P^T on MFMA,
 // the operands straight from memory into registers.
@@ -51,18 +52,41 @@ __device__ __forceinline__ float signed_byte(unsigned x) {
 __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
   return __builtin_amdgcn_perm(__builtin_bit_cast(unsigned, hi), __builtin_bit_cast(unsigned, lo), 0x07060302u);
 }
+// A power of two 2^e that fp16's operands of V are taken by: exact for all codes from 2^-15 to 2^7 (e4m3: 2^-9 to 448), or from 2^-24
+// to 2^5 (int8: 1152 * 2^5 is a number of fp16, too).  The other types' weights have the range that scales need.
+struct Times1 {
+  __device__ __forceinline__ explicit Times1(int = 0) {}
+};
+template <typename F>
+struct TimesPower {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  float f;         // 2^e
+  f16x2 h, minus;  // int8: 2^e and -1152 * 2^e twice
+  __device__ __forceinline__ explicit TimesPower(int e) : f(ldexpf(1.f, e)) {
+    if constexpr (__is_same(F, I8)) {
+      const _Float16 x = static_cast<_Float16>(f);
+      h = f16x2{x, x};
+      minus = h * f16x2{(_Float16)-1152.0f, (_Float16)-1152.0f};
+    }
+  }
+};
 // Pair HI (bytes 0 and 1, or 2 and 3) of the codes in x, as the bits of two 16-bit T.
-template <typename T, typename F, bool HI>
-__device__ __forceinline__ unsigned code_pair(unsigned x) {
+template <typename T, typename F, bool HI, typename P>
+__device__ __forceinline__ unsigned code_pair(unsigned x, const P& by) {
   if constexpr (__is_same(F, E4M3) && __is_same(T, __bf16)) {
     return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, HI));
   } else if constexpr (__is_same(F, E4M3)) {
-    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, HI));
+    float f = 1.0f;
+    if constexpr (!__is_same(P, Times1)) f = by.f;
+    return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, f, HI));
   } else if constexpr (__is_same(T, _Float16)) {
-    // The byte plus 128 in the last bits of 1024: exact, and so is the difference.
+    // The byte plus 128 in the last bits of 1024: exact, and so is the difference, and its product with the power of two.
     typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
     const unsigned h = __builtin_amdgcn_perm(0x64646464u, x ^ 0x80808080u, HI ? 0x05030402u : 0x05010400u);
-    return __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, h) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f});
+    if constexpr (__is_same(P, Times1))
+      return __builtin_bit_cast(unsigned, __builtin_bit_cast(f16x2, h) - f16x2{(_Float16)1152.0f, (_Float16)1152.0f});
+    else
+      return __builtin_bit_cast(unsigned, __builtin_elementwise_fma(__builtin_bit_cast(f16x2, h), by.h, by.minus));
   } else {
     return pack_bf16(signed_byte<HI ? 2 : 0>(x), signed_byte<HI ? 3 : 1>(x));
   }
@@ -77,15 +101,15 @@ __device__ __forceinline__ float code_float(unsigned x) {
 template <typename T, typename F>
 __device__ __forceinline__ typename Mfma<T>::vec8 code_vec8(unsigned lo, unsigned hi) {
   if constexpr (sizeof(T) == 2)
-    return __builtin_bit_cast(typename Mfma<T>::vec8, u32x4{code_pair<T, F, false>(lo), code_pair<T, F, true>(lo),
-                                                            code_pair<T, F, false>(hi), code_pair<T, F, true>(hi)});
+    return __builtin_bit_cast(typename Mfma<T>::vec8, u32x4{code_pair<T, F, false>(lo, Times1()), code_pair<T, F, true>(lo, Times1()),
+                                                            code_pair<T, F, false>(hi, Times1()), code_pair<T, F, true>(hi, Times1())});
   else
     return f32x8{code_float<F, 0>(lo), code_float<F, 1>(lo), code_float<F, 2>(lo), code_float<F, 3>(lo),
                  code_float<F, 0>(hi), code_float<F, 1>(hi), code_float<F, 2>(hi), code_float<F, 3>(hi)};
 }
 // Byte N of eight words as an operand.  Of two words at a time, the byte of both as a pair.
-template <typename T, typename F, int N>
-__device__ __forceinline__ typename Mfma<T>::vec8 byte_vec8(const unsigned (&w)[8]) {
+template <typename T, typename F, int N, typename P>
+__device__ __forceinline__ typename Mfma<T>::vec8 byte_vec8(const unsigned (&w)[8], const P& by) {
   if constexpr (sizeof(T) == 4) {
     f32x8 x;
 #pragma unroll
@@ -98,7 +122,7 @@ __device__ __forceinline__ typename Mfma<T>::vec8 byte_vec8(const unsigned (&w)[
       if constexpr (__is_same(F, I8) && __is_same(T, __bf16))
         x[e] = pack_bf16(signed_byte<N>(w[2 * e]), signed_byte<N>(w[2 * e + 1]));
       else  // (the permute serves the next byte, too)
-        x[e] = code_pair<T, F, (N & 1) != 0>(__builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], N & 2 ? 0x07030602u : 0x05010400u));
+        x[e] = code_pair<T, F, (N & 1) != 0>(__builtin_amdgcn_perm(w[2 * e + 1], w[2 * e], N & 2 ? 0x07030602u : 0x05010400u), by);
     }
     return __builtin_bit_cast(typename Mfma<T>::vec8, x);
   }
@@ -175,6 +199,8 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
   using M = Mfma<T>;
   using V8 = typename M::vec8;
   constexpr int DT = C::DT;
+  constexpr bool kCodesTakeScales = __is_same(T, _Float16);
+  constexpr int kMostPower = __is_same(F, E4M3) ? 7 : 5, kLeastPower = __is_same(F, E4M3) ? -15 : -20;  // (TimesPower)
   const TreeArgs& a = a8.t;
   __shared__ __align__(16) char smem[C::LDS_BYTES];
   __shared__ float sMax[kTree8Waves][32], sSum[kTree8Waves][32], sSig[kTree8Waves][32], sScale[kTree8Waves][32];
@@ -309,7 +335,9 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
   // State of the lane's row: scale, this half's share of the sum, O^T, and the sigma of the keys after the current ones.
   float m2 = kNegInf, lsum = 0.f, carry = 0.f;
   V8 pb[2];  // weights of the last tile
-  f32x16 acc[DT];
+  f32x16 acc[DT];  // in units of 2^unit
+  int unit = 0, power = 0;  // power: of the lane's codes of the tile whose values are held
+  bool first_scale = true;
 #pragma unroll
   for (int j = 0; j < DT; ++j) acc[j] = f32x16{};
 
@@ -381,7 +409,27 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
     lost |= !fine;
     return fine ? x.vs : 1.f;
   };
+  // What the weights take of a tile's scales of V.  fp16's have little room below the row's largest (subnormal below 2^-14), so there the
+  // codes take the scales' powers of two, relative to a unit of O that rises with the largest, as far as their products are exact
+  // (2^22 below it for e4m3, 2^25 for int8); the weights what is left, from 1 to 2.
+  auto take = [&](float vs) {
+    if constexpr (!kCodesTakeScales) return vs;
+    const int e = (int)(__builtin_bit_cast(unsigned, vs) >> 23) - 127;
+    const int most = max(__builtin_amdgcn_readlane(e, 0), __builtin_amdgcn_readlane(e, 32));
+    if (first_scale || most - unit > kMostPower) {
+      const int to = most - kMostPower;
+      const float f = ldexpf(1.f, unit - to);
+#pragma unroll
+      for (int j = 0; j < DT; ++j) acc[j] *= f;
+      unit = to;
+      first_scale = false;
+    }
+    power = max(e - unit, kLeastPower);
+    return ldexpf(vs, -(unit + power));
+  };
   auto add_values = [&](const Run<DT> (&v)[16], const V8 (&pb)[2]) {
+    using By = std::conditional_t<kCodesTakeScales, TimesPower<F>, Times1>;
+    const By by(power);
 #pragma unroll
     for (int st = 0; st < 2; ++st) {
 #pragma unroll
@@ -389,11 +437,11 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
         unsigned w[8];
 #pragma unroll
         for (int e = 0; e < 8; ++e) w[e] = v[8 * st + e].w[q4];
-        acc[4 * q4] = M::k16(byte_vec8<T, F, 0>(w), pb[st], acc[4 * q4]);
-        if constexpr (DT > 1) acc[4 * q4 + 1] = M::k16(byte_vec8<T, F, 1>(w), pb[st], acc[4 * q4 + 1]);
+        acc[4 * q4] = M::k16(byte_vec8<T, F, 0>(w, by), pb[st], acc[4 * q4]);
+        if constexpr (DT > 1) acc[4 * q4 + 1] = M::k16(byte_vec8<T, F, 1>(w, by), pb[st], acc[4 * q4 + 1]);
         if constexpr (DT > 2) {
-          acc[4 * q4 + 2] = M::k16(byte_vec8<T, F, 2>(w), pb[st], acc[4 * q4 + 2]);
-          acc[4 * q4 + 3] = M::k16(byte_vec8<T, F, 3>(w), pb[st], acc[4 * q4 + 3]);
+          acc[4 * q4 + 2] = M::k16(byte_vec8<T, F, 2>(w, by), pb[st], acc[4 * q4 + 2]);
+          acc[4 * q4 + 3] = M::k16(byte_vec8<T, F, 3>(w, by), pb[st], acc[4 * q4 + 3]);
         }
       }
     }
@@ -477,7 +525,7 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
     const int left = L - tile * 32 - 16 * hh;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[r] = r < left ? s[r] : kNegInf;
-    weigh(s, scale_of(kb));
+    weigh(s, take(scale_of(kb)));
     add_values(v, pb);
     --tile;
   }
@@ -502,7 +550,9 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
     for (int r = 1; r < 16; ++r) mt = __builtin_elementwise_maximum(mt, s[r]);
     held = __any(row_ok && !(lam2 >= 0.f && mt - lam2 * carry - m2 < __builtin_amdgcn_logf(lsum) - a.far));
     if (held) load_values(Inside{}, tile, f, v);
-    weigh_or_pass(s, scale_of(x), held);
+    float vs = scale_of(x);
+    if (held) vs = take(vs);
+    weigh_or_pass(s, vs, held);
     --tile;
   };
   while (tile >= t_first) {
@@ -549,7 +599,7 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
   }
   __syncthreads();
   float* const so = reinterpret_cast<float*>(smem) + (size_t)wave * 32 * C::LDO + hl * C::LDO;
-  const float f = sScale[wave][hl];
+  const float f = ldexpf(sScale[wave][hl], unit);
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const int d = DT * ((r >> 2) * 8 + hh * 4 + (r & 3));

@@ -148,7 +148,8 @@ def co_alibi_decode_tree_8bit(q, k, v, k_cache, v_cache, k_scale, v_scale, seq_l
     """``co_alibi_decode_tree`` over an 8-bit cache (see the module): everything else is the same.
 
     The cached keys and values are code * scale, and neither q nor the weights are rounded to 8 bits: only what the cache holds
-    is.  The new tokens' own k and v count as they are.  A sequence whose filled rows lie on a page outside the pool, or in a
+    is.  The new tokens' own k and v count as they are.  (In float16 weights of values whose block has a scale below 2^-22 (e4m3) or
+    2^-25 (int8) of the largest lose bits.)  A sequence whose filled rows lie on a page outside the pool, or in a
     block whose scale is not in [2^-40, 2^40], gets NaN.
     """
     return _decode_tree(q, k, v, (k_cache, v_cache), (k_scale, v_scale), seq_len, parents, block_table, sm_scale, bias_max,
