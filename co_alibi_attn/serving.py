@@ -120,9 +120,9 @@ def _decode_tree(q, k, v, caches, scales, seq_len, parents, block_table, sm_scal
         o, lse = ops.decode_tree(_detached(q), _detached(k), _detached(v), _detached(k_cache), _detached(v_cache), slopes, lens,
                                  parents, block_table, bound, float(sm_scale), bool(return_lse))
     else:
-        o, lse = ops.decode_tree_8bit(_detached(q), _detached(k), _detached(v), k_cache, v_cache, _detached(scales[0]),
-                                      _detached(scales[1]), slopes, lens, parents, block_table, bound, float(sm_scale),
-                                      bool(return_lse))
+        o, lse = ops.decode_tree_8bit(_detached(q), _detached(k), _detached(v), _detached(k_cache), _detached(v_cache),
+                                      _detached(scales[0]), _detached(scales[1]), slopes, lens, parents, block_table, bound,
+                                      float(sm_scale), bool(return_lse))
     return (o, lse) if return_lse else o
 
 
@@ -197,8 +197,8 @@ def co_alibi_cache_append_8bit(k, v, k_cache, v_cache, k_scale, v_scale, seq_len
     _check_8bit(k_cache, v_cache, k_scale, v_scale)
     _check_head_dim(k.shape[3], k.dtype)
     _check_table(block_table, k.shape[0])
-    if k_scale.requires_grad or v_scale.requires_grad:
-        raise ValueError("the scales are written in place and cannot require gradients")
+    if any(t.requires_grad for t in (k_cache, v_cache, k_scale, v_scale)):
+        raise ValueError("the caches and their scales are written in place and cannot require gradients")
     ops.cache_append_8bit(_detached(k), _detached(v), k_cache, v_cache, k_scale, v_scale, seq_lens, counts, rows, block_table)
 
 
@@ -218,7 +218,8 @@ def co_alibi_cache_read_8bit(k_cache, v_cache, k_scale, v_scale, seq_lens, rows,
     _check_table(block_table, seq_lens.shape[0])
     if int(rows) != rows or rows < 0:
         raise ValueError(f"rows must be a whole number >= 0, got {rows}")
-    return ops.cache_read_8bit(k_cache, v_cache, _detached(k_scale), _detached(v_scale), seq_lens, first, block_table, int(rows), dtype)
+    return ops.cache_read_8bit(_detached(k_cache), _detached(v_cache), _detached(k_scale), _detached(v_scale), seq_lens, first,
+                               block_table, int(rows), dtype)
 
 
 def co_alibi_beam_select(logits, scores, num_beams=None, finished=None, end_token=0):
