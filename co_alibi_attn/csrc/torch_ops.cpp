@@ -663,8 +663,16 @@ std::tuple<Tensor, Tensor> cache_read_8bit_hip(const Tensor& k_cache, const Tens
   TORCH_CHECK_VALUE(rows >= 0, fn, ": rows must be >= 0, got ", rows);
   const int64_t heads = k_cache.size(1), head_dim = k_cache.size(3);
   const auto options = k_cache.options().dtype(dtype);
-  if (k_cache.numel() == 0 || c.capacity == 0)
-    return {at::zeros({batch, heads, rows, head_dim}, options), at::zeros({batch, heads, rows, head_dim}, options)};
+  if (k_cache.numel() == 0 || c.capacity == 0) {
+    Tensor k = at::zeros({batch, heads, rows, head_dim}, options), v = at::zeros_like(k);
+    if (k.numel() != 0 && c.capacity != 0) {  // a pool without pages: filled rows lie outside it
+      Tensor row = at::arange(rows, lens.options().dtype(at::kLong)).unsqueeze(0);
+      if (from.defined()) row = row + from.unsqueeze(1);
+      const Tensor filled = row.ge(0).logical_and(row.lt(lens.clamp_max(c.capacity).unsqueeze(1)));
+      for (const Tensor& t : {k, v}) t.masked_fill_(filled.unsqueeze(1).unsqueeze(3), std::numeric_limits<double>::quiet_NaN());
+    }
+    return {k, v};
+  }
   Tensor k = at::empty({batch, heads, rows, head_dim}, options), v = at::empty_like(k);
   if (k.numel() == 0) return {k, v};
   const auto strides = all_strides<2>({k_cache, v_cache});
