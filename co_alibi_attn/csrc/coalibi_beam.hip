@@ -517,23 +517,24 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
           kbeam[rank] = xb;
         }
       }
-    } else
-    for (int i = lane; i < mine; i += 64) {
-      const u64 x = lscore[wave][i], xl = llogit[wave][i];
-      const int xb = lbeam[wave][i];
-      int rank = 0;
-      for (int w = 0; w < kSelectWaves; ++w)
-        for (int j = 0; j < listed[w]; ++j) {
-          const u64 y = lscore[w][j];
-          if (y > x)
-            ++rank;
-          else if (y == x)
-            rank += lbeam[w][j] < xb || (lbeam[w][j] == xb && llogit[w][j] > xl) ? 1 : 0;
+    } else {
+      for (int i = lane; i < mine; i += 64) {
+        const u64 x = lscore[wave][i], xl = llogit[wave][i];
+        const int xb = lbeam[wave][i];
+        int rank = 0;
+        for (int w = 0; w < kSelectWaves; ++w)
+          for (int j = 0; j < listed[w]; ++j) {
+            const u64 y = lscore[w][j];
+            if (y > x)
+              ++rank;
+            else if (y == x)
+              rank += lbeam[w][j] < xb || (lbeam[w][j] == xb && llogit[w][j] > xl) ? 1 : 0;
+          }
+        if (rank < a.N) {
+          kscore[rank] = x;
+          klogit[rank] = xl;
+          kbeam[rank] = xb;
         }
-      if (rank < a.N) {
-        kscore[rank] = x;
-        klogit[rank] = xl;
-        kbeam[rank] = xb;
       }
     }
     __syncthreads();

@@ -334,7 +334,10 @@ __global__ __launch_bounds__(kTree8Threads, (Tree8Cfg<T, D>::WGS_PER_CU)) void c
 
   // State of the lane's row: scale, this half's share of the sum, O^T, and the sigma of the keys after the current ones.
   float m2 = kNegInf, lsum = 0.f, carry = 0.f;
-  V8 pb[2];  // weights of the last tile
+  // Weights of the last tile, rounded to q's type for their product with V (their sum is not), as the other attentions of this library
+  // round them.  In two parts, the second what the first leaves, o has no rounding but its own, and it costs 6 % of the drafts and of
+  // the single token, 4 % of the 32 sequences.
+  V8 pb[2];
   f32x16 acc[DT];  // in units of 2^unit
   int unit = 0, power = 0;  // power: of the lane's codes of the tile whose values are held
   bool first_scale = true;
