@@ -1062,8 +1062,8 @@ int append_args(const char* fn, int dtype, bool eight, const void* k, const void
 }
 
 // Beam selection's segments of a row: the longest that give the GPU two work-groups per CU, else the shortest.  8 beams of 16
-// sequences over 131071 bf16 tokens, at most 2 / 4 / 8 chunks a thread, us: 25.6 / 23.2 / 24.0 (segments 14.5 / 13.8 / 16.3, their ranking
-// 11.5 / 9.3 / 8.4; before both became shorter by the same 2 or 3).
+// sequences over 131071 bf16 tokens, at most 2 / 4 / 8 chunks a thread, us: 23.3 / 21.7 / 24.5 (segments 15.2 / 14.2 / 16.9, their ranking
+// 8.5 / 8.0 / 7.9).
 struct SelectPlan {
   int segments, chunks;
 };

@@ -19,11 +19,12 @@
 //
 // What bounds it, by replayed graphs and counters (D 128; both kernels, of which the merge takes 4.7 us, for drafts 9.4):
 //   one token for each of 32 sequences of up to 8192 rows (32 / 8 heads, bf16, e4m3): 63 us; 259 of 301 MB are read (values of far
-//     keys are not) at 4.75 TB/s, VALU busy 40 %, MFMA 11 %;
-//   24 drafts for each of 16 (int8): 82 us; VALU busy 51 %, MFMA 11 %: int8 has no conversion to bf16 (three instructions for two
+//     keys are not) at 5.0 TB/s, VALU busy 39 %, MFMA 11 %;
+//   24 drafts for each of 16 (int8): 82 us; VALU busy 50 %, MFMA 11 %: int8 has no conversion to bf16 (three instructions for two
 //     codes, e4m3 has one), and about 12 of them go with each score;
-//   7 drafts over 131072 rows (fp16, e4m3): 56 us; 233 MB at 5.1 TB/s;
-//   one token over 500 rows of 12 heads (bf16 D 64): 9.5 us in one work-group a head, the latency of its tiles in a row.
+//   7 drafts over 131072 rows (fp16, e4m3): 57 us; 233 MB at 5.1 TB/s;
+//   one token over 500 rows of 12 heads (bf16 D 64): 9.5 us in one work-group a head, the latency of its tiles in a row;
+//   8 tokens for each of 4 over 8192 rows (8 heads, fp32, e4m3): 62 us: products of 32 rows for 8, at a 16th of bf16's rate.
 // Taken step by step for the 32 sequences, the drafts and the long one: keys and values loaded where they are used 71, 115 and 64
 // us; keys a tile ahead, values while a tile is weighed, their product with the weights a tile late 67, 117 and 57; plans by the
 // batch's own lengths, two rounds of work-groups where several row blocks share keys: drafts 86; splits by kv head, the
