@@ -104,34 +104,40 @@ __device__ __forceinline__ unsigned nth_of_wave(unsigned x, int larger, int n) {
   return lane_of(x, __builtin_amdgcn_readfirstlane(__ffsll(is) - 1));
 }
 
-// Sums of exp(x), as a factor of 2^reference(m) for the largest x, m: a whole number, so that sums of parts are brought to one
-// reference exactly, or m log2 e itself where that is no number of a few digits.
-constexpr float kOrdinary = 0x1p20f;
-constexpr double kLog2e64 = 0x1.71547652b82fep0, kLn2_64 = 0x1.62e42fefa39efp-1;
+// Sums of exp(x) are relative to that of their largest x, m: what is as large weighs 1 exactly, so that a row's only candidate scores
+// what its beam does.  Of ordinary m, m log2 e is a whole number and a rest in [-1/2, 1/2], off by 2^-25.
+constexpr float kOrdinary = 0x1p20f, kWhole = 0x1.8p23f;
+constexpr double kLog2e64 = 0x1.71547652b82fep0;
 constexpr float kLog2eRest = (float)(kLog2e64 - (double)kLog2e);
-__device__ __forceinline__ float whole_reference(float m) { return rintf(m * kLog2e); }
-__device__ __forceinline__ double reference(float m) {
-  return fabsf(m) < kOrdinary ? (double)whole_reference(m) : (double)m * kLog2e64;
-}
+struct Reference {
+  float whole, rest;
+  __device__ __forceinline__ explicit Reference(float m) : whole(fmaf(m, kLog2e, kWhole) - kWhole), rest(rest_of(m, whole)) {}
+  static __device__ __forceinline__ float rest_of(float x, float k) { return fmaf(x, kLog2eRest, fmaf(x, kLog2e, -k)); }
+};
 // A sum against `from` as one against `to`, which is not less.
 __device__ __forceinline__ double rescaled(double sum, float from, float to) {
   if (from == to) return sum;  // (infinities, too)
-  if (fabsf(from) < kOrdinary && fabsf(to) < kOrdinary) return ldexp(sum, (int)(whole_reference(from) - whole_reference(to)));
-  return sum * exp2(reference(from) - reference(to));
+  if (fabsf(from) < kOrdinary && fabsf(to) < kOrdinary) {
+    const Reference a(from), b(to);
+    return ldexp(sum * exp2((double)a.rest - (double)b.rest), (int)(a.whole - b.whole));
+  }
+  return sum * exp2(((double)from - (double)to) * kLog2e64);
 }
-// exp(x) against the reference of an ordinary m, for x <= m, or NaN.  x log2 e is split into a whole number and a rest in [-1/2, 1/2]
-// that is off by 2^-25: the rest's power is off by 2^-23 of itself (one step of v_exp_f32) and 2^-25.5, whatever x is.  (A product
-// that is rounded as a whole, 17 for a logit that 2^20 of make as heavy as the largest, is off by 2^-20.)  What is below 2^-126
-// of the largest may come to 0.
+// exp(x - m) for an ordinary m and x <= m, or NaN.  x log2 e is split as m's is, so that whatever x is the exponent is off by 3 * 2^-25,
+// the weight by 2^-24 of itself, and its power by 2^-23 (one step of v_exp_f32): 2^-22.  (A product that is rounded as a whole, 17 for
+// a logit that 2^20 of make as heavy as the largest, is off by 2^-20.)  What is below 2^-126 may come to 0.
 struct Weights {
-  float least, magic;
-  __device__ __forceinline__ Weights(float m) : least(m - 128.f), magic(0x1.8p23f - whole_reference(m)) {}
+  float least, magic, rest;
+  __device__ __forceinline__ explicit Weights(float m) : least(m - 128.f) {
+    const Reference r(m);
+    magic = kWhole - r.whole;
+    rest = r.rest;
+  }
   __device__ __forceinline__ double operator()(float x) const {
     x = x < least ? least : x;
-    const float t = fmaf(x, kLog2e, magic);  // the whole number in its last bits: t lies in [2^23, 2^24)
-    const float k = t - magic;
-    const float rest = fmaf(x, kLog2eRest, fmaf(x, kLog2e, -k));
-    return (double)ldexpf(fast_exp2(rest), __builtin_bit_cast(int, t) - __builtin_bit_cast(int, 0x1.8p23f));
+    const float t = fmaf(x, kLog2e, magic);  // the whole numbers' difference in its last bits: t lies in [2^23, 2^24)
+    const float d = Reference::rest_of(x, t - magic) - rest;
+    return (double)ldexpf(fast_exp2(d), __builtin_bit_cast(int, t) - __builtin_bit_cast(int, kWhole));
   }
 };
 
@@ -401,9 +407,7 @@ __global__ __launch_bounds__(kSelectThreads) void coalibi_select_beams_kernel(Se
       double sum = rescaled(s0, m0, m);
       for (int s = lane + 64; s < a.segments; s += 64) sum += rescaled(ps[s], pm[s], m);
       sum = wave_sum(sum);
-      // (What the reference is more than m goes with the sum, so that a logit counts by its distance to m.)
-      const double more = fabsf(m) < kOrdinary ? (double)whole_reference(m) * kLn2_64 - (double)m : 0.0;
-      if (!__any(nan) && m > kNegInf) base = (double)score - (log(sum) + more);
+      if (!__any(nan) && m > kNegInf) base = (double)score - log(sum);
     }
     if (lane == 0) {
       sbase[w] = score > kNegInf && score < __builtin_inff() ? base : __builtin_nan("");

@@ -86,3 +86,25 @@ def test_infinite_and_missing_numbers():
     logits[0, 4, :99000] = -math.inf
     logits[0, 5, ::2] = torch.finfo(F32).min
     check(logits, torch.zeros(1, 6), 20)
+
+
+@pytest.mark.parametrize("dtype", (F32, BF16, F16), ids=str)
+def test_a_sole_candidate_scores_what_its_beam_does(dtype):
+    """One token, or one that a mask leaves: log_softmax is 0 exactly, whatever the logit is, and beams of one score go in order; so do
+    those with the same number of equal logits."""
+    gen = torch.Generator().manual_seed(11)
+    for V in (1, 2, 9, 1000, 50257):
+        logits = torch.full((2, 16, V), -math.inf)
+        where = torch.randint(0, V, (2, 16, 1), generator=gen)
+        logits.scatter_(2, where, torch.randn(2, 16, 1, generator=gen) * torch.tensor([1.0, 300.0]).view(2, 1, 1))
+        scores = -torch.randint(0, 3, (2, 16), generator=gen).float() * 0.7
+        s, p, t = (x.cpu() for x in co_alibi_beam_select(logits.to(dtype).to(DEV), scores.to(DEV), 16))
+        order = scores.sort(dim=1, descending=True, stable=True)
+        assert torch.equal(s, order.values) and torch.equal(p.long(), order.indices)
+        assert torch.equal(t, where[:, :, 0].gather(1, order.indices))
+        if V > 500:
+            logits = torch.full((1, 8, V), -math.inf)
+            for w in range(8):
+                logits[0, w, torch.randperm(V, generator=gen)[:40]] = torch.tensor(1.7 * w - 5.3).to(dtype).float()
+            s, p, t = (x.cpu() for x in co_alibi_beam_select(logits.to(dtype).to(DEV), torch.zeros(1, 8, device=DEV), 64))
+            assert p[0].tolist() == [0] * 40 + [1] * 24 and (s == s[0, 0]).all() and abs(s[0, 0].item() + math.log(40)) < 2.0 ** -21
