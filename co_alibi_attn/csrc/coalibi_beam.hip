@@ -16,13 +16,13 @@
 // its rows.  That many are free, as no more than W are in use.  A wavefront works out a column's W beams by itself, a lane
 // each, for the tables and again for every copy, so that all is one launch.
 //
-// Measured in replayed graphs.  Selection, 8 beams of 16 sequences over 131071 bf16 logits, a third of them finished: 21.7 us, of which
-// the segments take 14.2 (22.5 MB, which a copy takes 4.6 us for: a segment's loads, its bound, its weights and its list follow one
-// another; VALU busy 34 %) and the ranking 8.0, loads and steps of one work-group per sequence in a row.  With exponents rounded as a
+// Measured in replayed graphs.  Selection, 8 beams of 16 sequences over 131071 bf16 logits, a third of them finished: 22.2 us, of which
+// the segments take 14.6 (22.5 MB, which a copy takes 4.6 us for: a segment's loads, its bound, its weights and its list follow one
+// another; VALU busy 37 %) and the ranking 7.9, loads and steps of one work-group per sequence in a row.  With exponents rounded as a
 // whole, up to 33 weights added in fp32 and rows read from their first 16-byte boundary on, log S was off by 1e-6 and equal rows got
 // different sums; it took 18.8, 11.9 and 7.4.  Against that: lists counted by one wavefront 13.8 and 9.4, a bound by counting 64 lanes in
 // the segments 14.4, weights against the work-group's maximum 12.9.  4 beams over 50304: 9.5 us.  16 beams of 8 sequences over 50304, 16
-// and 32 kept: 22.7 and 37.4 us; 32 of 16 beams over 131072 fp32 34 (groups' bounds for all N and lists one after the other were 1.5,
+// and 32 kept: 23.1 and 37.7 us; 32 of 16 beams over 131072 fp32 34 (groups' bounds for all N and lists one after the other were 1.5,
 // 2.4 and 6 times as long).
 // Reordering, 4 beams, 24 pools: 4.3 us.  8 beams of 16 sequences, 8 pools of codes and 8 of scales: 11.5 us for 21 MB, which a copy
 // takes 4.3 for: 2176 work-groups, of which most find nothing to copy (as many again take 3.5 us more), and three dependent

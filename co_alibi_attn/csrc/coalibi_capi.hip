@@ -1062,8 +1062,8 @@ int append_args(const char* fn, int dtype, bool eight, const void* k, const void
 }
 
 // Beam selection's segments of a row: the longest that give the GPU two work-groups per CU, else the shortest.  8 beams of 16
-// sequences over 131071 bf16 tokens, at most 2 / 4 / 8 chunks a thread, us: 23.3 / 21.7 / 24.5 (segments 15.2 / 14.2 / 16.9, their ranking
-// 8.5 / 8.0 / 7.9).
+// sequences over 131071 bf16 tokens, at most 2 / 4 / 8 chunks a thread, us: 24.2 / 22.2 / 24.8 (segments 16.1 / 14.9 / 17.4, their ranking
+// 8.4 / 7.9 / 7.8).
 struct SelectPlan {
   int segments, chunks;
 };
