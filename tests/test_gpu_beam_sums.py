@@ -1,7 +1,7 @@
 """co_alibi_beam_select's sums where the exponentials' errors do not cancel: many equal logits far below the largest.  Needs an MI355X.
 
-log S may be off by 2^-22: a weight's exponential by 2^-23 of itself (one step of its instruction), its reduced argument by 2^-25,
-in powers of two, which is 2^-25.5 of the weight; sums and powers of two are exact or fp64.  The score is rounded to fp32 once more:
+log S may be off by 2^-22: a weight's exponential by 2^-23 of itself (one step of its instruction), its reduced argument by three
+roundings of 2^-25, in powers of two, which is 2^-24 of the weight; sums and powers of two are exact or fp64.  The score is rounded to fp32 once more:
 2^-24 of itself.
 """
 import math
